@@ -136,6 +136,22 @@ int ops_rope_create(int device, ops_rope **out);
 int ops_rope_scheme(ops_rope *op, const ops_rope_args *args, size_t max_ws, size_t *ws_out);
 int ops_rope_launch(const ops_rope *op, const ops_rope_args *args, void *ws, size_t ws_len, void *stream);
 void ops_rope_destroy(ops_rope *op);
+/* Extension with no counterpart in the crate, which chains rms_norm (one launch per operand, its weight shared by all rows) and
+ * rope: the heads of x [nt, nh, dh] are normalised one by one, weighted and rotated in one pass.
+ *   n[d] = x[d] * w[h, d] / sqrt(mean_d(x[h, :]^2) + epsilon);  y[2k], y[2k+1] = the pair (n[2k], n[2k+1]) turned by pos / theta^(2k/dh)
+ * Everything is held in f32 and rounded once; the angle is formed and reduced in f64, so far positions lose nothing (ops_rope
+ * forms it in f32, as the crate does).  w [nh, dh], one row per head (stride 0 shares a row), so that the query and the key heads
+ * of a fused projection go through one launch.  y may be x.  f16 or bf16, w of the same type or f32, p u32 or u64, dh a multiple
+ * of 8 up to 256, 16-byte aligned rows; other layouts are answered with OPS_ARGS_NOT_SUPPORT (chain the two operators then). */
+typedef struct {
+  ops_layout y_layout; void *y_base;
+  ops_layout x_layout; const void *x_base;
+  ops_layout p_layout; const void *p_base;
+  ops_layout w_layout; const void *w_base;
+  float epsilon;
+  float theta;
+} ops_rope_norm_args;
+int ops_rope_norm_launch(const ops_rope *op, const ops_rope_norm_args *args, void *stream);
 /* Rope::build_pos (operators/src/rope/mod.rs:17-21, fill_pos :44-58): writes, for every (pos,len)
  * sequence in order, pos..pos+len into a HOST buffer of `nt` u32 or u64; the caller uploads it. */
 int ops_rope_build_pos(uint32_t dt, size_t nt, const size_t *seq_pos, const size_t *seq_len, size_t nseq, void *host_out);
@@ -270,6 +286,85 @@ int ops_attention_kv_cached_set_algo(ops_attention_kv_cached *op, int algo);
 int ops_attention_kv_cached_scheme(ops_attention_kv_cached *op, const ops_attention_kv_cached_args *args, size_t max_ws, size_t *ws_out);
 int ops_attention_kv_cached_launch(const ops_attention_kv_cached *op, const ops_attention_kv_cached_args *args, void *ws, size_t ws_len, void *stream);
 void ops_attention_kv_cached_destroy(ops_attention_kv_cached *op);
+
+/* ---------------------------------------------------------------------------------------------
+ * A batch of requests over a paged cache.  No counterpart in the crate, whose attention_kv_cached serves one sequence with one
+ * contiguous cache; the same step for many sequences of different lengths at once:
+ *     kv_append_paged: q, k rotated (and normalised per head if asked), k and v written into the sequences' pages
+ *     attention_paged: every new token attends to its sequence's pages
+ *
+ * The cache is k_pages, v_pages [npages, nkvh, page, dh] (any order of the dims in memory: the strides say), `page` a power of
+ * two from 8 to 65536.  The rows of the step are the new tokens of all sequences, packed: sequence i owns the rows
+ * [seq_start[i], seq_start[i + 1]) and, the new tokens included, the cache slots [0, kv_len[i]); slot s lies in page
+ * page_table[i, s / page] at s % page.  Rows in front of seq_start[0] and from seq_start[nseq] on belong to nobody and are left as
+ * they are, so a captured launch can be padded.  All three are device arrays of u32 (i32 is taken as its bits), read when the
+ * kernels run: a captured graph may be replayed after they have changed.
+ *
+ * What the arrays hold is checked where it is used; nothing outside the tensors is ever read or written.  What is wrong sets
+ * the handle's status word (the first code sticks), which ops_<op>_status reads (it synchronises the device):
+ *   OPS_PAGED_BAD_PAGE    a page number >= npages: its keys and values read as zeros, a token meant for it is not written
+ *   OPS_PAGED_BAD_LENGTH  kv_len[i] beyond the table's width x page (attention_paged cuts it to that), or, for kv_append_paged, fewer
+ *                         slots than new tokens; tokens without a slot of the table are not written
+ *   OPS_PAGED_BAD_ROWS    seq_start decreases or passes nt (cut to that), or a sequence has more new tokens than max_seq (attention
+ *                         leaves its rows as they are)
+ * Codes from 100 on: a bounded wait inside a kernel ran out (the launch's output is undefined then).
+ * ------------------------------------------------------------------------------------------- */
+enum { OPS_PAGED_BAD_PAGE = 1, OPS_PAGED_BAD_LENGTH = 2, OPS_PAGED_BAD_ROWS = 3 };
+typedef struct {
+  ops_layout page_table_layout; const void *page_table_base; /* [nseq, width], rows contiguous */
+  ops_layout seq_start_layout; const void *seq_start_base;   /* [nseq + 1] */
+  ops_layout kv_len_layout; const void *kv_len_base;         /* [nseq] */
+  size_t max_seq; /* no sequence has more new tokens than this; 0: unknown (a step of single tokens then costs an idle launch) */
+} ops_paged_batch;
+
+/* kv_append_paged: q_out <- rotated q (q_out may be q); k rotated and v as it is into the pages of their slots.  The rotation is
+ * rope's (adjacent pairs, angle pos / theta^(2k/dh), formed in f64); positions come from p [nt], as for rope.  With w given
+ * ([nh + nkvh, dh], query heads first; stride 0 shares a row) the heads of q and k are normalised first, as ops_rope_norm_launch
+ * does.  q, q_out [nt, nh, dh], k, v [nt, nkvh, dh]; f16 or bf16, all of one type; w of that type or f32, w_base NULL: no norm;
+ * dh a multiple of 8 up to 256; unit inner strides, every row 16-byte aligned. */
+typedef struct ops_kv_append_paged ops_kv_append_paged;
+typedef struct {
+  ops_layout q_out_layout; void *q_out_base;
+  ops_layout q_layout; const void *q_base;
+  ops_layout k_layout; const void *k_base;
+  ops_layout v_layout; const void *v_base;
+  ops_layout k_pages_layout; void *k_pages_base;
+  ops_layout v_pages_layout; void *v_pages_base;
+  ops_layout p_layout; const void *p_base;
+  ops_layout w_layout; const void *w_base;
+  ops_paged_batch batch;
+  float epsilon;
+  float theta;
+} ops_kv_append_paged_args;
+int ops_kv_append_paged_create(int device, ops_kv_append_paged **out);
+int ops_kv_append_paged_scheme(ops_kv_append_paged *op, const ops_kv_append_paged_args *args, size_t max_ws, size_t *ws_out);
+int ops_kv_append_paged_launch(const ops_kv_append_paged *op, const ops_kv_append_paged_args *args, void *ws, size_t ws_len, void *stream);
+int ops_kv_append_paged_status(const ops_kv_append_paged *op);
+int ops_kv_append_paged_status_reset(ops_kv_append_paged *op);
+void ops_kv_append_paged_destroy(ops_kv_append_paged *op);
+
+/* attention_paged: o = softmax_mask(scale q k^T) v over the sequence's own slots, grouped-query heads.  q, o [nh, nt, dh] (the order
+ * of ops_attention), nh a multiple of nkvh, up to 128 query heads per kv head.  With OPS_MASK_CAUSAL the j-th of n new tokens of a
+ * sequence sees the slots [0, kv_len - n + j + 1), with OPS_MASK_NONE all kv_len; a row that sees nothing becomes zeros.  Slots
+ * past kv_len are never used, whatever they hold.  Scores, softmax and sums are f32, the probabilities enter the second product
+ * in the element type, o is rounded once.  f16 or bf16, dh a multiple of 8 up to 128, unit inner strides, every row 16-byte
+ * aligned, no negative strides. */
+typedef struct ops_attention_paged ops_attention_paged;
+typedef struct {
+  ops_layout q_layout; const void *q_base;
+  ops_layout k_pages_layout; const void *k_pages_base;
+  ops_layout v_pages_layout; const void *v_pages_base;
+  ops_layout o_layout; void *o_base;
+  ops_paged_batch batch;
+  uint8_t mask;
+  float scale;
+} ops_attention_paged_args;
+int ops_attention_paged_create(int device, ops_attention_paged **out);
+int ops_attention_paged_scheme(ops_attention_paged *op, const ops_attention_paged_args *args, size_t max_ws, size_t *ws_out);
+int ops_attention_paged_launch(const ops_attention_paged *op, const ops_attention_paged_args *args, void *ws, size_t ws_len, void *stream);
+int ops_attention_paged_status(const ops_attention_paged *op);
+int ops_attention_paged_status_reset(ops_attention_paged *op);
+void ops_attention_paged_destroy(ops_attention_paged *op);
 
 /* ---------------------------------------------------------------------------------------------
  * random_sample — random_sample::Args, SampleArgs (operators/src/random_sample/args.rs:9-84);

@@ -37,6 +37,7 @@ REDUCE_SUM, REDUCE_PROD, REDUCE_MIN, REDUCE_MAX, REDUCE_MEAN = range(5)
 ATTENTION_CHAIN, ATTENTION_FUSED, ATTENTION_FUSED_ONE_TILE = 0, 1, 2
 ATTENTION_MAX_RUNS, ATTENTION_RUN_RECORD_BYTES = 4, 528  # OPS_ATTENTION_MAX_RUNS, OPS_ATTENTION_RUN_RECORD_BYTES
 ALL_REDUCE_AUTO, ALL_REDUCE_NCCL, ALL_REDUCE_P2P_ONE_SHOT, ALL_REDUCE_P2P_TWO_SHOT = range(4)
+PAGED_BAD_PAGE, PAGED_BAD_LENGTH, PAGED_BAD_ROWS = 1, 2, 3
 COMM_ID_BYTES, COMM_P2P_HANDLE_BYTES = 128, 128
 
 
@@ -227,10 +228,30 @@ _AddArgs = _struct("_AddArgs", [("c_layout", _Layout), ("c_base", ctypes.c_void_
                                 ("b_layout", _Layout), ("b_base", ctypes.c_void_p)])
 _AddRowsArgs = _struct("_AddRowsArgs", [("dst_layout", _Layout), ("dst_base", ctypes.c_void_p), ("src_layout", _Layout),
                                         ("src_base", ctypes.c_void_p), ("idx_layout", _Layout), ("idx_base", ctypes.c_void_p)])
+_RopeNormArgs = _struct("_RopeNormArgs", [("y_layout", _Layout), ("y_base", ctypes.c_void_p), ("x_layout", _Layout), ("x_base", ctypes.c_void_p),
+                                          ("p_layout", _Layout), ("p_base", ctypes.c_void_p), ("w_layout", _Layout), ("w_base", ctypes.c_void_p),
+                                          ("epsilon", ctypes.c_float), ("theta", ctypes.c_float)])
+_PagedBatch = _struct("_PagedBatch", [("page_table_layout", _Layout), ("page_table_base", ctypes.c_void_p), ("seq_start_layout", _Layout),
+                                      ("seq_start_base", ctypes.c_void_p), ("kv_len_layout", _Layout), ("kv_len_base", ctypes.c_void_p),
+                                      ("max_seq", ctypes.c_size_t)])
+_KvAppendPagedArgs = _struct("_KvAppendPagedArgs", [("q_out_layout", _Layout), ("q_out_base", ctypes.c_void_p), ("q_layout", _Layout),
+                                                    ("q_base", ctypes.c_void_p), ("k_layout", _Layout), ("k_base", ctypes.c_void_p),
+                                                    ("v_layout", _Layout), ("v_base", ctypes.c_void_p), ("k_pages_layout", _Layout),
+                                                    ("k_pages_base", ctypes.c_void_p), ("v_pages_layout", _Layout),
+                                                    ("v_pages_base", ctypes.c_void_p), ("p_layout", _Layout), ("p_base", ctypes.c_void_p),
+                                                    ("w_layout", _Layout), ("w_base", ctypes.c_void_p), ("batch", _PagedBatch),
+                                                    ("epsilon", ctypes.c_float), ("theta", ctypes.c_float)])
+_AttentionPagedArgs = _struct("_AttentionPagedArgs", [("q_layout", _Layout), ("q_base", ctypes.c_void_p), ("k_pages_layout", _Layout),
+                                                      ("k_pages_base", ctypes.c_void_p), ("v_pages_layout", _Layout),
+                                                      ("v_pages_base", ctypes.c_void_p), ("o_layout", _Layout), ("o_base", ctypes.c_void_p),
+                                                      ("batch", _PagedBatch), ("mask", ctypes.c_uint8), ("scale", ctypes.c_float)])
 
 
 def _lay(x):
     return x if isinstance(x, TensorLayout) else TensorLayout.of(x)
+
+
+_NO_WEIGHT = TensorLayout(F32, (), ())  # the layout beside a null weight: never looked at
 
 
 class RmsNormArgs(_ArgsBase):
@@ -357,6 +378,67 @@ class AttentionKvCachedArgs(_ArgsBase):
     @classmethod
     def of(cls, q, k, v, o, k_cache, v_cache, pos, mask=MASK_CAUSAL):
         return cls(q, q, k, k, v, v, o, o, k_cache, k_cache, v_cache, v_cache, mask, pos)
+
+
+class RopeNormArgs(_ArgsBase):
+    """Arguments of the extension ops_rope_norm_launch: y <- rotate(rms_norm of every head of x, weighted by w[head])."""
+
+    def __init__(self, y_layout, y_base, x_layout, x_base, p_layout, p_base, w_layout, w_base, epsilon, theta):
+        self._alive = (y_base, x_base, p_base, w_base)
+        self.keep = (_lay(y_layout), _lay(x_layout), _lay(p_layout), _lay(w_layout))
+        k = self.keep
+        self.c = _RopeNormArgs(k[0].c, _vp(y_base), k[1].c, _vp(x_base), k[2].c, _vp(p_base), k[3].c, _vp(w_base), epsilon, theta)
+
+    @classmethod
+    def of(cls, y, x, pos, w, epsilon, theta):
+        return cls(y, y, x, x, pos, pos, w, w, epsilon, theta)
+
+
+class PagedBatch:
+    """ops_paged_batch: which rows of a step belong to which sequence, and in which pages its keys and values lie.
+
+    page_table [nseq, width], seq_start [nseq + 1], kv_len [nseq]: device tensors of int32 or uint32, read when the kernels
+    run.  max_seq: no sequence has more new tokens than this (0: unknown)."""
+
+    def __init__(self, page_table, seq_start, kv_len, max_seq=0):
+        self._alive = (page_table, seq_start, kv_len)
+        self.keep = (_lay(page_table), _lay(seq_start), _lay(kv_len))
+        k = self.keep
+        base = [None if isinstance(t, TensorLayout) else t for t in self._alive]
+        self.c = _PagedBatch(k[0].c, _vp(base[0]), k[1].c, _vp(base[1]), k[2].c, _vp(base[2]), int(max_seq))
+
+
+class KvAppendPagedArgs(_ArgsBase):
+    """ops_kv_append_paged_args: rotate (and optionally normalise) q and k, write k and v into the pages of their slots."""
+
+    def __init__(self, q_out_layout, q_out_base, q_layout, q_base, k_layout, k_base, v_layout, v_base, k_pages_layout, k_pages_base,
+                 v_pages_layout, v_pages_base, p_layout, p_base, w_layout, w_base, batch, epsilon, theta):
+        self._alive = (q_out_base, q_base, k_base, v_base, k_pages_base, v_pages_base, p_base, w_base, batch)
+        self.keep = tuple(_lay(x) for x in (q_out_layout, q_layout, k_layout, v_layout, k_pages_layout, v_pages_layout, p_layout, w_layout))
+        k = self.keep
+        self.c = _KvAppendPagedArgs(k[0].c, _vp(q_out_base), k[1].c, _vp(q_base), k[2].c, _vp(k_base), k[3].c, _vp(v_base), k[4].c,
+                                    _vp(k_pages_base), k[5].c, _vp(v_pages_base), k[6].c, _vp(p_base), k[7].c, _vp(w_base), batch.c,
+                                    epsilon, theta)
+
+    @classmethod
+    def of(cls, q_out, q, k, v, k_pages, v_pages, pos, batch, theta, w=None, epsilon=1e-5):
+        return cls(q_out, q_out, q, q, k, k, v, v, k_pages, k_pages, v_pages, v_pages, pos, pos, _NO_WEIGHT if w is None else w, w, batch,
+                   epsilon, theta)
+
+
+class AttentionPagedArgs(_ArgsBase):
+    """ops_attention_paged_args: q, o [nh, nt, dh], k_pages, v_pages [npages, nkvh, page, dh]; scale None = 1 / sqrt(dh)."""
+
+    def __init__(self, q_layout, q_base, k_pages_layout, k_pages_base, v_pages_layout, v_pages_base, o_layout, o_base, batch, mask, scale):
+        self._alive = (q_base, k_pages_base, v_pages_base, o_base, batch)
+        self.keep = (_lay(q_layout), _lay(k_pages_layout), _lay(v_pages_layout), _lay(o_layout))
+        k = self.keep
+        self.c = _AttentionPagedArgs(k[0].c, _vp(q_base), k[1].c, _vp(k_pages_base), k[2].c, _vp(v_pages_base), k[3].c, _vp(o_base), batch.c,
+                                     mask, scale)
+
+    @classmethod
+    def of(cls, q, k_pages, v_pages, o, batch, mask=MASK_CAUSAL, scale=None):
+        return cls(q, q, k_pages, k_pages, v_pages, v_pages, o, o, batch, mask, q.shape[2] ** -0.5 if scale is None else scale)
 
 
 class SampleArgsError(ValueError):
@@ -536,6 +618,12 @@ class RmsNorm(Operator):
 class Rope(Operator):
     NAME = "rope"
 
+    def launch_norm(self, args, queue_alloc=None):
+        """ops_rope_norm_launch: every head normalised, weighted and rotated in one pass."""
+        qa = queue_alloc or TorchQueueAlloc()
+        self._last_args = args
+        _check(lib().ops_rope_norm_launch(self._h, args.byref(), ctypes.c_void_p(qa.queue())), True)
+
     @staticmethod
     def build_pos(dt, nt, seqs):
         """Rope::build_pos (operators/src/rope/mod.rs:17-21): seqs = [(pos, len), ...] -> host numpy array."""
@@ -603,6 +691,23 @@ class AttentionKvCached(Operator):
 
     def set_algo(self, algo):
         _check(lib().ops_attention_kv_cached_set_algo(self._h, ctypes.c_int(algo)), False)
+
+
+class _PagedOperator(Operator):
+    def status(self):
+        """0, or what the device found wrong first (PAGED_BAD_*; from 100 on a bounded wait ran out).  Synchronises."""
+        return getattr(lib(), f"ops_{self.NAME}_status")(self._h)
+
+    def status_reset(self):
+        _check(getattr(lib(), f"ops_{self.NAME}_status_reset")(self._h), False)
+
+
+class KvAppendPaged(_PagedOperator):
+    NAME = "kv_append_paged"
+
+
+class AttentionPaged(_PagedOperator):
+    NAME = "attention_paged"
 
 
 class RandomSample(Operator):
@@ -768,7 +873,8 @@ class AddRows(Operator):
 EXPORTS = [
     "ops_last_error", "ops_last_workspace_need", "ops_dtype_nbytes", "ops_device_count", "ops_build_info",
     *[f"ops_{op}_{fn}" for op in ("rms_norm", "rope", "fused_softmax", "swiglu", "rearrange", "mat_mul", "attention",
-                                  "attention_kv_cached", "random_sample", "all_reduce", "broadcast", "add", "add_rows")
+                                  "attention_kv_cached", "random_sample", "all_reduce", "broadcast", "add", "add_rows",
+                                  "kv_append_paged", "attention_paged")
       for fn in ("create", "scheme", "launch", "destroy")],
     "ops_rope_build_pos", "ops_rearrange_plan", "ops_mat_mul_status", "ops_mat_mul_status_reset", "ops_attention_set_algo", "ops_attention_status",
     "ops_attention_status_reset",
@@ -777,5 +883,7 @@ EXPORTS = [
     "ops_random_sample_noalloc_max_logits", "ops_random_sample_launch_noalloc", "ops_comm_unique_id",
     "ops_comm_init_rank", "ops_comm_rank", "ops_comm_group_size", "ops_comm_destroy", "ops_comm_p2p_export",
     "ops_comm_p2p_attach", "ops_comm_p2p_status", "ops_comm_p2p_reset", "ops_comm_p2p_direct", "ops_comm_nvls_attach", "ops_all_reduce_add_launch",
+    "ops_rope_norm_launch", "ops_kv_append_paged_status", "ops_kv_append_paged_status_reset", "ops_attention_paged_status",
+    "ops_attention_paged_status_reset",
     "ops_rms_norm_add_launch", "ops_comm_create_loopback", "ops_all_reduce_set_algo", "ops_add_rows_status", "ops_mat_mul_all_reduce_launch",
 ]

@@ -53,6 +53,24 @@ struct OpBase {
 };
 int init_base(OpBase *b, int device);
 
+// Makes `device` current for a launch and gives the caller's current device back.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(int device) {
+    if (cudaGetDevice(&before_) != cudaSuccess) before_ = device;
+    if (before_ != device) cudaSetDevice(device);
+    device_ = device;
+  }
+  ~DeviceGuard() {
+    if (before_ != device_) cudaSetDevice(before_);
+  }
+  DeviceGuard(const DeviceGuard &) = delete;
+  DeviceGuard &operator=(const DeviceGuard &) = delete;
+
+ private:
+  int before_ = 0, device_ = 0;
+};
+
 // Kernel launch epilogue: turns a launch-time CUDA error into ExecutionFailed.
 inline int check_launch(const char *what) {
   cudaError_t e = cudaGetLastError();

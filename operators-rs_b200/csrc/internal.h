@@ -20,4 +20,6 @@ usz attention_decode_ticket_bytes();
 int attention_decode_enqueue(const OpBase &base, const ops_attention_args *a, usz nh, usz nkvh, usz seq, usz att, usz dh, float *scratch,
                              unsigned int *tickets, cudaStream_t s);
 
+int rope_norm_enqueue(const OpBase *base, const ops_rope_norm_args *a, cudaStream_t s);
+
 }  // namespace ops

@@ -1,0 +1,37 @@
+// paged.cu — the status word of the paged operators' handles.
+#include "paged.h"
+
+namespace ops {
+
+int paged_create(PagedHandle *h, int device) {
+  h->status = nullptr;
+  OPS_TRY(init_base(&h->base, device));
+  DeviceGuard guard(device);
+  if (cudaMalloc(&h->status, sizeof(int)) != cudaSuccess || cudaMemset(h->status, 0, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    if (h->status) cudaFree(h->status);
+    return fail(OPS_EXECUTION_FAILED, "cannot allocate the status word");
+  }
+  return OPS_OK;
+}
+
+void paged_destroy(PagedHandle *h) {
+  if (h->status) cudaFree(h->status);
+}
+
+int paged_status(const PagedHandle *h) {
+  DeviceGuard guard(h->base.device);
+  int v = -1;
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(&v, h->status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
+  return v;
+}
+
+int paged_status_reset(PagedHandle *h) {
+  DeviceGuard guard(h->base.device);
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemset(h->status, 0, sizeof(int));
+  if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "status reset: %s", cudaGetErrorString(e));
+  return OPS_OK;
+}
+
+}  // namespace ops

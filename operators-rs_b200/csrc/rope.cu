@@ -12,6 +12,7 @@
 // from bit-identical divisors; the division is IEEE and sincosf is the full-range (non fast-math) one.
 #include "common.h"
 #include "device_utils.cuh"
+#include "internal.h"
 
 namespace ops {
 
@@ -173,6 +174,11 @@ OPS_API int ops_rope_launch(const ops_rope *op, const ops_rope_args *a, void *ws
 #undef ROPE_GENERIC
   }
   return check_launch("rope");
+}
+
+// Extension with no counterpart in the crate: norm, weight and rotation of every head in one pass (rope_norm.cu).
+OPS_API int ops_rope_norm_launch(const ops_rope *op, const ops_rope_norm_args *a, void *stream) {
+  return rope_norm_enqueue(op ? &op->base : nullptr, a, (cudaStream_t)stream);
 }
 
 // Rope::build_pos / fill_pos (operators/src/rope/mod.rs:44-58): positions of each (pos, len) run.

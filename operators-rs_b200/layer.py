@@ -13,8 +13,9 @@ how the partials and the residual meet.
 """
 from dataclasses import dataclass
 
-from . import (ALL_REDUCE_AUTO, ATTENTION_MAX_RUNS, ATTENTION_RUN_RECORD_BYTES, MASK_CAUSAL, AllReduce, AllReduceArgs, Attention, AttentionArgs, FusedSoftmax, MatMul,
-               MatMulArgs, Rearrange, RmsNorm, RmsNormArgs, Rope, RopeArgs, Swiglu, SwigluArgs)
+from . import (ALL_REDUCE_AUTO, ATTENTION_MAX_RUNS, ATTENTION_RUN_RECORD_BYTES, MASK_CAUSAL, AllReduce, AllReduceArgs, Attention, AttentionArgs, AttentionPaged,
+               AttentionPagedArgs, FusedSoftmax, KvAppendPaged, KvAppendPagedArgs, MatMul, MatMulArgs, Rearrange, RmsNorm, RmsNormArgs, Rope, RopeArgs,
+               RopeNormArgs, Swiglu, SwigluArgs)
 
 
 @dataclass
@@ -40,7 +41,7 @@ def shard_weights(w, rank, tp, cfg):
     """Column/row split of the full weights for `rank` of `tp` (works on numpy arrays and torch tensors).
 
     w: dict with w_norm1 [d], w_qkv [d, (nh+2*nkvh)*dh] (q heads | k heads | v heads), w_o [nh*dh, d],
-       w_norm2 [d], w_gu [d, 2*ffn] (gate | up), w_down [ffn, d].
+       w_norm2 [d], w_gu [d, 2*ffn] (gate | up), w_down [ffn, d]; optionally w_qk_norm [nh+nkvh, dh] (q heads | k heads).
     """
     if tp == 1:
         return dict(w)
@@ -52,7 +53,9 @@ def shard_weights(w, rank, tp, cfg):
                w["w_qkv"][:, k0 + rank * nkv * dh: k0 + (rank + 1) * nkv * dh],
                w["w_qkv"][:, v0 + rank * nkv * dh: v0 + (rank + 1) * nkv * dh]], 1)
     gu = cat([w["w_gu"][:, rank * f:(rank + 1) * f], w["w_gu"][:, cfg.ffn + rank * f: cfg.ffn + (rank + 1) * f]], 1)
-    return {"w_norm1": w["w_norm1"], "w_norm2": w["w_norm2"], "w_qkv": qkv, "w_gu": gu,
+    norm = {} if "w_qk_norm" not in w else {"w_qk_norm": cat([w["w_qk_norm"][rank * nq: (rank + 1) * nq],
+                                                              w["w_qk_norm"][cfg.nh + rank * nkv: cfg.nh + (rank + 1) * nkv]], 0)}
+    return {**norm, "w_norm1": w["w_norm1"], "w_norm2": w["w_norm2"], "w_qkv": qkv, "w_gu": gu,
             "w_o": _contig(w["w_o"][rank * nq * dh:(rank + 1) * nq * dh]), "w_down": _contig(w["w_down"][rank * f:(rank + 1) * f])}
 
 
@@ -95,6 +98,8 @@ class DecoderLayer:
     that wait at once could starve each other of SMs in opposite orders on different ranks) while the projections of the
     other chunk keep the tensor cores busy.  (Measured on 2 and 8 B200s it is slower than running in order — two
     persistent GEMMs and the exchange kernel contend for the same SMs — so the default is `pipeline` = 1.)
+    Weights that hold w_qk_norm [nh + nkvh, dh] make the layer normalise the heads of q and k in front of the rotation
+    (ops_rope_norm_launch in place of rope).  `forward_paged` runs the same layer for a batch of requests over a paged cache.
     With `direct_region` (the first half of an attached NVLink multicast buffer, Comm.nvls_attach) the partials are written
     there instead and the reduce-scatter half of the exchange is done inside the switch.
     """
@@ -113,6 +118,7 @@ class DecoderLayer:
         self.cfg, self.w, self.device, self.tp, self.rank = cfg, weights, device, tp, rank
         idx = device.index if device.index is not None else 0
         self.rope, self.attention = Rope(idx), Attention(idx)
+        self.kv_append_paged, self.attention_paged, self.paged_ws = KvAppendPaged(idx), AttentionPaged(idx), None
         self.all_reduce = None
         self.direct_buf = None
         if tp > 1:
@@ -151,15 +157,13 @@ class DecoderLayer:
         hooks; with it the tail runs unpipelined so that the hooks see one operator at a time)."""
         import torch
         cfg, T = self.cfg, x.shape[0]
-        assert T <= self.max_tokens
         mark = on_step or (lambda name: None)
-        h, qkv, att_out = self.h[:T], self.qkv[:T], self.att_out[:T]
-        self.rms_norm.launch(RmsNormArgs.of(h, x, self.w["w_norm1"], cfg.eps))
-        mark("rms_norm_1")
-        self.mat_mul.launch(MatMulArgs.of(qkv, 0.0, h, self.w["w_qkv"], 1.0))
-        mark("mat_mul_qkv")
-        heads = qkv.view(T, self.nq + 2 * self.nkv, cfg.dh)
-        self.rope.launch(RopeArgs.of(heads[:, : self.nq + self.nkv], pos, cfg.theta))
+        att_out, heads = self._project_qkv(x, mark)
+        qk = heads[:, : self.nq + self.nkv]
+        if "w_qk_norm" in self.w:
+            self.rope.launch_norm(RopeNormArgs.of(qk, qk, pos, self.w["w_qk_norm"], cfg.eps, cfg.theta))
+        else:
+            self.rope.launch(RopeArgs.of(qk, pos, cfg.theta))
         mark("rope")
         q = heads[:, : self.nq].permute(1, 0, 2)
         k = heads[:, self.nq: self.nq + self.nkv].permute(1, 0, 2)
@@ -189,6 +193,42 @@ class DecoderLayer:
         lane = self.lanes[0]
         xr = self._stage_o(lane, x, 0, T, mark)
         return self._stage_mlp(lane, xr, 0, T, mark)
+
+    def _project_qkv(self, x, mark):
+        """First norm and QKV projection of x [T, d]: (attention's output rows, the projection as [T, heads, dh])."""
+        cfg, T = self.cfg, x.shape[0]
+        assert T <= self.max_tokens
+        h, qkv = self.h[:T], self.qkv[:T]
+        self.rms_norm.launch(RmsNormArgs.of(h, x, self.w["w_norm1"], cfg.eps))
+        mark("rms_norm_1")
+        self.mat_mul.launch(MatMulArgs.of(qkv, 0.0, h, self.w["w_qkv"], 1.0))
+        mark("mat_mul_qkv")
+        return self.att_out[:T], qkv.view(T, self.nq + 2 * self.nkv, cfg.dh)
+
+    def forward_paged(self, x, pos, batch, k_pages, v_pages, on_step=None):
+        """The layer for one step of a batch of requests: x [T, d] holds the new tokens of all sequences, packed (updated in
+        place like `forward`'s), pos [T] their positions, `batch` (PagedBatch) says whose they are and where the cache
+        k_pages, v_pages [npages, nkvh / tp, page, dh] holds their keys and values; the new ones are written on the way.
+        Rows behind the last sequence (a padded batch) go through the row-wise operators and mean nothing."""
+        cfg, T = self.cfg, x.shape[0]
+        mark = on_step or (lambda name: None)
+        att_out, heads = self._project_qkv(x, mark)
+        q, k, v = heads[:, : self.nq], heads[:, self.nq: self.nq + self.nkv], heads[:, self.nq + self.nkv:]
+        self.kv_append_paged.launch(KvAppendPagedArgs.of(q, q, k, v, k_pages, v_pages, pos, batch, cfg.theta, self.w.get("w_qk_norm"), cfg.eps))
+        mark("kv_append_paged")
+        args = AttentionPagedArgs.of(q.permute(1, 0, 2), k_pages, v_pages, att_out.view(T, self.nq, cfg.dh).permute(1, 0, 2), batch, MASK_CAUSAL)
+        self.attention_paged.launch(args, self._paged_workspace(args))
+        mark("attention_paged")
+        lane = self.lanes[0]
+        return self._stage_mlp(lane, self._stage_o(lane, x, 0, T, mark), 0, T, mark)
+
+    def _paged_workspace(self, args):
+        """Scratch of attention_paged, kept between steps and grown when a step wants more."""
+        import torch
+        need = self.attention_paged.scheme(args)
+        if self.paged_ws is None or self.paged_ws.numel() < need:
+            self.paged_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return self.paged_ws
 
     def _use_direct(self, rows):
         return self.direct and rows * self.cfg.d * 2 >= self.DIRECT_MIN_BYTES

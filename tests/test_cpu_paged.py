@@ -1,0 +1,206 @@
+"""What the paged operators and rope_norm refuse, through the C ABI without a device: every check of arguments comes before the
+handle is looked at, so a null handle is enough (a call that passes all of them is answered with "null handle")."""
+import ctypes
+
+import pytest
+
+P16 = 1 << 20  # a base pointer that is aligned and never followed
+
+
+def L(pkg, dt, shape, strides=None):
+    return pkg.TensorLayout.new_contiguous(dt, shape) if strides is None else pkg.TensorLayout(dt, shape, strides)
+
+
+def batch(pkg, table=None, start=None, length=None, base=P16, max_seq=0):
+    b = pkg.PagedBatch(table or L(pkg, pkg.I32, (3, 5)), start or L(pkg, pkg.I32, (4,)), length or L(pkg, pkg.I32, (3,)), max_seq)
+    b.c.page_table_base = b.c.seq_start_base = b.c.kv_len_base = base
+    return b
+
+
+def attention_args(pkg, q=None, k=None, v=None, o=None, b=None, mask=1, scale=0.125, base=P16):
+    F16 = pkg.F16
+    return pkg.AttentionPagedArgs(q or L(pkg, F16, (8, 7, 64)), base, k or L(pkg, F16, (10, 2, 16, 64)), base, v or L(pkg, F16, (10, 2, 16, 64)), base,
+                                  o or L(pkg, F16, (8, 7, 64)), base, b or batch(pkg), mask, scale)
+
+
+def append_args(pkg, b=None, base=P16, theta=1e4, eps=1e-5, w_base=None, **kw):
+    F16 = pkg.F16
+    d = {"q_out": L(pkg, F16, (7, 8, 64)), "q": L(pkg, F16, (7, 8, 64)), "k": L(pkg, F16, (7, 2, 64)), "v": L(pkg, F16, (7, 2, 64)),
+         "k_pages": L(pkg, F16, (10, 2, 16, 64)), "v_pages": L(pkg, F16, (10, 2, 16, 64)), "p": L(pkg, pkg.U32, (7,)), "w": L(pkg, F16, (10, 64))}
+    d.update(kw)
+    return pkg.KvAppendPagedArgs(d["q_out"], base, d["q"], base, d["k"], base, d["v"], base, d["k_pages"], base, d["v_pages"], base, d["p"], base,
+                                 d["w"], w_base, b or batch(pkg), eps, theta)
+
+
+def norm_args(pkg, base=P16, theta=1e4, eps=1e-5, **kw):
+    F16 = pkg.F16
+    d = {"y": L(pkg, F16, (7, 10, 64)), "x": L(pkg, F16, (7, 10, 64)), "p": L(pkg, pkg.U32, (7,)), "w": L(pkg, F16, (10, 64))}
+    d.update(kw)
+    return pkg.RopeNormArgs(d["y"], base, d["x"], base, d["p"], base, d["w"], base, eps, theta)
+
+
+def scheme(pkg, op, args):
+    ws = ctypes.c_size_t(77)
+    return getattr(pkg.lib(), f"ops_{op}_scheme")(None, args.byref(), ctypes.c_size_t(pkg.DYN_SIZE), ctypes.byref(ws))
+
+
+def launch(pkg, op, args):
+    if op == "rope_norm":
+        return pkg.lib().ops_rope_norm_launch(None, args.byref(), None)
+    return getattr(pkg.lib(), f"ops_{op}_launch")(None, args.byref(), None, ctypes.c_size_t(0), None)
+
+
+def passes(pkg, op, args):
+    """Nothing but the missing handle is wrong."""
+    return launch(pkg, op, args) == pkg.ARGS_NOT_SUPPORT and "null handle" in pkg.last_error()
+
+
+def test_the_calls_that_the_others_are_bent_from_pass(pkg):
+    assert passes(pkg, "attention_paged", attention_args(pkg)) and scheme(pkg, "attention_paged", attention_args(pkg)) == 0
+    assert passes(pkg, "kv_append_paged", append_args(pkg)) and scheme(pkg, "kv_append_paged", append_args(pkg)) == 0
+    assert passes(pkg, "kv_append_paged", append_args(pkg, w_base=P16))
+    assert passes(pkg, "rope_norm", norm_args(pkg))
+    # any order of the cache's dims, a shared weight row, u32 arrays, padded rows
+    assert passes(pkg, "attention_paged", attention_args(pkg, k=L(pkg, pkg.F16, (10, 2, 16, 64), (4096, 128, 256, 2))))
+    assert passes(pkg, "rope_norm", norm_args(pkg, w=L(pkg, pkg.F32, (10, 64), (0, 4))))
+    assert passes(pkg, "attention_paged", attention_args(pkg, b=batch(pkg, L(pkg, pkg.U32, (3, 5), (40, 4)), L(pkg, pkg.U32, (4,)), L(pkg, pkg.U32, (3,)))))
+
+
+def test_attention_paged_refusals(pkg):
+    F16, op = pkg.F16, "attention_paged"
+
+    def bent(kind, **kw):
+        assert scheme(pkg, op, attention_args(pkg, **kw)) == kind, (kw, pkg.last_error())
+        assert launch(pkg, op, attention_args(pkg, **kw)) == kind, (kw, pkg.last_error())
+
+    bent(pkg.RANK_NOT_SUPPORT, q=L(pkg, F16, (8, 448)))
+    bent(pkg.RANK_NOT_SUPPORT, o=L(pkg, F16, (8, 448)))
+    bent(pkg.RANK_NOT_SUPPORT, k=L(pkg, F16, (10, 2, 1024)))
+    bent(pkg.RANK_NOT_SUPPORT, v=L(pkg, F16, (10, 2, 1024)))
+    bent(pkg.RANK_NOT_SUPPORT, b=batch(pkg, table=L(pkg, pkg.I32, (15,))))
+    bent(pkg.RANK_NOT_SUPPORT, b=batch(pkg, start=L(pkg, pkg.I32, (2, 2))))
+    bent(pkg.RANK_NOT_SUPPORT, b=batch(pkg, length=L(pkg, pkg.I32, ())))
+    bent(pkg.TYPE_NOT_SUPPORT, b=batch(pkg, table=L(pkg, pkg.I64, (3, 5))))
+    bent(pkg.TYPE_NOT_SUPPORT, b=batch(pkg, length=L(pkg, pkg.F32, (3,))))
+    bent(pkg.TYPE_NOT_SUPPORT, q=L(pkg, pkg.F32, (8, 7, 64)))
+    bent(pkg.TYPE_MISMATCH, o=L(pkg, pkg.BF16, (8, 7, 64)))
+    bent(pkg.TYPE_MISMATCH, v=L(pkg, pkg.BF16, (10, 2, 16, 64)))
+    bent(pkg.SHAPE_MISMATCH, o=L(pkg, F16, (8, 6, 64)))
+    bent(pkg.SHAPE_MISMATCH, o=L(pkg, F16, (4, 7, 64)))
+    bent(pkg.SHAPE_MISMATCH, v=L(pkg, F16, (9, 2, 16, 64)))
+    bent(pkg.SHAPE_MISMATCH, v=L(pkg, F16, (10, 2, 32, 64)))
+    bent(pkg.SHAPE_MISMATCH, v=L(pkg, F16, (10, 2, 16, 128)))
+    bent(pkg.SHAPE_MISMATCH, k=L(pkg, F16, (10, 3, 16, 64)), v=L(pkg, F16, (10, 3, 16, 64)))   # 8 heads over 3
+    bent(pkg.SHAPE_MISMATCH, b=batch(pkg, start=L(pkg, pkg.I32, (3,))))
+    bent(pkg.SHAPE_MISMATCH, b=batch(pkg, start=L(pkg, pkg.I32, (0,))))
+    bent(pkg.SHAPE_NOT_SUPPORT, k=L(pkg, F16, (10, 2, 24, 64)), v=L(pkg, F16, (10, 2, 24, 64)))  # pages: powers of two
+    bent(pkg.SHAPE_NOT_SUPPORT, k=L(pkg, F16, (10, 2, 4, 64)), v=L(pkg, F16, (10, 2, 4, 64)))
+    bent(pkg.SHAPE_NOT_SUPPORT, q=L(pkg, F16, (8, 7, 136)), o=L(pkg, F16, (8, 7, 136)), k=L(pkg, F16, (10, 2, 16, 136)), v=L(pkg, F16, (10, 2, 16, 136)))
+    bent(pkg.SHAPE_NOT_SUPPORT, q=L(pkg, F16, (8, 7, 60)), o=L(pkg, F16, (8, 7, 60)), k=L(pkg, F16, (10, 2, 16, 60)), v=L(pkg, F16, (10, 2, 16, 60)))
+    bent(pkg.SHAPE_NOT_SUPPORT, q=L(pkg, F16, (258, 7, 64)), o=L(pkg, F16, (258, 7, 64)))
+    bent(pkg.ARGS_NOT_SUPPORT, mask=2)
+
+    def at_launch(kind, **kw):
+        assert scheme(pkg, op, attention_args(pkg, **kw)) == 0, (kw, pkg.last_error())
+        assert launch(pkg, op, attention_args(pkg, **kw)) == kind, (kw, pkg.last_error())
+
+    D, S = pkg.DYN_SIZE, pkg.DYN_STRIDE
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, q=L(pkg, F16, (8, D, 64), (S, 128, 2)))
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, k=L(pkg, F16, (D, 2, 16, 64), (4096, 2048, 128, 2)))
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, v=L(pkg, F16, (10, 2, 16, 64), (S, 2048, 128, 2)))
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, b=batch(pkg, table=L(pkg, pkg.I32, (3, D), (S, 4))))
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, b=batch(pkg, base=None))
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, base=None)
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, scale=pkg.DYN_F32)
+    at_launch(pkg.STRIDES_NOT_SUPPORT, q=L(pkg, F16, (8, 7, 64), (896, 128, 4)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, q=L(pkg, F16, (8, 7, 64), (904, 128, 2)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, q=L(pkg, F16, (8, 7, 64), (896, -128, 2)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, o=L(pkg, F16, (8, 7, 64), (898, 128, 2)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, k=L(pkg, F16, (10, 2, 16, 64), (4096, 2048, 136, 2)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, v=L(pkg, F16, (10, 2, 16, 64), (4096, -2048, 128, 2)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, k=L(pkg, F16, (10, 2, 16, 64), (1 << 40, 2048, 128, 2)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, base=P16 + 8)
+    at_launch(pkg.STRIDES_NOT_SUPPORT, b=batch(pkg, base=P16 + 2))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, b=batch(pkg, table=L(pkg, pkg.I32, (3, 5), (40, 8))))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, b=batch(pkg, start=L(pkg, pkg.I32, (4,), (8,))))
+    at_launch(pkg.SHAPE_NOT_SUPPORT, b=batch(pkg, table=L(pkg, pkg.I32, (3, 1 << 27))))  # 2^31 slots a sequence
+    # nothing to do is not an error, null pointers or not
+    for kw in ({"q": L(pkg, F16, (8, 0, 64)), "o": L(pkg, F16, (8, 0, 64))},
+               {"b": batch(pkg, L(pkg, pkg.I32, (0, 5)), L(pkg, pkg.I32, (1,)), L(pkg, pkg.I32, (0,)))}):
+        assert launch(pkg, op, attention_args(pkg, **kw)) == 0, pkg.last_error()
+
+
+def test_kv_append_paged_refusals(pkg):
+    F16, op = pkg.F16, "kv_append_paged"
+
+    def bent(kind, **kw):
+        assert scheme(pkg, op, append_args(pkg, **kw)) == kind, (kw, pkg.last_error())
+        assert launch(pkg, op, append_args(pkg, **kw)) == kind, (kw, pkg.last_error())
+
+    for name in ("q", "q_out", "k", "v"):
+        bent(pkg.RANK_NOT_SUPPORT, **{name: L(pkg, F16, (7, 512))})
+        bent(pkg.TYPE_MISMATCH if name != "q" else pkg.TYPE_NOT_SUPPORT, **{name: L(pkg, pkg.F32, (7, 8 if "q" in name else 2, 64))})
+        bent(pkg.SHAPE_MISMATCH, **{name: L(pkg, F16, (6, 8 if "q" in name else 2, 64))})
+        bent(pkg.SHAPE_MISMATCH, **{name: L(pkg, F16, (7, 8 if "q" in name else 2, 32))})
+    bent(pkg.SHAPE_MISMATCH, k=L(pkg, F16, (7, 3, 64)))
+    bent(pkg.SHAPE_MISMATCH, p=L(pkg, pkg.U32, (8,)))
+    bent(pkg.RANK_NOT_SUPPORT, p=L(pkg, pkg.U32, (7, 1)))
+    bent(pkg.TYPE_NOT_SUPPORT, p=L(pkg, pkg.I32, (7,)))
+    bent(pkg.RANK_NOT_SUPPORT, w=L(pkg, F16, (64,)), w_base=P16)
+    bent(pkg.SHAPE_NOT_SUPPORT, k_pages=L(pkg, F16, (10, 2, 12, 64)), v_pages=L(pkg, F16, (10, 2, 12, 64)))
+    wide = {n: L(pkg, F16, s) for n, s in {"q": (7, 8, 264), "q_out": (7, 8, 264), "k": (7, 2, 264), "v": (7, 2, 264), "k_pages": (10, 2, 16, 264),
+                                           "v_pages": (10, 2, 16, 264)}.items()}
+    bent(pkg.SHAPE_NOT_SUPPORT, **wide)
+
+    def at_launch(kind, **kw):
+        assert scheme(pkg, op, append_args(pkg, **kw)) == 0, (kw, pkg.last_error())
+        assert launch(pkg, op, append_args(pkg, **kw)) == kind, (kw, pkg.last_error())
+
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, theta=pkg.DYN_F32)
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, eps=pkg.DYN_F32, w_base=P16)
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, base=None)
+    at_launch(pkg.DYNAMIC_NOT_SUPPORT, k=L(pkg, F16, (7, 2, 64), (pkg.DYN_STRIDE, 128, 2)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, q_out=L(pkg, F16, (7, 8, 64), (1032, 128, 2)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, v=L(pkg, F16, (7, 2, 64), (256, 128, 4)))
+    at_launch(pkg.STRIDES_NOT_SUPPORT, base=P16 + 8)
+    at_launch(pkg.STRIDES_NOT_SUPPORT, p=L(pkg, pkg.U32, (7,), (6,)))
+    at_launch(pkg.SHAPE_MISMATCH, w=L(pkg, F16, (8, 64)), w_base=P16)
+    at_launch(pkg.TYPE_NOT_SUPPORT, w=L(pkg, pkg.BF16, (10, 64)), w_base=P16)
+    at_launch(pkg.STRIDES_NOT_SUPPORT, w=L(pkg, F16, (10, 64), (136, 2)), w_base=P16)
+    at_launch(pkg.STRIDES_NOT_SUPPORT, w_base=P16 + 2)
+
+
+def test_rope_norm_refusals(pkg):
+    F16, op = pkg.F16, "rope_norm"
+
+    def bent(kind, **kw):
+        assert launch(pkg, op, norm_args(pkg, **kw)) == kind, (kw, pkg.last_error())
+
+    bent(pkg.RANK_NOT_SUPPORT, x=L(pkg, F16, (7, 640)))
+    bent(pkg.RANK_NOT_SUPPORT, w=L(pkg, F16, (64,)))
+    bent(pkg.TYPE_MISMATCH, y=L(pkg, pkg.BF16, (7, 10, 64)))
+    bent(pkg.TYPE_NOT_SUPPORT, p=L(pkg, pkg.I32, (7,)))
+    bent(pkg.TYPE_NOT_SUPPORT, w=L(pkg, pkg.BF16, (10, 64)))
+    bent(pkg.SHAPE_MISMATCH, y=L(pkg, F16, (7, 9, 64)))
+    bent(pkg.SHAPE_MISMATCH, w=L(pkg, F16, (9, 64)))
+    bent(pkg.SHAPE_MISMATCH, p=L(pkg, pkg.U32, (6,)))
+    bent(pkg.DYNAMIC_NOT_SUPPORT, theta=pkg.DYN_F32)
+    bent(pkg.DYNAMIC_NOT_SUPPORT, base=None)
+    bent(pkg.DYNAMIC_NOT_SUPPORT, x=L(pkg, F16, (pkg.DYN_SIZE, 10, 64), (1280, 128, 2)))
+    # what the chain of rms_norm and rope takes and this pass does not
+    bent(pkg.ARGS_NOT_SUPPORT, x=L(pkg, pkg.F32, (7, 10, 64), (2560, 256, 2)), y=L(pkg, pkg.F32, (7, 10, 64), (2560, 256, 2)), w=L(pkg, pkg.F32, (10, 64)))
+    bent(pkg.ARGS_NOT_SUPPORT, x=L(pkg, F16, (7, 10, 64), (1288, 128, 2)))
+    bent(pkg.ARGS_NOT_SUPPORT, x=L(pkg, F16, (7, 10, 64), (1280, 128, 4)))
+    bent(pkg.ARGS_NOT_SUPPORT, w=L(pkg, F16, (10, 64), (130, 2)))
+    bent(pkg.ARGS_NOT_SUPPORT, x=L(pkg, F16, (7, 10, 60), (1280, 128, 2)), y=L(pkg, F16, (7, 10, 60), (1280, 128, 2)), w=L(pkg, F16, (10, 60), (128, 2)))
+    assert "chain" in pkg.last_error()
+    assert launch(pkg, op, norm_args(pkg, x=L(pkg, F16, (0, 10, 64)), y=L(pkg, F16, (0, 10, 64)), p=L(pkg, pkg.U32, (0,)))) == 0
+
+
+@pytest.mark.parametrize("cls", ["KvAppendPaged", "AttentionPaged"])
+def test_no_device_no_operator(pkg, cls):
+    if pkg.device_count() > 0:
+        pytest.skip("a CUDA device is present")
+    with pytest.raises(pkg.SchemeError) as e:
+        getattr(pkg, cls)(0)
+    assert e.value.kind == pkg.EXECUTION_FAILED and "no CPU path" in e.value.info
