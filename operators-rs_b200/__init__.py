@@ -12,6 +12,7 @@ queue, `torch.empty` the workspace fallback.
 """
 import ctypes
 import os
+import struct
 
 from . import build as _build
 
@@ -93,11 +94,16 @@ class TensorLayout:
         return f"TensorLayout(dt={self.dt}, shape={self.shape}, strides={self.strides})"
 
 
+_TORCH_DT = {}
+
+
 def _torch_dt(dtype):
-    import torch
-    return {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.float64: F64, torch.uint8: U8,
-            torch.int8: I8, torch.int16: I16, torch.int32: I32, torch.int64: I64, torch.uint16: U16,
-            torch.uint32: U32, torch.uint64: U64}[dtype]
+    if not _TORCH_DT:  # filled on the first use: torch is imported only where a tensor comes in
+        import torch
+        _TORCH_DT.update({torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.float64: F64, torch.uint8: U8,
+                          torch.int8: I8, torch.int16: I16, torch.int32: I32, torch.int64: I64, torch.uint16: U16,
+                          torch.uint32: U32, torch.uint64: U64})
+    return _TORCH_DT[dtype]
 
 
 def _numpy_dt(dtype):
@@ -228,30 +234,55 @@ _AddArgs = _struct("_AddArgs", [("c_layout", _Layout), ("c_base", ctypes.c_void_
                                 ("b_layout", _Layout), ("b_base", ctypes.c_void_p)])
 _AddRowsArgs = _struct("_AddRowsArgs", [("dst_layout", _Layout), ("dst_base", ctypes.c_void_p), ("src_layout", _Layout),
                                         ("src_base", ctypes.c_void_p), ("idx_layout", _Layout), ("idx_base", ctypes.c_void_p)])
-_RopeNormArgs = _struct("_RopeNormArgs", [("y_layout", _Layout), ("y_base", ctypes.c_void_p), ("x_layout", _Layout), ("x_base", ctypes.c_void_p),
-                                          ("p_layout", _Layout), ("p_base", ctypes.c_void_p), ("w_layout", _Layout), ("w_base", ctypes.c_void_p),
-                                          ("epsilon", ctypes.c_float), ("theta", ctypes.c_float)])
-_PagedBatch = _struct("_PagedBatch", [("page_table_layout", _Layout), ("page_table_base", ctypes.c_void_p), ("seq_start_layout", _Layout),
-                                      ("seq_start_base", ctypes.c_void_p), ("kv_len_layout", _Layout), ("kv_len_base", ctypes.c_void_p),
-                                      ("max_seq", ctypes.c_size_t)])
-_KvAppendPagedArgs = _struct("_KvAppendPagedArgs", [("q_out_layout", _Layout), ("q_out_base", ctypes.c_void_p), ("q_layout", _Layout),
-                                                    ("q_base", ctypes.c_void_p), ("k_layout", _Layout), ("k_base", ctypes.c_void_p),
-                                                    ("v_layout", _Layout), ("v_base", ctypes.c_void_p), ("k_pages_layout", _Layout),
-                                                    ("k_pages_base", ctypes.c_void_p), ("v_pages_layout", _Layout),
-                                                    ("v_pages_base", ctypes.c_void_p), ("p_layout", _Layout), ("p_base", ctypes.c_void_p),
-                                                    ("w_layout", _Layout), ("w_base", ctypes.c_void_p), ("batch", _PagedBatch),
-                                                    ("epsilon", ctypes.c_float), ("theta", ctypes.c_float)])
-_AttentionPagedArgs = _struct("_AttentionPagedArgs", [("q_layout", _Layout), ("q_base", ctypes.c_void_p), ("k_pages_layout", _Layout),
-                                                      ("k_pages_base", ctypes.c_void_p), ("v_pages_layout", _Layout),
-                                                      ("v_pages_base", ctypes.c_void_p), ("o_layout", _Layout), ("o_base", ctypes.c_void_p),
-                                                      ("batch", _PagedBatch), ("mask", ctypes.c_uint8), ("scale", ctypes.c_float)])
-
-
 def _lay(x):
     return x if isinstance(x, TensorLayout) else TensorLayout.of(x)
 
 
-_NO_WEIGHT = TensorLayout(F32, (), ())  # the layout beside a null weight: never looked at
+def _dims(x):
+    """(dtype, shape, byte strides) of a TensorLayout or a tensor."""
+    if isinstance(x, TensorLayout):
+        return x.dt, x.shape, x.strides
+    if hasattr(x, "element_size"):
+        es = x.element_size()
+        return _torch_dt(x.dtype), x.shape, [s * es for s in x.stride()]
+    return _numpy_dt(x.dtype), x.shape, x.strides
+
+
+class _PackedArgs(_ArgsBase):
+    """An args struct written in one go: `operands` layouts, each followed by its base pointer, then TAIL; the shapes and
+    strides that the layouts point to lie behind it in the same buffer.  (A decode step makes several of these per layer: one
+    ctypes object per layout costs 5 us each, a step's kernels run for less.)"""
+    TAIL = ""   # struct format of what follows the operands
+    _plans = {}
+
+    def _fill(self, operands, tail):
+        """operands: (dtype, shape, byte strides, base address or None)."""
+        ranks = tuple([len(o[1]) for o in operands])
+        plan = self._plans.get((self.TAIL, ranks))
+        if plan is None:
+            front = "=" + "IIQQQ" * len(ranks) + self.TAIL
+            offset, at = [], struct.calcsize(front)
+            for n in ranks:
+                offset.append(at)
+                at += 16 * n
+            plan = self._plans[self.TAIL, ranks] = (struct.Struct(front + "".join(f"{n}Q{n}q" for n in ranks)), offset)
+        packer, offset = plan
+        self.c = ctypes.create_string_buffer(packer.size)
+        addr = ctypes.addressof(self.c)
+        values, dims = [], []
+        for (dt, shape, strides, base), at in zip(operands, offset):
+            n = len(shape)
+            values += (dt, n, addr + at, addr + at + 8 * n, base or 0)
+            dims += shape
+            dims += strides
+        packer.pack_into(self.c, 0, *values, *tail, *dims)
+
+
+def _operand(layout, base):
+    return (*_dims(layout), ptr(base))
+
+
+_NO_WEIGHT = (F32, (), (), None)  # beside a null weight the layout is never looked at
 
 
 class RmsNormArgs(_ArgsBase):
@@ -380,14 +411,14 @@ class AttentionKvCachedArgs(_ArgsBase):
         return cls(q, q, k, k, v, v, o, o, k_cache, k_cache, v_cache, v_cache, mask, pos)
 
 
-class RopeNormArgs(_ArgsBase):
+class RopeNormArgs(_PackedArgs):
     """Arguments of the extension ops_rope_norm_launch: y <- rotate(rms_norm of every head of x, weighted by w[head])."""
+    TAIL = "ff"  # epsilon, theta
 
     def __init__(self, y_layout, y_base, x_layout, x_base, p_layout, p_base, w_layout, w_base, epsilon, theta):
         self._alive = (y_base, x_base, p_base, w_base)
-        self.keep = (_lay(y_layout), _lay(x_layout), _lay(p_layout), _lay(w_layout))
-        k = self.keep
-        self.c = _RopeNormArgs(k[0].c, _vp(y_base), k[1].c, _vp(x_base), k[2].c, _vp(p_base), k[3].c, _vp(w_base), epsilon, theta)
+        self._fill((_operand(y_layout, y_base), _operand(x_layout, x_base), _operand(p_layout, p_base), _operand(w_layout, w_base)),
+                   (epsilon, theta))
 
     @classmethod
     def of(cls, y, x, pos, w, epsilon, theta):
@@ -398,43 +429,39 @@ class PagedBatch:
     """ops_paged_batch: which rows of a step belong to which sequence, and in which pages its keys and values lie.
 
     page_table [nseq, width], seq_start [nseq + 1], kv_len [nseq]: device tensors of int32 or uint32, read when the kernels
-    run.  max_seq: no sequence has more new tokens than this (0: unknown)."""
+    run (or layouts, without memory: for `scheme`).  max_seq: no sequence has more new tokens than this (0: unknown).  One
+    batch serves every layer of a step."""
 
     def __init__(self, page_table, seq_start, kv_len, max_seq=0):
         self._alive = (page_table, seq_start, kv_len)
-        self.keep = (_lay(page_table), _lay(seq_start), _lay(kv_len))
-        k = self.keep
-        base = [None if isinstance(t, TensorLayout) else t for t in self._alive]
-        self.c = _PagedBatch(k[0].c, _vp(base[0]), k[1].c, _vp(base[1]), k[2].c, _vp(base[2]), int(max_seq))
+        self.operands = tuple([_operand(t, None if isinstance(t, TensorLayout) else t) for t in self._alive])
+        self.max_seq = int(max_seq)
 
 
-class KvAppendPagedArgs(_ArgsBase):
+class KvAppendPagedArgs(_PackedArgs):
     """ops_kv_append_paged_args: rotate (and optionally normalise) q and k, write k and v into the pages of their slots."""
+    TAIL = "Qff"  # batch.max_seq, epsilon, theta
 
     def __init__(self, q_out_layout, q_out_base, q_layout, q_base, k_layout, k_base, v_layout, v_base, k_pages_layout, k_pages_base,
                  v_pages_layout, v_pages_base, p_layout, p_base, w_layout, w_base, batch, epsilon, theta):
         self._alive = (q_out_base, q_base, k_base, v_base, k_pages_base, v_pages_base, p_base, w_base, batch)
-        self.keep = tuple(_lay(x) for x in (q_out_layout, q_layout, k_layout, v_layout, k_pages_layout, v_pages_layout, p_layout, w_layout))
-        k = self.keep
-        self.c = _KvAppendPagedArgs(k[0].c, _vp(q_out_base), k[1].c, _vp(q_base), k[2].c, _vp(k_base), k[3].c, _vp(v_base), k[4].c,
-                                    _vp(k_pages_base), k[5].c, _vp(v_pages_base), k[6].c, _vp(p_base), k[7].c, _vp(w_base), batch.c,
-                                    epsilon, theta)
+        self._fill((_operand(q_out_layout, q_out_base), _operand(q_layout, q_base), _operand(k_layout, k_base), _operand(v_layout, v_base),
+                    _operand(k_pages_layout, k_pages_base), _operand(v_pages_layout, v_pages_base), _operand(p_layout, p_base),
+                    _NO_WEIGHT if w_layout is None else _operand(w_layout, w_base), *batch.operands), (batch.max_seq, epsilon, theta))
 
     @classmethod
     def of(cls, q_out, q, k, v, k_pages, v_pages, pos, batch, theta, w=None, epsilon=1e-5):
-        return cls(q_out, q_out, q, q, k, k, v, v, k_pages, k_pages, v_pages, v_pages, pos, pos, _NO_WEIGHT if w is None else w, w, batch,
-                   epsilon, theta)
+        return cls(q_out, q_out, q, q, k, k, v, v, k_pages, k_pages, v_pages, v_pages, pos, pos, w, w, batch, epsilon, theta)
 
 
-class AttentionPagedArgs(_ArgsBase):
+class AttentionPagedArgs(_PackedArgs):
     """ops_attention_paged_args: q, o [nh, nt, dh], k_pages, v_pages [npages, nkvh, page, dh]; scale None = 1 / sqrt(dh)."""
+    TAIL = "QB3xf"  # batch.max_seq, mask, scale
 
     def __init__(self, q_layout, q_base, k_pages_layout, k_pages_base, v_pages_layout, v_pages_base, o_layout, o_base, batch, mask, scale):
         self._alive = (q_base, k_pages_base, v_pages_base, o_base, batch)
-        self.keep = (_lay(q_layout), _lay(k_pages_layout), _lay(v_pages_layout), _lay(o_layout))
-        k = self.keep
-        self.c = _AttentionPagedArgs(k[0].c, _vp(q_base), k[1].c, _vp(k_pages_base), k[2].c, _vp(v_pages_base), k[3].c, _vp(o_base), batch.c,
-                                     mask, scale)
+        self._fill((_operand(q_layout, q_base), _operand(k_pages_layout, k_pages_base), _operand(v_pages_layout, v_pages_base),
+                    _operand(o_layout, o_base), *batch.operands), (batch.max_seq, mask, scale))
 
     @classmethod
     def of(cls, q, k_pages, v_pages, o, batch, mask=MASK_CAUSAL, scale=None):

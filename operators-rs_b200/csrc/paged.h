@@ -3,6 +3,7 @@
 #include <new>
 
 #include "common.h"
+#include "paged_schedule.h"
 
 namespace ops {
 
@@ -15,11 +16,6 @@ struct PagedBatch {
   uint32_t npages, max_seq;             // max_seq: 0xffffffff when unknown
   int page_log2;
   int *status;
-};
-
-// A sequence's rows [row, row + n) of the step and its cache slots [0, len).
-struct PagedSeq {
-  int row, n, len;
 };
 
 #ifdef __CUDACC__

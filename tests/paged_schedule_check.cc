@@ -1,0 +1,125 @@
+// Walks the schedule of random batches on the CPU: every key block of every unit belongs to exactly one CTA, a CTA parks at most
+// one part in each of its two slots, shares are even, and a unit's parts are found again from the cuts as the joining kernel does.
+#include <cstdio>
+#include <cstdlib>
+#include <map>
+#include <random>
+#include <tuple>
+#include <vector>
+
+#include "../operators-rs_b200/csrc/paged_schedule.h"
+
+using namespace ops;
+
+#define CHECK(x)                                                            \
+  do {                                                                      \
+    if (!(x)) {                                                             \
+      printf("round %d: %s failed (line %d)\n", round_no, #x, __LINE__);    \
+      return 1;                                                             \
+    }                                                                       \
+  } while (0)
+
+int main() {
+  std::mt19937 rng(7);
+  auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+  for (int round_no = 0; round_no < 3000; ++round_no) {
+    PagedLine l;
+    l.group = std::vector<int>{1, 2, 4, 7, 8, 16, 32}[pick(0, 6)];
+    l.nkvh = pick(1, 9);
+    l.causal = pick(0, 3) > 0;
+    const bool tile = pick(0, 1);
+    const int few = 16;
+    l.rows_lo = tile ? few + 1 : 1;
+    l.rows_hi = tile ? 0x7fffffff : few;
+    l.max_seq = pick(0, 4) ? 0x7fffffff : pick(1, 40);
+    l.tokens = tile ? 2 * (128 / l.group) : few;
+    l.block = tile ? 128 : 64;
+    l.overhead = pick(1, 600);
+    l.min_share = pick(1, 900);
+    l.ctas = std::vector<int>{1, 3, 148, 296}[pick(0, 3)];
+    std::vector<PagedSeq> seqs(pick(0, round_no % 10 ? 12 : 400));
+    const int big = round_no % 7 ? 300 : 20000;
+    int row = 0;
+    for (auto &s : seqs) {
+      s.n = pick(0, 2) ? pick(0, 3) : pick(0, big);
+      s.len = pick(0, 9) ? s.n + pick(0, big) : pick(0, 5);
+      s.row = row;
+      row += s.n;
+    }
+    const int nseq = (int)seqs.size();
+    i64 total = 0;
+    for (auto &s : seqs) total += paged_span(l, s).head * l.nkvh;
+    if (total == 0) continue;
+    const int active = paged_active(l, total);
+    CHECK(active >= 1 && active <= l.ctas);
+    CHECK(paged_cut(total, active, 0) == 0 && paged_cut(total, active, active) == total);
+    auto at = [&](int i) { return seqs[i]; };
+    std::map<std::tuple<int, int, int>, std::vector<std::tuple<int, int, int>>> units;  // (seq, head, tile) -> (lo, hi, cta * 2 + slot) of the parts
+    std::map<std::tuple<int, int, int>, int> blocks;
+    std::map<int, int> parked;
+    for (int c = 0; c < active; ++c) {
+      PagedWalk w{0, 0, paged_cut(total, active, c), paged_cut(total, active, c + 1)};
+      i64 keys = 0;
+      int steps = 0;
+      for (PagedPiece q = paged_next(l, nseq, w, at); q.seq >= 0; q = paged_next(l, nseq, w, at)) {
+        CHECK(++steps < 1000000);
+        CHECK(q.lo < q.hi && q.hi <= q.blocks);
+        if (!q.whole()) CHECK(++parked[c * 2 + q.slot()] == 1);
+        units[{q.seq, q.head, q.tile}].push_back({q.lo, q.hi, c * 2 + q.slot()});
+        blocks[{q.seq, q.head, q.tile}] = q.blocks;
+        keys += (q.hi - q.lo);
+      }
+      // a share is its points' blocks, to within the roundings at its two ends and the short last block and tile of a unit
+      CHECK(keys <= (paged_cut(total, active, c + 1) - paged_cut(total, active, c)) / l.block + 2 + 2 * steps);
+    }
+    size_t want = 0;
+    for (int i = 0; i < nseq; ++i) {
+      const PagedSpan p = paged_span(l, seqs[i]);
+      const i64 rows = (i64)seqs[i].n * l.group;
+      CHECK((p.tiles > 0) == (seqs[i].n > 0 && rows >= l.rows_lo && rows <= l.rows_hi && seqs[i].n <= l.max_seq));
+      if (p.tiles) CHECK((i64)p.tiles * l.tokens >= seqs[i].n && (i64)(p.tiles - 1) * l.tokens < seqs[i].n);
+      want += (size_t)p.tiles * l.nkvh;
+    }
+    CHECK(units.size() == want);
+    for (auto &u : units) {
+      int next = 0;
+      for (auto &part : u.second) {
+        CHECK(std::get<0>(part) == next);
+        next = std::get<1>(part);
+      }
+      CHECK(next == blocks[u.first]);
+      const PagedSeq &s = seqs[std::get<0>(u.first)];
+      const int keys = paged_keys(l, s, (std::get<2>(u.first) + 1) * l.tokens);
+      CHECK((i64)blocks[u.first] * l.block >= keys && (keys == 0 || (i64)(blocks[u.first] - 1) * l.block < keys));
+    }
+    // the joining kernel's view: the first cut inside a unit leads to all its parts
+    size_t joined = 0, split = 0;
+    for (auto &u : units) split += u.second.size() > 1;
+    for (int c = 1; c < active; ++c) {
+      const i64 cut = paged_cut(total, active, c);
+      i64 begin = 0;
+      int i = 0;
+      while (begin + paged_span(l, seqs[i]).head * l.nkvh <= cut) begin += paged_span(l, seqs[i++]).head * l.nkvh;
+      const PagedUnit u = paged_unit(l, paged_span(l, seqs[i]), cut - begin);
+      if (cut == begin + u.begin || paged_cut(total, active, c - 1) > begin + u.begin) continue;
+      const int nb = paged_blocks(l, seqs[i], u.tile);
+      std::vector<std::tuple<int, int, int>> parts;
+      for (int d = c - 1; d < active && paged_cut(total, active, d) < begin + u.begin + u.cost; ++d) {
+        const int lo = paged_block(l, u, nb, paged_cut(total, active, d) - begin), hi = paged_block(l, u, nb, paged_cut(total, active, d + 1) - begin);
+        if (lo < hi) parts.push_back({lo, hi, d * 2 + (lo > 0 ? 0 : 1)});
+      }
+      auto found = units.find({i, u.head, u.tile});
+      CHECK(found != units.end() && found->second == parts);
+      joined += parts.size() > 1;
+    }
+    CHECK(joined == split);
+    for (int k = 0; k < 20; ++k) {
+      const i64 x = k ? 1 + (i64)(rng() % (unsigned long long)total) : total;
+      int c = 0;
+      while (c < active && paged_cut(total, active, c) < x) ++c;
+      CHECK(paged_first_behind(total, active, x) == c);
+    }
+  }
+  printf("schedule ok\n");
+  return 0;
+}

@@ -1,6 +1,9 @@
 """What the paged operators and rope_norm refuse, through the C ABI without a device: every check of arguments comes before the
 handle is looked at, so a null handle is enough (a call that passes all of them is answered with "null handle")."""
 import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
 
@@ -13,7 +16,7 @@ def L(pkg, dt, shape, strides=None):
 
 def batch(pkg, table=None, start=None, length=None, base=P16, max_seq=0):
     b = pkg.PagedBatch(table or L(pkg, pkg.I32, (3, 5)), start or L(pkg, pkg.I32, (4,)), length or L(pkg, pkg.I32, (3,)), max_seq)
-    b.c.page_table_base = b.c.seq_start_base = b.c.kv_len_base = base
+    b.operands = tuple((*o[:3], base) for o in b.operands)
     return b
 
 
@@ -195,6 +198,16 @@ def test_rope_norm_refusals(pkg):
     bent(pkg.ARGS_NOT_SUPPORT, x=L(pkg, F16, (7, 10, 60), (1280, 128, 2)), y=L(pkg, F16, (7, 10, 60), (1280, 128, 2)), w=L(pkg, F16, (10, 60), (128, 2)))
     assert "chain" in pkg.last_error()
     assert launch(pkg, op, norm_args(pkg, x=L(pkg, F16, (0, 10, 64)), y=L(pkg, F16, (0, 10, 64)), p=L(pkg, pkg.U32, (0,)))) == 0
+
+
+def test_schedule_on_the_cpu(tmp_path):
+    """The arithmetic that deals a batch to the CTAs (csrc/paged_schedule.h), compiled for the host, over random batches."""
+    exe = str(tmp_path / "paged_schedule_check")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "paged_schedule_check.cc")
+    built = subprocess.run([shutil.which("g++") or "g++", "-O2", "-std=c++17", src, "-o", exe], capture_output=True, text=True)
+    assert built.returncode == 0, built.stderr
+    ran = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert ran.returncode == 0 and "schedule ok" in ran.stdout, ran.stdout
 
 
 @pytest.mark.parametrize("cls", ["KvAppendPaged", "AttentionPaged"])
