@@ -348,7 +348,7 @@ void ops_kv_append_paged_destroy(ops_kv_append_paged *op);
  * sequence sees the slots [0, kv_len - n + j + 1), with OPS_MASK_NONE all kv_len; a row that sees nothing becomes zeros.  Slots
  * past kv_len are never used, whatever they hold.  Scores, softmax and sums are f32, the probabilities enter the second product
  * in the element type, o is rounded once.  f16 or bf16, dh a multiple of 8 up to 128, unit inner strides, every row 16-byte
- * aligned, no negative strides. */
+ * aligned, positive strides. */
 typedef struct ops_attention_paged ops_attention_paged;
 typedef struct {
   ops_layout q_layout; const void *q_base;

@@ -7,71 +7,6 @@
 
 namespace ops {
 
-// One warp per (token, head).
-template <class E>
-__global__ void __launch_bounds__(128) attention_paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int tok = (int)(item / a.nh), head = (int)(item - (long long)tok * a.nh), kvh = head / a.line.group;
-  if (tok >= a.batch.nt) return;
-  const int i = paged_find(a.batch, (uint32_t)tok);
-  if (i < 0) return;
-  const PagedSeq s = paged_seq(a.batch, i, lane == 0);
-  if (tok - s.row >= s.n || (uint32_t)s.n > a.batch.max_seq) return;
-  if (s.n * a.line.group < a.line.rows_lo) return;
-  const int seen = a.line.causal ? max(0, s.len - s.n + (tok - s.row) + 1) : s.len;
-  const E *q = reinterpret_cast<const E *>(a.q + (long long)tok * a.q_t + (long long)head * a.q_h);
-  __shared__ float q_s[4][AP_MAX_DH];
-  float *qw = q_s[threadIdx.x >> 5];
-  for (int d = lane; d < a.dh; d += 32) qw[d] = to_f32(q[d]);
-  __syncwarp();
-  const uint32_t *table = a.batch.table + (long long)i * a.batch.table_ld;
-  const int mask = (1 << a.batch.page_log2) - 1;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < seen; k0 += 32) {
-    const int key = k0 + lane;
-    uint32_t page = 0xffffffffu;
-    float x = -INFINITY;
-    if (key < seen) {
-      page = table[key >> a.batch.page_log2];
-      x = 0.f;
-      if (page < a.batch.npages) {
-        const E *k = reinterpret_cast<const E *>(a.k + (long long)page * a.kp_p + (long long)kvh * a.kp_h + (long long)(key & mask) * a.kp_s);
-        for (int d = 0; d < a.dh; d += 8) {
-          Vec8<E> kv;
-          kv.u = ld_global_16(k + d);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x = fmaf(qw[d + e], to_f32(kv.h[e]), x);
-        }
-      } else {
-        atomicCAS(a.batch.status, 0, OPS_PAGED_BAD_PAGE);
-      }
-      x *= a.scale_log2;
-    }
-    const float m_new = fmaxf(m, warp_max(x));
-    const float at = m_new == -INFINITY ? 0.f : m_new;
-    const float p = exp2f(x - at), alpha = exp2f(m - at);
-    l = fmaf(l, alpha, warp_sum(p));
-    m = m_new;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= alpha;
-    for (int j = 0; j < min(32, seen - k0); ++j) {
-      const uint32_t pg = __shfl_sync(0xffffffffu, page, j);
-      const float pj = __shfl_sync(0xffffffffu, p, j);
-      if (pg < a.batch.npages && lane * 4 < a.dh) {
-        const E *v = reinterpret_cast<const E *>(a.v + (long long)pg * a.vp_p + (long long)kvh * a.vp_h + (long long)((k0 + j) & mask) * a.vp_s) + lane * 4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(pj, to_f32(v[e]), o[e]);
-      }
-    }
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  E *out = reinterpret_cast<E *>(a.o + (long long)tok * a.o_t + (long long)head * a.o_h) + lane * 4;
-  if (lane * 4 < a.dh)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = from_f32<E>(o[e] * inv);
-}
-
 // Joins the parts of the units that several CTAs share:
 //   o = sum_d 2^(m_d - M) O_d / sum_d 2^(m_d - M) l_d,  M = max_d m_d, parts in the order of their keys.
 // Block (c, y) takes rows [16 y, 16 y + 16) of the unit whose first blocks CTA c had.  With fewer rows a row's parts are dealt to
@@ -132,6 +67,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_paged_join_kernel(c
       }
 #pragma unroll
       for (int e = 0; e < DEEP; ++e) {
+        if (ml[e].x == -INFINITY) continue;  // a part in which the row sees nothing may have left its o unwritten
         const float top = fmaxf(m, ml[e].x);
         const float at = top == -INFINITY ? 0.f : top;
         const float wa = ap_ex2(m - at), wb = ap_ex2(ml[e].x - at);
@@ -249,7 +185,16 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
   } else {
     p.tile.rows_lo = 1;
   }
-  p.tile.rows_hi = 0x7fffffff;
+  if (most >= (usz)p.tile.rows_lo) {
+    p.tile.rows_hi = 0x7fffffff;
+    p.tile.tokens = AP_TILE_ROWS / 2 / (int)group * 2;
+    p.tile.block = AP_TILE_BLOCK;
+    p.tile.overhead = 256;
+    p.tile.min_share = 512;
+    p.tile.ctas = std::min(base.sm_count, AP_MAX_CTAS);
+    p.tile_joins = up256(sizeof(PagedJoin) * (usz)p.tile.ctas);
+    p.tile_parts = up256(2 * (usz)p.tile.ctas * AP_TILE_ROWS * (p.part_dh + AP_PAD) * sizeof(float));
+  }
   return p;
 }
 
@@ -313,18 +258,13 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   few.joins = (PagedJoin *)at;
   few.parts = (float *)(at + plan.few_joins);
   tile.line = plan.tile;
+  tile.joins = (PagedJoin *)(at + plan.few_joins + plan.few_parts);
+  tile.parts = (float *)(at + plan.few_joins + plan.few_parts + plan.tile_joins);
   if (plan.few.ctas) OPS_TRY(attention_paged_few(few, plan.few_rows, bf16, s));
-  if (g.batch.max_seq * (unsigned long long)plan.tile.group >= (unsigned long long)plan.tile.rows_lo) {
-    const unsigned long long items = (unsigned long long)m.nt * m.nh;
-    if (items > 0x7fffffffull) return fail(OPS_SHAPE_NOT_SUPPORT, "attention_paged: shape too large");
-    const unsigned grid = (unsigned)((items + 3) / 4);
-    if (bf16) attention_paged_rows_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(tile);
-    else attention_paged_rows_kernel<__half><<<grid, 128, 0, s>>>(tile);
-    OPS_TRY(check_launch(name));
-  }
-  if (plan.few.ctas) {
+  if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, s));
+  if (plan.few.ctas + plan.tile.ctas) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(plan.few.ctas + plan.tile.ctas), 1);
+    cfg.gridDim = dim3((unsigned)(plan.few.ctas + plan.tile.ctas), plan.tile.ctas ? AP_TILE_ROWS / JOIN_ROWS : 1);
     cfg.blockDim = dim3(JOIN_WARPS * 32);
     cfg.stream = s;
     cudaLaunchAttribute attr;
@@ -332,8 +272,8 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaError_t e = bf16 ? cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<true>, few, tile, plan.few_rows, 256, plan.part_dh)
-                         : cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<false>, few, tile, plan.few_rows, 256, plan.part_dh);
+    cudaError_t e = bf16 ? cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<true>, few, tile, plan.few_rows, AP_TILE_ROWS, plan.part_dh)
+                         : cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<false>, few, tile, plan.few_rows, AP_TILE_ROWS, plan.part_dh);
     if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: launch of the joining kernel failed: %s", cudaGetErrorString(e));
   }
   return OPS_OK;

@@ -35,7 +35,9 @@ struct PagedAttnArgs {
 
 int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, cudaStream_t s);
 int attention_paged_few_ctas(const OpBase &base, int rows);
-constexpr int AP_FEW_BLOCK = 128;  // keys of a block of that kernel
+int attention_paged_tile(const PagedAttnArgs &a, bool bf16, cudaStream_t s);
+constexpr int AP_FEW_BLOCK = 128, AP_TILE_BLOCK = 128;  // keys of a block of either kernel
+constexpr int AP_TILE_ROWS = 256;                       // query rows of a unit of the tile kernel: two tiles
 
 #ifdef __CUDACC__
 __device__ __forceinline__ float ap_ex2(float x) {

@@ -1,0 +1,618 @@
+// attention_paged_tile.cu — attention over a paged cache for sequences with more query rows than the few-rows kernel holds: chunks
+// of a prompt, whole prompts, many query heads per kv head.
+//
+//   o_r = sum_j 2^(x_rj - m_r) v_j / sum_j 2^(x_rj - m_r),  x_rj = scale log2(e) q_r . k_j,  one pass with a running m_r
+//
+// Tensor-bound: 4 dh flops a (query head, key) pair against 4 dh bytes a key that 256 query rows share.  The two products run on
+// tcgen05 with S, P and O in tensor memory, as in attention_fused.cu's two-tile kernel, whose arithmetic this one shares: a unit
+// is TWO tiles of 128 query rows, so that the tensor pipe runs one tile's products while the other tile's exponentials are in
+// flight; two threads per row; the reference point m follows the row maximum only when that has moved by 2^8 (lazy rescaling; the
+// factor cancels in o / l; the probabilities stay below 256, exact to half a step in the 16-bit operand that the second product
+// takes).  What a paged batch of ragged chunks changes:
+//   - A tile's rows are tokens x query heads of one kv head, token by token: a chunk of 33 tokens fills its rows whatever its
+//     length, and the heads of a group share every K and V block in shared memory.
+//   - K and V come page by page: a block of 128 keys is 128 / min(page, 64) boxes of a 4-d tensor map over the whole cache, each
+//     issued by its own lane, which has looked its page up a block ahead.  A box behind the sequence's end, or of a page that is
+//     not there, is asked for outside the map and arrives as zeros; the slots behind the end inside the last page are zeroed in
+//     shared memory (a zero probability does not hide a NaN there).
+//   - One persistent CTA per SM takes an equal share of the line of all units' keys (paged_schedule.h): ragged chunks, one long
+//     chunk and few heads over a long past are all the same to it.  The pieces of its share follow each other without a
+//     pause: the scheduler warp posts them ahead, K, V and Q of the next piece load and its first scores run while the softmax
+//     warps still write out the one before.
+//
+//   warp 0   Q and K producer        warps 4-11   softmax of tile 0, half a row a thread
+//   warp 1   tcgen05.mma issuer      warps 12-19  softmax of tile 1
+//   warp 2   V producer; zeroes what lies behind the end of a sequence in its last block (within the time that the block in
+//            front takes the tensor pipe: the next stage is not free earlier)
+//   warp 3   scheduler
+// Every wait is bounded; when one runs out its code goes to the status word and all roles unwind to the common teardown.
+#include <cuda.h>
+
+#include "attention_paged.h"
+#include "device_utils.cuh"
+#include "sm100_ptx.cuh"
+
+namespace ops {
+
+using namespace sm100;
+
+constexpr int TL_THREADS = 640;
+constexpr int TL_ROWS = 128;  // of a tile
+constexpr int TL_KEYS = AP_TILE_BLOCK;
+constexpr int TL_RING = 4;    // pieces posted ahead
+constexpr int TL_READERS = 19;  // warps that read the ring: all but the scheduler
+
+// A piece as the scheduler posts it.
+struct TilePiece {
+  int valid;
+  int row;        // of the step: first token of the unit
+  int tokens;     // of the sequence from there on
+  int off;        // causal token x of the unit sees slots <= off + x
+  int len, seq, head;
+  int lo, hi;     // key blocks of the unit that this CTA walks
+  int blocks[2];  // ... of each tile, counted from lo
+  int clean;      // local block whose V rows from len on are zeroed; -1: none
+  int park;       // -1: the piece is the whole unit; else the slot of the parts
+};
+
+template <int DH> struct TileSmem {
+  static constexpr int HALVES = DH / 64;
+  static constexpr int STAGES = DH == 64 ? 4 : 2;
+  static constexpr int TILE = TL_ROWS * DH * 2;  // a Q tile, a K block or a V block
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + 2 * TILE;
+  static constexpr int OFF_V = OFF_K + STAGES * TILE;
+  static constexpr int OFF_BAR = OFF_V + STAGES * TILE;
+  static constexpr int NUM_BARS = 18 + 2 * TL_RING + 5 * STAGES;
+  static constexpr int OFF_TMEM_SLOT = OFF_BAR + NUM_BARS * 8;
+  static constexpr int OFF_RING = (OFF_TMEM_SLOT + 16 + 15) / 16 * 16;
+  static constexpr int OFF_MAX = (OFF_RING + TL_RING * (int)sizeof(TilePiece) + 15) / 16 * 16;  // [2 tiles][2 halves][128] f32
+  static constexpr int OFF_L = OFF_MAX + 4 * TL_ROWS * 4;
+  static constexpr int BYTES = OFF_L + 4 * TL_ROWS * 4 + 1024;  // 1024: alignment
+};
+
+struct TileArgs {
+  PagedAttnArgs a;
+  int per_tile;   // tokens of a tile: 128 / group
+  int box_log2;   // rows of a K or V box: min(page, 64)
+};
+
+__device__ __forceinline__ float tl_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+template <int DH, bool BF>
+__global__ void __launch_bounds__(TL_THREADS, 1)
+    attention_paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                                const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ TileArgs g) {
+  typedef TileSmem<DH> Smem;
+  constexpr int HALVES = Smem::HALVES, ST = Smem::STAGES, TILE = Smem::TILE;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bar0 = base + Smem::OFF_BAR;
+  auto q_full = [&](int t) { return bar0 + 8u * (0 + t); };
+  auto q_empty = [&](int t) { return bar0 + 8u * (2 + t); };    // last QK of the piece's tile done
+  auto s_full = [&](int t) { return bar0 + 8u * (4 + t); };     // S complete (tensor pipe -> softmax)
+  auto p_full = [&](int t) { return bar0 + 8u * (6 + t); };     // P written, O rescaled if needed, the last piece's O read (softmax -> issuer)
+  auto o_final = [&](int t) { return bar0 + 8u * (8 + t); };    // last PV of the piece's tile done (tensor pipe -> softmax)
+  auto pair_bar = [&](int i) { return bar0 + 8u * (10 + i); };  // the two warps that share 32 rows of a tile
+  auto ring_full = [&](int i) { return bar0 + 8u * (18 + i); };
+  auto ring_empty = [&](int i) { return bar0 + 8u * (18 + TL_RING + i); };
+  auto k_full = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + s); };
+  auto k_empty = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + ST + s); };
+  auto v_full = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + 2 * ST + s); };
+  auto v_empty = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + 3 * ST + s); };
+  auto v_clean = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + 4 * ST + s); };  // a stage's, so that no phase is overrun
+  const uint32_t tmem_slot = base + Smem::OFF_TMEM_SLOT;
+  uint32_t *tmem_slot_ptr = reinterpret_cast<uint32_t *>(base_ptr + Smem::OFF_TMEM_SLOT);
+  volatile TilePiece *ring = reinterpret_cast<volatile TilePiece *>(base_ptr + Smem::OFF_RING);
+  float *max_s = reinterpret_cast<float *>(base_ptr + Smem::OFF_MAX);
+  float *l_s = reinterpret_cast<float *>(base_ptr + Smem::OFF_L);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedBatch &batch = g.a.batch;
+  const PagedLine &line = g.a.line;
+  const int group = line.group;
+  int *status = batch.status + 1;  // of the waits
+  __shared__ int gave_up;
+
+  pdl_let_next_come();
+  i64 total;
+  PagedWalk walk = paged_locate<TL_THREADS>(batch, line, blockIdx.x, blockIdx.x == 0, &total);
+  if (walk.at >= walk.end) {  // nothing for this CTA (all its threads agree)
+    PagedPiece none;
+    none.seq = -1;
+    if (threadIdx.x == 0) paged_note_join(g.a, blockIdx.x, none, walk, total);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    gave_up = 0;
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(q_full(t), 1);
+      mbar_init(q_empty(t), 1);
+      mbar_init(s_full(t), 1);
+      mbar_init(p_full(t), 8);
+      mbar_init(o_final(t), 1);
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(pair_bar(i), 2);
+    for (int i = 0; i < TL_RING; ++i) {
+      mbar_init(ring_full(i), 1);
+      mbar_init(ring_empty(i), TL_READERS);
+    }
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 1);
+      mbar_init(v_clean(s), 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot_ptr;
+  // tensor memory columns: S0 | S1 | O0 | O1, 128 each; the P of keys [64h, 64h+64) of a tile overwrites columns
+  // [64h, 64h+32) of its S (the first half of what the thread that wrote it had read)
+  auto s_col = [&](int t) { return (uint32_t)(t * 128); };
+  auto o_col = [&](int t) { return (uint32_t)(256 + t * 128); };
+
+  if (warp < 4) {
+    setmaxnreg_dec<64>();
+    if (warp == 0 || warp == 2) {
+      // ------------------------------------------------------------------ producers: one warp, a lane per box
+      const bool keys = warp == 0;
+      const int box = 1 << g.box_log2, boxes = TL_KEYS >> g.box_log2;
+      const int lg = batch.page_log2, in_page = (1 << lg) - 1;
+      uint32_t count = 0, q_count[2] = {0, 0};
+      bool ok = true;
+      for (uint32_t i = 0; ok; ++i) {
+        const int slot = i % TL_RING;
+        ok = mbar_wait(ring_full(slot), (i / TL_RING) & 1u, status, keys ? 101 : 102);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        volatile TilePiece &p = ring[slot];
+        const int valid = p.valid, row = p.row, len = p.len, seq = p.seq, head = p.head, lo = p.lo, hi = p.hi;
+        const int n0 = p.blocks[0], n1 = p.blocks[1], clean = keys ? -1 : p.clean;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ring_empty(slot));
+        if (!valid) break;
+        const uint32_t *table = batch.table + (long long)seq * batch.table_ld;
+        // the page of this lane's box of block j, outside the map where there is nothing to read
+        auto look_up = [&](int j) -> int {
+          const int key = j * TL_KEYS + lane * box;
+          if (lane >= boxes || j >= hi || key >= len) return (int)batch.npages;
+          const uint32_t page = table[key >> lg];
+          if (page < batch.npages) return (int)page;
+          atomicCAS(batch.status, 0, OPS_PAGED_BAD_PAGE);
+          return (int)batch.npages;
+        };
+        int page = look_up(lo);
+        if (keys)
+          for (int t = 0; t < 2 && ok; ++t) {
+            if ((t ? n1 : n0) == 0) continue;
+            if (lane == 0) {
+              ok = mbar_wait(q_empty(t), (q_count[t] & 1u) ^ 1u, status, 103 + t);
+              if (ok) {
+                mbar_arrive_expect_tx(q_full(t), (uint32_t)(group * g.per_tile * HALVES * 128));
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h)
+                  tma_load_4d(base + Smem::OFF_Q + t * TILE + h * (TL_ROWS * 128), &tmap_q, q_full(t), h * 64, 0, row + t * g.per_tile, head);
+              }
+            }
+            ++q_count[t];
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0);
+          }
+        for (int j = lo; j < hi && ok; ++j, ++count) {
+          const int s = count % ST;
+          const uint32_t full = keys ? k_full(s) : v_full(s);
+          if (lane == 0) {
+            ok = mbar_wait(keys ? k_empty(s) : v_empty(s), ((count / ST) & 1u) ^ 1u, status, keys ? 105 : 106);
+            if (ok) mbar_arrive_expect_tx(full, TILE);
+          }
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0);
+          if (!ok) break;
+          const int next = look_up(j + 1);
+          if (lane < boxes) {
+            const int r = lane * box;  // first row of the block
+            const int at = (j * TL_KEYS + r) & in_page;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+              if (keys)  // [half][128 keys][128 B]
+                tma_load_4d(base + Smem::OFF_K + s * TILE + h * (TL_KEYS * 128) + r * 128, &tmap_k, full, h * 64, at, head, page);
+              else  // [64 keys][half][64 keys][128 B]
+                tma_load_4d(base + Smem::OFF_V + s * TILE + ((r >> 6) * HALVES + h) * 8192 + (r & 63) * 128, &tmap_v, full, h * 64, at, head, page);
+            }
+          }
+          page = next;
+          if (j - lo == clean) {
+            // the slots behind the end share a page with the last ones and may hold anything, a NaN too
+            ok = __all_sync(0xffffffffu, mbar_wait(full, (count / ST) & 1u, status, 107));
+            if (!ok) break;
+            const int r0 = len % TL_KEYS, r1 = (r0 + box - 1) >> g.box_log2 << g.box_log2;
+            for (int e = lane; e < (r1 - r0) * HALVES * 8; e += 32) {
+              const int r = r0 + e / (HALVES * 8), piece = e % (HALVES * 8);
+              *reinterpret_cast<uint4 *>(base_ptr + Smem::OFF_V + s * TILE + ((r >> 6) * HALVES + (piece >> 3)) * 8192 + (r & 63) * 128 + (piece & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();  // the MMA reads these writes through the async proxy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_clean(s));
+          }
+        }
+      }
+      if (!ok) gave_up = 1;
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMA issuer
+      if (lane == 0) {
+        const uint32_t idesc_qk = make_idesc_f16(TL_ROWS, TL_KEYS, 0, 0, BF ? 1 : 0);
+        const uint32_t idesc_pv = make_idesc_f16(TL_ROWS, DH, 0, 1, BF ? 1 : 0);
+        uint32_t count = 0, cleaned = 0 /* a bit per stage */, q_count[2] = {0, 0}, p_count[2] = {0, 0};
+        bool ok = true;
+        for (uint32_t i = 0; ok; ++i) {
+          const int slot = i % TL_RING;
+          if (!(ok = mbar_wait(ring_full(slot), (i / TL_RING) & 1u, status, 120))) break;
+          volatile TilePiece &p = ring[slot];
+          const int valid = p.valid, blocks = p.hi - p.lo, clean = p.clean;
+          const int n0 = p.blocks[0], n1 = p.blocks[1];
+          mbar_arrive(ring_empty(slot));
+          if (!valid) break;
+          // S(t) = Q(t) K_j^T.  Tile 1 sees every block that tile 0 sees, if it is there at all.
+          auto issue_qk = [&](int t, int j) -> bool {
+            const uint32_t c = count + (uint32_t)j;
+            const int s = c % ST;
+            if (!mbar_wait(k_full(s), (c / ST) & 1u, status, 121)) return false;
+            tc_fence_after();
+            const uint32_t qa = base + Smem::OFF_Q + t * TILE, ka = base + Smem::OFF_K + s * TILE;
+            const uint32_t d = tmem_base + s_col(t);
+#pragma unroll
+            for (int ks = 0; ks < DH / 16; ++ks) {
+              const uint64_t da = make_smem_desc_sw128(qa + (ks >> 2) * (TL_ROWS * 128) + (ks & 3) * 32, 16, 1024);
+              const uint64_t db = make_smem_desc_sw128(ka + (ks >> 2) * (TL_KEYS * 128) + (ks & 3) * 32, 16, 1024);
+              umma_f16_ss(d, da, db, idesc_qk, ks != 0 ? 1u : 0u);
+            }
+            umma_commit(s_full(t));
+            if (t == 1 || n1 == 0) umma_commit(k_empty(s));
+            if (j == (t ? n1 : n0) - 1) umma_commit(q_empty(t));
+            return true;
+          };
+          // O(t) (+)= P(t) V_j, P from tensor memory
+          auto issue_pv = [&](int t, int j) -> bool {
+            const uint32_t c = count + (uint32_t)j;
+            const int s = c % ST;
+            if (!mbar_wait(v_full(s), (c / ST) & 1u, status, 122)) return false;
+            if (j == clean && !mbar_wait(v_clean(s), (cleaned >> s) & 1u, status, 123)) return false;
+            if (!mbar_wait(p_full(t), p_count[t] & 1u, status, 124)) return false;
+            ++p_count[t];
+            tc_fence_after();
+            const uint32_t va = base + Smem::OFF_V + s * TILE;
+            const uint32_t d = tmem_base + o_col(t);
+            const uint32_t pa = tmem_base + s_col(t);
+#pragma unroll
+            for (int ks = 0; ks < TL_KEYS / 16; ++ks) {
+              const uint64_t db = make_smem_desc_sw128(va + (ks >> 2) * (HALVES * 8192) + (ks & 3) * 2048, 8192, 1024);
+              // 16 keys = 8 packed columns; keys 64.. sit behind the second half row's S columns
+              umma_f16_ts(d, pa + (uint32_t)((ks >> 2) * 64 + (ks & 3) * 8), db, idesc_pv, (j != 0 || ks != 0) ? 1u : 0u);
+            }
+            if (j == (t ? n1 : n0) - 1) umma_commit(o_final(t));
+            if (t == 1 || n1 == 0) umma_commit(v_empty(s));
+            return true;
+          };
+          for (int t = 0; t < 2 && ok; ++t) {
+            if ((t ? n1 : n0) == 0) continue;
+            ok = mbar_wait(q_full(t), q_count[t] & 1u, status, 125) && issue_qk(t, 0);
+            ++q_count[t];
+          }
+          for (int j = 0; j < blocks && ok; ++j)
+            for (int t = 0; t < 2 && ok; ++t) {
+              const int n = t ? n1 : n0;
+              if (j < n) ok = issue_pv(t, j);
+              if (ok && j + 1 < n) ok = issue_qk(t, j + 1);
+            }
+          if (clean >= 0) cleaned ^= 1u << ((count + (uint32_t)clean) % ST);
+          count += (uint32_t)blocks;
+        }
+        if (!ok) gave_up = 1;
+      }
+    } else {
+      // ------------------------------------------------------------------ scheduler
+      PagedPiece cur = paged_step(batch, line, walk);
+      i64 begin = walk.begin;  // of cur's sequence
+      bool ok = true;
+      auto post = [&](const PagedPiece &q, uint32_t i) -> bool {
+        TilePiece told;
+        memset(&told, 0, sizeof(told));
+        told.clean = -1;
+        if (q.seq >= 0) {
+          const int t0 = q.tile * line.tokens;
+          told.valid = 1;
+          told.row = q.s.row + t0;
+          told.tokens = q.s.n - t0;
+          told.off = q.s.len - q.s.n + t0;
+          told.len = q.s.len;
+          told.seq = q.seq;
+          told.head = q.head;
+          told.lo = q.lo;
+          told.hi = q.hi;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int keys_seen = paged_keys(line, q.s, t0 + (t + 1) * g.per_tile);
+            const int all = t * g.per_tile < told.tokens ? max(1, (keys_seen + TL_KEYS - 1) / TL_KEYS) : 0;
+            told.blocks[t] = max(0, min(all, q.hi) - q.lo);
+          }
+          const int last = q.s.len / TL_KEYS;  // the block the sequence ends in
+          if ((q.s.len & ((1 << g.box_log2) - 1)) && last >= q.lo && last < q.hi) told.clean = last - q.lo;
+          told.park = q.whole() ? -1 : (int)blockIdx.x * 2 + q.slot();
+        }
+        const int slot = i % TL_RING;
+        if (!__all_sync(0xffffffffu, mbar_wait(ring_empty(slot), ((i / TL_RING) & 1u) ^ 1u, status, 130))) return false;
+        volatile int *to = reinterpret_cast<volatile int *>(&ring[slot]);
+        const int *from = reinterpret_cast<const int *>(&told);
+#pragma unroll
+        for (int w = 0; w < (int)(sizeof(TilePiece) / 4); ++w)
+          if (lane == w % 32) to[w] = from[w];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ring_full(slot));
+        return true;
+      };
+      ok = post(cur, 0);
+      for (uint32_t i = 0; ok; ++i) {
+        const PagedPiece last = cur;
+        const i64 last_begin = begin;
+        cur = paged_step(batch, line, walk);
+        begin = walk.begin;
+        ok = post(cur, i + 1);
+        if (!ok) break;
+        if (cur.seq < 0) {
+          PagedWalk w = walk;
+          w.begin = last_begin;
+          if (lane == 0) paged_note_join(g.a, blockIdx.x, last, w, total);
+          break;
+        }
+      }
+      if (!ok) gave_up = 1;
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax, rescaling, output: two threads per q row
+    setmaxnreg_inc<104>();
+    const int idx = warp - 4;
+    const int t = idx >> 3;          // q tile
+    const int h = (idx >> 2) & 1;    // which 64 keys of a block, and which half of O's columns
+    const int quarter = idx & 3;     // = warp & 3: tensor-memory lanes [32 * quarter, +32)
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const int tok = r / group, gi = r - tok * group;
+    const uint32_t pair = pair_bar(t * 4 + quarter);
+    float *max_mine = max_s + (t * 2 + h) * TL_ROWS + r, *max_other = max_s + (t * 2 + (h ^ 1)) * TL_ROWS + r;
+    uint32_t met = 0, s_count = 0, o_count = 0;
+    bool ok = true;
+    // the two warps of these rows: what either wrote before is read by the other after
+    auto meet = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair);
+      return mbar_wait(pair, met++ & 1u, status, 140);
+    };
+    for (uint32_t i = 0; ok; ++i) {
+      const int slot = i % TL_RING;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(ring_full(slot), (i / TL_RING) & 1u, status, 141)))) break;
+      volatile TilePiece &p = ring[slot];
+      const int valid = p.valid, nblk = p.blocks[t], lo = p.lo, park = p.park;
+      const int mine = t * g.per_tile + tok;  // token of the unit
+      const bool there = tok < g.per_tile && mine < p.tokens;
+      const int limit = line.causal ? min(p.len - 1, p.off + mine) : p.len - 1;  // last slot this row may see
+      const long long row = p.row + mine;
+      const int q_head = p.head * group + gi;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ring_empty(slot));
+      if (!valid) break;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nblk && ok; ++j) {
+        const int kv0 = (lo + j) * TL_KEYS + h * 64;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), s_count++ & 1u, status, 142)))) break;
+        tc_fence_after();
+        const uint32_t ta = tmem_base + lane_addr + s_col(t) + (uint32_t)(h * 64);
+        uint32_t s0[32], s1[32];
+        tmem_ld_32x32(ta, s0);
+        tmem_ld_32x32(ta + 32u, s1);
+        tmem_wait_ld();
+        const bool need_mask = kv0 + 63 > limit;
+        auto chunk_max = [&](const uint32_t (&v)[32], int k0, float mx) -> float {
+          if (need_mask) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (k0 + e <= limit) mx = fmaxf(mx, __uint_as_float(v[e]) * g.a.scale_log2);
+            return mx;
+          }
+          float m0 = -INFINITY, m1 = -INFINITY;
+          if (g.a.scale_log2 >= 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              m0 = tl_max3(m0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+              m1 = tl_max3(m1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+            }
+            return fmaxf(mx, fmaxf(m0, m1) * g.a.scale_log2);
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) m0 = fmaxf(m0, __uint_as_float(v[e]) * g.a.scale_log2);
+          return fmaxf(mx, m0);
+        };
+        float mx = fmaxf(chunk_max(s0, kv0, -INFINITY), chunk_max(s1, kv0 + 32, -INFINITY));
+        // the other half of the row: its maximum over its 64 keys.  A slot is rewritten one block later, after the partner has
+        // published the probabilities of this block, i.e. after it has read the slot.
+        *max_mine = mx;
+        if (!(ok = __all_sync(0xffffffffu, meet()))) break;
+        mx = fmaxf(mx, *max_other);
+        const float m_raw = fmaxf(m, mx);
+        const bool move = m_raw > m + 8.f;                       // also true on the first block (m = -inf)
+        const float m_next = move ? m_raw : m;
+        const float m_new = m_next == -INFINITY ? 0.f : m_next;  // a row with nothing visible yet: keep the arithmetic finite
+        const float alpha = move ? ap_ex2(m - m_new) : 1.f;      // 0 on the first block
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          // some row maximum of these 32 rows moved: rescale this thread's columns of O.  S of block j being complete says that
+          // PV of block j-1 has completed too (the tensor pipe retires in order), so O is stable.
+          const uint32_t to = tmem_base + lane_addr + o_col(t) + (uint32_t)(h * (DH / 2));
+#pragma unroll 1
+          for (int c = 0; c < DH / 2; c += 16) {
+            uint32_t v[16];
+            tmem_ld_32x16(to + (uint32_t)c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+            tmem_st_32x16(to + (uint32_t)c, v);
+          }
+        }
+        // probabilities -> tensor memory, packed pairs over the first 32 of this thread's 64 S columns; row sum
+        float rs0 = 0.f, rs1 = 0.f;
+        auto emit = [&](const uint32_t (&v)[32], int c) {  // c = first key (0 or 32) of these 32 values within the half row
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float p0 = ap_ex2(fmaf(__uint_as_float(v[e]), g.a.scale_log2, -m_new));
+            float p1 = ap_ex2(fmaf(__uint_as_float(v[e + 1]), g.a.scale_log2, -m_new));
+            if (need_mask) {
+              if (kv0 + c + e > limit) p0 = 0.f;
+              if (kv0 + c + e + 1 > limit) p1 = 0.f;
+            }
+            rs0 += p0;
+            rs1 += p1;
+            packed[e >> 1] = ap_pack<BF>(p0, p1);
+          }
+          tmem_st_32x16(ta + (uint32_t)(c >> 1), packed);
+        };
+        emit(s0, 0);
+        emit(s1, 32);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(t));
+        l = fmaf(l, alpha, rs0 + rs1);
+        m = m_next;
+      }
+      if (!ok) break;
+      // whole-row sum: both halves carry the same reference point
+      l_s[(t * 2 + h) * TL_ROWS + r] = l;
+      if (!(ok = __all_sync(0xffffffffu, meet()))) break;
+      l += l_s[(t * 2 + (h ^ 1)) * TL_ROWS + r];
+      if (nblk == 0) {  // the tile has no block in this part of the unit, or no token at all
+        if (park >= 0 && h == 0)
+          *reinterpret_cast<float2 *>(g.a.parts + ((long long)park * (2 * TL_ROWS) + t * TL_ROWS + r) * (DH + AP_PAD) + DH) = make_float2(-INFINITY, 0.f);
+        continue;
+      }
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_final(t), o_count++ & 1u, status, 143)))) break;
+      tc_fence_after();
+      const uint32_t to = tmem_base + lane_addr + o_col(t) + (uint32_t)(h * (DH / 2));
+      if (park >= 0) {
+        // one part of several: park the unnormalised O with its reference point and row sum
+        float *prow = g.a.parts + ((long long)park * (2 * TL_ROWS) + t * TL_ROWS + r) * (DH + AP_PAD);
+        if (there && h == 0) *reinterpret_cast<float2 *>(prow + DH) = make_float2(m, l);
+#pragma unroll 1
+        for (int c = 0; c < DH / 2; c += 16) {
+          uint32_t v[16];
+          tmem_ld_32x16(to + (uint32_t)c, v);
+          tmem_wait_ld();
+          if (there)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4 *>(prow + h * (DH / 2) + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        }
+      } else {
+        const float inv = l > 0.f ? __frcp_rn(l) : 0.f;  // a row that sees nothing: zeros
+        char *orow = g.a.o + row * g.a.o_t + (long long)q_head * g.a.o_h;
+#pragma unroll 1
+        for (int c = 0; c < DH / 2; c += 16) {
+          uint32_t v[16];
+          tmem_ld_32x16(to + (uint32_t)c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+            const int col = h * (DH / 2) + c + e;
+            if (there && col < g.a.dh) {
+              uint4 out;
+              out.x = ap_pack<BF>(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
+              out.y = ap_pack<BF>(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
+              out.z = ap_pack<BF>(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv);
+              out.w = ap_pack<BF>(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv);
+              st_global_16(orow + col * 2, out);
+            }
+          }
+        }
+      }
+      tc_fence_before();  // the next P of this tile says that O has been read
+    }
+    if (!ok) gave_up = 1;
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (gave_up) __nanosleep(1000000);  // a wait ran out: let stray copies land before the CTA goes away
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn tl_encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+    return (EncodeTiledFn)p;
+  }();
+  return fn;
+}
+
+// A 4-d map of 16-bit elements, 64 of the innermost dim and `box1` x `box2` of the next two a box, 128-byte swizzle.
+static bool tl_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2) {
+  EncodeTiledFn fn = tl_encode_fn();
+  if (!fn) return false;
+  cuuint64_t d[4], st[3];
+  for (int i = 0; i < 4; ++i) d[i] = dims[i];
+  for (int i = 0; i < 3; ++i) st[i] = dims[i + 1] > 1 ? (cuuint64_t)strides[i] : (cuuint64_t)(dims[0] * 2);  // never stepped over
+  cuuint32_t box[4] = {64, box1, box2, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(ptr), d, st, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DH, bool BF>
+static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
+  const int bytes = TileSmem<DH>::BYTES;
+  cudaError_t e = cudaFuncSetAttribute(attention_paged_tile_kernel<DH, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+  attention_paged_tile_kernel<DH, BF><<<g.a.line.ctas, TL_THREADS, bytes, s>>>(q, k, v, g);
+  return check_launch("attention_paged(tiles)");
+}
+
+int attention_paged_tile(const PagedAttnArgs &a, bool bf16, cudaStream_t s) {
+  TileArgs g;
+  g.a = a;
+  g.per_tile = TL_ROWS / a.line.group;
+  g.box_log2 = a.batch.page_log2 < 6 ? a.batch.page_log2 : 6;
+  CUtensorMap q, k, v;
+  const usz nkvh = (usz)a.line.nkvh, page = (usz)1 << a.batch.page_log2, dh = (usz)a.dh;
+  const usz q_dims[4] = {dh, (usz)a.line.group, (usz)a.batch.nt, nkvh}, dims[4] = {dh, page, nkvh, a.batch.npages};
+  const isz q_st[3] = {a.q_h, a.q_t, a.q_h * a.line.group}, k_st[3] = {a.kp_s, a.kp_h, a.kp_p}, v_st[3] = {a.vp_s, a.vp_h, a.vp_p};
+  if (!tl_encode(&q, bf16, a.q, q_dims, q_st, (uint32_t)a.line.group, (uint32_t)g.per_tile) ||
+      !tl_encode(&k, bf16, a.k, dims, k_st, 1u << g.box_log2, 1) || !tl_encode(&v, bf16, a.v, dims, v_st, 1u << g.box_log2, 1))
+    return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
+  if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, s) : tile_launch<64, false>(g, q, k, v, s);
+  return bf16 ? tile_launch<128, true>(g, q, k, v, s) : tile_launch<128, false>(g, q, k, v, s);
+}
+
+}  // namespace ops

@@ -1,4 +1,4 @@
-// paged.cu — the status word of the paged operators' handles.
+// paged.cu — the status words of the paged operators' handles.
 #include "paged.h"
 
 namespace ops {
@@ -7,10 +7,10 @@ int paged_create(PagedHandle *h, int device) {
   h->status = nullptr;
   OPS_TRY(init_base(&h->base, device));
   DeviceGuard guard(device);
-  if (cudaMalloc(&h->status, sizeof(int)) != cudaSuccess || cudaMemset(h->status, 0, sizeof(int)) != cudaSuccess) {
+  if (cudaMalloc(&h->status, 2 * sizeof(int)) != cudaSuccess || cudaMemset(h->status, 0, 2 * sizeof(int)) != cudaSuccess) {
     cudaGetLastError();
     if (h->status) cudaFree(h->status);
-    return fail(OPS_EXECUTION_FAILED, "cannot allocate the status word");
+    return fail(OPS_EXECUTION_FAILED, "cannot allocate the status words");
   }
   return OPS_OK;
 }
@@ -21,15 +21,15 @@ void paged_destroy(PagedHandle *h) {
 
 int paged_status(const PagedHandle *h) {
   DeviceGuard guard(h->base.device);
-  int v = -1;
-  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(&v, h->status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
-  return v;
+  int v[2];
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(v, h->status, sizeof(v), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
+  return v[1] ? v[1] : v[0];
 }
 
 int paged_status_reset(PagedHandle *h) {
   DeviceGuard guard(h->base.device);
   cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMemset(h->status, 0, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemset(h->status, 0, 2 * sizeof(int));
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "status reset: %s", cudaGetErrorString(e));
   return OPS_OK;
 }

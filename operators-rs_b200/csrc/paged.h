@@ -1,4 +1,4 @@
-// paged.h — what the operators of a paged serving batch share: the batch as the kernels see it, its checks, the status word.
+// paged.h — what the operators of a paged serving batch share: the batch as the kernels see it, its checks, the status words.
 #pragma once
 #include <new>
 
@@ -112,8 +112,8 @@ inline int paged_launch_checks(const char *op, const ops_paged_batch *b, const o
   for (int i = 0; i < 2; ++i) {
     if (caches[i]->strides[3] != 2) return fail(OPS_STRIDES_NOT_SUPPORT, "%s: last dim of the cache must be contiguous", op);
     for (int d = 0; d < 3; ++d)
-      if (dims[d] > 1 && (caches[i]->strides[d] % 16 || caches[i]->strides[d] < 0 || caches[i]->strides[d] >= ((isz)1 << 40)))
-        return fail(OPS_STRIDES_NOT_SUPPORT, "%s: strides of the cache must be multiples of 16 bytes, not negative and below 2^40", op);
+      if (dims[d] > 1 && (caches[i]->strides[d] % 16 || caches[i]->strides[d] <= 0 || caches[i]->strides[d] >= ((isz)1 << 40)))
+        return fail(OPS_STRIDES_NOT_SUPPORT, "%s: strides of the cache must be multiples of 16 bytes, positive and below 2^40", op);
   }
   if (nt == 0 || m.nseq == 0) return OPS_OK;
   if (!b->seq_start_base || !b->kv_len_base || (m.width && !b->page_table_base))
@@ -140,7 +140,7 @@ inline int paged_launch_checks(const char *op, const ops_paged_batch *b, const o
 }
 
 // Rows of 16-bit elements that are read and written 16 bytes at a time: dims in front of dh, unit inner stride.
-inline int rows16_checks(const char *op, const char *what, const ops_layout *l, const void *base, bool negative_ok) {
+inline int rows16_checks(const char *op, const char *what, const ops_layout *l, const void *base, bool any_sign) {
   const int last = (int)l->ndim - 1;
   bool empty = false;
   for (int d = 0; d <= last; ++d) {
@@ -149,15 +149,15 @@ inline int rows16_checks(const char *op, const char *what, const ops_layout *l, 
   }
   if (l->strides[last] != 2) return fail(OPS_STRIDES_NOT_SUPPORT, "%s: last dim of %s must be contiguous", op, what);
   for (int d = 0; d < last; ++d)
-    if (l->shape[d] > 1 && (l->strides[d] % 16 || (!negative_ok && l->strides[d] < 0) || l->strides[d] >= ((isz)1 << 40)))
-      return fail(OPS_STRIDES_NOT_SUPPORT, "%s: strides of %s must be multiples of 16 bytes%s", op, what, negative_ok ? "" : " and not negative");
+    if (l->shape[d] > 1 && (l->strides[d] % 16 || (!any_sign && l->strides[d] <= 0) || l->strides[d] >= ((isz)1 << 40)))
+      return fail(OPS_STRIDES_NOT_SUPPORT, "%s: strides of %s must be multiples of 16 bytes%s", op, what, any_sign ? "" : " and positive");
   if (empty) return OPS_OK;
   if (!base) return fail(OPS_DYNAMIC_NOT_SUPPORT, "%s: null base pointer of %s at launch", op, what);
   if (!aligned(base, 16)) return fail(OPS_STRIDES_NOT_SUPPORT, "%s: %s must be 16-byte aligned", op, what);
   return OPS_OK;
 }
 
-// A handle that owns a status word on its device.
+// A handle that owns two status words on its device: what was wrong with a batch, and which bounded wait ran out.
 struct PagedHandle {
   OpBase base;
   int *status;
