@@ -94,16 +94,22 @@ class TensorLayout:
         return f"TensorLayout(dt={self.dt}, shape={self.shape}, strides={self.strides})"
 
 
-_TORCH_DT = {}
+_TORCH_DT = {}  # torch dtype -> (element type, bytes); filled on the first use: torch is imported only where a tensor comes in
+
+
+def _torch_info(dtype):
+    info = _TORCH_DT.get(dtype)
+    if info is None:
+        import torch
+        _TORCH_DT.update({getattr(torch, name): (dt, _NBYTES[dt]) for name, dt in
+                          (("float16", F16), ("bfloat16", BF16), ("float32", F32), ("float64", F64), ("uint8", U8), ("int8", I8), ("int16", I16),
+                           ("int32", I32), ("int64", I64), ("uint16", U16), ("uint32", U32), ("uint64", U64))})
+        info = _TORCH_DT[dtype]
+    return info
 
 
 def _torch_dt(dtype):
-    if not _TORCH_DT:  # filled on the first use: torch is imported only where a tensor comes in
-        import torch
-        _TORCH_DT.update({torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.float64: F64, torch.uint8: U8,
-                          torch.int8: I8, torch.int16: I16, torch.int32: I32, torch.int64: I64, torch.uint16: U16,
-                          torch.uint32: U32, torch.uint64: U64})
-    return _TORCH_DT[dtype]
+    return _torch_info(dtype)[0]
 
 
 def _numpy_dt(dtype):
@@ -238,14 +244,14 @@ def _lay(x):
     return x if isinstance(x, TensorLayout) else TensorLayout.of(x)
 
 
-def _dims(x):
-    """(dtype, shape, byte strides) of a TensorLayout or a tensor."""
-    if isinstance(x, TensorLayout):
-        return x.dt, x.shape, x.strides
-    if hasattr(x, "element_size"):
-        es = x.element_size()
-        return _torch_dt(x.dtype), x.shape, [s * es for s in x.stride()]
-    return _numpy_dt(x.dtype), x.shape, x.strides
+def _operand(layout, base):
+    """(dtype, shape, byte strides, address) of an operand; layout: a TensorLayout, or the tensor itself."""
+    if type(layout) is TensorLayout:
+        return layout.dt, layout.shape, layout.strides, ptr(base)
+    if hasattr(layout, "data_ptr"):
+        dt, es = _torch_info(layout.dtype)
+        return dt, layout.shape, [s * es for s in layout.stride()], layout.data_ptr() if base is layout else ptr(base)
+    return _numpy_dt(layout.dtype), layout.shape, layout.strides, ptr(base)
 
 
 class _PackedArgs(_ArgsBase):
@@ -267,19 +273,15 @@ class _PackedArgs(_ArgsBase):
                 at += 16 * n
             plan = self._plans[self.TAIL, ranks] = (struct.Struct(front + "".join(f"{n}Q{n}q" for n in ranks)), offset)
         packer, offset = plan
-        self.c = ctypes.create_string_buffer(packer.size)
-        addr = ctypes.addressof(self.c)
+        self.c = buf = ctypes.create_string_buffer(packer.size)
+        addr = ctypes.addressof(buf)
         values, dims = [], []
-        for (dt, shape, strides, base), at in zip(operands, offset):
-            n = len(shape)
-            values += (dt, n, addr + at, addr + at + 8 * n, base or 0)
+        for (dt, shape, strides, base), n, at in zip(operands, ranks, offset):
+            at += addr
+            values += (dt, n, at, at + 8 * n, base or 0)
             dims += shape
             dims += strides
-        packer.pack_into(self.c, 0, *values, *tail, *dims)
-
-
-def _operand(layout, base):
-    return (*_dims(layout), ptr(base))
+        packer.pack_into(buf, 0, *values, *tail, *dims)
 
 
 _NO_WEIGHT = (F32, (), (), None)  # beside a null weight the layout is never looked at
@@ -562,9 +564,10 @@ class AddRowsArgs(_ArgsBase):
 # ---------------------------------------------------------------------------------------------------
 # operators
 # ---------------------------------------------------------------------------------------------------
-def current_stream():
+def current_stream(device=None):
+    """Torch's current stream of a device (an index; None: the current device)."""
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 class TorchQueueAlloc:
@@ -574,7 +577,7 @@ class TorchQueueAlloc:
         self.device, self.stream = device, stream
 
     def queue(self):
-        return self.stream if self.stream is not None else current_stream()
+        return self.stream if self.stream is not None else current_stream(self.device)
 
     def alloc(self, size):
         import torch
@@ -611,7 +614,7 @@ class Operator:
     def launch(self, args, workspace=None, queue_alloc=None):
         """Enqueue on queue_alloc.queue().  A short workspace is topped up from queue_alloc and the
         call repeated, as Workspace::new does in the crate (operators/src/common/workspace.rs:12-21)."""
-        qa = queue_alloc or TorchQueueAlloc()
+        qa = queue_alloc or TorchQueueAlloc(self.device)
         stream = ctypes.c_void_p(qa.queue())
         self._last_args = args  # the enqueued kernels read these buffers: keep them until the next launch
         ws_ptr, ws_len = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
@@ -647,7 +650,7 @@ class Rope(Operator):
 
     def launch_norm(self, args, queue_alloc=None):
         """ops_rope_norm_launch: every head normalised, weighted and rotated in one pass."""
-        qa = queue_alloc or TorchQueueAlloc()
+        qa = queue_alloc or TorchQueueAlloc(self.device)
         self._last_args = args
         _check(lib().ops_rope_norm_launch(self._h, args.byref(), ctypes.c_void_p(qa.queue())), True)
 

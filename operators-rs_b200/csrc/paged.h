@@ -147,11 +147,11 @@ inline int rows16_checks(const char *op, const char *what, const ops_layout *l, 
     if (dyn(l->shape[d]) || dyn(l->strides[d])) return fail(OPS_DYNAMIC_NOT_SUPPORT, "%s: every shape and stride of %s must be static at launch", op, what);
     empty |= l->shape[d] == 0;
   }
+  if (empty) return OPS_OK;
   if (l->strides[last] != 2) return fail(OPS_STRIDES_NOT_SUPPORT, "%s: last dim of %s must be contiguous", op, what);
   for (int d = 0; d < last; ++d)
     if (l->shape[d] > 1 && (l->strides[d] % 16 || (!any_sign && l->strides[d] <= 0) || l->strides[d] >= ((isz)1 << 40)))
       return fail(OPS_STRIDES_NOT_SUPPORT, "%s: strides of %s must be multiples of 16 bytes%s", op, what, any_sign ? "" : " and positive");
-  if (empty) return OPS_OK;
   if (!base) return fail(OPS_DYNAMIC_NOT_SUPPORT, "%s: null base pointer of %s at launch", op, what);
   if (!aligned(base, 16)) return fail(OPS_STRIDES_NOT_SUPPORT, "%s: %s must be 16-byte aligned", op, what);
   return OPS_OK;

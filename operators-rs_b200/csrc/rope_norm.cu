@@ -9,9 +9,14 @@
 // HBM-bound: every head vector is read once and written once, 4 dh bytes a head.  A lane holds 8 consecutive elements (one
 // 128-bit access), so a head takes dh / 8 lanes (rounded up to a power of two) and its sum of squares a few shuffles.  A warp
 // walks heads of ONE token: the lane's four (sin, cos) are the same for all of them and are computed once, in registers, with no
-// shared memory and no barrier; UNROLL vectors are in flight per lane.  With few tokens the heads of a token are dealt to several
-// warps, so that a decode step fills the machine.  Everything is f32 and rounded once; the angle is taken in turns,
+// shared memory and no barrier; two or four vectors are in flight per lane.  With few tokens the heads of a token are dealt to
+// several warps, so that a decode step fills the machine.  Everything is f32 and rounded once; the angle is taken in turns,
 // pos * (theta^(-2k/dh) / 2 pi), in f64 and reduced there: in f32 it would be off by pos * 2^-24 rad.
+// What bounded it first was instruction issue (full-range sincospi, 64-bit address arithmetic per vector: 70 us for 8192 rows of
+// 40 heads of 128); with angles reduced in f64 in front of the special-function unit, pointers that step and packed f32 pairs
+// it streams: 33 us, 5.1 TB/s.  Reads and writes both bypass what other kernels keep in L2 (either alone changes nothing: 43 us).
+#include <type_traits>
+
 #include "device_utils.cuh"
 #include "internal.h"
 #include "paged.h"
@@ -20,7 +25,6 @@ namespace ops {
 
 constexpr int RN_MAX_PAIRS = 128;  // dh <= 256
 constexpr int RN_WARPS = 4;
-constexpr int RN_UNROLL = 4;
 
 struct RotateTurns {
   double v[RN_MAX_PAIRS];  // theta^(-2k/dh) / 2 pi
@@ -36,7 +40,7 @@ struct RotateArgs {
   int pos64;
   const char *w;  // null: no norm
   long long w_h;
-  float eps;
+  float eps, inv_dh;
   int nt, nh, nkvh;     // without APPEND nkvh = 0
   int dh, lanes;        // lanes of a warp that hold one head: dh / 8 rounded up to a power of two
   int slices, per_slice;  // warps per token, heads each of them walks
@@ -46,25 +50,35 @@ struct RotateArgs {
   PagedBatch batch;
 };
 
-__device__ __forceinline__ void w8(const __half *p, float (&f)[8]) {
-  Vec8<__half> t;
-  t.u = ld_global_16(p);
+// 8 consecutive elements as pairs of f32
+__device__ __forceinline__ void pairs_of(uint4 v, float2 (&f)[4], __half) {
+  const __half2 *h = reinterpret_cast<const __half2 *>(&v);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = to_f32(t.h[e]);
+  for (int e = 0; e < 4; ++e) f[e] = __half22float2(h[e]);
 }
-__device__ __forceinline__ void w8(const __nv_bfloat16 *p, float (&f)[8]) {
-  Vec8<__nv_bfloat16> t;
-  t.u = ld_global_16(p);
+__device__ __forceinline__ void pairs_of(uint4 v, float2 (&f)[4], __nv_bfloat16) {
+  const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = to_f32(t.h[e]);
+  for (int e = 0; e < 4; ++e) f[e] = __bfloat1622float2(h[e]);
 }
-__device__ __forceinline__ void w8(const float *p, float (&f)[8]) {
+template <class T> __device__ __forceinline__ void load_pairs(const T *p, float2 (&f)[4]) { pairs_of(ld_global_16(p), f, T()); }
+__device__ __forceinline__ void load_pairs(const float *p, float2 (&f)[4]) {
   const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  f[0] = make_float2(a.x, a.y);
+  f[1] = make_float2(a.z, a.w);
+  f[2] = make_float2(b.x, b.y);
+  f[3] = make_float2(b.z, b.w);
+}
+__device__ __forceinline__ uint32_t pair_to(float2 v, __half) {
+  const __half2 h = __float22half2_rn(v);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pair_to(float2 v, __nv_bfloat16) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(v);
+  return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-template <class E, class W, bool NORM, bool APPEND>
+template <class E, class W, bool NORM, bool APPEND, int RN_UNROLL>
 __global__ void __launch_bounds__(RN_WARPS * 32) rotate_heads_kernel(const __grid_constant__ RotateArgs a, const __grid_constant__ RotateTurns turns) {
   const int lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * RN_WARPS + (threadIdx.x >> 5);
@@ -75,7 +89,7 @@ __global__ void __launch_bounds__(RN_WARPS * 32) rotate_heads_kernel(const __gri
   const int at_once = 32 / a.lanes;
   const bool active = sub * 8 < a.dh;
   const int heads = a.nh + (APPEND ? 2 * a.nkvh : 0);
-  const int h_end = min(heads, (slice + 1) * a.per_slice);
+  const int h_begin = slice * a.per_slice, h_end = min(heads, h_begin + a.per_slice);
 
   if (APPEND) {  // rows of nobody are left as they are
     const uint32_t lo = a.batch.start[0], hi = a.batch.start[a.batch.nseq];
@@ -83,88 +97,96 @@ __global__ void __launch_bounds__(RN_WARPS * 32) rotate_heads_kernel(const __gri
   }
   const double pos = a.pos64 ? (double)*reinterpret_cast<const unsigned long long *>(reinterpret_cast<const char *>(a.pos) + tok * a.pos_t)
                              : (double)*reinterpret_cast<const uint32_t *>(reinterpret_cast<const char *>(a.pos) + tok * a.pos_t);
-  char *k_slot = nullptr, *v_slot = nullptr;  // the token's slot in the cache, head 0
-  if (APPEND && h_end > a.nh) {
-    const int i = paged_find(a.batch, (uint32_t)tok);
-    if (i >= 0) {
-      const PagedSeq s = paged_seq(a.batch, i, slice == a.slices - 1 && lane == 0);
-      const long long slot = (long long)a.batch.len[i] - s.n + (tok - s.row);  // by the length as given: a cut one would move the token
-      if (tok - s.row >= s.n) {
-        if (lane == 0) atomicCAS(a.batch.status, 0, OPS_PAGED_BAD_ROWS);
-      } else if (slot < 0 || slot >= ((long long)a.batch.width << a.batch.page_log2)) {
-        if (lane == 0) atomicCAS(a.batch.status, 0, OPS_PAGED_BAD_LENGTH);
-      } else {
-        const uint32_t page = a.batch.table[(long long)i * a.batch.table_ld + (slot >> a.batch.page_log2)];
-        const int at = (int)slot & ((1 << a.batch.page_log2) - 1);
-        if (page < a.batch.npages) {
-          k_slot = a.k_pages + (long long)page * a.kp_p + (long long)at * a.kp_s;
-          v_slot = a.v_pages + (long long)page * a.vp_p + (long long)at * a.vp_s;
-        } else if (lane == 0) {
-          atomicCAS(a.batch.status, 0, OPS_PAGED_BAD_PAGE);
-        }
-      }
-    }
-  }
   float sn[4], cs[4];
+  bool turned = false;
+  auto turn = [&]() {
+    if (turned) return;
+    turned = true;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const double turn = pos * turns.v[min(sub * 4 + e, RN_MAX_PAIRS - 1)];
-    sincospif(2.f * (float)(turn - rint(turn)), &sn[e], &cs[e]);
-  }
+    for (int e = 0; e < 4; ++e) {
+      // reduced to half a turn either way in f64; the special-function unit is off by less than 2^-20 there, a five-hundredth
+      // of the 16-bit result's half step
+      const double t = pos * turns.v[min(sub * 4 + e, RN_MAX_PAIRS - 1)];
+      __sincosf(6.283185307f * (float)(t - rint(t)), &sn[e], &cs[e]);
+    }
+  };
 
-  for (int h0 = slice * a.per_slice; h0 < h_end; h0 += at_once * RN_UNROLL) {
-    Vec8<E> x[RN_UNROLL];
-    char *dst[RN_UNROLL];
+  // Heads [lo, hi) of one operand, counted from its first head; dst null: nowhere to write.  The loads of a round are issued before
+  // the first is used, those of the first round before the angles are there.
+  auto walk = [&](const char *src, long long src_h, char *dst, long long dst_h, const char *w, int lo, int hi, auto rotated) {
+    if (lo >= hi) return;
+    src += (long long)(lo + first) * src_h + sub * 16;
+    dst += (long long)(lo + first) * dst_h + sub * 16;
+    if (NORM) w += (long long)(lo + first) * a.w_h + sub * 8 * (int)sizeof(W);
+    const long long src_step = at_once * src_h, dst_step = at_once * dst_h, w_step = at_once * a.w_h;
+    for (int h = lo + first; h - first < hi; h += at_once * RN_UNROLL) {
+      uint4 x[RN_UNROLL];
 #pragma unroll
-    for (int u = 0; u < RN_UNROLL; ++u) {
-      const int h = h0 + u * at_once + first;
-      dst[u] = nullptr;
-      x[u].u = make_uint4(0, 0, 0, 0);
-      if (h < h_end && active) {
-        const char *src;
-        if (h < a.nh) {
-          src = a.q + (long long)tok * a.q_t + (long long)h * a.q_h;
-          dst[u] = a.qo + (long long)tok * a.qo_t + (long long)h * a.qo_h;
-        } else if (h < a.nh + a.nkvh) {
-          src = a.k + (long long)tok * a.k_t + (long long)(h - a.nh) * a.k_h;
-          dst[u] = k_slot ? k_slot + (long long)(h - a.nh) * a.kp_h : nullptr;
-        } else {
-          src = a.v + (long long)tok * a.v_t + (long long)(h - a.nh - a.nkvh) * a.v_h;
-          dst[u] = v_slot ? v_slot + (long long)(h - a.nh - a.nkvh) * a.vp_h : nullptr;
+      for (int u = 0; u < RN_UNROLL; ++u) {
+        x[u] = make_uint4(0, 0, 0, 0);
+        if (active && h + u * at_once < hi) x[u] = ld_stream_16(src + u * src_step);
+      }
+      if (rotated) turn();
+#pragma unroll
+      for (int u = 0; u < RN_UNROLL; ++u) {
+        const bool there = active && h + u * at_once < hi;
+        if (rotated) {
+          float2 f[4];
+          pairs_of(x[u], f, E());
+          if (NORM) {
+            float2 ss = __fmul2_rn(f[0], f[0]);
+#pragma unroll
+            for (int e = 1; e < 4; ++e) ss = __ffma2_rn(f[e], f[e], ss);
+            float sum = ss.x + ss.y;
+            for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float r = rsqrtf(fmaf(sum, a.inv_dh, a.eps));
+            float2 wt[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) wt[e] = make_float2(0.f, 0.f);
+            if (there) load_pairs(reinterpret_cast<const W *>(w + u * w_step), wt);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = __fmul2_rn(f[e], __fmul2_rn(wt[e], make_float2(r, r)));
+          }
+          uint32_t y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            y[e] = pair_to(make_float2(f[e].x * cs[e] - f[e].y * sn[e], f[e].x * sn[e] + f[e].y * cs[e]), E());
+          x[u] = make_uint4(y[0], y[1], y[2], y[3]);
         }
-        x[u].u = ld_global_16(src + sub * 16);
+        if (there) st_stream_16(dst + u * dst_step, x[u]);
       }
+      src += RN_UNROLL * src_step;
+      dst += RN_UNROLL * dst_step;
+      if (NORM) w += RN_UNROLL * w_step;
     }
-#pragma unroll
-    for (int u = 0; u < RN_UNROLL; ++u) {
-      const int h = h0 + u * at_once + first;
-      const bool rotated = !APPEND || h < a.nh + a.nkvh;
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = to_f32(x[u].h[e]);
-      if (NORM) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
-        for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float r = rsqrtf(ss / (float)a.dh + a.eps);
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = 0.f;
-        if (dst[u] && rotated) w8(reinterpret_cast<const W *>(a.w + (long long)h * a.w_h) + sub * 8, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = f[e] * r * w[e];
-      }
-      if (rotated) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[u].h[2 * e] = from_f32<E>(f[2 * e] * cs[e] - f[2 * e + 1] * sn[e]);
-          x[u].h[2 * e + 1] = from_f32<E>(f[2 * e] * sn[e] + f[2 * e + 1] * cs[e]);
-        }
-      }
-      if (dst[u]) st_global_16(dst[u] + sub * 16, x[u].u);
-    }
+  };
+  walk(a.q + (long long)tok * a.q_t, a.q_h, a.qo + (long long)tok * a.qo_t, a.qo_h, a.w, h_begin, min(h_end, a.nh), std::true_type());
+  if (!APPEND || h_end <= a.nh) return;
+
+  // the token's slot in the cache
+  const int i = paged_find(a.batch, (uint32_t)tok);
+  if (i < 0) return;
+  const PagedSeq s = paged_seq(a.batch, i, slice == a.slices - 1 && lane == 0);
+  const long long slot = (long long)a.batch.len[i] - s.n + (tok - s.row);  // by the length as given: a cut one would move the token
+  int wrong = 0;
+  uint32_t page = 0;
+  if (tok - s.row >= s.n) {
+    wrong = OPS_PAGED_BAD_ROWS;
+  } else if (slot < 0 || slot >= ((long long)a.batch.width << a.batch.page_log2)) {
+    wrong = OPS_PAGED_BAD_LENGTH;
+  } else {
+    page = a.batch.table[(long long)i * a.batch.table_ld + (slot >> a.batch.page_log2)];
+    if (page >= a.batch.npages) wrong = OPS_PAGED_BAD_PAGE;
   }
+  if (wrong) {
+    if (lane == 0) atomicCAS(a.batch.status, 0, wrong);
+    return;
+  }
+  const int at = (int)slot & ((1 << a.batch.page_log2) - 1);
+  walk(a.k + (long long)tok * a.k_t, a.k_h, a.k_pages + (long long)page * a.kp_p + (long long)at * a.kp_s, a.kp_h,
+       NORM ? a.w + (long long)a.nh * a.w_h : nullptr, max(0, h_begin - a.nh), min(h_end - a.nh, a.nkvh), std::true_type());
+  walk(a.v + (long long)tok * a.v_t, a.v_h, a.v_pages + (long long)page * a.vp_p + (long long)at * a.vp_s, a.vp_h, nullptr,
+       max(0, h_begin - a.nh - a.nkvh), min(h_end - a.nh - a.nkvh, a.nkvh), std::false_type());
 }
 
 static RotateTurns rotate_turns(float theta, usz dh) {
@@ -174,24 +196,32 @@ static RotateTurns rotate_turns(float theta, usz dh) {
   return t;
 }
 
-// Warps per token: a launch wants about 16 warps an SM to hide a round trip to memory; beyond that a warp walks a whole token,
-// so that its sines are computed once.
-static void rotate_split(const OpBase &base, RotateArgs *a, int heads) {
+// Warps per token.  About 16 warps an SM hide a round trip to memory; with no more than that, and few heads a warp, a round of two
+// vectors a lane is enough (a round of four spends instructions on vectors that are not there: 64 rows of 40 heads 3.8 against
+// 3.3 us, 1777 rows of 5 heads 5.5 against 4.5).  Otherwise a warp walks a whole token in rounds of four, or half of one as long
+// as that makes no more than 48 warps an SM (8192 rows of 40 heads: 33.0 us against 36.4 in rounds of two, 36.4 with twice the
+// warps; ragged prompts of 48 heads: 30.8 us against 33.4 with 16 warps an SM).
+static int rotate_split(const OpBase &base, RotateArgs *a, int heads) {
   a->lanes = 1;
   while (a->lanes * 8 < a->dh) a->lanes *= 2;
   const int at_once = 32 / a->lanes, passes = (heads + at_once - 1) / at_once;
-  const long long want = 16ll * base.sm_count;
-  const int most = (int)std::min<long long>(passes, std::max<long long>(1, (want + a->nt - 1) / a->nt));
-  const int each = (passes + most - 1) / most;
-  a->per_slice = each * at_once;
-  a->slices = (passes + each - 1) / each;
+  auto split = [&](long long per_sm) {
+    const long long most = std::min<long long>(passes, std::max<long long>(1, (per_sm * base.sm_count + a->nt - 1) / a->nt));
+    const int each = (int)((passes + most - 1) / most);
+    a->per_slice = each * at_once;
+    a->slices = (passes + each - 1) / each;
+    return each;
+  };
+  if (split(16) <= 4) return 2;
+  split(48);
+  return 4;
 }
 
-template <bool APPEND>
+template <bool APPEND, int RN_UNROLL>
 static int rotate_launch(const char *what, const RotateArgs &a, const RotateTurns &turns, bool bf16, uint32_t w_dt, cudaStream_t s) {
   const unsigned long long items = (unsigned long long)a.nt * a.slices;
   const unsigned grid = (unsigned)((items + RN_WARPS - 1) / RN_WARPS);
-#define RN_GO(E, W, NORM) rotate_heads_kernel<E, W, NORM, APPEND><<<grid, RN_WARPS * 32, 0, s>>>(a, turns)
+#define RN_GO(E, W, NORM) rotate_heads_kernel<E, W, NORM, APPEND, RN_UNROLL><<<grid, RN_WARPS * 32, 0, s>>>(a, turns)
   if (!a.w) {
     if (bf16) RN_GO(__nv_bfloat16, float, false);
     else RN_GO(__half, float, false);
@@ -285,10 +315,11 @@ int rope_norm_enqueue(const OpBase *base, const ops_rope_norm_args *a, cudaStrea
   g.nt = (int)nt;
   g.nh = (int)nh;
   g.dh = (int)dh;
-  rotate_split(*base, &g, (int)nh);
+  g.inv_dh = 1.f / (float)dh;
+  const int unroll = rotate_split(*base, &g, (int)nh);
   if ((unsigned long long)nt * g.slices > 0x7fffffffull) return fail(OPS_SHAPE_NOT_SUPPORT, "rope_norm: shape too large");
   DeviceGuard guard(base->device);
-  return rotate_launch<false>(op, g, rotate_turns(a->theta, dh), dt == OPS_DT_BF16, a->w_layout.dt, s);
+  return (unroll == 2 ? rotate_launch<false, 2> : rotate_launch<false, 4>)(op, g, rotate_turns(a->theta, dh), dt == OPS_DT_BF16, a->w_layout.dt, s);
 }
 
 struct AppendMeta {
@@ -390,8 +421,9 @@ OPS_API int ops_kv_append_paged_launch(const ops_kv_append_paged *op, const ops_
   g.vp_p = sv[0];
   g.vp_h = sv[1];
   g.vp_s = sv[2];
-  rotate_split(op->h.base, &g, g.nh + 2 * g.nkvh);
+  g.inv_dh = 1.f / (float)m.dh;
+  const int unroll = rotate_split(op->h.base, &g, g.nh + 2 * g.nkvh);
   if ((unsigned long long)m.nt * g.slices > 0x7fffffffull) return fail(OPS_SHAPE_NOT_SUPPORT, "kv_append_paged: shape too large");
   DeviceGuard guard(op->h.base.device);
-  return rotate_launch<true>(name, g, rotate_turns(a->theta, m.dh), m.dt == OPS_DT_BF16, a->w_base ? a->w_layout.dt : (uint32_t)OPS_DT_F32, (cudaStream_t)stream);
+  return (unroll == 2 ? rotate_launch<true, 2> : rotate_launch<true, 4>)(name, g, rotate_turns(a->theta, m.dh), m.dt == OPS_DT_BF16, a->w_base ? a->w_layout.dt : (uint32_t)OPS_DT_F32, (cudaStream_t)stream);
 }
