@@ -9,102 +9,176 @@ namespace ops {
 
 // Joins the parts of the units that several CTAs share:
 //   o = sum_d 2^(m_d - M) O_d / sum_d 2^(m_d - M) l_d,  M = max_d m_d, parts in the order of their keys.
-// Block (c, y) takes rows [16 y, 16 y + 16) of the unit whose first blocks CTA c had.  With fewer rows a row's parts are dealt to
-// several warps, which meet in shared memory; a lane holds 4 columns.
-constexpr int JOIN_WARPS = 16, JOIN_ROWS = 16;
+// An item is 16 rows of a unit.  How many units there are, and of how many rows and parts, only the records tell (one long
+// sequence: few units of a hundred parts; a prompt: a unit per CTA, of two), so every block counts the items of all records and
+// the blocks deal them out among themselves.  With fewer than 16 rows a row's parts go to several warps, which meet in shared
+// memory; a lane holds 4 columns.
+constexpr int JOIN_WARPS = 16, JOIN_THREADS = JOIN_WARPS * 32, JOIN_ROWS = 16;
+constexpr int JOIN_BLOCKS_PER_SM = 2;
 
 template <bool BF>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) attention_paged_join_kernel(const __grid_constant__ PagedAttnArgs few, const __grid_constant__ PagedAttnArgs tile,
-                                                                              int few_rows, int tile_rows, int part_dh) {
-  pdl_wait_for_front();
-  const bool on_tile = (int)blockIdx.x >= few.line.ctas;
-  const PagedAttnArgs &a = on_tile ? tile : few;
-  const int first = on_tile ? blockIdx.x - few.line.ctas : blockIdx.x;
-  const PagedJoin j = a.joins[first];
-  const int group = a.line.group, rows = j.ctas ? j.tokens * group : 0;
-  const int row0 = blockIdx.y * JOIN_ROWS, here = min(JOIN_ROWS, rows - row0);
-  if (here <= 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int share = JOIN_WARPS / here;  // warps per row
-  const int mine = warp / share, part = warp - mine * share;
-  const int r = row0 + mine;
-  // where the row lies in a parked unit: tiles of 128 rows, whole tokens each
-  const int tok = r / group, gi = r - tok * group;
-  const int per_tile = on_tile ? 128 / group : JOIN_ROWS, t = tok / per_tile;
-  const int parked = t * 128 + (tok - t * per_tile) * group + gi;
-  const long long ld = part_dh + AP_PAD, unit = (long long)(on_tile ? tile_rows : few_rows) * ld;
-  __shared__ float meet[JOIN_WARPS][AP_MAX_DH + 2];
+__global__ void __launch_bounds__(JOIN_THREADS, JOIN_BLOCKS_PER_SM)
+    attention_paged_join_kernel(const __grid_constant__ PagedAttnArgs few, const __grid_constant__ PagedAttnArgs tile, int few_rows, int part_dh) {
+  __shared__ int first_item[2 * AP_MAX_CTAS + 1];  // of every record
+  __shared__ int warp_items[JOIN_WARPS];
+  __shared__ __align__(16) float meet[JOIN_WARPS][AP_MAX_DH + AP_PAD];  // o, m, l; 16-byte rows
   __shared__ short slot_s[AP_MAX_CTAS];  // of the part of the d-th CTA behind the first; -1: the cut left it none
-  for (int d = threadIdx.x; d < j.ctas; d += JOIN_WARPS * 32) {
-    PagedUnit u;
-    u.head = u.tile = 0;
-    u.begin = j.begin;
-    u.cost = j.cost;
-    const int c = first + d;
-    const int lo = paged_block(a.line, u, j.blocks, paged_cut(j.total, j.active, c));
-    const int hi = paged_block(a.line, u, j.blocks, c + 1 < j.active ? paged_cut(j.total, j.active, c + 1) : j.total);
-    slot_s[d] = (short)(lo >= hi ? -1 : c * 2 + (lo > 0 ? 0 : 1));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int records = few.line.ctas + tile.line.ctas;
+  const int per = (records + JOIN_THREADS - 1) / JOIN_THREADS;
+  pdl_wait_for_front();
+  // items of this thread's records, then a prefix sum over the block
+  int mine = 0;
+  for (int e = 0; e < per; ++e) {
+    const int j = threadIdx.x * per + e;
+    if (j < records) {
+      const bool on_tile = j >= few.line.ctas;
+      const PagedJoin *rec = on_tile ? tile.joins + (j - few.line.ctas) : few.joins + j;
+      first_item[j] = mine;
+      if (rec->ctas) mine += (rec->tokens * few.line.group + JOIN_ROWS - 1) / JOIN_ROWS;
+    }
   }
-  __syncthreads();
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (mine < here) {
-    constexpr int DEEP = 4;
-    for (int d0 = part; d0 < j.ctas; d0 += share * DEEP) {
-      float4 v[DEEP];
-      float2 ml[DEEP];
+  int upto = mine;
 #pragma unroll
-      for (int e = 0; e < DEEP; ++e) {
-        const int d = d0 + e * share;
-        v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-        ml[e] = make_float2(-INFINITY, 0.f);
-        const int slot = d < j.ctas ? slot_s[d] : -1;
-        if (slot >= 0) {
-          const float *from = a.parts + slot * unit + parked * ld;
-          ml[e] = __ldcg(reinterpret_cast<const float2 *>(from + part_dh));
-          if (lane * 4 < a.dh) v[e] = __ldcg(reinterpret_cast<const float4 *>(from + lane * 4));
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) warp_items[warp] = upto;
+  __syncthreads();
+  int items = 0;
+#pragma unroll
+  for (int w = 0; w < JOIN_WARPS; ++w) {
+    if (w == warp) upto += items;
+    items += warp_items[w];
+  }
+  for (int e = 0; e < per; ++e)
+    if (threadIdx.x * per + e < records) first_item[threadIdx.x * per + e] += upto - mine;
+  __syncthreads();
+
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    int lo = 0, hi = records;  // the last record whose first item is at or before this one has it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (first_item[mid] <= item) lo = mid;
+      else hi = mid;
+    }
+    const bool on_tile = lo >= few.line.ctas;
+    const PagedAttnArgs &a = on_tile ? tile : few;
+    const int first = on_tile ? lo - few.line.ctas : lo;
+    const PagedJoin j = a.joins[first];
+    const int group = a.line.group, row0 = (item - first_item[lo]) * JOIN_ROWS, here = min(JOIN_ROWS, j.tokens * group - row0);
+    for (int d = threadIdx.x; d < j.ctas; d += JOIN_THREADS) {
+      const int c = first + d;
+      const int b0 = paged_block(a.line.overhead, j.cost, j.blocks, paged_cut(j.total, j.active, c) - j.begin);
+      const int b1 = paged_block(a.line.overhead, j.cost, j.blocks, paged_cut(j.total, j.active, c + 1) - j.begin);
+      slot_s[d] = (short)(b0 >= b1 ? -1 : c * 2 + (b0 > 0 ? 0 : 1));
+    }
+    __syncthreads();
+    const int share = JOIN_WARPS / here;  // warps per row
+    const int own = warp / share, part = warp - own * share;
+    const int r = row0 + own;
+    // where the row lies in a parked unit: tiles of 128 rows, whole tokens each
+    const int tok = r / group, gi = r - tok * group;
+    const int per_tile = on_tile ? AP_TILE_ROWS / 2 / group : JOIN_ROWS, t = tok / per_tile;
+    const int parked = t * (AP_TILE_ROWS / 2) + (tok - t * per_tile) * group + gi;
+    const long long ld = part_dh + AP_PAD, unit = (long long)(on_tile ? AP_TILE_ROWS : few_rows) * ld;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (own < here) {
+      constexpr int DEEP = 4;
+      for (int d0 = part; d0 < j.ctas; d0 += share * DEEP) {
+        float4 v[DEEP];
+        float2 ml[DEEP];
+#pragma unroll
+        for (int e = 0; e < DEEP; ++e) {
+          const int d = d0 + e * share;
+          v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+          ml[e] = make_float2(-INFINITY, 0.f);
+          const int slot = d < j.ctas ? slot_s[d] : -1;
+          if (slot >= 0) {
+            const float *from = a.parts + slot * unit + parked * ld;
+            ml[e] = __ldcg(reinterpret_cast<const float2 *>(from + part_dh));
+            if (lane * 4 < a.dh) v[e] = __ldcg(reinterpret_cast<const float4 *>(from + lane * 4));
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < DEEP; ++e) {
+          if (ml[e].x == -INFINITY) continue;  // a part in which the row sees nothing may have left its o unwritten
+          const float top = fmaxf(m, ml[e].x);
+          const float wa = ap_ex2(m - top), wb = ap_ex2(ml[e].x - top);
+          l = l * wa + ml[e].y * wb;
+          acc.x = acc.x * wa + v[e].x * wb;
+          acc.y = acc.y * wa + v[e].y * wb;
+          acc.z = acc.z * wa + v[e].z * wb;
+          acc.w = acc.w * wa + v[e].w * wb;
+          m = top;
         }
       }
-#pragma unroll
-      for (int e = 0; e < DEEP; ++e) {
-        if (ml[e].x == -INFINITY) continue;  // a part in which the row sees nothing may have left its o unwritten
-        const float top = fmaxf(m, ml[e].x);
-        const float at = top == -INFINITY ? 0.f : top;
-        const float wa = ap_ex2(m - at), wb = ap_ex2(ml[e].x - at);
-        l = l * wa + ml[e].y * wb;
-        acc.x = acc.x * wa + v[e].x * wb;
-        acc.y = acc.y * wa + v[e].y * wb;
-        acc.z = acc.z * wa + v[e].z * wb;
-        acc.w = acc.w * wa + v[e].w * wb;
+      if (part > 0) {
+        *reinterpret_cast<float4 *>(&meet[warp][lane * 4]) = acc;
+        if (lane == 0) {
+          meet[warp][AP_MAX_DH] = m;
+          meet[warp][AP_MAX_DH + 1] = l;
+        }
+      }
+    }
+    __syncthreads();
+    if (own < here && part == 0) {
+      for (int w = warp + 1; w < warp + share; ++w) {
+        const float mw = meet[w][AP_MAX_DH], top = fmaxf(m, mw);
+        if (mw == -INFINITY) continue;
+        const float wa = ap_ex2(m - top), wb = ap_ex2(mw - top);
+        l = l * wa + meet[w][AP_MAX_DH + 1] * wb;
+        const float4 v = *reinterpret_cast<const float4 *>(&meet[w][lane * 4]);
+        acc.x = acc.x * wa + v.x * wb;
+        acc.y = acc.y * wa + v.y * wb;
+        acc.z = acc.z * wa + v.z * wb;
+        acc.w = acc.w * wa + v.w * wb;
         m = top;
       }
-    }
-    if (part > 0) {
-      *reinterpret_cast<float2 *>(&meet[warp][lane * 4]) = make_float2(acc.x, acc.y);
-      *reinterpret_cast<float2 *>(&meet[warp][lane * 4 + 2]) = make_float2(acc.z, acc.w);
-      if (lane == 0) {
-        meet[warp][AP_MAX_DH] = m;
-        meet[warp][AP_MAX_DH + 1] = l;
+      if (lane * 4 < a.dh) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        char *to = a.o + (long long)(j.row + tok) * a.o_t + (long long)(j.head * group + gi) * a.o_h + lane * 8;
+        *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
       }
     }
+    __syncthreads();  // slot_s and meet are free again
   }
-  __syncthreads();
-  if (mine >= here || part > 0) return;
-  for (int w = warp + 1; w < warp + share; ++w) {
-    const float mw = meet[w][AP_MAX_DH], top = fmaxf(m, mw);
-    const float at = top == -INFINITY ? 0.f : top;
-    const float wa = ap_ex2(m - at), wb = ap_ex2(mw - at);
-    l = l * wa + meet[w][AP_MAX_DH + 1] * wb;
-    acc.x = acc.x * wa + meet[w][lane * 4] * wb;
-    acc.y = acc.y * wa + meet[w][lane * 4 + 1] * wb;
-    acc.z = acc.z * wa + meet[w][lane * 4 + 2] * wb;
-    acc.w = acc.w * wa + meet[w][lane * 4 + 3] * wb;
-    m = top;
-  }
-  if (lane * 4 >= a.dh) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  char *to = a.o + (long long)(j.row + tok) * a.o_t + (long long)(j.head * group + gi) * a.o_h + lane * 8;
-  *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+    return (EncodeTiledFn)p;
+  }();
+  return fn;
+}
+
+bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t d[4], st[3];
+  for (int i = 0; i < 4; ++i) d[i] = dims[i];
+  for (int i = 0; i < 3; ++i) st[i] = dims[i + 1] > 1 ? (cuuint64_t)strides[i] : (cuuint64_t)(dims[0] * 2);  // never stepped over
+  cuuint32_t box[4] = {64, box1, box2, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(ptr), d, st, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int attention_paged_maps(const PagedAttnArgs &a, bool bf16, uint32_t rows, CUtensorMap *k, CUtensorMap *v) {
+  const usz dims[4] = {(usz)a.dh, (usz)1 << a.batch.page_log2, (usz)a.line.nkvh, a.batch.npages};
+  const isz ks[3] = {a.kp_s, a.kp_h, a.kp_p}, vs[3] = {a.vp_s, a.vp_h, a.vp_p};
+  if (!ap_encode(k, bf16, a.k, dims, ks, rows, 1) || !ap_encode(v, bf16, a.v, dims, vs, rows, 1))
+    return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
+  return OPS_OK;
 }
 
 struct PagedAttnMeta {
@@ -157,11 +231,21 @@ struct PagedAttnPlan {
 
 static usz up256(usz n) { return (n + 255) / 256 * 256; }
 
-static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, usz dh, bool causal, uint32_t max_seq) {
+// The least shift with which a line cannot pass 31 bits: units, at most all rows in tiles and one more per sequence, of at most
+// all slots and rows.  `overhead`, `min_share`: keys.
+static void line_scale(PagedLine *l, usz nt, usz nseq, usz slots, int overhead, int min_share) {
+  const double units = ((double)(nt / (usz)l->tokens) + (double)nseq) * l->nkvh, keys = (double)slots + (double)nt + l->tokens + overhead;
+  l->shift = 0;
+  while (l->shift < 30 && units * (std::ldexp(keys, -l->shift) + 4.0) > 2147483647.0) ++l->shift;
+  l->overhead = std::max(1, overhead >> l->shift);
+  l->min_share = std::max(1, min_share >> l->shift);
+}
+
+static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, usz dh, bool causal, uint32_t max_seq, usz nt, usz nseq, usz slots) {
   PagedAttnPlan p;
   memset(&p, 0, sizeof(p));
   const usz group = nh / nkvh, most = max_seq == 0xffffffffu ? 0xffffffffull : (usz)max_seq * group;
-  // 16 rows cost the kernel half its CTAs; 8 are enough for one token of up to 8 heads
+  // 16 rows cost the kernel a third of its ring; 8 are enough for one token of up to 8 heads
   p.few_rows = group <= 8 && !(most > 8 && most <= 16) ? 8 : 16;
   p.part_dh = dh <= 64 ? 64 : 128;
   PagedLine l;
@@ -175,10 +259,9 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
     p.few.rows_lo = 1;
     p.few.rows_hi = p.few_rows;
     p.few.tokens = p.few_rows;
-    p.few.block = AP_FEW_BLOCK;
-    p.few.overhead = 128;
-    p.few.min_share = 256;
-    p.few.ctas = std::min(attention_paged_few_ctas(base, p.few_rows), AP_MAX_CTAS);
+    p.few.block_log2 = AP_FEW_BLOCK_LOG2;
+    line_scale(&p.few, nt, nseq, slots, 128, 256);
+    p.few.ctas = std::min(attention_paged_few_ctas(base), AP_MAX_CTAS);
     p.few_joins = up256(sizeof(PagedJoin) * (usz)p.few.ctas);
     p.few_parts = up256(2 * (usz)p.few.ctas * p.few_rows * (p.part_dh + AP_PAD) * sizeof(float));
     p.tile.rows_lo = p.few_rows + 1;
@@ -188,9 +271,8 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
   if (most >= (usz)p.tile.rows_lo) {
     p.tile.rows_hi = 0x7fffffff;
     p.tile.tokens = AP_TILE_ROWS / 2 / (int)group * 2;
-    p.tile.block = AP_TILE_BLOCK;
-    p.tile.overhead = 256;
-    p.tile.min_share = 512;
+    p.tile.block_log2 = AP_TILE_BLOCK_LOG2;
+    line_scale(&p.tile, nt, nseq, slots, 256, 512);
     p.tile.ctas = std::min(base.sm_count, AP_MAX_CTAS);
     p.tile_joins = up256(sizeof(PagedJoin) * (usz)p.tile.ctas);
     p.tile_parts = up256(2 * (usz)p.tile.ctas * AP_TILE_ROWS * (p.part_dh + AP_PAD) * sizeof(float));
@@ -208,7 +290,7 @@ OPS_API int ops_attention_paged_scheme(ops_attention_paged *op, const ops_attent
     if (!dyn(m.nh) && !dyn(m.paged.nkvh) && !dyn(m.dh) && m.nh && m.paged.nkvh) {
       OpBase none{0, 148};
       const uint32_t max_seq = args->batch.max_seq == 0 || args->batch.max_seq > 0xfffffffeu ? 0xffffffffu : (uint32_t)args->batch.max_seq;
-      const usz need = attention_paged_plan(op ? op->h.base : none, m.nh, m.paged.nkvh, m.dh, args->mask == OPS_MASK_CAUSAL, max_seq).bytes();
+      const usz need = attention_paged_plan(op ? op->h.base : none, m.nh, m.paged.nkvh, m.dh, args->mask == OPS_MASK_CAUSAL, max_seq, 1, 1, 1).bytes();
       *ws_out = need <= max_ws ? need : 0;
     }
   }
@@ -229,7 +311,8 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   if (m.nt == 0 || m.nh == 0 || m.dh == 0 || m.paged.nseq == 0) return OPS_OK;
   if (!op) return fail(OPS_ARGS_NOT_SUPPORT, "null handle");
   const OpBase &base = op->h.base;
-  const PagedAttnPlan plan = attention_paged_plan(base, m.nh, m.paged.nkvh, m.dh, a->mask == OPS_MASK_CAUSAL, g.batch.max_seq);
+  const PagedAttnPlan plan = attention_paged_plan(base, m.nh, m.paged.nkvh, m.dh, a->mask == OPS_MASK_CAUSAL, g.batch.max_seq, m.nt, m.paged.nseq,
+                                                m.paged.width * m.paged.page);
   if (!ws || ws_len < plan.bytes()) return need_workspace(plan.bytes());
   g.q = (const char *)a->q_base;
   g.q_h = a->q_layout.strides[0];
@@ -264,16 +347,16 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, s));
   if (plan.few.ctas + plan.tile.ctas) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(plan.few.ctas + plan.tile.ctas), plan.tile.ctas ? AP_TILE_ROWS / JOIN_ROWS : 1);
-    cfg.blockDim = dim3(JOIN_WARPS * 32);
+    cfg.gridDim = dim3((unsigned)(JOIN_BLOCKS_PER_SM * base.sm_count));
+    cfg.blockDim = dim3(JOIN_THREADS);
     cfg.stream = s;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaError_t e = bf16 ? cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<true>, few, tile, plan.few_rows, AP_TILE_ROWS, plan.part_dh)
-                         : cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<false>, few, tile, plan.few_rows, AP_TILE_ROWS, plan.part_dh);
+    cudaError_t e = bf16 ? cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<true>, few, tile, plan.few_rows, plan.part_dh)
+                         : cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<false>, few, tile, plan.few_rows, plan.part_dh);
     if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: launch of the joining kernel failed: %s", cudaGetErrorString(e));
   }
   return OPS_OK;

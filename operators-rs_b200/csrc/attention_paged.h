@@ -1,5 +1,6 @@
 // attention_paged.h — what the kernels of attention_paged share: arguments, the way a CTA finds its share, parked parts.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -17,7 +18,7 @@ struct PagedJoin {
   int ctas;               // that have points of the unit, the writer and those behind it; 0: nothing to join
   int row, tokens, head;  // first row of the step, query tokens, kv head
   int blocks, active;     // of the unit; of the launch
-  i64 begin, cost, total;  // unit on the line; points of the line
+  int begin, cost, total;  // unit on the line; points of the line
 };
 
 struct PagedAttnArgs {
@@ -33,10 +34,14 @@ struct PagedAttnArgs {
   float *parts;      // [2 * line.ctas][rows of a unit][DH + AP_PAD]
 };
 
+// Tensor maps over the whole cache, boxes of 64 columns x `rows` slots of one head of one page, 128-byte swizzle.
+int attention_paged_maps(const PagedAttnArgs &a, bool bf16, uint32_t rows, CUtensorMap *k, CUtensorMap *v);
+// A 4-d map of 16-bit elements, 64 of the innermost dim and `box1` x `box2` of the next two a box, 128-byte swizzle.
+bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2);
 int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, cudaStream_t s);
-int attention_paged_few_ctas(const OpBase &base, int rows);
+int attention_paged_few_ctas(const OpBase &base);
 int attention_paged_tile(const PagedAttnArgs &a, bool bf16, cudaStream_t s);
-constexpr int AP_FEW_BLOCK = 128, AP_TILE_BLOCK = 128;  // keys of a block of either kernel
+constexpr int AP_FEW_BLOCK_LOG2 = 5, AP_FEW_BLOCK = 32, AP_TILE_BLOCK_LOG2 = 7, AP_TILE_BLOCK = 128;  // keys of a block
 constexpr int AP_TILE_ROWS = 256;                       // query rows of a unit of the tile kernel: two tiles
 
 #ifdef __CUDACC__
@@ -56,68 +61,66 @@ __device__ __forceinline__ uint32_t ap_pack(float lo, float hi) {  // first valu
   return *reinterpret_cast<uint32_t *>(&t);
 }
 
-// CTA `cta`'s share of the line, found by all THREADS of a block together: a prefix sum over the sequences.  `report` says
-// whether this block is the one that looks for what is wrong with the batch.  total: the line's points.
-template <int THREADS>
-__device__ PagedWalk paged_locate(const PagedBatch &b, const PagedLine &l, int cta, bool report, i64 *total_out) {
-  __shared__ i64 warp_sums[THREADS / 32];
-  __shared__ PagedWalk found;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (b.nseq + THREADS - 1) / THREADS, i0 = min(b.nseq, (int)threadIdx.x * per), i1 = min(b.nseq, i0 + per);
-  i64 mine = 0;
-  for (int i = i0; i < i1; ++i) mine += paged_span(l, paged_seq(b, i, report)).head * l.nkvh;
-  i64 upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const i64 x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
-  }
-  if (lane == 31) warp_sums[warp] = upto;
-  __syncthreads();
-  i64 total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w == warp) upto += total;
-    total += warp_sums[w];
-  }
-  const int active = paged_active(l, total);
-  *total_out = total;
-  PagedWalk w;
-  w.seq = 0;
-  w.begin = w.at = w.end = 0;
-  if (cta >= active) return w;  // the whole block
-  const i64 lo = paged_cut(total, active, cta), hi = paged_cut(total, active, cta + 1);
-  i64 begin = upto - mine;
-  if (begin <= lo && lo < upto) {
-    int i = i0;
-    while (true) {
-      const i64 all = paged_span(l, paged_seq(b, i, false)).head * l.nkvh;
-      if (begin + all > lo) break;
-      begin += all;
-      ++i;
-    }
-    found.seq = i;
-    found.begin = begin;
-    found.at = lo;
-    found.end = hi;
-  }
-  __syncthreads();
-  return found;
+// Points of one sequence on the line.  Out of line, like everything of the schedule: a small launch spends its time on fetching code.
+static __device__ __noinline__ long long paged_cost(const PagedBatch &b, const PagedLine &l, int i, bool report) {
+  return (long long)paged_span(l, paged_seq(b, i, report)).head * l.nkvh;
 }
 
+// CTA `cta`'s share of the line, by one warp: the points of all sequences, then the one its share begins in.  `report` says
+// whether this CTA is the one that looks for what is wrong with the batch.  All lanes get the answer (at == end: nothing).
+__device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLine &l, int cta, bool report, PagedWalk *walk, int *total_out) {
+  const int lane = threadIdx.x & 31;
+  walk->seq = walk->begin = walk->at = walk->end = 0;
+  long long sum = 0, cost = 0;
+#pragma unroll 1
+  for (int i = lane; i < b.nseq; i += 32) sum += cost = paged_cost(b, l, i, report);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  // sequences that share rows (seq_start falls) can put more on the line than the host allowed for: nothing is done then
+  const int total = sum <= 0x7fffffff ? (int)sum : 0;
+  if (report && total != sum && lane == 0) atomicCAS(b.status, 0, OPS_PAGED_BAD_ROWS);
+  *total_out = total;
+  const int active = paged_active(l, total);
+  if (total == 0 || cta >= active) return;
+  const int lo = paged_cut(total, active, cta);
+  int before = 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < b.nseq; i0 += 32) {
+    const int i = i0 + lane;
+    int mine = (int)cost;  // of up to 32 sequences they are known already
+    if (b.nseq > 32) mine = i < b.nseq ? (int)paged_cost(b, l, i, false) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, before + upto - mine <= lo && lo < before + upto);
+    if (here) {
+      const int at = __ffs(here) - 1;
+      walk->seq = i0 + at;
+      walk->begin = before + __shfl_sync(0xffffffffu, upto - mine, at);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  walk->at = lo;
+  walk->end = paged_cut(total, active, cta + 1);
+}
+
+// By one thread.
 __device__ __forceinline__ PagedPiece paged_step(const PagedBatch &b, const PagedLine &l, PagedWalk &w) {
   return paged_next(l, b.nseq, w, [&](int i) { return paged_seq(b, i, false); });
 }
 
 // The CTA's record for the joining kernel, written by one thread: `piece` is the last of its share (its unit goes on in the next
-// CTAs' shares if it is not the end of it), or seq < 0.  walk: as the piece left it.
-__device__ __forceinline__ void paged_note_join(const PagedAttnArgs &a, int cta, const PagedPiece &piece, const PagedWalk &walk, i64 total) {
+// CTAs' shares if it is not the end of it), or seq < 0.
+__device__ __forceinline__ void paged_note_join(const PagedAttnArgs &a, int cta, const PagedPiece &piece, int total) {
   PagedJoin j;
   memset(&j, 0, sizeof(j));
   if (piece.seq >= 0 && piece.lo == 0 && piece.hi < piece.blocks) {
-    const PagedSpan p = paged_span(a.line, piece.s);
-    j.begin = walk.begin + piece.head * p.head + paged_tile_begin(a.line, p, piece.tile);
-    j.cost = a.line.overhead + p.base + (i64)p.ramp * (piece.tile + 1);
+    j.begin = piece.begin;
+    j.cost = piece.cost;
     j.total = total;
     j.active = paged_active(a.line, total);
     j.ctas = paged_first_behind(total, j.active, j.begin + j.cost) - cta;

@@ -4,342 +4,453 @@
 //   o_r = sum_j 2^(x_rj - m_r) v_j / sum_j 2^(x_rj - m_r),  x_rj = scale log2(e) q_r . k_j,  one pass with a running m_r
 //
 // The work is reading K and V once, 4 dh bytes a key and kv head, HBM-bound.  The keys of all (sequence, kv head) pairs form one
-// line of which every CTA takes an equal share (paged_schedule.h), so ragged lengths cost nothing.  A CTA of 8 warps
-// walks blocks of 128 keys, 16 a warp; a lane issues all sixteen 128-bit loads of its K and V pieces (64 KB a CTA in flight,
-// two CTAs an SM) before it uses one, with the page numbers fetched a block ahead, and the first loads of the next piece
-// are issued before the current one is brought together.  The arithmetic rides on m16n8k16 warp MMAs (a 128-row tcgen05 tile has
-// nothing to chew on here), as in attention_decode.cu: lane (g, c) = (lane / 4, lane % 4),
-//   S[rows x 8 keys] = Q K^T: A = q rows g (and g + 8), B = K rows straight from global; the contraction is permuted so that one
-//                      128-bit load of a K row serves two k-steps;
-//   O^T[16 dh x 8 rows] = V^T P^T: A = byte-permuted V rows, B = the S fragments, exponentiated.
-// Slots past the sequence's length are not loaded (their registers are zero), so whatever they hold stays out.  The 8 warps of a
-// CTA meet in shared memory at the end of a piece.
+// line of which every CTA, one per SM, takes an equal share (paged_schedule.h), so ragged lengths cost nothing.  What keeps the
+// memory busy is bytes in flight: 6.4 TB/s at a loaded latency of about 3 us is 130 KB per SM, more than registers hold
+// (with every lane's loads in registers, 64 KB a CTA and two CTAs an SM: 3.7 TB/s).  So one warp streams pages into a ring
+// of 32-key stages by TMA, 192 KB deep and on through the ends of pieces, and four warps take the stages in turn:
+//
+//   warps 0-3  stage i goes to warp i % 4, which alone waits for it and frees it: S = Q K^T and O += P V for its 32 keys on
+//              m16n8k16 warp MMAs (the rows are the 16 of the MMA; a 128-row tcgen05 tile has nothing to chew on here), both
+//              operands by ldmatrix from the 128-byte-swizzled stage, the probabilities straight from the S registers.  At the
+//              end of a piece the four meet in shared memory.
+//   warp 4     producer: a lane per box of a stage (32 / min(page, 32) boxes of K and of V), pages looked up a stage ahead
+//   warp 5     scheduler: finds the CTA's share, posts its pieces ahead
+//
+// A box behind the sequence's end, or of a page that is not there, is asked for outside the map and arrives as zeros; the slots
+// behind the end inside the last page are zeroed in the stage by the warp that owns it (a zero probability does not hide a
+// NaN there).  Every wait is bounded; when one runs out its code goes to the status word and all roles unwind.
+#include <cuda.h>
+
 #include "attention_paged.h"
 #include "device_utils.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ops {
 
-constexpr int FEW_WARPS = 8, FEW_THREADS = FEW_WARPS * 32;
-constexpr int FEW_BLOCK = AP_FEW_BLOCK;
-static_assert(FEW_BLOCK == FEW_WARPS * 16, "16 keys a warp");
+using namespace sm100;
+
+constexpr int FEW_CONSUMERS = 4, FEW_PRODUCERS = 4, FEW_THREADS = (FEW_CONSUMERS + FEW_PRODUCERS + 1) * 32;
+constexpr int FEW_KEYS = 32;  // of a stage
+constexpr int FEW_RING = 4;   // pieces posted ahead
+static_assert(FEW_KEYS == AP_FEW_BLOCK, "a block is a stage");
 
 // d += a . b, one warp, m16n8k16, f32 accumulate
 template <bool BF>
-__device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void few_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (BF)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t few_word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
 
-__device__ __forceinline__ void cp_async_16(void *dst, const void *src, bool there) {  // zeros where nothing is
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-}
+// A piece as the scheduler posts it.
+struct FewPiece {
+  int seq;  // -1: no more
+  int row, n, len, head;
+  int k0, k1;  // keys
+  int park;    // -1: the whole unit; else the slot of its part
+};
 
 template <int DH, int NR> struct FewSmem {
   static constexpr int ROWS = NR * 8;
-  static constexpr int LD = DH + 4;  // padded: the lanes of a column pair write other banks
-  static constexpr int OFF_Q = 0;                                        // [2][ROWS][DH] 16-bit: this piece's and the next one's
-  static constexpr int OFF_M = OFF_Q + 2 * ROWS * DH * 2;                // [warps][ROWS]
-  static constexpr int OFF_L = OFF_M + FEW_WARPS * ROWS * 4;             // [warps][ROWS]
-  static constexpr int OFF_O = OFF_L + FEW_WARPS * ROWS * 4;             // [warps][ROWS][LD]
-  static constexpr int BYTES = OFF_O + FEW_WARPS * ROWS * LD * 4;
+  static constexpr int HALVES = DH / 64;
+  static constexpr int OPERAND = FEW_KEYS * DH * 2;  // K or V of a stage: [half][32 keys][128 B], swizzled
+  // a multiple of the consumers, so that a slot of the ring is always the same warp's
+  static constexpr int STAGES = DH == 64 ? 24 : NR == 1 ? 12 : 8;
+  static constexpr int Q_LD = DH + 8;  // elements; rows fall on other banks
+  static constexpr int O_LD = DH + 4;
+  static constexpr int OFF_RING = 0;
+  static constexpr int OFF_Q = OFF_RING + STAGES * 2 * OPERAND;                 // [2][16][Q_LD] 16-bit
+  static constexpr int OFF_O = OFF_Q + 2 * 16 * Q_LD * 2;                       // [consumers][ROWS][O_LD] f32
+  static constexpr int OFF_ML = OFF_O + FEW_CONSUMERS * ROWS * O_LD * 4;        // [ROWS][consumers] (m, l)
+  static constexpr int OFF_PIECES = OFF_ML + ROWS * FEW_CONSUMERS * 8;
+  static constexpr int OFF_BAR = OFF_PIECES + FEW_RING * (int)sizeof(FewPiece);
+  static constexpr int NUM_BARS = 2 * STAGES + 4 + 2 * FEW_RING + 1;
+  static constexpr int BYTES = OFF_BAR + NUM_BARS * 8 + 1024;  // 1024: alignment
+  static_assert(STAGES % FEW_CONSUMERS == 0 && STAGES % FEW_PRODUCERS == 0 && OFF_BAR % 8 == 0 && OFF_O % 16 == 0, "layout");
+};
+
+struct FewArgs {
+  PagedAttnArgs a;
+  int box_log2;  // rows of a box: min(page, 32)
 };
 
 template <int DH, bool BF, int NR>
-__global__ void __launch_bounds__(FEW_THREADS, NR == 1 ? 2 : 1) attention_paged_few_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+    attention_paged_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ FewArgs f) {
   typedef FewSmem<DH, NR> Smem;
-  constexpr int ROWS = Smem::ROWS, LD = Smem::LD;
-  constexpr int CH = DH / 32;  // 128-bit loads per K row per lane
-  constexpr int HH = DH / 64;  // 64-wide halves of a V row
-  extern __shared__ __align__(16) uint8_t smem[];
-  unsigned short *q_s = reinterpret_cast<unsigned short *>(smem + Smem::OFF_Q);
-  float *red_m = reinterpret_cast<float *>(smem + Smem::OFF_M), *red_l = reinterpret_cast<float *>(smem + Smem::OFF_L);
-  float *red_o = reinterpret_cast<float *>(smem + Smem::OFF_O);
+  constexpr int ST = Smem::STAGES, ROWS = Smem::ROWS;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bar0 = base + Smem::OFF_BAR;
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
+  auto q_full = [&](int b) { return bar0 + 8u * (2 * ST + b); };
+  auto q_empty = [&](int b) { return bar0 + 8u * (2 * ST + 2 + b); };
+  auto piece_full = [&](int i) { return bar0 + 8u * (2 * ST + 4 + i); };
+  auto piece_empty = [&](int i) { return bar0 + 8u * (2 * ST + 4 + FEW_RING + i); };
+  const uint32_t meet_bar = bar0 + 8u * (2 * ST + 4 + 2 * FEW_RING);
+  volatile FewPiece *pieces = reinterpret_cast<volatile FewPiece *>(base_ptr + Smem::OFF_PIECES);
+  __shared__ int gave_up;
+  const PagedAttnArgs &a = f.a;
+  int *status = a.batch.status + 1;  // of the waits
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, c = lane & 3;
-  const int group = a.line.group, lg = a.batch.page_log2, mask = (1 << lg) - 1;
+  const int group = a.line.group;
 
   pdl_let_next_come();
-  i64 total;
-  PagedWalk walk = paged_locate<FEW_THREADS>(a.batch, a.line, blockIdx.x, blockIdx.x == 0, &total);
-  PagedPiece cur = paged_step(a.batch, a.line, walk);
-  if (cur.seq < 0) {
-    if (threadIdx.x == 0) paged_note_join(a, blockIdx.x, cur, walk, total);
-    return;
+  PagedWalk walk;
+  int total = 0;
+  if (warp == FEW_CONSUMERS + FEW_PRODUCERS) {
+    paged_locate(a.batch, a.line, blockIdx.x, blockIdx.x == 0, &walk, &total);
+  } else if (warp == FEW_CONSUMERS) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmap_k);
+      tma_prefetch_desc(&tmap_v);
+    }
+  } else if (threadIdx.x == 0) {
+    gave_up = 0;
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(q_full(b), 1);
+      mbar_init(q_empty(b), FEW_CONSUMERS);
+    }
+    for (int i = 0; i < FEW_RING; ++i) {
+      mbar_init(piece_full(i), 1);
+      mbar_init(piece_empty(i), FEW_CONSUMERS + FEW_PRODUCERS);
+    }
+    mbar_init(meet_bar, FEW_CONSUMERS);
+    fence_barrier_init();
   }
-
-  uint4 kq[2][CH], vq[HH][4];
-  uint32_t pg0, pg1;  // pages of the warp's 16 keys, first and second eight
-  auto pages = [&](const PagedPiece &p, int kb, int k_end) {
-    const uint32_t *table = a.batch.table + (long long)p.seq * a.batch.table_ld;
-    pg0 = kb < k_end ? table[kb >> lg] : 0u;
-    pg1 = kb + 8 < k_end ? table[(kb + 8) >> lg] : 0u;
-  };
-  // keys kb .. kb+15 of this warp; what lies at or past k_end, or in a page that is not there, is zeros
-  auto issue_k = [&](const PagedPiece &p, int kb, int k_end) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int key = kb + j * 8 + g;
-      const uint32_t pg = j ? pg1 : pg0;
-      const bool ok = key < k_end && pg < a.batch.npages;
-      const char *kr = a.k + (long long)pg * a.kp_p + (long long)p.head * a.kp_h + (long long)(key & mask) * a.kp_s + c * 16;
-#pragma unroll
-      for (int ch = 0; ch < CH; ++ch) {
-        kq[j][ch] = make_uint4(0, 0, 0, 0);
-        if (ok && ch * 32 + c * 8 < a.dh) kq[j][ch] = __ldcs(reinterpret_cast<const uint4 *>(kr + ch * 64));
-      }
-    }
-  };
-  auto issue_v = [&](const PagedPiece &p, int kb, int k_end) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int key = kb + 2 * c + (j & 1) + (j >> 1) * 8;
-      const uint32_t pg = (j >> 1) ? pg1 : pg0;
-      const bool ok = key < k_end && pg < a.batch.npages;
-      const char *vr = a.v + (long long)pg * a.vp_p + (long long)p.head * a.vp_h + (long long)(key & mask) * a.vp_s + g * 16;
-#pragma unroll
-      for (int hh = 0; hh < HH; ++hh) {
-        vq[hh][j] = make_uint4(0, 0, 0, 0);
-        if (ok && hh * 64 + g * 8 < a.dh) vq[hh][j] = __ldcs(reinterpret_cast<const uint4 *>(vr + hh * 128));
-      }
-    }
-  };
-  auto bad_page = [&](int kb, int k_end) {
-    if ((kb < k_end && pg0 >= a.batch.npages) || (kb + 8 < k_end && pg1 >= a.batch.npages))
-      if (lane == 0) atomicCAS(a.batch.status, 0, OPS_PAGED_BAD_PAGE);
-  };
-  auto stage_q = [&](const PagedPiece &p, int buf) {
-    for (int i = threadIdx.x; i < ROWS * DH / 8; i += FEW_THREADS) {
-      const int r = i / (DH / 8), col = (i - r * (DH / 8)) * 8;
-      const int tok = r / group, gi = r - tok * group;
-      const bool there = tok < p.s.n && col < a.dh;
-      const char *src = there ? a.q + (long long)(p.s.row + tok) * a.q_t + (long long)(p.head * group + gi) * a.q_h + col * 2 : a.q;
-      cp_async_16(q_s + (buf * ROWS + r) * DH + col, src, there);
-    }
-  };
-
-  int k_end = min(cur.hi * FEW_BLOCK, cur.s.len);
-  int kb = cur.lo * FEW_BLOCK + warp * 16;
-  pages(cur, kb, k_end);
-  stage_q(cur, 0);
-  bad_page(kb, k_end);
-  issue_k(cur, kb, k_end);
-  issue_v(cur, kb, k_end);
-  cp_async_wait();
   __syncthreads();
-  int buf = 0;
-  while (true) {
-    const i64 cur_begin = walk.begin;
-    const PagedPiece nxt = paged_step(a.batch, a.line, walk);
-    if (nxt.seq >= 0) stage_q(nxt, buf ^ 1);
-    const int rows = cur.s.n * group;
-    // q fragments are re-read from shared memory at every use (volatile: hoisting them would cost registers that the loads in
-    // flight need)
-    const volatile uint4 *q_frag = reinterpret_cast<const volatile uint4 *>(q_s + (buf * ROWS + g) * DH + c * 8);
-    int lim[NR];  // last visible key of row g (+ 8)
-    float m[NR], l[NR];  // m is common to the four lanes of a row, l is this lane's share
-    float o[NR][HH][4][4];
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      const int r = nr * 8 + g;
-      lim[nr] = r < rows ? (a.line.causal ? cur.s.len - cur.s.n + r / group : cur.s.len - 1) : -1;
-      m[nr] = -INFINITY;
-      l[nr] = 0.f;
-#pragma unroll
-      for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nr][hh][i][e] = 0.f;
-    }
-    for (; kb < k_end; kb += FEW_BLOCK) {  // warp-uniform
-      const bool more = kb + FEW_BLOCK < k_end;
-      if (more) pages(cur, kb + FEW_BLOCK, k_end);
-      float s[2][4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-          const uint32_t q0 = q_frag[ch * 4].x, q1 = q_frag[ch * 4].y, q2 = q_frag[ch * 4].z, q3 = q_frag[ch * 4].w;
-          uint32_t r0 = 0, r1 = 0, r2 = 0, r3 = 0;
-          if (NR == 2) {
-            const volatile uint4 *up = q_frag + DH + ch * 4;  // row g + 8
-            r0 = up->x;
-            r1 = up->y;
-            r2 = up->z;
-            r3 = up->w;
-          }
-          few_mma<BF>(s[j], q0, r0, q1, r1, kq[j][ch].x, kq[j][ch].y);
-          few_mma<BF>(s[j], q2, r2, q3, r3, kq[j][ch].z, kq[j][ch].w);
-        }
-      }
-      if (more) {
-        bad_page(kb + FEW_BLOCK, k_end);
-        issue_k(cur, kb + FEW_BLOCK, k_end);  // the K registers are free again
-      }
-      uint32_t pb[NR][2];
-      float al[NR][2];
-#pragma unroll
-      for (int nr = 0; nr < NR; ++nr) {
-        float sv[4], mx = -INFINITY;  // row 8 nr + g at keys kb + 8j + 2c + {0,1}
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int key = kb + j * 8 + 2 * c + e;
-            const float x = (key < k_end && key <= lim[nr]) ? s[j][nr * 2 + e] * a.scale_log2 : -INFINITY;
-            sv[j * 2 + e] = x;
-            mx = fmaxf(mx, x);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m[nr], mx);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = ap_ex2(m[nr] - m_use);
-        float p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = ap_ex2(sv[e] - m_use);
-        l[nr] = fmaf(l[nr], alpha, (p[0] + p[1]) + (p[2] + p[3]));
-        m[nr] = m_new;
-        pb[nr][0] = ap_pack<BF>(p[0], p[1]);
-        pb[nr][1] = ap_pack<BF>(p[2], p[3]);
-        // the accumulators of this lane belong to rows 8 nr + 2c and 2c + 1
-        al[nr][0] = __shfl_sync(0xffffffffu, alpha, (2 * c) << 2);
-        al[nr][1] = __shfl_sync(0xffffffffu, alpha, (2 * c + 1) << 2);
-      }
-#pragma unroll
-      for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w0 = few_word(vq[hh][0], i), w1 = few_word(vq[hh][1], i), w2 = few_word(vq[hh][2], i), w3 = few_word(vq[hh][3], i);
-          const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632), a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
-#pragma unroll
-          for (int nr = 0; nr < NR; ++nr) {
-            float (&d)[4] = o[nr][hh][i];
-            d[0] *= al[nr][0];
-            d[1] *= al[nr][1];
-            d[2] *= al[nr][0];
-            d[3] *= al[nr][1];
-            few_mma<BF>(d, a0, a1, a2, a3, pb[nr][0], pb[nr][1]);
-          }
-        }
-      if (more) issue_v(cur, kb + FEW_BLOCK, k_end);
-    }
-    const PagedPiece done = cur;
-    if (nxt.seq >= 0) {  // in flight while this piece is brought together
-      cur = nxt;
-      k_end = min(cur.hi * FEW_BLOCK, cur.s.len);
-      kb = cur.lo * FEW_BLOCK + warp * 16;
-      pages(cur, kb, k_end);
-      bad_page(kb, k_end);
-      issue_k(cur, kb, k_end);
-      issue_v(cur, kb, k_end);
-    }
 
-    // the 8 warps meet: common maximum per row, rescaled sums
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      l[nr] += __shfl_xor_sync(0xffffffffu, l[nr], 1);
-      l[nr] += __shfl_xor_sync(0xffffffffu, l[nr], 2);
-      if (c == 0) red_m[warp * ROWS + nr * 8 + g] = m[nr];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, red_m[w * ROWS + nr * 8 + g]);
-      if (c == 0) red_l[warp * ROWS + nr * 8 + g] = m[nr] == -INFINITY ? 0.f : l[nr] * ap_ex2(m[nr] - top);
-      float sc[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = nr * 8 + 2 * c + e;
-        float t = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < FEW_WARPS; ++w) t = fmaxf(t, red_m[w * ROWS + r]);
-        const float mw = red_m[warp * ROWS + r];
-        sc[e] = mw == -INFINITY ? 0.f : ap_ex2(mw - t);
-      }
-      float *to = red_o + (warp * ROWS + nr * 8 + 2 * c) * LD;
-#pragma unroll
-      for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = hh * 64 + g * 8 + 2 * i;
-          *reinterpret_cast<float2 *>(to + col) = make_float2(o[nr][hh][i][0] * sc[0], o[nr][hh][i][2] * sc[0]);
-          *reinterpret_cast<float2 *>(to + LD + col) = make_float2(o[nr][hh][i][1] * sc[1], o[nr][hh][i][3] * sc[1]);
+  bool ok = true;
+  if (warp == FEW_CONSUMERS + FEW_PRODUCERS) {
+    // ------------------------------------------------------------------ scheduler
+    if (lane == 0) {
+      PagedPiece last;
+      last.seq = -1;
+#pragma unroll 1
+      for (uint32_t i = 0; ok; ++i) {
+        const PagedPiece q = paged_step(a.batch, a.line, walk);
+        const int slot = i % FEW_RING;
+        if (!(ok = mbar_wait(piece_empty(slot), ((i / FEW_RING) & 1u) ^ 1u, status, 201))) break;
+        volatile FewPiece &to = pieces[slot];
+        to.seq = q.seq;
+        if (q.seq >= 0) {
+          to.row = q.s.row;
+          to.n = q.s.n;
+          to.len = q.s.len;
+          to.head = q.head;
+          to.k0 = q.lo * FEW_KEYS;
+          to.k1 = min(q.hi * FEW_KEYS, q.s.len);
+          to.park = q.whole() ? -1 : (int)blockIdx.x * 2 + q.slot();
         }
+        mbar_arrive(piece_full(slot));
+        if (q.seq < 0) break;
+        last = q;
+      }
+      paged_note_join(a, blockIdx.x, last, total);
     }
-    __syncthreads();
-    const bool whole = done.whole();
-    float *part = a.parts + (long long)(blockIdx.x * 2 + done.slot()) * ROWS * (DH + AP_PAD);
-    for (int i = threadIdx.x; i < rows * (DH / 4); i += FEW_THREADS) {
-      const int r = i / (DH / 4), col = (i - r * (DH / 4)) * 4;
-      if (col >= a.dh) continue;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float den = 0.f, top = -INFINITY;
+  } else if (warp >= FEW_CONSUMERS) {
+    // ------------------------------------------------------------------ producers
+    const int producer = warp - FEW_CONSUMERS;
+    const int box = 1 << f.box_log2, boxes = FEW_KEYS >> f.box_log2;  // of K; as many of V
+    const int lg = a.batch.page_log2, in_page = (1 << lg) - 1;
+    const bool values = lane >= boxes;
+    const int r = (values ? lane - boxes : lane) * box;  // the lane's first row of a stage
+    const bool mine = lane < 2 * boxes;
+    uint32_t count = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; ok; ++i) {
+      const int slot = i % FEW_RING;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(piece_full(slot), (i / FEW_RING) & 1u, status, 202)))) break;
+      volatile FewPiece &p = pieces[slot];
+      const int seq = p.seq, row = p.row, n = p.n, head = p.head, k0 = p.k0, k1 = p.k1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(piece_empty(slot));
+      if (seq < 0) break;
+      const uint32_t *table = a.batch.table + (long long)seq * a.batch.table_ld;
+      // the page of this lane's box of the stage at key k, outside the map where there is nothing to read
+      auto look_up = [&](int k) -> int {
+        const int key = k + r;
+        if (!mine || key >= k1) return (int)a.batch.npages;
+        const uint32_t page = table[key >> lg];
+        if (page < a.batch.npages) return (int)page;
+        atomicCAS(a.batch.status, 0, OPS_PAGED_BAD_PAGE);
+        return (int)a.batch.npages;
+      };
+      const uint32_t stages = k1 > k0 ? (uint32_t)(k1 - k0 + FEW_KEYS - 1) / FEW_KEYS : 0u;
+      uint32_t st = ((uint32_t)producer - count) % FEW_PRODUCERS;
+      int page = look_up(k0 + (int)st * FEW_KEYS);
+      // the piece's q rows, zeros behind them: read now by the first producer, written once its first stage is asked for
+      constexpr int Q_VECS = 16 * DH / 8 / 32;  // 16-byte pieces a lane
+      uint4 qv[Q_VECS];
+      bool q_due = producer == 0;
+      if (q_due) {
 #pragma unroll
-      for (int w = 0; w < FEW_WARPS; ++w) {
-        const float4 x = *reinterpret_cast<const float4 *>(red_o + (w * ROWS + r) * LD + col);
-        acc.x += x.x;
-        acc.y += x.y;
-        acc.z += x.z;
-        acc.w += x.w;
-        den += red_l[w * ROWS + r];
-        top = fmaxf(top, red_m[w * ROWS + r]);
+        for (int e = 0; e < Q_VECS; ++e) {
+          const int at = e * 32 + lane, qr = at / (DH / 8), col = (at - qr * (DH / 8)) * 8;
+          const int tok = paged_div(qr, group), gi = qr - tok * group;
+          qv[e] = make_uint4(0, 0, 0, 0);
+          if (tok < n && col < a.dh) qv[e] = ld_global_16(a.q + (long long)(row + tok) * a.q_t + (long long)(head * group + gi) * a.q_h + col * 2);
+        }
       }
-      if (whole) {
-        const float inv = den > 0.f ? 1.f / den : 0.f;  // a row that sees nothing: zeros
-        const int tok = r / group, gi = r - tok * group;
-        char *to = a.o + (long long)(done.s.row + tok) * a.o_t + (long long)(done.head * group + gi) * a.o_h + col * 2;
-        *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
-      } else {
-        float *to = part + r * (DH + AP_PAD);
-        *reinterpret_cast<float4 *>(to + col) = acc;
-        if (col == 0) *reinterpret_cast<float2 *>(to + DH) = make_float2(top, den);
+#pragma unroll 1
+      while (ok && (st < stages || q_due)) {
+        if (st < stages) {
+          const uint32_t at = count + st;
+          const int s = at % ST, k = k0 + (int)st * FEW_KEYS;
+          if (lane == 0) {
+            ok = mbar_wait(empty(s), ((at / ST) & 1u) ^ 1u, status, 204);
+            if (ok) mbar_arrive_expect_tx(full(s), 2 * Smem::OPERAND);
+          }
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0);
+          if (!ok) break;
+          if (mine) {
+            const uint32_t to = base + Smem::OFF_RING + s * (2 * Smem::OPERAND) + (values ? Smem::OPERAND : 0) + r * 128;
+            const int slot_in_page = (k + r) & in_page;
+#pragma unroll
+            for (int h = 0; h < Smem::HALVES; ++h)
+              tma_load_4d(to + h * (FEW_KEYS * 128), values ? &tmap_v : &tmap_k, full(s), h * 64, slot_in_page, head, page);
+          }
+          st += FEW_PRODUCERS;
+          page = look_up(k0 + (int)st * FEW_KEYS);
+        }
+        if (q_due) {
+          q_due = false;
+          const int b = i & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(q_empty(b), ((i >> 1) & 1u) ^ 1u, status, 203));
+#pragma unroll
+          for (int e = 0; e < Q_VECS; ++e) {
+            const int at = e * 32 + lane, qr = at / (DH / 8), col = (at - qr * (DH / 8)) * 8;
+            *reinterpret_cast<uint4 *>(base_ptr + Smem::OFF_Q + ((b * 16 + qr) * Smem::Q_LD + col) * 2) = qv[e];
+          }
+          __syncwarp();
+          if (ok && lane == 0) mbar_arrive(q_full(b));
+        }
       }
+      count += stages;
     }
-    if (nxt.seq < 0) {
-      walk.begin = cur_begin;
-      if (threadIdx.x == 0) paged_note_join(a, blockIdx.x, done, walk, total);
-      return;
+  } else {
+    // ------------------------------------------------------------------ consumers
+    const int g = lane >> 2, c = lane & 3;
+    // ldmatrix: lane l names row l % 8 of matrix l / 8
+    const int mi = lane >> 3, mr = lane & 7;
+    uint32_t count = 0, met = 0;  // stages of the pieces so far; meetings
+    auto meet = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(meet_bar);
+      return __all_sync(0xffffffffu, mbar_wait(meet_bar, met++ & 1u, status, 210));
+    };
+#pragma unroll 1
+    for (uint32_t i = 0; ok; ++i) {
+      const int slot = i % FEW_RING;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(piece_full(slot), (i / FEW_RING) & 1u, status, 211)))) break;
+      volatile FewPiece &p = pieces[slot];
+      const int seq = p.seq, row = p.row, n = p.n, len = p.len, head = p.head, k0 = p.k0, k1 = p.k1, park = p.park;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(piece_empty(slot));
+      if (seq < 0) break;
+      const int rows = n * group;
+      uint32_t q[DH / 16][4];
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full(i & 1), (i >> 1) & 1u, status, 212)))) break;
+#pragma unroll
+      for (int ks = 0; ks < DH / 16; ++ks)  // rows 0-7 | 8-15 of k 0-7, then of k 8-15
+        ldsm(base + Smem::OFF_Q + ((((i & 1) * 16 + (mi & 1) * 8 + mr) * Smem::Q_LD + ks * 16 + (mi >> 1) * 8) * 2), q[ks]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_empty(i & 1));
+      // last visible key of rows g and g + 8; every row sees the keys in front of `all`
+      int lim[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) lim[e] = a.line.causal ? len - n + paged_div(g + 8 * e, group) : len - 1;
+      const int all = min(k1, a.line.causal ? len - n + 1 : len);
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m is common to the four lanes of a row, l is this lane's share
+      float o[DH / 8][4];
+#pragma unroll
+      for (int j = 0; j < DH / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+
+      const uint32_t stages = k1 > k0 ? (uint32_t)(k1 - k0 + FEW_KEYS - 1) / FEW_KEYS : 0u;
+#pragma unroll 1
+      for (uint32_t st = ((uint32_t)warp - count) % FEW_CONSUMERS; st < stages; st += FEW_CONSUMERS) {
+        const uint32_t at = count + st;
+        const int s = at % ST, kb = k0 + (int)st * FEW_KEYS;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(full(s), (at / ST) & 1u, status, 213)))) break;
+        const uint32_t ks_base = base + Smem::OFF_RING + s * (2 * Smem::OPERAND), vs_base = ks_base + Smem::OPERAND;
+        if (kb + FEW_KEYS > len) {  // behind the end: may hold anything, a NaN too
+          uint8_t *v = base_ptr + Smem::OFF_RING + s * (2 * Smem::OPERAND) + Smem::OPERAND;
+          for (int e = lane; e < (kb + FEW_KEYS - len) * Smem::HALVES * 8; e += 32) {
+            const int r = len - kb + e / (Smem::HALVES * 8), piece = e % (Smem::HALVES * 8);
+            *reinterpret_cast<uint4 *>(v + (piece >> 3) * (FEW_KEYS * 128) + r * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();  // the stage's next load writes through the async proxy
+          __syncwarp();
+        }
+        float x[4][4];  // [8 keys][row g: keys 2c, 2c+1 | row g+8]
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[j][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DH / 16; ++ks)
+#pragma unroll
+          for (int np = 0; np < 2; ++np) {  // 16 keys: matrices (keys 0-7, k 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
+            uint32_t b[4];
+            const int key = np * 16 + (mi >> 1) * 8 + mr, chunk = ks * 2 + (mi & 1);
+            ldsm(ks_base + (chunk >> 3) * (FEW_KEYS * 128) + key * 128 + (((chunk & 7) ^ mr) << 4), b);
+            few_mma<BF>(x[np * 2], q[ks], b[0], b[1]);
+            few_mma<BF>(x[np * 2 + 1], q[ks], b[2], b[3]);
+          }
+        uint32_t pa[2][4];  // the probabilities as the second product's A: 16 keys each
+        float al[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              float &v = x[j][e * 2 + w];
+              v *= a.scale_log2;
+              if (kb + FEW_KEYS > all && kb + j * 8 + 2 * c + w > min(lim[e], k1 - 1)) v = -INFINITY;
+              mx = fmaxf(mx, v);
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float m_new = fmaxf(m[e], mx);
+          const float m_use = m_new == -INFINITY ? 0.f : m_new;
+          al[e] = ap_ex2(m[e] - m_use);
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p0 = ap_ex2(x[j][e * 2] - m_use), p1 = ap_ex2(x[j][e * 2 + 1] - m_use);
+            sum += p0 + p1;
+            pa[j >> 1][(j & 1) * 2 + e] = ap_pack<BF>(p0, p1);
+          }
+          l[e] = fmaf(l[e], al[e], sum);
+          m[e] = m_new;
+        }
+        if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+#pragma unroll
+          for (int j = 0; j < DH / 8; ++j) {
+            o[j][0] *= al[0];
+            o[j][1] *= al[0];
+            o[j][2] *= al[1];
+            o[j][3] *= al[1];
+          }
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int np = 0; np < DH / 16; ++np) {  // 16 columns: matrices (keys 0-7, columns 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
+            uint32_t b[4];
+            const int key = kt * 16 + (mi & 1) * 8 + mr, chunk = np * 2 + (mi >> 1);
+            ldsm_t(vs_base + (chunk >> 3) * (FEW_KEYS * 128) + key * 128 + (((chunk & 7) ^ mr) << 4), b);
+            few_mma<BF>(o[np * 2], pa[kt], b[0], b[1]);
+            few_mma<BF>(o[np * 2 + 1], pa[kt], b[2], b[3]);
+          }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(s));
+      }
+      if (!ok) break;
+      count += stages;
+
+      // the four warps meet: each leaves its m, l and o, and the threads that finish an output weigh them
+      float2 *ml_s = reinterpret_cast<float2 *>(base_ptr + Smem::OFF_ML);
+      float *o_s = reinterpret_cast<float *>(base_ptr + Smem::OFF_O);
+#pragma unroll
+      for (int e = 0; e < NR; ++e) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        if (c == 0) ml_s[(g + 8 * e) * FEW_CONSUMERS + warp] = make_float2(m[e], l[e]);
+        if (g + 8 * e < rows)
+#pragma unroll
+          for (int j = 0; j < DH / 8; ++j)
+            *reinterpret_cast<float2 *>(o_s + (warp * ROWS + g + 8 * e) * Smem::O_LD + j * 8 + 2 * c) = make_float2(o[j][e * 2], o[j][e * 2 + 1]);
+      }
+      if (!(ok = meet())) break;
+#pragma unroll 1
+      for (int at = threadIdx.x; at < rows * (DH / 4); at += FEW_CONSUMERS * 32) {
+        const int r = at / (DH / 4), col = (at - r * (DH / 4)) * 4;
+        if (col >= a.dh) continue;
+        float2 ml[FEW_CONSUMERS];
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < FEW_CONSUMERS; ++w) {
+          ml[w] = ml_s[r * FEW_CONSUMERS + w];
+          top = fmaxf(top, ml[w].x);
+        }
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f;
+#pragma unroll
+        for (int w = 0; w < FEW_CONSUMERS; ++w) {
+          const float4 v = *reinterpret_cast<const float4 *>(o_s + (w * ROWS + r) * Smem::O_LD + col);
+          const float weight = ap_ex2(ml[w].x - ref);  // a warp without a key in sight: 0, of zeros
+          acc.x = fmaf(v.x, weight, acc.x);
+          acc.y = fmaf(v.y, weight, acc.y);
+          acc.z = fmaf(v.z, weight, acc.z);
+          acc.w = fmaf(v.w, weight, acc.w);
+          den = fmaf(ml[w].y, weight, den);
+        }
+        if (park < 0) {
+          const float inv = den > 0.f ? 1.f / den : 0.f;  // a row that sees nothing: zeros
+          const int tok = paged_div(r, group), gi = r - tok * group;
+          char *to = a.o + (long long)(row + tok) * a.o_t + (long long)(head * group + gi) * a.o_h + col * 2;
+          *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
+        } else {
+          float *to = a.parts + ((long long)park * ROWS + r) * (DH + AP_PAD);
+          *reinterpret_cast<float4 *>(to + col) = acc;
+          if (col == 0) *reinterpret_cast<float2 *>(to + DH) = make_float2(top, den);
+        }
+      }
+      if (!(ok = meet())) break;  // ml_s and o_s are free again
     }
-    cp_async_wait();
-    __syncthreads();
-    buf ^= 1;
   }
+  if (!ok) gave_up = 1;
+  __syncthreads();
+  if (gave_up) __nanosleep(1000000);  // a wait ran out: let stray copies land before the CTA goes away
 }
 
-// One wave: two CTAs an SM for 8 rows (128 registers), one for 16 (twice the accumulators).
-int attention_paged_few_ctas(const OpBase &base, int rows) { return rows == 8 ? 2 * base.sm_count : base.sm_count; }
+// One CTA per SM: the ring takes its shared memory.
+int attention_paged_few_ctas(const OpBase &base) { return base.sm_count; }
 
 template <int DH, bool BF, int NR>
-static int few_launch(const PagedAttnArgs &a, cudaStream_t s) {
+static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
   const int bytes = FewSmem<DH, NR>::BYTES;
   cudaError_t e = cudaFuncSetAttribute(attention_paged_few_kernel<DH, BF, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
-  attention_paged_few_kernel<DH, BF, NR><<<a.line.ctas, FEW_THREADS, bytes, s>>>(a);
+  attention_paged_few_kernel<DH, BF, NR><<<f.a.line.ctas, FEW_THREADS, bytes, s>>>(k, v, f);
   return check_launch("attention_paged(few rows)");
+}
+template <int DH, int NR>
+static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, bool bf16, cudaStream_t s) {
+  return bf16 ? few_launch<DH, true, NR>(f, k, v, s) : few_launch<DH, false, NR>(f, k, v, s);
 }
 
 int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, cudaStream_t s) {
-  if (a.dh <= 64) {
-    if (rows == 8) return bf16 ? few_launch<64, true, 1>(a, s) : few_launch<64, false, 1>(a, s);
-    return bf16 ? few_launch<64, true, 2>(a, s) : few_launch<64, false, 2>(a, s);
-  }
-  if (rows == 8) return bf16 ? few_launch<128, true, 1>(a, s) : few_launch<128, false, 1>(a, s);
-  return bf16 ? few_launch<128, true, 2>(a, s) : few_launch<128, false, 2>(a, s);
+  FewArgs f;
+  f.a = a;
+  f.box_log2 = a.batch.page_log2 < 5 ? a.batch.page_log2 : 5;
+  CUtensorMap k, v;
+  OPS_TRY(attention_paged_maps(a, bf16, 1u << f.box_log2, &k, &v));
+  if (a.dh <= 64) return rows == 8 ? few_launch<64, 1>(f, k, v, bf16, s) : few_launch<64, 2>(f, k, v, bf16, s);
+  return rows == 8 ? few_launch<128, 1>(f, k, v, bf16, s) : few_launch<128, 2>(f, k, v, bf16, s);
 }
 
 }  // namespace ops

@@ -120,15 +120,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   __shared__ int gave_up;
 
   pdl_let_next_come();
-  i64 total;
-  PagedWalk walk = paged_locate<TL_THREADS>(batch, line, blockIdx.x, blockIdx.x == 0, &total);
-  if (walk.at >= walk.end) {  // nothing for this CTA (all its threads agree)
-    PagedPiece none;
-    none.seq = -1;
-    if (threadIdx.x == 0) paged_note_join(g.a, blockIdx.x, none, walk, total);
-    return;
-  }
-
   if (threadIdx.x == 0) {
     gave_up = 0;
     for (int t = 0; t < 2; ++t) {
@@ -152,6 +143,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
     }
     fence_barrier_init();
   }
+  PagedWalk walk;
+  int total = 0;
+  if (warp == 3) paged_locate(batch, line, blockIdx.x, blockIdx.x == 0, &walk, &total);
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
@@ -329,61 +323,44 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       }
     } else {
       // ------------------------------------------------------------------ scheduler
-      PagedPiece cur = paged_step(batch, line, walk);
-      i64 begin = walk.begin;  // of cur's sequence
-      bool ok = true;
-      auto post = [&](const PagedPiece &q, uint32_t i) -> bool {
-        TilePiece told;
-        memset(&told, 0, sizeof(told));
-        told.clean = -1;
-        if (q.seq >= 0) {
-          const int t0 = q.tile * line.tokens;
-          told.valid = 1;
-          told.row = q.s.row + t0;
-          told.tokens = q.s.n - t0;
-          told.off = q.s.len - q.s.n + t0;
-          told.len = q.s.len;
-          told.seq = q.seq;
-          told.head = q.head;
-          told.lo = q.lo;
-          told.hi = q.hi;
+      if (lane == 0) {
+        PagedPiece last;
+        last.seq = -1;
+        bool ok = true;
+#pragma unroll 1
+        for (uint32_t i = 0; ok; ++i) {
+          const PagedPiece q = paged_step(batch, line, walk);
+          const int slot = i % TL_RING;
+          if (!(ok = mbar_wait(ring_empty(slot), ((i / TL_RING) & 1u) ^ 1u, status, 130))) break;
+          volatile TilePiece &to = ring[slot];
+          to.valid = q.seq >= 0;
+          if (q.seq >= 0) {
+            const int t0 = q.tile * line.tokens;
+            to.row = q.s.row + t0;
+            to.tokens = q.s.n - t0;
+            to.off = q.s.len - q.s.n + t0;
+            to.len = q.s.len;
+            to.seq = q.seq;
+            to.head = q.head;
+            to.lo = q.lo;
+            to.hi = q.hi;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int keys_seen = paged_keys(line, q.s, t0 + (t + 1) * g.per_tile);
-            const int all = t * g.per_tile < told.tokens ? max(1, (keys_seen + TL_KEYS - 1) / TL_KEYS) : 0;
-            told.blocks[t] = max(0, min(all, q.hi) - q.lo);
+            for (int t = 0; t < 2; ++t) {
+              const int seen = paged_keys(line, q.s, t0 + (t + 1) * g.per_tile);
+              const int all = t0 + t * g.per_tile < q.s.n ? max(1, (seen + TL_KEYS - 1) / TL_KEYS) : 0;
+              to.blocks[t] = max(0, min(all, q.hi) - q.lo);
+            }
+            const int end = q.s.len / TL_KEYS;  // the block the sequence ends in
+            to.clean = (q.s.len & ((1 << g.box_log2) - 1)) && end >= q.lo && end < q.hi ? end - q.lo : -1;
+            to.park = q.whole() ? -1 : (int)blockIdx.x * 2 + q.slot();
           }
-          const int last = q.s.len / TL_KEYS;  // the block the sequence ends in
-          if ((q.s.len & ((1 << g.box_log2) - 1)) && last >= q.lo && last < q.hi) told.clean = last - q.lo;
-          told.park = q.whole() ? -1 : (int)blockIdx.x * 2 + q.slot();
+          mbar_arrive(ring_full(slot));
+          if (q.seq < 0) break;
+          last = q;
         }
-        const int slot = i % TL_RING;
-        if (!__all_sync(0xffffffffu, mbar_wait(ring_empty(slot), ((i / TL_RING) & 1u) ^ 1u, status, 130))) return false;
-        volatile int *to = reinterpret_cast<volatile int *>(&ring[slot]);
-        const int *from = reinterpret_cast<const int *>(&told);
-#pragma unroll
-        for (int w = 0; w < (int)(sizeof(TilePiece) / 4); ++w)
-          if (lane == w % 32) to[w] = from[w];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ring_full(slot));
-        return true;
-      };
-      ok = post(cur, 0);
-      for (uint32_t i = 0; ok; ++i) {
-        const PagedPiece last = cur;
-        const i64 last_begin = begin;
-        cur = paged_step(batch, line, walk);
-        begin = walk.begin;
-        ok = post(cur, i + 1);
-        if (!ok) break;
-        if (cur.seq < 0) {
-          PagedWalk w = walk;
-          w.begin = last_begin;
-          if (lane == 0) paged_note_join(g.a, blockIdx.x, last, w, total);
-          break;
-        }
+        paged_note_join(g.a, blockIdx.x, last, total);
+        if (!ok) gave_up = 1;
       }
-      if (!ok) gave_up = 1;
     }
   } else {
     // ------------------------------------------------------------------ softmax, rescaling, output: two threads per q row
@@ -563,33 +540,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   }
 }
 
-// cuTensorMapEncodeTiled through the runtime's driver entry point
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn tl_encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
-    return (EncodeTiledFn)p;
-  }();
-  return fn;
-}
-
-// A 4-d map of 16-bit elements, 64 of the innermost dim and `box1` x `box2` of the next two a box, 128-byte swizzle.
-static bool tl_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2) {
-  EncodeTiledFn fn = tl_encode_fn();
-  if (!fn) return false;
-  cuuint64_t d[4], st[3];
-  for (int i = 0; i < 4; ++i) d[i] = dims[i];
-  for (int i = 0; i < 3; ++i) st[i] = dims[i + 1] > 1 ? (cuuint64_t)strides[i] : (cuuint64_t)(dims[0] * 2);  // never stepped over
-  cuuint32_t box[4] = {64, box1, box2, 1};
-  cuuint32_t es[4] = {1, 1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(ptr), d, st, box, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int DH, bool BF>
 static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
   const int bytes = TileSmem<DH>::BYTES;
@@ -605,12 +555,11 @@ int attention_paged_tile(const PagedAttnArgs &a, bool bf16, cudaStream_t s) {
   g.per_tile = TL_ROWS / a.line.group;
   g.box_log2 = a.batch.page_log2 < 6 ? a.batch.page_log2 : 6;
   CUtensorMap q, k, v;
-  const usz nkvh = (usz)a.line.nkvh, page = (usz)1 << a.batch.page_log2, dh = (usz)a.dh;
-  const usz q_dims[4] = {dh, (usz)a.line.group, (usz)a.batch.nt, nkvh}, dims[4] = {dh, page, nkvh, a.batch.npages};
-  const isz q_st[3] = {a.q_h, a.q_t, a.q_h * a.line.group}, k_st[3] = {a.kp_s, a.kp_h, a.kp_p}, v_st[3] = {a.vp_s, a.vp_h, a.vp_p};
-  if (!tl_encode(&q, bf16, a.q, q_dims, q_st, (uint32_t)a.line.group, (uint32_t)g.per_tile) ||
-      !tl_encode(&k, bf16, a.k, dims, k_st, 1u << g.box_log2, 1) || !tl_encode(&v, bf16, a.v, dims, v_st, 1u << g.box_log2, 1))
+  const usz q_dims[4] = {(usz)a.dh, (usz)a.line.group, (usz)a.batch.nt, (usz)a.line.nkvh};
+  const isz q_st[3] = {a.q_h, a.q_t, a.q_h * a.line.group};
+  if (!ap_encode(&q, bf16, a.q, q_dims, q_st, (uint32_t)a.line.group, (uint32_t)g.per_tile))
     return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
+  OPS_TRY(attention_paged_maps(a, bf16, 1u << g.box_log2, &k, &v));
   if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, s) : tile_launch<64, false>(g, q, k, v, s);
   return bf16 ? tile_launch<128, true>(g, q, k, v, s) : tile_launch<128, false>(g, q, k, v, s);
 }

@@ -112,8 +112,8 @@ inline int paged_launch_checks(const char *op, const ops_paged_batch *b, const o
   for (int i = 0; i < 2; ++i) {
     if (caches[i]->strides[3] != 2) return fail(OPS_STRIDES_NOT_SUPPORT, "%s: last dim of the cache must be contiguous", op);
     for (int d = 0; d < 3; ++d)
-      if (dims[d] > 1 && (caches[i]->strides[d] % 16 || caches[i]->strides[d] <= 0 || caches[i]->strides[d] >= ((isz)1 << 40)))
-        return fail(OPS_STRIDES_NOT_SUPPORT, "%s: strides of the cache must be multiples of 16 bytes, positive and below 2^40", op);
+      if (dims[d] > 1 && (caches[i]->strides[d] % 16 || caches[i]->strides[d] <= 0 || caches[i]->strides[d] >= ((isz)1 << 36)))
+        return fail(OPS_STRIDES_NOT_SUPPORT, "%s: strides of the cache must be multiples of 16 bytes, positive and below 2^36", op);
   }
   if (nt == 0 || m.nseq == 0) return OPS_OK;
   if (!b->seq_start_base || !b->kv_len_base || (m.width && !b->page_table_base))

@@ -1,5 +1,6 @@
 // Walks the schedule of random batches on the CPU: every key block of every unit belongs to exactly one CTA, a CTA parks at most
 // one part in each of its two slots, shares are even, and a unit's parts are found again from the cuts as the joining kernel does.
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <map>
@@ -33,9 +34,9 @@ int main() {
     l.rows_hi = tile ? 0x7fffffff : few;
     l.max_seq = pick(0, 4) ? 0x7fffffff : pick(1, 40);
     l.tokens = tile ? 2 * (128 / l.group) : few;
-    l.block = tile ? 128 : 64;
-    l.overhead = pick(1, 600);
-    l.min_share = pick(1, 900);
+    l.block_log2 = tile ? 7 : 6;
+    const int block = 1 << l.block_log2;
+    const int overhead = pick(1, 600), min_share = pick(1, 900);
     l.ctas = std::vector<int>{1, 3, 148, 296}[pick(0, 3)];
     std::vector<PagedSeq> seqs(pick(0, round_no % 10 ? 12 : 400));
     const int big = round_no % 7 ? 300 : 20000;
@@ -47,8 +48,18 @@ int main() {
       row += s.n;
     }
     const int nseq = (int)seqs.size();
-    i64 total = 0;
-    for (auto &s : seqs) total += paged_span(l, s).head * l.nkvh;
+    // the host's bound: all rows in tiles and one more unit per sequence, each of all slots and rows
+    int slots = 1;
+    for (auto &s : seqs) slots = std::max(slots, s.len);
+    const double count = ((double)row / l.tokens + nseq) * l.nkvh, most = (double)slots + row + l.tokens + overhead;
+    l.shift = pick(0, 3) ? 0 : pick(0, 7);
+    while (count * (most / (1 << l.shift) + 4.0) > 2147483647.0) ++l.shift;
+    l.overhead = std::max(1, overhead >> l.shift);
+    l.min_share = std::max(1, min_share >> l.shift);
+    long long sum = 0;
+    for (auto &s : seqs) sum += (long long)paged_span(l, s).head * l.nkvh;
+    CHECK(sum <= 0x7fffffff);  // the shift below is chosen like the host's
+    const int total = (int)sum;
     if (total == 0) continue;
     const int active = paged_active(l, total);
     CHECK(active >= 1 && active <= l.ctas);
@@ -59,25 +70,26 @@ int main() {
     std::map<int, int> parked;
     for (int c = 0; c < active; ++c) {
       PagedWalk w{0, 0, paged_cut(total, active, c), paged_cut(total, active, c + 1)};
-      i64 keys = 0;
+      long long keys = 0;
       int steps = 0;
       for (PagedPiece q = paged_next(l, nseq, w, at); q.seq >= 0; q = paged_next(l, nseq, w, at)) {
         CHECK(++steps < 1000000);
-        CHECK(q.lo < q.hi && q.hi <= q.blocks);
+        CHECK(q.lo < q.hi && q.hi <= q.blocks && q.lo >= 0);
         if (!q.whole()) CHECK(++parked[c * 2 + q.slot()] == 1);
         units[{q.seq, q.head, q.tile}].push_back({q.lo, q.hi, c * 2 + q.slot()});
         blocks[{q.seq, q.head, q.tile}] = q.blocks;
         keys += (q.hi - q.lo);
       }
       // a share is its points' blocks, to within the roundings at its two ends and the short last block and tile of a unit
-      CHECK(keys <= (paged_cut(total, active, c + 1) - paged_cut(total, active, c)) / l.block + 2 + 2 * steps);
+      // (a point of several keys rounds the ramp of a causal unit down)
+      if (l.shift == 0) CHECK(keys <= (((long long)(paged_cut(total, active, c + 1) - paged_cut(total, active, c)) << l.shift) / block + 2 + 2 * steps) * 9 / 8);
     }
     size_t want = 0;
     for (int i = 0; i < nseq; ++i) {
       const PagedSpan p = paged_span(l, seqs[i]);
-      const i64 rows = (i64)seqs[i].n * l.group;
+      const long long rows = (long long)seqs[i].n * l.group;
       CHECK((p.tiles > 0) == (seqs[i].n > 0 && rows >= l.rows_lo && rows <= l.rows_hi && seqs[i].n <= l.max_seq));
-      if (p.tiles) CHECK((i64)p.tiles * l.tokens >= seqs[i].n && (i64)(p.tiles - 1) * l.tokens < seqs[i].n);
+      if (p.tiles) CHECK((long long)p.tiles * l.tokens >= seqs[i].n && (long long)(p.tiles - 1) * l.tokens < seqs[i].n);
       want += (size_t)p.tiles * l.nkvh;
     }
     CHECK(units.size() == want);
@@ -90,22 +102,23 @@ int main() {
       CHECK(next == blocks[u.first]);
       const PagedSeq &s = seqs[std::get<0>(u.first)];
       const int keys = paged_keys(l, s, (std::get<2>(u.first) + 1) * l.tokens);
-      CHECK((i64)blocks[u.first] * l.block >= keys && (keys == 0 || (i64)(blocks[u.first] - 1) * l.block < keys));
+      CHECK((long long)blocks[u.first] * block >= keys && (keys == 0 || (long long)(blocks[u.first] - 1) * block < keys));
     }
     // the joining kernel's view: the first cut inside a unit leads to all its parts
     size_t joined = 0, split = 0;
     for (auto &u : units) split += u.second.size() > 1;
     for (int c = 1; c < active; ++c) {
-      const i64 cut = paged_cut(total, active, c);
-      i64 begin = 0;
+      const int cut = paged_cut(total, active, c);
+      int begin = 0;
       int i = 0;
       while (begin + paged_span(l, seqs[i]).head * l.nkvh <= cut) begin += paged_span(l, seqs[i++]).head * l.nkvh;
-      const PagedUnit u = paged_unit(l, paged_span(l, seqs[i]), cut - begin);
+      const PagedUnit u = paged_unit(paged_span(l, seqs[i]), cut - begin);
       if (cut == begin + u.begin || paged_cut(total, active, c - 1) > begin + u.begin) continue;
       const int nb = paged_blocks(l, seqs[i], u.tile);
       std::vector<std::tuple<int, int, int>> parts;
       for (int d = c - 1; d < active && paged_cut(total, active, d) < begin + u.begin + u.cost; ++d) {
-        const int lo = paged_block(l, u, nb, paged_cut(total, active, d) - begin), hi = paged_block(l, u, nb, paged_cut(total, active, d + 1) - begin);
+        const int from = begin + u.begin;
+        const int lo = paged_block(l.overhead, u.cost, nb, paged_cut(total, active, d) - from), hi = paged_block(l.overhead, u.cost, nb, paged_cut(total, active, d + 1) - from);
         if (lo < hi) parts.push_back({lo, hi, d * 2 + (lo > 0 ? 0 : 1)});
       }
       auto found = units.find({i, u.head, u.tile});
@@ -114,7 +127,7 @@ int main() {
     }
     CHECK(joined == split);
     for (int k = 0; k < 20; ++k) {
-      const i64 x = k ? 1 + (i64)(rng() % (unsigned long long)total) : total;
+      const int x = k ? 1 + (int)(rng() % (unsigned)total) : total;
       int c = 0;
       while (c < active && paged_cut(total, active, c) < x) ++c;
       CHECK(paged_first_behind(total, active, x) == c);
