@@ -19,45 +19,46 @@ constexpr int JOIN_BLOCKS_PER_SM = 2;
 template <bool BF>
 __global__ void __launch_bounds__(JOIN_THREADS, JOIN_BLOCKS_PER_SM)
     attention_paged_join_kernel(const __grid_constant__ PagedAttnArgs few, const __grid_constant__ PagedAttnArgs tile, int few_rows, int part_dh) {
-  __shared__ int first_item[2 * AP_MAX_CTAS + 1];  // of every record
+  __shared__ int first_item[2 * AP_MAX_CTAS];  // of every record
+  __shared__ PagedJoin joins[2 * AP_MAX_CTAS];
   __shared__ int warp_items[JOIN_WARPS];
   __shared__ __align__(16) float meet[JOIN_WARPS][AP_MAX_DH + AP_PAD];  // o, m, l; 16-byte rows
-  __shared__ short slot_s[AP_MAX_CTAS];  // of the part of the d-th CTA behind the first; -1: the cut left it none
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int records = few.line.ctas + tile.line.ctas;
-  const int per = (records + JOIN_THREADS - 1) / JOIN_THREADS;
+  const int records = few.line.ctas + tile.line.ctas, group = few.line.group;
   pdl_wait_for_front();
-  // items of this thread's records, then a prefix sum over the block
-  int mine = 0;
-  for (int e = 0; e < per; ++e) {
-    const int j = threadIdx.x * per + e;
-    if (j < records) {
-      const bool on_tile = j >= few.line.ctas;
-      const PagedJoin *rec = on_tile ? tile.joins + (j - few.line.ctas) : few.joins + j;
-      first_item[j] = mine;
-      if (rec->ctas) mine += (rec->tokens * few.line.group + JOIN_ROWS - 1) / JOIN_ROWS;
-    }
-  }
-  int upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
-  }
-  if (lane == 31) warp_items[warp] = upto;
-  __syncthreads();
+  // items in front of every record's: a prefix sum over rounds of a record per thread
   int items = 0;
+  for (int j0 = 0; j0 < records; j0 += JOIN_THREADS) {
+    const int j = j0 + threadIdx.x;
+    int mine = 0;
+    if (j < records) {
+      const PagedJoin rec = j < few.line.ctas ? few.joins[j] : tile.joins[j - few.line.ctas];
+      joins[j] = rec;
+      if (rec.ctas) mine = paged_div(rec.tokens * group + JOIN_ROWS - 1, JOIN_ROWS);
+    }
+    int upto = mine;
 #pragma unroll
-  for (int w = 0; w < JOIN_WARPS; ++w) {
-    if (w == warp) upto += items;
-    items += warp_items[w];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) warp_items[warp] = upto;
+    __syncthreads();
+    int sum = warp_items[lane & (JOIN_WARPS - 1)];  // of all warps, by every warp for itself
+#pragma unroll
+    for (int o = 1; o < JOIN_WARPS; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if ((lane & (JOIN_WARPS - 1)) >= o) sum += x;
+    }
+    const int front = warp == 0 ? 0 : __shfl_sync(0xffffffffu, sum, warp - 1);
+    if (j < records) first_item[j] = items + front + upto - mine;
+    items += __shfl_sync(0xffffffffu, sum, JOIN_WARPS - 1);
+    __syncthreads();
   }
-  for (int e = 0; e < per; ++e)
-    if (threadIdx.x * per + e < records) first_item[threadIdx.x * per + e] += upto - mine;
-  __syncthreads();
 
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
     int lo = 0, hi = records;  // the last record whose first item is at or before this one has it
+#pragma unroll 1
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
       if (first_item[mid] <= item) lo = mid;
@@ -65,22 +66,15 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_BLOCKS_PER_SM)
     }
     const bool on_tile = lo >= few.line.ctas;
     const PagedAttnArgs &a = on_tile ? tile : few;
+    const PagedJoin &j = joins[lo];
     const int first = on_tile ? lo - few.line.ctas : lo;
-    const PagedJoin j = a.joins[first];
-    const int group = a.line.group, row0 = (item - first_item[lo]) * JOIN_ROWS, here = min(JOIN_ROWS, j.tokens * group - row0);
-    for (int d = threadIdx.x; d < j.ctas; d += JOIN_THREADS) {
-      const int c = first + d;
-      const int b0 = paged_block(a.line.overhead, j.cost, j.blocks, paged_cut(j.total, j.active, c) - j.begin);
-      const int b1 = paged_block(a.line.overhead, j.cost, j.blocks, paged_cut(j.total, j.active, c + 1) - j.begin);
-      slot_s[d] = (short)(b0 >= b1 ? -1 : c * 2 + (b0 > 0 ? 0 : 1));
-    }
-    __syncthreads();
-    const int share = JOIN_WARPS / here;  // warps per row
-    const int own = warp / share, part = warp - own * share;
+    const int row0 = (item - first_item[lo]) * JOIN_ROWS, here = min(JOIN_ROWS, j.tokens * group - row0);
+    const int share = paged_div(JOIN_WARPS, here);  // warps per row
+    const int own = paged_div(warp, share), part = warp - own * share;
     const int r = row0 + own;
     // where the row lies in a parked unit: tiles of 128 rows, whole tokens each
-    const int tok = r / group, gi = r - tok * group;
-    const int per_tile = on_tile ? AP_TILE_ROWS / 2 / group : JOIN_ROWS, t = tok / per_tile;
+    const int tok = paged_div(r, group), gi = r - tok * group;
+    const int per_tile = on_tile ? tile.line.tokens / 2 : JOIN_ROWS, t = paged_div(tok, per_tile);
     const int parked = t * (AP_TILE_ROWS / 2) + (tok - t * per_tile) * group + gi;
     const long long ld = part_dh + AP_PAD, unit = (long long)(on_tile ? AP_TILE_ROWS : few_rows) * ld;
     float m = -INFINITY, l = 0.f;
@@ -95,7 +89,8 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_BLOCKS_PER_SM)
           const int d = d0 + e * share;
           v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
           ml[e] = make_float2(-INFINITY, 0.f);
-          const int slot = d < j.ctas ? slot_s[d] : -1;
+          // the first has the unit's beginning in its second slot; a cut may have left one of the others none
+          const int slot = d >= j.ctas ? -1 : d == 0 ? first * 2 + 1 : joins[lo + d].front ? (first + d) * 2 : -1;
           if (slot >= 0) {
             const float *from = a.parts + slot * unit + parked * ld;
             ml[e] = __ldcg(reinterpret_cast<const float2 *>(from + part_dh));
@@ -143,7 +138,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_BLOCKS_PER_SM)
         *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
       }
     }
-    __syncthreads();  // slot_s and meet are free again
+    __syncthreads();  // meet is free again
   }
 }
 
@@ -260,7 +255,7 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
     p.few.rows_hi = p.few_rows;
     p.few.tokens = p.few_rows;
     p.few.block_log2 = AP_FEW_BLOCK_LOG2;
-    line_scale(&p.few, nt, nseq, slots, 128, 256);
+    line_scale(&p.few, nt, nseq, slots, 128, 128);
     p.few.ctas = std::min(attention_paged_few_ctas(base), AP_MAX_CTAS);
     p.few_joins = up256(sizeof(PagedJoin) * (usz)p.few.ctas);
     p.few_parts = up256(2 * (usz)p.few.ctas * p.few_rows * (p.part_dh + AP_PAD) * sizeof(float));

@@ -10,15 +10,15 @@ namespace ops {
 
 constexpr int AP_MAX_DH = 128;
 constexpr int AP_MAX_GROUP = 128;
-constexpr int AP_MAX_CTAS = 1024;
+constexpr int AP_MAX_CTAS = 256;  // of a kernel: the joining kernel holds a record of each
 constexpr int AP_PAD = 4;  // a parked row: DH floats of unnormalised o, its reference point m and its sum l; 16-byte aligned
 
-// A unit that several CTAs share, as the one that has its first blocks writes it down for the kernel that joins the parts.
-struct PagedJoin {
-  int ctas;               // that have points of the unit, the writer and those behind it; 0: nothing to join
-  int row, tokens, head;  // first row of the step, query tokens, kv head
-  int blocks, active;     // of the unit; of the launch
-  int begin, cost, total;  // unit on the line; points of the line
+// What a CTA leaves for the kernel that joins the parts of units that several CTAs share.
+struct __align__(16) PagedJoin {
+  int ctas;                 // that have points of the unit this CTA has the first blocks of, and not the last: it and those behind it; else 0
+  int row, tokens, head;    // of that unit: first row of the step, query tokens, kv head
+  int front;                // whether this CTA's slot 0 holds a part (of the unit that its share begins in)
+  int unused[3];
 };
 
 struct PagedAttnArgs {
@@ -113,21 +113,17 @@ __device__ __forceinline__ PagedPiece paged_step(const PagedBatch &b, const Page
   return paged_next(l, b.nseq, w, [&](int i) { return paged_seq(b, i, false); });
 }
 
-// The CTA's record for the joining kernel, written by one thread: `piece` is the last of its share (its unit goes on in the next
-// CTAs' shares if it is not the end of it), or seq < 0.
-__device__ __forceinline__ void paged_note_join(const PagedAttnArgs &a, int cta, const PagedPiece &piece, int total) {
+// The CTA's record for the joining kernel, written by one thread: `last` is the last piece of its share (its unit goes on in the
+// next CTAs' shares if it is not the end of it), or seq < 0; front: its first piece is not the beginning of a unit.
+__device__ __forceinline__ void paged_note_join(const PagedAttnArgs &a, int cta, const PagedPiece &last, bool front, int total) {
   PagedJoin j;
   memset(&j, 0, sizeof(j));
-  if (piece.seq >= 0 && piece.lo == 0 && piece.hi < piece.blocks) {
-    j.begin = piece.begin;
-    j.cost = piece.cost;
-    j.total = total;
-    j.active = paged_active(a.line, total);
-    j.ctas = paged_first_behind(total, j.active, j.begin + j.cost) - cta;
-    j.row = piece.s.row + piece.tile * a.line.tokens;
-    j.tokens = min(a.line.tokens, piece.s.n - piece.tile * a.line.tokens);
-    j.head = piece.head;
-    j.blocks = piece.blocks;
+  j.front = front;
+  if (last.seq >= 0 && last.lo == 0 && last.hi < last.blocks) {
+    j.ctas = paged_first_behind(total, paged_active(a.line, total), last.begin + last.cost) - cta;
+    j.row = last.s.row + last.tile * a.line.tokens;
+    j.tokens = min(a.line.tokens, last.s.n - last.tile * a.line.tokens);
+    j.head = last.head;
   }
   a.joins[cta] = j;
 }

@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     if (lane == 0) {
       PagedPiece last;
       last.seq = -1;
+      bool front = false;
 #pragma unroll 1
       for (uint32_t i = 0; ok; ++i) {
         const PagedPiece q = paged_step(a.batch, a.line, walk);
@@ -161,9 +162,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
         mbar_arrive(piece_full(slot));
         if (q.seq < 0) break;
+        if (last.seq < 0) front = q.lo > 0;
         last = q;
       }
-      paged_note_join(a, blockIdx.x, last, total);
+      paged_note_join(a, blockIdx.x, last, front, total);
     }
   } else if (warp >= FEW_CONSUMERS) {
     // ------------------------------------------------------------------ producers

@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       if (lane == 0) {
         PagedPiece last;
         last.seq = -1;
+        bool front = false;
         bool ok = true;
 #pragma unroll 1
         for (uint32_t i = 0; ok; ++i) {
@@ -356,9 +357,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           }
           mbar_arrive(ring_full(slot));
           if (q.seq < 0) break;
+          if (last.seq < 0) front = q.lo > 0;
           last = q;
         }
-        paged_note_join(g.a, blockIdx.x, last, total);
+        paged_note_join(g.a, blockIdx.x, last, front, total);
         if (!ok) gave_up = 1;
       }
     }
