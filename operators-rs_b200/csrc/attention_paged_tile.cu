@@ -75,6 +75,7 @@ struct TileArgs {
   PagedAttnArgs a;
   int per_tile;   // tokens of a tile: 128 / group
   int box_log2;   // rows of a K or V box: min(page, 64)
+  int odd_scale;  // scale <= 0
 };
 
 __device__ __forceinline__ float tl_max3(float a, float b, float c) {
@@ -377,6 +378,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
     const uint32_t pair = pair_bar(t * 4 + quarter);
     float *max_mine = max_s + (t * 2 + h) * TL_ROWS + r, *max_other = max_s + (t * 2 + (h ^ 1)) * TL_ROWS + r;
     uint32_t met = 0, s_count = 0, o_count = 0;
+    const float mult = g.odd_scale ? 1.f : g.a.scale_log2;
     bool ok = true;
     // the two warps of these rows: what either wrote before is read by the other after
     auto meet = [&]() -> bool {
@@ -407,28 +409,29 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         tmem_ld_32x32(ta, s0);
         tmem_ld_32x32(ta + 32u, s1);
         tmem_wait_ld();
-        const bool need_mask = kv0 + 63 > limit;
-        auto chunk_max = [&](const uint32_t (&v)[32], int k0, float mx) -> float {
-          if (need_mask) {
+        // Rare cases first, each in a branch of its own that whole warps take or leave, so that the common path is an addition, a
+        // power, a multiply-add and half a maximum and half a conversion per score.
+        if (g.odd_scale) {  // not positive: the maximum of the products is not the product of the maximum
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (k0 + e <= limit) mx = fmaxf(mx, __uint_as_float(v[e]) * g.a.scale_log2);
-            return mx;
+          for (int e = 0; e < 32; ++e) {
+            s0[e] = __float_as_uint(__uint_as_float(s0[e]) * g.a.scale_log2);
+            s1[e] = __float_as_uint(__uint_as_float(s1[e]) * g.a.scale_log2);
           }
-          float m0 = -INFINITY, m1 = -INFINITY;
-          if (g.a.scale_log2 >= 0.f) {
+        }
+        if (__any_sync(0xffffffffu, kv0 + 63 > limit)) {  // the diagonal, or the end: what a row does not see weighs nothing
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              m0 = tl_max3(m0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-              m1 = tl_max3(m1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-            }
-            return fmaxf(mx, fmaxf(m0, m1) * g.a.scale_log2);
+          for (int e = 0; e < 32; ++e) {
+            if (kv0 + e > limit) s0[e] = 0xff800000u;  // -infinity
+            if (kv0 + 32 + e > limit) s1[e] = 0xff800000u;
           }
+        }
+        float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) m0 = fmaxf(m0, __uint_as_float(v[e]) * g.a.scale_log2);
-          return fmaxf(mx, m0);
-        };
-        float mx = fmaxf(chunk_max(s0, kv0, -INFINITY), chunk_max(s1, kv0 + 32, -INFINITY));
+        for (int e = 0; e < 32; e += 2) {
+          m0 = tl_max3(m0, __uint_as_float(s0[e]), __uint_as_float(s0[e + 1]));
+          m1 = tl_max3(m1, __uint_as_float(s1[e]), __uint_as_float(s1[e + 1]));
+        }
+        float mx = fmaxf(m0, m1) * mult;
         // the other half of the row: its maximum over its 64 keys.  A slot is rewritten one block later, after the partner has
         // published the probabilities of this block, i.e. after it has read the slot.
         *max_mine = mx;
@@ -454,20 +457,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           }
         }
         // probabilities -> tensor memory, packed pairs over the first 32 of this thread's 64 S columns; row sum
-        float rs0 = 0.f, rs1 = 0.f;
+        float2 sum = make_float2(0.f, 0.f);
+        const float2 by = make_float2(mult, mult), less = make_float2(-m_new, -m_new);
         auto emit = [&](const uint32_t (&v)[32], int c) {  // c = first key (0 or 32) of these 32 values within the half row
           uint32_t packed[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float p0 = ap_ex2(fmaf(__uint_as_float(v[e]), g.a.scale_log2, -m_new));
-            float p1 = ap_ex2(fmaf(__uint_as_float(v[e + 1]), g.a.scale_log2, -m_new));
-            if (need_mask) {
-              if (kv0 + c + e > limit) p0 = 0.f;
-              if (kv0 + c + e + 1 > limit) p1 = 0.f;
-            }
-            rs0 += p0;
-            rs1 += p1;
-            packed[e >> 1] = ap_pack<BF>(p0, p1);
+            float2 x = __ffma2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), by, less);
+            x.x = ap_ex2(x.x);
+            x.y = ap_ex2(x.y);
+            sum = __fadd2_rn(sum, x);
+            packed[e >> 1] = ap_pack<BF>(x.x, x.y);
           }
           tmem_st_32x16(ta + (uint32_t)(c >> 1), packed);
         };
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(t));
-        l = fmaf(l, alpha, rs0 + rs1);
+        l = fmaf(l, alpha, sum.x + sum.y);
         m = m_next;
       }
       if (!ok) break;
@@ -555,6 +555,7 @@ int attention_paged_tile(const PagedAttnArgs &a, bool bf16, cudaStream_t s) {
   TileArgs g;
   g.a = a;
   g.per_tile = TL_ROWS / a.line.group;
+  g.odd_scale = !(a.scale_log2 > 0.f);
   g.box_log2 = a.batch.page_log2 < 6 ? a.batch.page_log2 : 6;
   CUtensorMap q, k, v;
   const usz q_dims[4] = {(usz)a.dh, (usz)a.line.group, (usz)a.batch.nt, (usz)a.line.nkvh};
