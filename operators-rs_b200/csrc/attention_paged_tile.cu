@@ -6,9 +6,11 @@
 // Tensor-bound: 4 dh flops a (query head, key) pair against 4 dh bytes a key that 256 query rows share.  The two products run on
 // tcgen05 with S, P and O in tensor memory, as in attention_fused.cu's two-tile kernel, whose arithmetic this one shares: a unit
 // is TWO tiles of 128 query rows, so that the tensor pipe runs one tile's products while the other tile's exponentials are in
-// flight; two threads per row; the reference point m follows the row maximum only when that has moved by 2^8 (lazy rescaling; the
+// flight; the reference point m follows the row maximum only when that has moved by 2^8 (lazy rescaling; the
 // factor cancels in o / l; the probabilities stay below 256, exact to half a step in the 16-bit operand that the second product
 // takes).  What a paged batch of ragged chunks changes:
+//   - A thread per row, a warp of each tile on every scheduler: a whole row's maximum needs no meeting of threads, and the first
+//     half of a block's probabilities feeds the second product while the other half's powers are taken.
 //   - A tile's rows are tokens x query heads of one kv head, token by token: a chunk of 33 tokens fills its rows whatever its
 //     length, and the heads of a group share every K and V block in shared memory.
 //   - K and V come page by page: a block of 128 keys is 128 / min(page, 64) boxes of a 4-d tensor map over the whole cache, each
@@ -20,8 +22,8 @@
 //     pause: the scheduler warp posts them ahead, K, V and Q of the next piece load and its first scores run while the softmax
 //     warps still write out the one before.
 //
-//   warp 0   Q and K producer        warps 4-11   softmax of tile 0, half a row a thread
-//   warp 1   tcgen05.mma issuer      warps 12-19  softmax of tile 1
+//   warp 0   Q and K producer        warps 4-7    softmax of tile 0, a row a thread
+//   warp 1   tcgen05.mma issuer      warps 8-11   softmax of tile 1
 //   warp 2   V producer; zeroes what lies behind the end of a sequence in its last block (within the time that the block in
 //            front takes the tensor pipe: the next stage is not free earlier)
 //   warp 3   scheduler
@@ -36,11 +38,11 @@ namespace ops {
 
 using namespace sm100;
 
-constexpr int TL_THREADS = 640;
+constexpr int TL_THREADS = 384;
 constexpr int TL_ROWS = 128;  // of a tile
 constexpr int TL_KEYS = AP_TILE_BLOCK;
 constexpr int TL_RING = 4;    // pieces posted ahead
-constexpr int TL_READERS = 19;  // warps that read the ring: all but the scheduler
+constexpr int TL_READERS = 11;  // warps that read the ring: all but the scheduler
 
 // A piece as the scheduler posts it.
 struct TilePiece {
@@ -63,12 +65,10 @@ template <int DH> struct TileSmem {
   static constexpr int OFF_K = OFF_Q + 2 * TILE;
   static constexpr int OFF_V = OFF_K + STAGES * TILE;
   static constexpr int OFF_BAR = OFF_V + STAGES * TILE;
-  static constexpr int NUM_BARS = 18 + 2 * TL_RING + 5 * STAGES;
+  static constexpr int NUM_BARS = 12 + 2 * TL_RING + 5 * STAGES;
   static constexpr int OFF_TMEM_SLOT = OFF_BAR + NUM_BARS * 8;
   static constexpr int OFF_RING = (OFF_TMEM_SLOT + 16 + 15) / 16 * 16;
-  static constexpr int OFF_MAX = (OFF_RING + TL_RING * (int)sizeof(TilePiece) + 15) / 16 * 16;  // [2 tiles][2 halves][128] f32
-  static constexpr int OFF_L = OFF_MAX + 4 * TL_ROWS * 4;
-  static constexpr int BYTES = OFF_L + 4 * TL_ROWS * 4 + 1024;  // 1024: alignment
+  static constexpr int BYTES = OFF_RING + TL_RING * (int)sizeof(TilePiece) + 1024;  // 1024: alignment
 };
 
 struct TileArgs {
@@ -97,21 +97,18 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   auto q_full = [&](int t) { return bar0 + 8u * (0 + t); };
   auto q_empty = [&](int t) { return bar0 + 8u * (2 + t); };    // last QK of the piece's tile done
   auto s_full = [&](int t) { return bar0 + 8u * (4 + t); };     // S complete (tensor pipe -> softmax)
-  auto p_full = [&](int t) { return bar0 + 8u * (6 + t); };     // P written, O rescaled if needed, the last piece's O read (softmax -> issuer)
-  auto o_final = [&](int t) { return bar0 + 8u * (8 + t); };    // last PV of the piece's tile done (tensor pipe -> softmax)
-  auto pair_bar = [&](int i) { return bar0 + 8u * (10 + i); };  // the two warps that share 32 rows of a tile
-  auto ring_full = [&](int i) { return bar0 + 8u * (18 + i); };
-  auto ring_empty = [&](int i) { return bar0 + 8u * (18 + TL_RING + i); };
-  auto k_full = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + s); };
-  auto k_empty = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + ST + s); };
-  auto v_full = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + 2 * ST + s); };
-  auto v_empty = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + 3 * ST + s); };
-  auto v_clean = [&](int s) { return bar0 + 8u * (18 + 2 * TL_RING + 4 * ST + s); };  // a stage's, so that no phase is overrun
+  auto p_full = [&](int t, int h) { return bar0 + 8u * (6 + 2 * t + h); };  // P of the h-th 64 keys written (softmax -> issuer)
+  auto o_final = [&](int t) { return bar0 + 8u * (10 + t); };   // last PV of the piece's tile done (tensor pipe -> softmax)
+  auto ring_full = [&](int i) { return bar0 + 8u * (12 + i); };
+  auto ring_empty = [&](int i) { return bar0 + 8u * (12 + TL_RING + i); };
+  auto k_full = [&](int s) { return bar0 + 8u * (12 + 2 * TL_RING + s); };
+  auto k_empty = [&](int s) { return bar0 + 8u * (12 + 2 * TL_RING + ST + s); };
+  auto v_full = [&](int s) { return bar0 + 8u * (12 + 2 * TL_RING + 2 * ST + s); };
+  auto v_empty = [&](int s) { return bar0 + 8u * (12 + 2 * TL_RING + 3 * ST + s); };
+  auto v_clean = [&](int s) { return bar0 + 8u * (12 + 2 * TL_RING + 4 * ST + s); };  // a stage's, so that no phase is overrun
   const uint32_t tmem_slot = base + Smem::OFF_TMEM_SLOT;
   uint32_t *tmem_slot_ptr = reinterpret_cast<uint32_t *>(base_ptr + Smem::OFF_TMEM_SLOT);
   volatile TilePiece *ring = reinterpret_cast<volatile TilePiece *>(base_ptr + Smem::OFF_RING);
-  float *max_s = reinterpret_cast<float *>(base_ptr + Smem::OFF_MAX);
-  float *l_s = reinterpret_cast<float *>(base_ptr + Smem::OFF_L);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedBatch &batch = g.a.batch;
@@ -127,10 +124,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       mbar_init(q_full(t), 1);
       mbar_init(q_empty(t), 1);
       mbar_init(s_full(t), 1);
-      mbar_init(p_full(t), 8);
+      mbar_init(p_full(t, 0), 4);
+      mbar_init(p_full(t, 1), 4);
       mbar_init(o_final(t), 1);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(pair_bar(i), 2);
     for (int i = 0; i < TL_RING; ++i) {
       mbar_init(ring_full(i), 1);
       mbar_init(ring_empty(i), TL_READERS);
@@ -160,13 +157,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot_ptr;
-  // tensor memory columns: S0 | S1 | O0 | O1, 128 each; the P of keys [64h, 64h+64) of a tile overwrites columns
-  // [64h, 64h+32) of its S (the first half of what the thread that wrote it had read)
+  // tensor memory columns: S0 | S1 | O0 | O1, 128 each; the P of a tile overwrites the first 64 columns of its S
   auto s_col = [&](int t) { return (uint32_t)(t * 128); };
   auto o_col = [&](int t) { return (uint32_t)(256 + t * 128); };
 
   if (warp < 4) {
-    setmaxnreg_dec<64>();
+    setmaxnreg_dec<88>();
     if (warp == 0 || warp == 2) {
       // ------------------------------------------------------------------ producers: one warp, a lane per box
       const bool keys = warp == 0;
@@ -290,18 +286,22 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
             const int s = c % ST;
             if (!mbar_wait(v_full(s), (c / ST) & 1u, status, 122)) return false;
             if (j == clean && !mbar_wait(v_clean(s), (cleaned >> s) & 1u, status, 123)) return false;
-            if (!mbar_wait(p_full(t), p_count[t] & 1u, status, 124)) return false;
-            ++p_count[t];
-            tc_fence_after();
             const uint32_t va = base + Smem::OFF_V + s * TILE;
             const uint32_t d = tmem_base + o_col(t);
             const uint32_t pa = tmem_base + s_col(t);
+            // the first 64 keys' products run while the others' powers are taken
 #pragma unroll
-            for (int ks = 0; ks < TL_KEYS / 16; ++ks) {
-              const uint64_t db = make_smem_desc_sw128(va + (ks >> 2) * (HALVES * 8192) + (ks & 3) * 2048, 8192, 1024);
-              // 16 keys = 8 packed columns; keys 64.. sit behind the second half row's S columns
-              umma_f16_ts(d, pa + (uint32_t)((ks >> 2) * 64 + (ks & 3) * 8), db, idesc_pv, (j != 0 || ks != 0) ? 1u : 0u);
+            for (int h = 0; h < 2; ++h) {
+              if (!mbar_wait(p_full(t, h), p_count[t] & 1u, status, 124)) return false;
+              tc_fence_after();
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4) {
+                const int ks = h * 4 + k4;
+                const uint64_t db = make_smem_desc_sw128(va + h * (HALVES * 8192) + k4 * 2048, 8192, 1024);
+                umma_f16_ts(d, pa + (uint32_t)(ks * 8), db, idesc_pv, (j != 0 || ks != 0) ? 1u : 0u);  // 16 keys = 8 packed columns
+              }
             }
+            ++p_count[t];
             if (j == (t ? n1 : n0) - 1) umma_commit(o_final(t));
             if (t == 1 || n1 == 0) umma_commit(v_empty(s));
             return true;
@@ -366,164 +366,150 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       }
     }
   } else {
-    // ------------------------------------------------------------------ softmax, rescaling, output: two threads per q row
-    setmaxnreg_inc<104>();
-    const int idx = warp - 4;
-    const int t = idx >> 3;          // q tile
-    const int h = (idx >> 2) & 1;    // which 64 keys of a block, and which half of O's columns
-    const int quarter = idx & 3;     // = warp & 3: tensor-memory lanes [32 * quarter, +32)
+    // ------------------------------------------------------------------ softmax, rescaling, output: a thread per q row
+    setmaxnreg_inc<208>();
+    const int t = (warp - 4) >> 2;   // q tile
+    const int quarter = warp & 3;    // tensor-memory lanes [32 * quarter, +32)
     const int r = quarter * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const int tok = r / group, gi = r - tok * group;
-    const uint32_t pair = pair_bar(t * 4 + quarter);
-    float *max_mine = max_s + (t * 2 + h) * TL_ROWS + r, *max_other = max_s + (t * 2 + (h ^ 1)) * TL_ROWS + r;
-    uint32_t met = 0, s_count = 0, o_count = 0;
+    const int tok = paged_div(r, group), gi = r - tok * group;
+    const uint32_t ta = tmem_base + lane_addr + s_col(t), to = tmem_base + lane_addr + o_col(t);
     const float mult = g.odd_scale ? 1.f : g.a.scale_log2;
+    uint32_t s_count = 0, o_count = 0;
     bool ok = true;
-    // the two warps of these rows: what either wrote before is read by the other after
-    auto meet = [&]() -> bool {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(pair);
-      return mbar_wait(pair, met++ & 1u, status, 140);
-    };
+#pragma unroll 1
     for (uint32_t i = 0; ok; ++i) {
       const int slot = i % TL_RING;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(ring_full(slot), (i / TL_RING) & 1u, status, 141)))) break;
       volatile TilePiece &p = ring[slot];
-      const int valid = p.valid, nblk = p.blocks[t], lo = p.lo, park = p.park;
+      if (!p.valid) break;
+      const int nblk = p.blocks[t];
       const int mine = t * g.per_tile + tok;  // token of the unit
-      const bool there = tok < g.per_tile && mine < p.tokens;
       const int limit = line.causal ? min(p.len - 1, p.off + mine) : p.len - 1;  // last slot this row may see
-      const long long row = p.row + mine;
-      const int q_head = p.head * group + gi;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ring_empty(slot));
-      if (!valid) break;
+      int kv0 = p.lo * TL_KEYS;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < nblk && ok; ++j) {
-        const int kv0 = (lo + j) * TL_KEYS + h * 64;
+#pragma unroll 1
+      for (int j = 0; j < nblk; ++j, kv0 += TL_KEYS) {
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), s_count++ & 1u, status, 142)))) break;
         tc_fence_after();
-        const uint32_t ta = tmem_base + lane_addr + s_col(t) + (uint32_t)(h * 64);
-        uint32_t s0[32], s1[32];
-        tmem_ld_32x32(ta, s0);
-        tmem_ld_32x32(ta + 32u, s1);
+        uint32_t x[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld_32x32(ta + 32u * q, x[q]);
         tmem_wait_ld();
         // Rare cases first, each in a branch of its own that whole warps take or leave, so that the common path is an addition, a
         // power, a multiply-add and half a maximum and half a conversion per score.
         if (g.odd_scale) {  // not positive: the maximum of the products is not the product of the maximum
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            s0[e] = __float_as_uint(__uint_as_float(s0[e]) * g.a.scale_log2);
-            s1[e] = __float_as_uint(__uint_as_float(s1[e]) * g.a.scale_log2);
-          }
-        }
-        if (__any_sync(0xffffffffu, kv0 + 63 > limit)) {  // the diagonal, or the end: what a row does not see weighs nothing
+          for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if (kv0 + e > limit) s0[e] = 0xff800000u;  // -infinity
-            if (kv0 + 32 + e > limit) s1[e] = 0xff800000u;
-          }
+            for (int e = 0; e < 32; ++e) x[q][e] = __float_as_uint(__uint_as_float(x[q][e]) * g.a.scale_log2);
         }
-        float m0 = -INFINITY, m1 = -INFINITY;
+        if (__any_sync(0xffffffffu, kv0 + TL_KEYS - 1 > limit)) {  // the diagonal, or the end: what a row does not see weighs nothing
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          m0 = tl_max3(m0, __uint_as_float(s0[e]), __uint_as_float(s0[e + 1]));
-          m1 = tl_max3(m1, __uint_as_float(s1[e]), __uint_as_float(s1[e + 1]));
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (kv0 + q * 32 + e > limit) x[q][e] = 0xff800000u;  // -infinity
         }
-        float mx = fmaxf(m0, m1) * mult;
-        // the other half of the row: its maximum over its 64 keys.  A slot is rewritten one block later, after the partner has
-        // published the probabilities of this block, i.e. after it has read the slot.
-        *max_mine = mx;
-        if (!(ok = __all_sync(0xffffffffu, meet()))) break;
-        mx = fmaxf(mx, *max_other);
-        const float m_raw = fmaxf(m, mx);
+        float mx[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          mx[q] = __uint_as_float(x[q][0]);
+#pragma unroll
+          for (int e = 1; e < 31; e += 2) mx[q] = tl_max3(mx[q], __uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1]));
+          mx[q] = fmaxf(mx[q], __uint_as_float(x[q][31]));
+        }
+        // Lazy rescaling: the reference point m of the powers follows the row maximum only when that has moved by more than 2^8.
+        // Until then the probabilities are taken relative to the older, smaller m: they stay below 256, exact to half a step in
+        // the 16-bit operand, and the f32 row sum and O carry the same factor, which cancels in o = O / l.
+        const float m_raw = fmaxf(m, fmaxf(tl_max3(mx[0], mx[1], mx[2]), mx[3]) * mult);
         const bool move = m_raw > m + 8.f;                       // also true on the first block (m = -inf)
         const float m_next = move ? m_raw : m;
         const float m_new = m_next == -INFINITY ? 0.f : m_next;  // a row with nothing visible yet: keep the arithmetic finite
-        const float alpha = move ? ap_ex2(m - m_new) : 1.f;      // 0 on the first block
-        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          // some row maximum of these 32 rows moved: rescale this thread's columns of O.  S of block j being complete says that
-          // PV of block j-1 has completed too (the tensor pipe retires in order), so O is stable.
-          const uint32_t to = tmem_base + lane_addr + o_col(t) + (uint32_t)(h * (DH / 2));
+        if (__any_sync(0xffffffffu, move)) {
+          const float alpha = move ? ap_ex2(m - m_new) : 1.f;    // 0 on the first block
+          l *= alpha;
+          if (j > 0) {
+            // S of block j being complete says that PV of block j-1 has completed too (the tensor pipe retires in order): O is stable
 #pragma unroll 1
-          for (int c = 0; c < DH / 2; c += 16) {
-            uint32_t v[16];
-            tmem_ld_32x16(to + (uint32_t)c, v);
-            tmem_wait_ld();
+            for (int c = 0; c < DH; c += 16) {
+              uint32_t v[16];
+              tmem_ld_32x16(to + (uint32_t)c, v);
+              tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-            tmem_st_32x16(to + (uint32_t)c, v);
+              for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+              tmem_st_32x16(to + (uint32_t)c, v);
+            }
           }
         }
-        // probabilities -> tensor memory, packed pairs over the first 32 of this thread's 64 S columns; row sum
+        m = m_next;
+        // probabilities -> tensor memory as packed pairs, in two halves; row sum
         float2 sum = make_float2(0.f, 0.f);
         const float2 by = make_float2(mult, mult), less = make_float2(-m_new, -m_new);
-        auto emit = [&](const uint32_t (&v)[32], int c) {  // c = first key (0 or 32) of these 32 values within the half row
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
           uint32_t packed[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float2 x = __ffma2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), by, less);
-            x.x = ap_ex2(x.x);
-            x.y = ap_ex2(x.y);
-            sum = __fadd2_rn(sum, x);
-            packed[e >> 1] = ap_pack<BF>(x.x, x.y);
+            float2 y = __ffma2_rn(make_float2(__uint_as_float(x[q][e]), __uint_as_float(x[q][e + 1])), by, less);
+            y.x = ap_ex2(y.x);
+            y.y = ap_ex2(y.y);
+            sum = __fadd2_rn(sum, y);
+            packed[e >> 1] = ap_pack<BF>(y.x, y.y);
           }
-          tmem_st_32x16(ta + (uint32_t)(c >> 1), packed);
-        };
-        emit(s0, 0);
-        emit(s1, 32);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(t));
-        l = fmaf(l, alpha, sum.x + sum.y);
-        m = m_next;
+          tmem_st_32x16(ta + 16u * q, packed);
+          if (q & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(t, q >> 1));
+          }
+        }
+        l += sum.x + sum.y;
       }
       if (!ok) break;
-      // whole-row sum: both halves carry the same reference point
-      l_s[(t * 2 + h) * TL_ROWS + r] = l;
-      if (!(ok = __all_sync(0xffffffffu, meet()))) break;
-      l += l_s[(t * 2 + (h ^ 1)) * TL_ROWS + r];
+      const bool there = tok < g.per_tile && mine < p.tokens;
+      const int park = p.park;
+      const long long row = p.row + mine;
+      const int q_head = p.head * group + gi;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ring_empty(slot));
+      float *parked = g.a.parts + ((long long)park * (2 * TL_ROWS) + t * TL_ROWS + r) * (DH + AP_PAD);
       if (nblk == 0) {  // the tile has no block in this part of the unit, or no token at all
-        if (park >= 0 && h == 0)
-          *reinterpret_cast<float2 *>(g.a.parts + ((long long)park * (2 * TL_ROWS) + t * TL_ROWS + r) * (DH + AP_PAD) + DH) = make_float2(-INFINITY, 0.f);
+        if (park >= 0) *reinterpret_cast<float2 *>(parked + DH) = make_float2(-INFINITY, 0.f);
         continue;
       }
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_final(t), o_count++ & 1u, status, 143)))) break;
       tc_fence_after();
-      const uint32_t to = tmem_base + lane_addr + o_col(t) + (uint32_t)(h * (DH / 2));
       if (park >= 0) {
         // one part of several: park the unnormalised O with its reference point and row sum
-        float *prow = g.a.parts + ((long long)park * (2 * TL_ROWS) + t * TL_ROWS + r) * (DH + AP_PAD);
-        if (there && h == 0) *reinterpret_cast<float2 *>(prow + DH) = make_float2(m, l);
+        if (there) *reinterpret_cast<float2 *>(parked + DH) = make_float2(m, l);
 #pragma unroll 1
-        for (int c = 0; c < DH / 2; c += 16) {
-          uint32_t v[16];
-          tmem_ld_32x16(to + (uint32_t)c, v);
+        for (int c = 0; c < DH; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32(to + (uint32_t)c, v);
           tmem_wait_ld();
           if (there)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4 *>(prow + h * (DH / 2) + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(parked + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
         }
       } else {
         const float inv = l > 0.f ? __frcp_rn(l) : 0.f;  // a row that sees nothing: zeros
         char *orow = g.a.o + row * g.a.o_t + (long long)q_head * g.a.o_h;
 #pragma unroll 1
-        for (int c = 0; c < DH / 2; c += 16) {
-          uint32_t v[16];
-          tmem_ld_32x16(to + (uint32_t)c, v);
+        for (int c = 0; c < DH; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32(to + (uint32_t)c, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; e += 8) {
-            const int col = h * (DH / 2) + c + e;
-            if (there && col < g.a.dh) {
+          for (int e = 0; e < 32; e += 8) {
+            if (there && c + e < g.a.dh) {
               uint4 out;
               out.x = ap_pack<BF>(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
               out.y = ap_pack<BF>(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
               out.z = ap_pack<BF>(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv);
               out.w = ap_pack<BF>(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv);
-              st_global_16(orow + col * 2, out);
+              st_global_16(orow + (c + e) * 2, out);
             }
           }
         }
