@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   uint32_t *tmem_slot_ptr = reinterpret_cast<uint32_t *>(base_ptr + Smem::OFF_TMEM_SLOT);
   volatile TilePiece *ring = reinterpret_cast<volatile TilePiece *>(base_ptr + Smem::OFF_RING);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // known to be uniform
   const PagedBatch &batch = g.a.batch;
   const PagedLine &line = g.a.line;
   const int group = line.group;
@@ -248,67 +248,72 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       if (!ok) gave_up = 1;
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMA issuer
-      if (lane == 0) {
+      // the whole warp walks along, one lane issues
+      {
+        const uint32_t leader = elect_one() ? 1u : 0u;
         const uint32_t idesc_qk = make_idesc_f16(TL_ROWS, TL_KEYS, 0, 0, BF ? 1 : 0);
         const uint32_t idesc_pv = make_idesc_f16(TL_ROWS, DH, 0, 1, BF ? 1 : 0);
+        // a descriptor's address is its low bits, in 16 bytes: adding steps to one made once keeps the issue of an MMA short
+        const uint64_t q_desc = make_smem_desc_sw128(base + Smem::OFF_Q, 16, 1024), k_desc = make_smem_desc_sw128(base + Smem::OFF_K, 16, 1024);
+        const uint64_t v_desc = make_smem_desc_sw128(base + Smem::OFF_V, 8192, 1024);
+        auto all_wait = [&](uint32_t bar, uint32_t parity, int code) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code)); };
         uint32_t count = 0, cleaned = 0 /* a bit per stage */, q_count[2] = {0, 0}, p_count[2] = {0, 0};
         bool ok = true;
         for (uint32_t i = 0; ok; ++i) {
           const int slot = i % TL_RING;
-          if (!(ok = mbar_wait(ring_full(slot), (i / TL_RING) & 1u, status, 120))) break;
+          if (!(ok = all_wait(ring_full(slot), (i / TL_RING) & 1u, 120))) break;
           volatile TilePiece &p = ring[slot];
-          const int valid = p.valid, blocks = p.hi - p.lo, clean = p.clean;
-          const int n0 = p.blocks[0], n1 = p.blocks[1];
-          mbar_arrive(ring_empty(slot));
+          auto uniform = [&](int v) -> int { return __shfl_sync(0xffffffffu, v, 0); };
+          const int valid = uniform(p.valid), blocks = uniform(p.hi - p.lo), clean = uniform(p.clean);
+          const int n0 = uniform(p.blocks[0]), n1 = uniform(p.blocks[1]);
+          if (lane == 0) mbar_arrive(ring_empty(slot));
           if (!valid) break;
           // S(t) = Q(t) K_j^T.  Tile 1 sees every block that tile 0 sees, if it is there at all.
           auto issue_qk = [&](int t, int j) -> bool {
             const uint32_t c = count + (uint32_t)j;
             const int s = c % ST;
-            if (!mbar_wait(k_full(s), (c / ST) & 1u, status, 121)) return false;
+            if (!all_wait(k_full(s), (c / ST) & 1u, 121)) return false;
             tc_fence_after();
-            const uint32_t qa = base + Smem::OFF_Q + t * TILE, ka = base + Smem::OFF_K + s * TILE;
+            const uint64_t da = q_desc + (uint32_t)(t * (TILE >> 4)), db = k_desc + (uint32_t)(s * (TILE >> 4));
             const uint32_t d = tmem_base + s_col(t);
 #pragma unroll
             for (int ks = 0; ks < DH / 16; ++ks) {
-              const uint64_t da = make_smem_desc_sw128(qa + (ks >> 2) * (TL_ROWS * 128) + (ks & 3) * 32, 16, 1024);
-              const uint64_t db = make_smem_desc_sw128(ka + (ks >> 2) * (TL_KEYS * 128) + (ks & 3) * 32, 16, 1024);
-              umma_f16_ss(d, da, db, idesc_qk, ks != 0 ? 1u : 0u);
+              const uint32_t step = (ks >> 2) * (TL_ROWS * 128 >> 4) + (ks & 3) * 2;  // rows of Q and keys of a block are as many
+              umma_f16_ss_by(leader, d, da + step, db + step, idesc_qk, ks != 0 ? 1u : 0u);
             }
-            umma_commit(s_full(t));
-            if (t == 1 || n1 == 0) umma_commit(k_empty(s));
-            if (j == (t ? n1 : n0) - 1) umma_commit(q_empty(t));
+            umma_commit_by(leader, s_full(t));
+            if (t == 1 || n1 == 0) umma_commit_by(leader, k_empty(s));
+            if (j == (t ? n1 : n0) - 1) umma_commit_by(leader, q_empty(t));
             return true;
           };
           // O(t) (+)= P(t) V_j, P from tensor memory
           auto issue_pv = [&](int t, int j) -> bool {
             const uint32_t c = count + (uint32_t)j;
             const int s = c % ST;
-            if (!mbar_wait(v_full(s), (c / ST) & 1u, status, 122)) return false;
-            if (j == clean && !mbar_wait(v_clean(s), (cleaned >> s) & 1u, status, 123)) return false;
-            const uint32_t va = base + Smem::OFF_V + s * TILE;
+            if (!all_wait(v_full(s), (c / ST) & 1u, 122)) return false;
+            if (j == clean && !all_wait(v_clean(s), (cleaned >> s) & 1u, 123)) return false;
+            const uint64_t db = v_desc + (uint32_t)(s * (TILE >> 4));
             const uint32_t d = tmem_base + o_col(t);
             const uint32_t pa = tmem_base + s_col(t);
             // the first 64 keys' products run while the others' powers are taken
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (!mbar_wait(p_full(t, h), p_count[t] & 1u, status, 124)) return false;
+              if (!all_wait(p_full(t, h), p_count[t] & 1u, 124)) return false;
               tc_fence_after();
 #pragma unroll
               for (int k4 = 0; k4 < 4; ++k4) {
                 const int ks = h * 4 + k4;
-                const uint64_t db = make_smem_desc_sw128(va + h * (HALVES * 8192) + k4 * 2048, 8192, 1024);
-                umma_f16_ts(d, pa + (uint32_t)(ks * 8), db, idesc_pv, (j != 0 || ks != 0) ? 1u : 0u);  // 16 keys = 8 packed columns
+                umma_f16_ts_by(leader, d, pa + (uint32_t)(ks * 8), db + (uint32_t)((h * (HALVES * 8192) + k4 * 2048) >> 4), idesc_pv, (j != 0 || ks != 0) ? 1u : 0u);  // 16 keys = 8 packed columns
               }
             }
             ++p_count[t];
-            if (j == (t ? n1 : n0) - 1) umma_commit(o_final(t));
-            if (t == 1 || n1 == 0) umma_commit(v_empty(s));
+            if (j == (t ? n1 : n0) - 1) umma_commit_by(leader, o_final(t));
+            if (t == 1 || n1 == 0) umma_commit_by(leader, v_empty(s));
             return true;
           };
           for (int t = 0; t < 2 && ok; ++t) {
             if ((t ? n1 : n0) == 0) continue;
-            ok = mbar_wait(q_full(t), q_count[t] & 1u, status, 125) && issue_qk(t, 0);
+            ok = all_wait(q_full(t), q_count[t] & 1u, 125) && issue_qk(t, 0);
             ++q_count[t];
           }
           for (int j = 0; j < blocks && ok; ++j)
