@@ -267,7 +267,7 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
     p.tile.rows_hi = 0x7fffffff;
     p.tile.tokens = AP_TILE_ROWS / 2 / (int)group * 2;
     p.tile.block_log2 = AP_TILE_BLOCK_LOG2;
-    line_scale(&p.tile, nt, nseq, slots, 256, 512);
+    line_scale(&p.tile, nt, nseq, slots, 512, 512);
     p.tile.ctas = std::min(base.sm_count, AP_MAX_CTAS);
     p.tile_joins = up256(sizeof(PagedJoin) * (usz)p.tile.ctas);
     p.tile_parts = up256(2 * (usz)p.tile.ctas * AP_TILE_ROWS * (p.part_dh + AP_PAD) * sizeof(float));
@@ -339,20 +339,9 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   tile.joins = (PagedJoin *)(at + plan.few_joins + plan.few_parts);
   tile.parts = (float *)(at + plan.few_joins + plan.few_parts + plan.tile_joins);
   if (plan.few.ctas) OPS_TRY(attention_paged_few(few, plan.few_rows, bf16, s));
-  if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, s));
-  if (plan.few.ctas + plan.tile.ctas) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(JOIN_BLOCKS_PER_SM * base.sm_count));
-    cfg.blockDim = dim3(JOIN_THREADS);
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cudaError_t e = bf16 ? cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<true>, few, tile, plan.few_rows, plan.part_dh)
-                         : cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<false>, few, tile, plan.few_rows, plan.part_dh);
-    if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: launch of the joining kernel failed: %s", cudaGetErrorString(e));
-  }
+  if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, plan.few.ctas != 0, s));
+  if (plan.few.ctas + plan.tile.ctas)
+    return ap_launch_beside("attention_paged(join)", bf16 ? attention_paged_join_kernel<true> : attention_paged_join_kernel<false>,
+                            JOIN_BLOCKS_PER_SM * base.sm_count, JOIN_THREADS, 0, s, true, few, tile, plan.few_rows, plan.part_dh);
   return OPS_OK;
 }

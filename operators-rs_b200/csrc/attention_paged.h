@@ -40,7 +40,8 @@ int attention_paged_maps(const PagedAttnArgs &a, bool bf16, uint32_t rows, CUten
 bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2);
 int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, cudaStream_t s);
 int attention_paged_few_ctas(const OpBase &base);
-int attention_paged_tile(const PagedAttnArgs &a, bool bf16, cudaStream_t s);
+// beside: it may start while the launch in front of it, the few-rows kernel's, still runs; it ends behind it all the same.
+int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool beside, cudaStream_t s);
 constexpr int AP_FEW_BLOCK_LOG2 = 5, AP_FEW_BLOCK = 32, AP_TILE_BLOCK_LOG2 = 7, AP_TILE_BLOCK = 128;  // keys of a block
 constexpr int AP_TILE_ROWS = 256;                       // query rows of a unit of the tile kernel: two tiles
 
@@ -132,6 +133,26 @@ __device__ __forceinline__ void paged_note_join(const PagedAttnArgs &a, int cta,
 // may come, the other waits for all of its results.
 __device__ __forceinline__ void pdl_let_next_come() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_for_front() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+#endif
+
+#ifdef __CUDACC__
+// A launch, with `beside` one that may start while the one in front of it in the stream still runs.
+template <class Kernel, class... Args>
+int ap_launch_beside(const char *what, Kernel kernel, int grid, int block, int bytes, cudaStream_t s, bool beside, const Args &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = (size_t)bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = beside ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "%s: %s", what, cudaGetErrorString(e));
+  return OPS_OK;
+}
 #endif
 
 }  // namespace ops

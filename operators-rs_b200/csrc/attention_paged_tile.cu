@@ -68,7 +68,8 @@ template <int DH> struct TileSmem {
   static constexpr int NUM_BARS = 12 + 2 * TL_RING + 5 * STAGES;
   static constexpr int OFF_TMEM_SLOT = OFF_BAR + NUM_BARS * 8;
   static constexpr int OFF_RING = (OFF_TMEM_SLOT + 16 + 15) / 16 * 16;
-  static constexpr int BYTES = OFF_RING + TL_RING * (int)sizeof(TilePiece) + 1024;  // 1024: alignment
+  static constexpr int OFF_STAGE = (OFF_RING + TL_RING * (int)sizeof(TilePiece) + 15) / 16 * 16;  // 4 KB a softmax warp: 32 rows x 128 B
+  static constexpr int BYTES = OFF_STAGE + 8 * 4096 + 1024;  // 1024: alignment
 };
 
 struct TileArgs {
@@ -486,37 +487,59 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       }
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_final(t), o_count++ & 1u, status, 143)))) break;
       tc_fence_after();
+      // A row is one thread's, 512 or 256 bytes of it: written as it is, every store of a warp would touch 32 lines.  128 bytes of
+      // the warp's 32 rows at a time turn in shared memory instead, 16-byte pieces swizzled by the row, and leave as whole lines
+      // (a piece's end 5000 -> 1900 cycles).
+      uint8_t *stage = base_ptr + Smem::OFF_STAGE + (warp - 4) * 4096;
+      auto turn = [&](int e, uint4 v) { *reinterpret_cast<uint4 *>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) = v; };  // e-th piece of the own row
+      auto leave = [&](auto &&address) {  // address(row of the warp, piece) -> where it goes, or null
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int rr = k * 4 + (lane >> 3), e = lane & 7;
+          const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * 128 + ((e ^ (rr & 7)) << 4));
+          if (char *where = address(rr, e)) st_global_16(where, v);
+        }
+        __syncwarp();
+      };
       if (park >= 0) {
-        // one part of several: park the unnormalised O with its reference point and row sum
-        if (there) *reinterpret_cast<float2 *>(parked + DH) = make_float2(m, l);
+        // one part of several: park the unnormalised O with its reference point and row sum (rows that are not there too: in bounds
+        // and never read)
+        *reinterpret_cast<float2 *>(parked + DH) = make_float2(m, l);
+        char *warp_rows = reinterpret_cast<char *>(parked) - (long long)lane * ((DH + AP_PAD) * 4);
 #pragma unroll 1
         for (int c = 0; c < DH; c += 32) {
           uint32_t v[32];
           tmem_ld_32x32(to + (uint32_t)c, v);
           tmem_wait_ld();
-          if (there)
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(parked + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          for (int e = 0; e < 8; ++e) turn(e, make_uint4(v[e * 4], v[e * 4 + 1], v[e * 4 + 2], v[e * 4 + 3]));
+          leave([&](int rr, int e) { return warp_rows + (long long)rr * ((DH + AP_PAD) * 4) + c * 4 + e * 16; });
         }
       } else {
         const float inv = l > 0.f ? __frcp_rn(l) : 0.f;  // a row that sees nothing: zeros
-        char *orow = g.a.o + row * g.a.o_t + (long long)q_head * g.a.o_h;
+        char *orow = there ? g.a.o + row * g.a.o_t + (long long)q_head * g.a.o_h : nullptr;
 #pragma unroll 1
-        for (int c = 0; c < DH; c += 32) {
-          uint32_t v[32];
-          tmem_ld_32x32(to + (uint32_t)c, v);
-          tmem_wait_ld();
+        for (int c = 0; c < DH; c += 64) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (there && c + e < g.a.dh) {
+          for (int half = 0; half < 2; ++half) {
+            uint32_t v[32];
+            tmem_ld_32x32(to + (uint32_t)(c + half * 32), v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
               uint4 out;
               out.x = ap_pack<BF>(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
               out.y = ap_pack<BF>(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
               out.z = ap_pack<BF>(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv);
               out.w = ap_pack<BF>(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv);
-              st_global_16(orow + (c + e) * 2, out);
+              turn(half * 4 + e / 8, out);
             }
           }
+          leave([&](int rr, int e) -> char * {
+            char *whose = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), rr));
+            return whose && c + e * 8 < g.a.dh ? whose + (c + e * 8) * 2 : nullptr;
+          });
         }
       }
       tc_fence_before();  // the next P of this tile says that O has been read
@@ -524,6 +547,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
     if (!ok) gave_up = 1;
   }
 
+  if (warp == 3) pdl_wait_for_front();  // the few-rows kernel, beside which this one started, has ended when this one has
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -534,15 +558,14 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
 }
 
 template <int DH, bool BF>
-static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
+static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, bool beside, cudaStream_t s) {
   const int bytes = TileSmem<DH>::BYTES;
   cudaError_t e = cudaFuncSetAttribute(attention_paged_tile_kernel<DH, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
-  attention_paged_tile_kernel<DH, BF><<<g.a.line.ctas, TL_THREADS, bytes, s>>>(q, k, v, g);
-  return check_launch("attention_paged(tiles)");
+  return ap_launch_beside("attention_paged(tiles)", attention_paged_tile_kernel<DH, BF>, g.a.line.ctas, TL_THREADS, bytes, s, beside, q, k, v, g);
 }
 
-int attention_paged_tile(const PagedAttnArgs &a, bool bf16, cudaStream_t s) {
+int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool beside, cudaStream_t s) {
   TileArgs g;
   g.a = a;
   g.per_tile = TL_ROWS / a.line.group;
@@ -554,8 +577,8 @@ int attention_paged_tile(const PagedAttnArgs &a, bool bf16, cudaStream_t s) {
   if (!ap_encode(&q, bf16, a.q, q_dims, q_st, (uint32_t)a.line.group, (uint32_t)g.per_tile))
     return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
   OPS_TRY(attention_paged_maps(a, bf16, 1u << g.box_log2, &k, &v));
-  if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, s) : tile_launch<64, false>(g, q, k, v, s);
-  return bf16 ? tile_launch<128, true>(g, q, k, v, s) : tile_launch<128, false>(g, q, k, v, s);
+  if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, beside, s) : tile_launch<64, false>(g, q, k, v, beside, s);
+  return bf16 ? tile_launch<128, true>(g, q, k, v, beside, s) : tile_launch<128, false>(g, q, k, v, beside, s);
 }
 
 }  // namespace ops
