@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_BLOCKS_PER_SM)
     if (j < records) {
       const PagedJoin rec = j < few.line.ctas ? few.joins[j] : tile.joins[j - few.line.ctas];
       joins[j] = rec;
-      if (rec.ctas) mine = paged_div(rec.tokens * group + JOIN_ROWS - 1, JOIN_ROWS);
+      if (rec.ctas) mine = (rec.tokens * group + JOIN_ROWS - 1) / JOIN_ROWS;
     }
     int upto = mine;
 #pragma unroll
@@ -69,12 +69,12 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_BLOCKS_PER_SM)
     const PagedJoin &j = joins[lo];
     const int first = on_tile ? lo - few.line.ctas : lo;
     const int row0 = (item - first_item[lo]) * JOIN_ROWS, here = min(JOIN_ROWS, j.tokens * group - row0);
-    const int share = paged_div(JOIN_WARPS, here);  // warps per row
-    const int own = paged_div(warp, share), part = warp - own * share;
+    const int share = here > 8 ? 1 : here > 5 ? 2 : here > 4 ? 3 : here > 3 ? 4 : here > 2 ? 5 : here > 1 ? 8 : 16;  // JOIN_WARPS / here warps per row
+    const int own = paged_guess((float)warp + 0.5f, (float)share), part = warp - own * share;  // warp / share
     const int r = row0 + own;
     // where the row lies in a parked unit: tiles of 128 rows, whole tokens each
-    const int tok = paged_div(r, group), gi = r - tok * group;
-    const int per_tile = on_tile ? tile.line.tokens / 2 : JOIN_ROWS, t = paged_div(tok, per_tile);
+    const int tok = paged_div(r, few.line.by_group), gi = r - tok * group;
+    const int per_tile = on_tile ? tile.line.tokens / 2 : JOIN_ROWS, t = tok >= per_tile;
     const int parked = t * (AP_TILE_ROWS / 2) + (tok - t * per_tile) * group + gi;
     const long long ld = part_dh + AP_PAD, unit = (long long)(on_tile ? AP_TILE_ROWS : few_rows) * ld;
     float m = -INFINITY, l = 0.f;
@@ -233,7 +233,11 @@ static void line_scale(PagedLine *l, usz nt, usz nseq, usz slots, int overhead, 
   l->shift = 0;
   while (l->shift < 30 && units * (std::ldexp(keys, -l->shift) + 4.0) > 2147483647.0) ++l->shift;
   l->overhead = std::max(1, overhead >> l->shift);
-  l->min_share = std::max(1, min_share >> l->shift);
+  l->min_share = std::max(1, min_share >> l->shift);  // a power of two
+  l->min_share_log2 = 0;
+  while ((1 << l->min_share_log2) < l->min_share) ++l->min_share_log2;
+  l->by_tokens = paged_div_by((uint32_t)l->tokens);
+  l->by_ctas = paged_div_by((uint32_t)l->ctas);
 }
 
 static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, usz dh, bool causal, uint32_t max_seq, usz nt, usz nseq, usz slots) {
@@ -247,6 +251,7 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
   memset(&l, 0, sizeof(l));
   l.nkvh = (int)nkvh;
   l.group = (int)group;
+  l.by_group = paged_div_by((uint32_t)group);
   l.causal = causal;
   l.max_seq = max_seq > 0x7fffffffu ? 0x7fffffff : (int)max_seq;
   p.few = p.tile = l;
@@ -255,8 +260,8 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
     p.few.rows_hi = p.few_rows;
     p.few.tokens = p.few_rows;
     p.few.block_log2 = AP_FEW_BLOCK_LOG2;
-    line_scale(&p.few, nt, nseq, slots, 128, 128);
     p.few.ctas = std::min(attention_paged_few_ctas(base), AP_MAX_CTAS);
+    line_scale(&p.few, nt, nseq, slots, 128, 128);
     p.few_joins = up256(sizeof(PagedJoin) * (usz)p.few.ctas);
     p.few_parts = up256(2 * (usz)p.few.ctas * p.few_rows * (p.part_dh + AP_PAD) * sizeof(float));
     p.tile.rows_lo = p.few_rows + 1;
@@ -267,8 +272,8 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
     p.tile.rows_hi = 0x7fffffff;
     p.tile.tokens = AP_TILE_ROWS / 2 / (int)group * 2;
     p.tile.block_log2 = AP_TILE_BLOCK_LOG2;
-    line_scale(&p.tile, nt, nseq, slots, 512, 512);
     p.tile.ctas = std::min(base.sm_count, AP_MAX_CTAS);
+    line_scale(&p.tile, nt, nseq, slots, 512, 512);
     p.tile_joins = up256(sizeof(PagedJoin) * (usz)p.tile.ctas);
     p.tile_parts = up256(2 * (usz)p.tile.ctas * AP_TILE_ROWS * (p.part_dh + AP_PAD) * sizeof(float));
   }

@@ -75,15 +75,14 @@ __device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLin
   long long sum = 0, cost = 0;
 #pragma unroll 1
   for (int i = lane; i < b.nseq; i += 32) sum += cost = paged_cost(b, l, i, report);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  // (a lane's sum stays below 2^47: 2^16 sequences of 2^31 points; its halves add up in 32 bits)
+  sum = (long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum & 0xffffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum >> 24)) << 24);
   // sequences that share rows (seq_start falls) can put more on the line than the host allowed for: nothing is done then
   const int total = sum <= 0x7fffffff ? (int)sum : 0;
   if (report && total != sum && lane == 0) atomicCAS(b.status, 0, OPS_PAGED_BAD_ROWS);
   *total_out = total;
-  const int active = paged_active(l, total);
-  if (total == 0 || cta >= active) return;
-  const int lo = paged_cut(total, active, cta);
+  const int lo = paged_cut(l, total, cta), hi = paged_cut(l, total, cta + 1);
+  if (lo >= hi) return;
   int before = 0;
 #pragma unroll 1
   for (int i0 = 0; i0 < b.nseq; i0 += 32) {
@@ -106,7 +105,7 @@ __device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLin
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
   walk->at = lo;
-  walk->end = paged_cut(total, active, cta + 1);
+  walk->end = hi;
 }
 
 // By one thread.
@@ -121,7 +120,7 @@ __device__ __forceinline__ void paged_note_join(const PagedAttnArgs &a, int cta,
   memset(&j, 0, sizeof(j));
   j.front = front;
   if (last.seq >= 0 && last.lo == 0 && last.hi < last.blocks) {
-    j.ctas = paged_first_behind(total, paged_active(a.line, total), last.begin + last.cost) - cta;
+    j.ctas = paged_first_behind(a.line, total, last.begin + last.cost) - cta;
     j.row = last.s.row + last.tile * a.line.tokens;
     j.tokens = min(a.line.tokens, last.s.n - last.tile * a.line.tokens);
     j.head = last.head;

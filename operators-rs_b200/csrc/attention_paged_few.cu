@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < Q_VECS; ++e) {
           const int at = e * 32 + lane, qr = at / (DH / 8), col = (at - qr * (DH / 8)) * 8;
-          const int tok = paged_div(qr, group), gi = qr - tok * group;
+          const int tok = paged_div(qr, a.line.by_group), gi = qr - tok * group;
           qv[e] = make_uint4(0, 0, 0, 0);
           if (tok < n && col < a.dh) qv[e] = ld_global_16(a.q + (long long)(row + tok) * a.q_t + (long long)(head * group + gi) * a.q_h + col * 2);
         }
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       // last visible key of rows g and g + 8; every row sees the keys in front of `all`
       int lim[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) lim[e] = a.line.causal ? len - n + paged_div(g + 8 * e, group) : len - 1;
+      for (int e = 0; e < 2; ++e) lim[e] = a.line.causal ? len - n + paged_div(g + 8 * e, a.line.by_group) : len - 1;
       const int all = min(k1, a.line.causal ? len - n + 1 : len);
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m is common to the four lanes of a row, l is this lane's share
       float o[DH / 8][4];
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
         if (park < 0) {
           const float inv = den > 0.f ? 1.f / den : 0.f;  // a row that sees nothing: zeros
-          const int tok = paged_div(r, group), gi = r - tok * group;
+          const int tok = paged_div(r, a.line.by_group), gi = r - tok * group;
           char *to = a.o + (long long)(row + tok) * a.o_t + (long long)(head * group + gi) * a.o_h + col * 2;
           *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
         } else {

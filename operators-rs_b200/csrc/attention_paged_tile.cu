@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
     const int quarter = warp & 3;    // tensor-memory lanes [32 * quarter, +32)
     const int r = quarter * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const int tok = paged_div(r, group), gi = r - tok * group;
+    const int tok = paged_div(r, line.by_group), gi = r - tok * group;
     const uint32_t ta = tmem_base + lane_addr + s_col(t), to = tmem_base + lane_addr + o_col(t);
     const float mult = g.odd_scale ? 1.f : g.a.scale_log2;
     uint32_t s_count = 0, o_count = 0;

@@ -10,8 +10,8 @@
 // So the scratch depends on G alone, and the result on the batch alone: no atomics, no order of arrival.
 //
 // A point is 2^shift keys, with the least shift that keeps every line the host can expect within 31 bits: the arithmetic is
-// 32-bit throughout, and one thread of a CTA does it.  (In 64 bits and in every thread it was three quarters of a kernel's code,
-// and fetching that was most of a small launch: 17 us for one token over 1000 keys.)
+// 32-bit throughout, without a division by anything but what the host knows, and one warp of a CTA does it.  What the others
+// wait for at the start of a launch is this.
 #pragma once
 #include <cstdint>
 
@@ -25,12 +25,28 @@
 
 namespace ops {
 
-// a / b of numbers that are not negative, b > 0
+// n / d for 0 <= n < 2^31 with a divisor that the host knows: a multiplication and a shift.  (A division by a variable takes some
+// 200 clocks, and a thread that finds a CTA's share is what all others wait for.)
+struct PagedDiv {
+  uint32_t mul;
+  int shift;
+};
+inline PagedDiv paged_div_by(uint32_t d) {  // mul = ceil(2^(31 + shift) / d), 2^(shift - 1) < d <= 2^shift
+  PagedDiv v;
+  v.shift = 0;
+  while ((1ull << v.shift) < d) ++v.shift;
+  v.mul = (uint32_t)(((1ull << (31 + v.shift)) + d - 1) / d);
+  return v;
+}
+// near enough to be put right by one
+OPS_HD int paged_guess(float a, float b) {
 #ifdef __CUDA_ARCH__
-static __device__ __noinline__ int paged_div(unsigned a, unsigned b) { return (int)(a / b); }  // one copy of a divider's code
+  return (int)__fdividef(a, b);
 #else
-inline int paged_div(unsigned a, unsigned b) { return (int)(a / b); }
+  return (int)(a / b);
 #endif
+}
+OPS_HD int paged_div(int n, const PagedDiv &d) { return (int)(((unsigned long long)(unsigned)n * d.mul) >> (31 + d.shift)); }
 
 // A sequence's rows [row, row + n) of the step and its cache slots [0, len).
 struct PagedSeq {
@@ -45,8 +61,9 @@ struct PagedLine {
   int block_log2;        // keys of a block
   int shift;             // log2 of the keys of a point
   int overhead;          // points in front of a unit's keys
-  int min_share;         // no CTA gets fewer points than this, as long as one has any
+  int min_share, min_share_log2;  // no CTA gets fewer points than this, a power of two, as long as one has any
   int ctas;
+  PagedDiv by_group, by_tokens, by_ctas;
 };
 
 // What one sequence puts on the line: per kv head `tiles` units, the p-th of base + ramp * (p + 1) points, the overhead among
@@ -65,7 +82,7 @@ OPS_HD PagedSpan paged_span(const PagedLine &l, const PagedSeq &s) {
   p.tiles = p.base = p.ramp = p.head = 0;
   const long long rows = (long long)s.n * l.group;
   if (s.n <= 0 || s.n > l.max_seq || rows < l.rows_lo || rows > l.rows_hi) return p;
-  p.tiles = s.n <= l.tokens ? 1 : paged_div(s.n + l.tokens - 1, l.tokens);
+  p.tiles = s.n <= l.tokens ? 1 : paged_div(s.n + l.tokens - 1, l.by_tokens);
   const bool ramped = l.causal && p.tiles > 1;
   p.base = l.overhead + paged_points(l, ramped ? (s.len > s.n ? s.len - s.n : 0) : (s.len > 0 ? s.len : 1));
   p.ramp = ramped ? l.tokens >> l.shift : 0;
@@ -81,7 +98,9 @@ struct PagedUnit {
 // The unit that holds point `at` of the sequence's stretch, 0 <= at < nkvh * head.
 OPS_HD PagedUnit paged_unit(const PagedSpan &p, int at) {
   PagedUnit u;
-  u.head = paged_div(at, p.head);
+  u.head = paged_guess((float)at, (float)p.head);  // heads are few: off by one at most
+  if (u.head * p.head > at) --u.head;
+  else if (at - u.head * p.head >= p.head) ++u.head;
   const int in_head = at - u.head * p.head;
   int lo = 0, hi = p.tiles;  // begin(lo) <= in_head < begin(hi)
   OPS_ROLLED while (hi - lo > 1) {
@@ -107,31 +126,39 @@ OPS_HD int paged_blocks(const PagedLine &l, const PagedSeq &s, int tile) {
   return k > 0 ? (k + (1 << l.block_log2) - 1) >> l.block_log2 : 1;
 }
 
-// First block behind a cut `at` points behind the beginning of a unit.
-OPS_HD int paged_block(int overhead, int cost, int blocks, int at) {
+// First block behind a cut `at` points behind the beginning of a unit.  (The points of a ramped unit may stand for a few keys more
+// than its last blocks hold: those cuts fall behind its end.)
+OPS_HD int paged_block(const PagedLine &l, int cost, int blocks, int at) {
   if (at >= cost) return blocks;
-  const int t = at - overhead;
+  const int t = at - l.overhead;
   if (t <= 0) return 0;
-  const int each = paged_div(cost - overhead + blocks - 1, blocks);  // points of a block
-  return paged_div(t, each);                                        // < blocks: t < cost - overhead <= each * blocks
+  const int b = l.shift <= l.block_log2 ? t >> (l.block_log2 - l.shift) : t << (l.shift - l.block_log2);
+  return b < blocks ? b : blocks;
 }
 
+// Shares: equal ones if every CTA gets min_share points at least, else shares of min_share for as many as there are points for.
 // CTAs that get anything, and where CTA c's share begins.
+OPS_HD bool paged_all(const PagedLine &l, int total) { return total >= l.min_share * l.ctas; }
 OPS_HD int paged_active(const PagedLine &l, int total) {
-  const int most = paged_div(total, l.min_share) + 1;
-  return most < l.ctas ? most : l.ctas;
+  if (paged_all(l, total)) return l.ctas;
+  return (total + l.min_share - 1) >> l.min_share_log2;
 }
-OPS_HD int paged_cut(int total, int active, int c) {
-  const int each = paged_div(total, active);
-  return each * c + paged_div((unsigned)(total - each * active) * (unsigned)c, active);
+OPS_HD int paged_cut(const PagedLine &l, int total, int c) {
+  if (paged_all(l, total)) {
+    const int each = paged_div(total, l.by_ctas);
+    return each * c + paged_div((total - each * l.ctas) * c, l.by_ctas);
+  }
+  const int cut = c * l.min_share;
+  return cut < total ? cut : total;
 }
 
 // The first CTA whose share begins at or behind point x, 0 < x <= total (`active` if there is none).
-OPS_HD int paged_first_behind(int total, int active, int x) {
-  int c = (int)((float)x * (float)active / (float)total);
+OPS_HD int paged_first_behind(const PagedLine &l, int total, int x) {
+  const int active = paged_active(l, total);
+  int c = paged_guess((float)x * (float)active, (float)total);
   if (c > active) c = active;
-  OPS_ROLLED while (c > 0 && paged_cut(total, active, c) >= x) --c;
-  OPS_ROLLED while (c < active && paged_cut(total, active, c) < x) ++c;
+  OPS_ROLLED while (c > 0 && paged_cut(l, total, c) >= x) --c;
+  OPS_ROLLED while (c < active && paged_cut(l, total, c) < x) ++c;
   return c;
 }
 
@@ -171,9 +198,9 @@ template <class Seqs> OPS_HD PagedPiece paged_next(const PagedLine &l, int nseq,
     q.begin = w.begin + u.begin;
     q.cost = u.cost;
     q.blocks = paged_blocks(l, q.s, u.tile);
-    q.lo = paged_block(l.overhead, u.cost, q.blocks, w.at - q.begin);
+    q.lo = paged_block(l, u.cost, q.blocks, w.at - q.begin);
     w.at = q.begin + u.cost < w.end ? q.begin + u.cost : w.end;
-    q.hi = paged_block(l.overhead, u.cost, q.blocks, w.at - q.begin);
+    q.hi = paged_block(l, u.cost, q.blocks, w.at - q.begin);
     if (q.lo == q.hi) continue;
     q.seq = w.seq;
     break;

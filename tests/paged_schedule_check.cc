@@ -22,6 +22,10 @@ using namespace ops;
 
 int main() {
   std::mt19937 rng(7);
+  const int round_no = -1;
+  for (uint32_t d = 1; d <= 70000; d += d < 300 ? 1 : 97)
+    for (uint32_t n : {0u, 1u, d - 1, d, d + 1, 2 * d - 1, 1000 * d - 1, 1000 * d, 0x7fffffffu, 0x7fffffffu - d, 0x7fffffffu / d * d, 0x7fffffffu / d * d - 1, (uint32_t)(rng() >> 1)})
+      if (n <= 0x7fffffffu) CHECK(paged_div((int)n, paged_div_by(d)) == (int)(n / d));
   auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
   for (int round_no = 0; round_no < 3000; ++round_no) {
     PagedLine l;
@@ -55,7 +59,13 @@ int main() {
     l.shift = pick(0, 3) ? 0 : pick(0, 7);
     while (count * (most / (1 << l.shift) + 4.0) > 2147483647.0) ++l.shift;
     l.overhead = std::max(1, overhead >> l.shift);
-    l.min_share = std::max(1, min_share >> l.shift);
+    l.min_share = 1;
+    while (l.min_share * 2 <= std::max(1, min_share >> l.shift)) l.min_share *= 2;
+    l.min_share_log2 = 0;
+    while ((1 << l.min_share_log2) < l.min_share) ++l.min_share_log2;
+    l.by_group = paged_div_by(l.group);
+    l.by_tokens = paged_div_by(l.tokens);
+    l.by_ctas = paged_div_by(l.ctas);
     long long sum = 0;
     for (auto &s : seqs) sum += (long long)paged_span(l, s).head * l.nkvh;
     CHECK(sum <= 0x7fffffff);  // the shift below is chosen like the host's
@@ -63,13 +73,13 @@ int main() {
     if (total == 0) continue;
     const int active = paged_active(l, total);
     CHECK(active >= 1 && active <= l.ctas);
-    CHECK(paged_cut(total, active, 0) == 0 && paged_cut(total, active, active) == total);
+    CHECK(paged_cut(l, total, 0) == 0 && paged_cut(l, total, active) == total);
     auto at = [&](int i) { return seqs[i]; };
     std::map<std::tuple<int, int, int>, std::vector<std::tuple<int, int, int>>> units;  // (seq, head, tile) -> (lo, hi, cta * 2 + slot) of the parts
     std::map<std::tuple<int, int, int>, int> blocks;
     std::map<int, int> parked;
     for (int c = 0; c < active; ++c) {
-      PagedWalk w{0, 0, paged_cut(total, active, c), paged_cut(total, active, c + 1)};
+      PagedWalk w{0, 0, paged_cut(l, total, c), paged_cut(l, total, c + 1)};
       long long keys = 0;
       int steps = 0;
       for (PagedPiece q = paged_next(l, nseq, w, at); q.seq >= 0; q = paged_next(l, nseq, w, at)) {
@@ -82,7 +92,7 @@ int main() {
       }
       // a share is its points' blocks, to within the roundings at its two ends and the short last block and tile of a unit
       // (a point of several keys rounds the ramp of a causal unit down)
-      if (l.shift == 0) CHECK(keys <= (((long long)(paged_cut(total, active, c + 1) - paged_cut(total, active, c)) << l.shift) / block + 2 + 2 * steps) * 9 / 8);
+      if (l.shift == 0) CHECK(keys <= (((long long)(paged_cut(l, total, c + 1) - paged_cut(l, total, c)) << l.shift) / block + 2 + 2 * steps) * 9 / 8);
     }
     size_t want = 0;
     for (int i = 0; i < nseq; ++i) {
@@ -108,17 +118,17 @@ int main() {
     size_t joined = 0, split = 0;
     for (auto &u : units) split += u.second.size() > 1;
     for (int c = 1; c < active; ++c) {
-      const int cut = paged_cut(total, active, c);
+      const int cut = paged_cut(l, total, c);
       int begin = 0;
       int i = 0;
       while (begin + paged_span(l, seqs[i]).head * l.nkvh <= cut) begin += paged_span(l, seqs[i++]).head * l.nkvh;
       const PagedUnit u = paged_unit(paged_span(l, seqs[i]), cut - begin);
-      if (cut == begin + u.begin || paged_cut(total, active, c - 1) > begin + u.begin) continue;
+      if (cut == begin + u.begin || paged_cut(l, total, c - 1) > begin + u.begin) continue;
       const int nb = paged_blocks(l, seqs[i], u.tile);
       std::vector<std::tuple<int, int, int>> parts;
-      for (int d = c - 1; d < active && paged_cut(total, active, d) < begin + u.begin + u.cost; ++d) {
+      for (int d = c - 1; d < active && paged_cut(l, total, d) < begin + u.begin + u.cost; ++d) {
         const int from = begin + u.begin;
-        const int lo = paged_block(l.overhead, u.cost, nb, paged_cut(total, active, d) - from), hi = paged_block(l.overhead, u.cost, nb, paged_cut(total, active, d + 1) - from);
+        const int lo = paged_block(l, u.cost, nb, paged_cut(l, total, d) - from), hi = paged_block(l, u.cost, nb, paged_cut(l, total, d + 1) - from);
         if (lo < hi) parts.push_back({lo, hi, d * 2 + (lo > 0 ? 0 : 1)});
       }
       auto found = units.find({i, u.head, u.tile});
@@ -129,8 +139,8 @@ int main() {
     for (int k = 0; k < 20; ++k) {
       const int x = k ? 1 + (int)(rng() % (unsigned)total) : total;
       int c = 0;
-      while (c < active && paged_cut(total, active, c) < x) ++c;
-      CHECK(paged_first_behind(total, active, x) == c);
+      while (c < active && paged_cut(l, total, c) < x) ++c;
+      CHECK(paged_first_behind(l, total, x) == c);
     }
   }
   printf("schedule ok\n");
