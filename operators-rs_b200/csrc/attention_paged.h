@@ -62,44 +62,50 @@ __device__ __forceinline__ uint32_t ap_pack(float lo, float hi) {  // first valu
   return *reinterpret_cast<uint32_t *>(&t);
 }
 
-// Points of one sequence on the line.  Out of line, like everything of the schedule: a small launch spends its time on fetching code.
-static __device__ __noinline__ long long paged_cost(const PagedBatch &b, const PagedLine &l, int i, bool report) {
-  return (long long)paged_span(l, paged_seq(b, i, report)).head * l.nkvh;
-}
-
 // CTA `cta`'s share of the line, by one warp: the points of all sequences, then the one its share begins in.  `report` says
 // whether this CTA is the one that looks for what is wrong with the batch.  All lanes get the answer (at == end: nothing).
 __device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLine &l, int cta, bool report, PagedWalk *walk, int *total_out) {
   const int lane = threadIdx.x & 31;
   walk->seq = walk->begin = walk->at = walk->end = 0;
-  long long sum = 0, cost = 0;
+  *total_out = 0;
+  long long sum = 0;
+  int lo = 0, hi = 0, before = 0;
+  // two passes through one copy of the code: all sequences for the sum, then up to the one that is looked for
+  bool looking = false;
 #pragma unroll 1
-  for (int i = lane; i < b.nseq; i += 32) sum += cost = paged_cost(b, l, i, report);
-  // (a lane's sum stays below 2^47: 2^16 sequences of 2^31 points; its halves add up in 32 bits)
-  sum = (long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum & 0xffffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum >> 24)) << 24);
-  // sequences that share rows (seq_start falls) can put more on the line than the host allowed for: nothing is done then
-  const int total = sum <= 0x7fffffff ? (int)sum : 0;
-  if (report && total != sum && lane == 0) atomicCAS(b.status, 0, OPS_PAGED_BAD_ROWS);
-  *total_out = total;
-  const int lo = paged_cut(l, total, cta), hi = paged_cut(l, total, cta + 1);
-  if (lo >= hi) return;
-  int before = 0;
-#pragma unroll 1
-  for (int i0 = 0; i0 < b.nseq; i0 += 32) {
+  for (int i0 = 0; i0 < b.nseq;) {
     const int i = i0 + lane;
-    int mine = (int)cost;  // of up to 32 sequences they are known already
-    if (b.nseq > 32) mine = i < b.nseq ? (int)paged_cost(b, l, i, false) : 0;
-    int upto = mine;
+    long long cost = 0;
+    if (i < b.nseq) cost = (long long)paged_span(l, paged_seq(b, i, report && !looking)).head * l.nkvh;
+    i0 += 32;
+    if (!looking) {
+      sum += cost;
+      if (i0 < b.nseq) continue;
+      // (a lane's sum stays below 2^47: 2^16 sequences of 2^31 points; its halves add up in 32 bits)
+      sum = (long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum & 0xffffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum >> 24)) << 24);
+      // sequences that share rows (seq_start falls) can put more on the line than the host allowed for: nothing is done then
+      const int total = sum <= 0x7fffffff ? (int)sum : 0;
+      if (report && total != sum && lane == 0) atomicCAS(b.status, 0, OPS_PAGED_BAD_ROWS);
+      *total_out = total;
+      lo = paged_cut(l, total, cta);
+      hi = paged_cut(l, total, cta + 1);
+      if (lo >= hi) return;
+      looking = true;
+      i0 = 0;
+      if (b.nseq > 32) continue;
+      i0 = 32;  // of up to 32 sequences the costs are at hand
+    }
+    int upto = (int)cost;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
-    const unsigned here = __ballot_sync(0xffffffffu, before + upto - mine <= lo && lo < before + upto);
+    const unsigned here = __ballot_sync(0xffffffffu, before + upto - (int)cost <= lo && lo < before + upto);
     if (here) {
       const int at = __ffs(here) - 1;
-      walk->seq = i0 + at;
-      walk->begin = before + __shfl_sync(0xffffffffu, upto - mine, at);
+      walk->seq = i0 - 32 + at;
+      walk->begin = before + __shfl_sync(0xffffffffu, upto - (int)cost, at);
       break;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
