@@ -156,6 +156,7 @@ def _declare(L):
     L.ops_dtype_nbytes.restype = ctypes.c_size_t
     L.ops_dtype_nbytes.argtypes = [ctypes.c_uint32]
     L.ops_build_info.restype = ctypes.c_char_p
+    L.ops_rope_norm_launch.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
     L.ops_random_sample_batched_workspace.restype = ctypes.c_size_t
     L.ops_random_sample_batched_workspace.argtypes = [ctypes.c_uint32, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_void_p]
     for name in EXPORTS:
@@ -245,13 +246,15 @@ def _lay(x):
 
 
 def _operand(layout, base):
-    """(dtype, shape, byte strides, address) of an operand; layout: a TensorLayout, or the tensor itself."""
+    """(dtype, shape, strides, bytes of a stride's unit, address) of an operand; layout: a TensorLayout, or the tensor itself."""
     if type(layout) is TensorLayout:
-        return layout.dt, layout.shape, layout.strides, ptr(base)
-    if hasattr(layout, "data_ptr"):
-        dt, es = _torch_info(layout.dtype)
-        return dt, layout.shape, [s * es for s in layout.stride()], layout.data_ptr() if base is layout else ptr(base)
-    return _numpy_dt(layout.dtype), layout.shape, layout.strides, ptr(base)
+        return layout.dt, layout.shape, layout.strides, 1, ptr(base)
+    info = _TORCH_DT.get(layout.dtype)
+    if info is None:
+        if not hasattr(layout, "data_ptr"):
+            return _numpy_dt(layout.dtype), layout.shape, layout.strides, 1, ptr(base)
+        info = _torch_info(layout.dtype)
+    return info[0], layout.shape, layout.stride(), info[1], layout.data_ptr() if base is layout else ptr(base)
 
 
 class _PackedArgs(_ArgsBase):
@@ -262,7 +265,7 @@ class _PackedArgs(_ArgsBase):
     _plans = {}
 
     def _fill(self, operands, tail):
-        """operands: (dtype, shape, byte strides, base address or None)."""
+        """operands: as `_operand` makes them."""
         ranks = tuple([len(o[1]) for o in operands])
         plan = self._plans.get((self.TAIL, ranks))
         if plan is None:
@@ -276,15 +279,15 @@ class _PackedArgs(_ArgsBase):
         self.c = buf = ctypes.create_string_buffer(packer.size)
         addr = ctypes.addressof(buf)
         values, dims = [], []
-        for (dt, shape, strides, base), n, at in zip(operands, ranks, offset):
+        for (dt, shape, strides, unit, base), n, at in zip(operands, ranks, offset):
             at += addr
             values += (dt, n, at, at + 8 * n, base or 0)
             dims += shape
-            dims += strides
+            dims += [s * unit for s in strides]
         packer.pack_into(buf, 0, *values, *tail, *dims)
 
 
-_NO_WEIGHT = (F32, (), (), None)  # beside a null weight the layout is never looked at
+_NO_WEIGHT = (F32, (), (), 1, None)  # beside a null weight the layout is never looked at
 
 
 class RmsNormArgs(_ArgsBase):
@@ -564,10 +567,18 @@ class AddRowsArgs(_ArgsBase):
 # ---------------------------------------------------------------------------------------------------
 # operators
 # ---------------------------------------------------------------------------------------------------
+_raw_stream = None  # torch's own accessor, once CUDA is up: a hundredth of the public call's time
+
+
 def current_stream(device=None):
     """Torch's current stream of a device (an index; None: the current device)."""
+    global _raw_stream
+    if _raw_stream is not None and device is not None:
+        return _raw_stream(device)
     import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    stream = torch.cuda.current_stream(device).cuda_stream
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return stream
 
 
 class TorchQueueAlloc:
@@ -596,6 +607,7 @@ class Operator:
         self._destroy.restype = None
         self._scheme = getattr(L, f"ops_{self.NAME}_scheme")
         self._launch = getattr(L, f"ops_{self.NAME}_launch")
+        self._launch.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         self._create(L, node)
 
     def _create(self, L, node):
@@ -614,17 +626,17 @@ class Operator:
     def launch(self, args, workspace=None, queue_alloc=None):
         """Enqueue on queue_alloc.queue().  A short workspace is topped up from queue_alloc and the
         call repeated, as Workspace::new does in the crate (operators/src/common/workspace.rs:12-21)."""
-        qa = queue_alloc or TorchQueueAlloc(self.device)
-        stream = ctypes.c_void_p(qa.queue())
+        stream = current_stream(self.device) if queue_alloc is None else queue_alloc.queue()
         self._last_args = args  # the enqueued kernels read these buffers: keep them until the next launch
         ws_ptr, ws_len = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
-        rc = self._launch(self._h, args.byref(), ctypes.c_void_p(ws_ptr), ctypes.c_size_t(ws_len), stream)
+        rc = self._launch(self._h, args.byref(), ws_ptr, ws_len, stream)
         if rc == WORKSPACE_TOO_SMALL:
             need = lib().ops_last_workspace_need()
-            own = qa.alloc(need)
-            rc = self._launch(self._h, args.byref(), ctypes.c_void_p(own.data_ptr()), ctypes.c_size_t(need), stream)
+            own = (queue_alloc or TorchQueueAlloc(self.device)).alloc(need)
+            rc = self._launch(self._h, args.byref(), own.data_ptr(), need, stream)
             self._last_ws = own  # stream-ordered reuse by torch's allocator keeps this safe once dropped
-        _check(rc, True)
+        if rc != OK:
+            _check(rc, True)
 
     def __del__(self):
         h, self._h = getattr(self, "_h", None), None
@@ -650,9 +662,10 @@ class Rope(Operator):
 
     def launch_norm(self, args, queue_alloc=None):
         """ops_rope_norm_launch: every head normalised, weighted and rotated in one pass."""
-        qa = queue_alloc or TorchQueueAlloc(self.device)
         self._last_args = args
-        _check(lib().ops_rope_norm_launch(self._h, args.byref(), ctypes.c_void_p(qa.queue())), True)
+        rc = lib().ops_rope_norm_launch(self._h, args.byref(), current_stream(self.device) if queue_alloc is None else queue_alloc.queue())
+        if rc != OK:
+            _check(rc, True)
 
     @staticmethod
     def build_pos(dt, nt, seqs):

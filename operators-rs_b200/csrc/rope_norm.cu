@@ -189,10 +189,17 @@ __global__ void __launch_bounds__(RN_WARPS * 32) rotate_heads_kernel(const __gri
        max(0, h_begin - a.nh - a.nkvh), min(h_end - a.nh - a.nkvh, a.nkvh), std::false_type());
 }
 
-static RotateTurns rotate_turns(float theta, usz dh) {
-  RotateTurns t;
-  for (int k = 0; k < RN_MAX_PAIRS; ++k)
-    t.v[k] = (usz)k < dh / 2 ? std::pow((double)theta, -2.0 * k / (double)dh) / 6.283185307179586476925 : 0.0;
+// (Sixty-four calls of pow are a third of what a small launch costs the host: a thread keeps the last table it made.)
+static const RotateTurns &rotate_turns(float theta, usz dh) {
+  static thread_local RotateTurns t;
+  static thread_local float for_theta = 0.f;
+  static thread_local usz for_dh = 0;
+  if (for_dh != dh || memcmp(&for_theta, &theta, sizeof(theta)) != 0) {
+    for (int k = 0; k < RN_MAX_PAIRS; ++k)
+      t.v[k] = (usz)k < dh / 2 ? std::pow((double)theta, -2.0 * k / (double)dh) / 6.283185307179586476925 : 0.0;
+    for_theta = theta;
+    for_dh = dh;
+  }
   return t;
 }
 

@@ -16,7 +16,7 @@ def L(pkg, dt, shape, strides=None):
 
 def batch(pkg, table=None, start=None, length=None, base=P16, max_seq=0):
     b = pkg.PagedBatch(table or L(pkg, pkg.I32, (3, 5)), start or L(pkg, pkg.I32, (4,)), length or L(pkg, pkg.I32, (3,)), max_seq)
-    b.operands = tuple((*o[:3], base) for o in b.operands)
+    b.operands = tuple((*o[:-1], base) for o in b.operands)
     return b
 
 
