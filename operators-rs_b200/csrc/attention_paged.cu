@@ -7,139 +7,10 @@
 
 namespace ops {
 
-// Joins the parts of the units that several CTAs share:
-//   o = sum_d 2^(m_d - M) O_d / sum_d 2^(m_d - M) l_d,  M = max_d m_d, parts in the order of their keys.
-// An item is 16 rows of a unit.  How many units there are, and of how many rows and parts, only the records tell (one long
-// sequence: few units of a hundred parts; a prompt: a unit per CTA, of two), so every block counts the items of all records and
-// the blocks deal them out among themselves.  With fewer than 16 rows a row's parts go to several warps, which meet in shared
-// memory; a lane holds 4 columns.
-constexpr int JOIN_WARPS = 16, JOIN_THREADS = JOIN_WARPS * 32, JOIN_ROWS = 16;
-constexpr int JOIN_BLOCKS_PER_SM = 2;
-
-template <bool BF>
-__global__ void __launch_bounds__(JOIN_THREADS, JOIN_BLOCKS_PER_SM)
-    attention_paged_join_kernel(const __grid_constant__ PagedAttnArgs few, const __grid_constant__ PagedAttnArgs tile, int few_rows, int part_dh) {
-  __shared__ int first_item[2 * AP_MAX_CTAS];  // of every record
-  __shared__ PagedJoin joins[2 * AP_MAX_CTAS];
-  __shared__ int warp_items[JOIN_WARPS];
-  __shared__ __align__(16) float meet[JOIN_WARPS][AP_MAX_DH + AP_PAD];  // o, m, l; 16-byte rows
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int records = few.line.ctas + tile.line.ctas, group = few.line.group;
-  pdl_wait_for_front();
-  // items in front of every record's: a prefix sum over rounds of a record per thread
-  int items = 0;
-  for (int j0 = 0; j0 < records; j0 += JOIN_THREADS) {
-    const int j = j0 + threadIdx.x;
-    int mine = 0;
-    if (j < records) {
-      const PagedJoin rec = j < few.line.ctas ? few.joins[j] : tile.joins[j - few.line.ctas];
-      joins[j] = rec;
-      if (rec.ctas) mine = (rec.tokens * group + JOIN_ROWS - 1) / JOIN_ROWS;
-    }
-    int upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    if (lane == 31) warp_items[warp] = upto;
-    __syncthreads();
-    int sum = warp_items[lane & (JOIN_WARPS - 1)];  // of all warps, by every warp for itself
-#pragma unroll
-    for (int o = 1; o < JOIN_WARPS; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if ((lane & (JOIN_WARPS - 1)) >= o) sum += x;
-    }
-    const int front = warp == 0 ? 0 : __shfl_sync(0xffffffffu, sum, warp - 1);
-    if (j < records) first_item[j] = items + front + upto - mine;
-    items += __shfl_sync(0xffffffffu, sum, JOIN_WARPS - 1);
-    __syncthreads();
-  }
-
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    int lo = 0, hi = records;  // the last record whose first item is at or before this one has it
-#pragma unroll 1
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (first_item[mid] <= item) lo = mid;
-      else hi = mid;
-    }
-    const bool on_tile = lo >= few.line.ctas;
-    const PagedAttnArgs &a = on_tile ? tile : few;
-    const PagedJoin &j = joins[lo];
-    const int first = on_tile ? lo - few.line.ctas : lo;
-    const int row0 = (item - first_item[lo]) * JOIN_ROWS, here = min(JOIN_ROWS, j.tokens * group - row0);
-    const int share = here > 8 ? 1 : here > 5 ? 2 : here > 4 ? 3 : here > 3 ? 4 : here > 2 ? 5 : here > 1 ? 8 : 16;  // JOIN_WARPS / here warps per row
-    const int own = paged_guess((float)warp + 0.5f, (float)share), part = warp - own * share;  // warp / share
-    const int r = row0 + own;
-    // where the row lies in a parked unit: tiles of 128 rows, whole tokens each
-    const int tok = paged_div(r, few.line.by_group), gi = r - tok * group;
-    const int per_tile = on_tile ? tile.line.tokens / 2 : JOIN_ROWS, t = tok >= per_tile;
-    const int parked = t * (AP_TILE_ROWS / 2) + (tok - t * per_tile) * group + gi;
-    const long long ld = part_dh + AP_PAD, unit = (long long)(on_tile ? AP_TILE_ROWS : few_rows) * ld;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (own < here) {
-      constexpr int DEEP = 4;
-      for (int d0 = part; d0 < j.ctas; d0 += share * DEEP) {
-        float4 v[DEEP];
-        float2 ml[DEEP];
-#pragma unroll
-        for (int e = 0; e < DEEP; ++e) {
-          const int d = d0 + e * share;
-          v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-          ml[e] = make_float2(-INFINITY, 0.f);
-          // the first has the unit's beginning in its second slot; a cut may have left one of the others none
-          const int slot = d >= j.ctas ? -1 : d == 0 ? first * 2 + 1 : joins[lo + d].front ? (first + d) * 2 : -1;
-          if (slot >= 0) {
-            const float *from = a.parts + slot * unit + parked * ld;
-            ml[e] = __ldcg(reinterpret_cast<const float2 *>(from + part_dh));
-            if (lane * 4 < a.dh) v[e] = __ldcg(reinterpret_cast<const float4 *>(from + lane * 4));
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < DEEP; ++e) {
-          if (ml[e].x == -INFINITY) continue;  // a part in which the row sees nothing may have left its o unwritten
-          const float top = fmaxf(m, ml[e].x);
-          const float wa = ap_ex2(m - top), wb = ap_ex2(ml[e].x - top);
-          l = l * wa + ml[e].y * wb;
-          acc.x = acc.x * wa + v[e].x * wb;
-          acc.y = acc.y * wa + v[e].y * wb;
-          acc.z = acc.z * wa + v[e].z * wb;
-          acc.w = acc.w * wa + v[e].w * wb;
-          m = top;
-        }
-      }
-      if (part > 0) {
-        *reinterpret_cast<float4 *>(&meet[warp][lane * 4]) = acc;
-        if (lane == 0) {
-          meet[warp][AP_MAX_DH] = m;
-          meet[warp][AP_MAX_DH + 1] = l;
-        }
-      }
-    }
-    __syncthreads();
-    if (own < here && part == 0) {
-      for (int w = warp + 1; w < warp + share; ++w) {
-        const float mw = meet[w][AP_MAX_DH], top = fmaxf(m, mw);
-        if (mw == -INFINITY) continue;
-        const float wa = ap_ex2(m - top), wb = ap_ex2(mw - top);
-        l = l * wa + meet[w][AP_MAX_DH + 1] * wb;
-        const float4 v = *reinterpret_cast<const float4 *>(&meet[w][lane * 4]);
-        acc.x = acc.x * wa + v.x * wb;
-        acc.y = acc.y * wa + v.y * wb;
-        acc.z = acc.z * wa + v.z * wb;
-        acc.w = acc.w * wa + v.w * wb;
-        m = top;
-      }
-      if (lane * 4 < a.dh) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        char *to = a.o + (long long)(j.row + tok) * a.o_t + (long long)(j.head * group + gi) * a.o_h + lane * 8;
-        *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
-      }
-    }
-    __syncthreads();  // meet is free again
-  }
+// Clears the counters of the launch.  The kernels that use them start beside it and wait for it where they first need them.
+__global__ void __launch_bounds__(1024) attention_paged_clear_kernel(uint4 *counters, int n) {
+  pdl_let_next_come();
+  for (int i = threadIdx.x; i < n; i += 1024) counters[i] = make_uint4(0, 0, 0, 0);
 }
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point
@@ -220,8 +91,8 @@ namespace ops {
 struct PagedAttnPlan {
   PagedLine few, tile;  // ctas == 0: not launched
   int few_rows, part_dh;
-  usz few_joins, few_parts, tile_joins, tile_parts;  // bytes
-  usz bytes() const { return few_joins + few_parts + tile_joins + tile_parts + 256; }
+  usz few_arrived, tile_arrived, few_parts, tile_parts;  // bytes
+  usz bytes() const { return few_arrived + tile_arrived + few_parts + tile_parts + 256; }
 };
 
 static usz up256(usz n) { return (n + 255) / 256 * 256; }
@@ -262,8 +133,8 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
     p.few.block_log2 = AP_FEW_BLOCK_LOG2;
     p.few.ctas = std::min(attention_paged_few_ctas(base), AP_MAX_CTAS);
     line_scale(&p.few, nt, nseq, slots, 128, 128);
-    p.few_joins = up256(sizeof(PagedJoin) * (usz)p.few.ctas);
-    p.few_parts = up256(2 * (usz)p.few.ctas * p.few_rows * (p.part_dh + AP_PAD) * sizeof(float));
+    p.few_arrived = up256((usz)AP_LEVELS * p.few.ctas * 8 * sizeof(uint32_t));
+    p.few_parts = up256(3 * (usz)p.few.ctas * p.few_rows * (p.part_dh + 2) * sizeof(float));
     p.tile.rows_lo = p.few_rows + 1;
   } else {
     p.tile.rows_lo = 1;
@@ -274,8 +145,8 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
     p.tile.block_log2 = AP_TILE_BLOCK_LOG2;
     p.tile.ctas = std::min(base.sm_count, AP_MAX_CTAS);
     line_scale(&p.tile, nt, nseq, slots, 512, 512);
-    p.tile_joins = up256(sizeof(PagedJoin) * (usz)p.tile.ctas);
-    p.tile_parts = up256(2 * (usz)p.tile.ctas * AP_TILE_ROWS * (p.part_dh + AP_PAD) * sizeof(float));
+    p.tile_arrived = up256((usz)AP_LEVELS * p.tile.ctas * 8 * sizeof(uint32_t));
+    p.tile_parts = up256(2 * (usz)p.tile.ctas * AP_TILE_ROWS * (p.part_dh + 2) * sizeof(float));
   }
   return p;
 }
@@ -338,15 +209,16 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   char *at = (char *)(((uintptr_t)ws + 255) / 256 * 256);
   PagedAttnArgs few = g, tile = g;
   few.line = plan.few;
-  few.joins = (PagedJoin *)at;
-  few.parts = (float *)(at + plan.few_joins);
+  few.arrived = (uint32_t *)at;
+  few.parts = (float *)(at + plan.few_arrived + plan.tile_arrived);
+  few.parts_ml = (float2 *)(few.parts + 3 * (usz)plan.few.ctas * plan.few_rows * plan.part_dh);
   tile.line = plan.tile;
-  tile.joins = (PagedJoin *)(at + plan.few_joins + plan.few_parts);
-  tile.parts = (float *)(at + plan.few_joins + plan.few_parts + plan.tile_joins);
+  tile.arrived = (uint32_t *)(at + plan.few_arrived);
+  tile.parts = (float *)(at + plan.few_arrived + plan.tile_arrived + plan.few_parts);
+  tile.parts_ml = (float2 *)(tile.parts + 2 * (usz)plan.tile.ctas * AP_TILE_ROWS * plan.part_dh);
+  attention_paged_clear_kernel<<<1, 1024, 0, s>>>((uint4 *)at, (int)((plan.few_arrived + plan.tile_arrived) / 16));
+  OPS_TRY(check_launch("attention_paged(clear)"));
   if (plan.few.ctas) OPS_TRY(attention_paged_few(few, plan.few_rows, bf16, s));
-  if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, plan.few.ctas != 0, s));
-  if (plan.few.ctas + plan.tile.ctas)
-    return ap_launch_beside("attention_paged(join)", bf16 ? attention_paged_join_kernel<true> : attention_paged_join_kernel<false>,
-                            JOIN_BLOCKS_PER_SM * base.sm_count, JOIN_THREADS, 0, s, true, few, tile, plan.few_rows, plan.part_dh);
+  if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, plan.few.ctas == 0, s));
   return OPS_OK;
 }

@@ -10,16 +10,8 @@ namespace ops {
 
 constexpr int AP_MAX_DH = 128;
 constexpr int AP_MAX_GROUP = 128;
-constexpr int AP_MAX_CTAS = 256;  // of a kernel: the joining kernel holds a record of each
-constexpr int AP_PAD = 4;  // a parked row: DH floats of unnormalised o, its reference point m and its sum l; 16-byte aligned
-
-// What a CTA leaves for the kernel that joins the parts of units that several CTAs share.
-struct __align__(16) PagedJoin {
-  int ctas;                 // that have points of the unit this CTA has the first blocks of, and not the last: it and those behind it; else 0
-  int row, tokens, head;    // of that unit: first row of the step, query tokens, kv head
-  int front;                // whether this CTA's slot 0 holds a part (of the unit that its share begins in)
-  int unused[3];
-};
+constexpr int AP_MAX_CTAS = 256;  // of a kernel
+constexpr int AP_FEW_JOIN = 16, AP_LEVELS = 2;  // parts are joined in groups, the groups in turn: 16^2 is AP_MAX_CTAS
 
 struct PagedAttnArgs {
   const char *q, *k, *v;
@@ -30,8 +22,11 @@ struct PagedAttnArgs {
   float scale_log2;  // scale * log2(e): the softmax runs in powers of two
   PagedBatch batch;
   PagedLine line;
-  PagedJoin *joins;  // [line.ctas]
-  float *parts;      // [2 * line.ctas][rows of a unit][DH + AP_PAD]
+  uint32_t *arrived;  // [AP_LEVELS][line.ctas][8]: parts of a group that are parked; zero when the launch begins
+  // parked parts, [2 * line.ctas, and line.ctas more for the few-rows kernel][rows of a unit]: unnormalised o, DH floats in whole
+  // lines, and (m, l), its reference point and sum
+  float *parts;
+  float2 *parts_ml;
 };
 
 // Tensor maps over the whole cache, boxes of 64 columns x `rows` slots of one head of one page, 128-byte swizzle.
@@ -40,8 +35,7 @@ int attention_paged_maps(const PagedAttnArgs &a, bool bf16, uint32_t rows, CUten
 bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2);
 int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, cudaStream_t s);
 int attention_paged_few_ctas(const OpBase &base);
-// beside: it may start while the launch in front of it, the few-rows kernel's, still runs; it ends behind it all the same.
-int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool beside, cudaStream_t s);
+int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, cudaStream_t s);
 constexpr int AP_FEW_BLOCK_LOG2 = 5, AP_FEW_BLOCK = 32, AP_TILE_BLOCK_LOG2 = 7, AP_TILE_BLOCK = 128;  // keys of a block
 constexpr int AP_TILE_ROWS = 256;                       // query rows of a unit of the tile kernel: two tiles
 
@@ -119,19 +113,24 @@ __device__ __forceinline__ PagedPiece paged_step(const PagedBatch &b, const Page
   return paged_next(l, b.nseq, w, [&](int i) { return paged_seq(b, i, false); });
 }
 
-// The CTA's record for the joining kernel, written by one thread: `last` is the last piece of its share (its unit goes on in the
-// next CTAs' shares if it is not the end of it), or seq < 0; front: its first piece is not the beginning of a unit.
-__device__ __forceinline__ void paged_note_join(const PagedAttnArgs &a, int cta, const PagedPiece &last, bool front, int total) {
-  PagedJoin j;
-  memset(&j, 0, sizeof(j));
-  j.front = front;
-  if (last.seq >= 0 && last.lo == 0 && last.hi < last.blocks) {
-    j.ctas = paged_first_behind(a.line, total, last.begin + last.cost) - cta;
-    j.row = last.s.row + last.tile * a.line.tokens;
-    j.tokens = min(a.line.tokens, last.s.n - last.tile * a.line.tokens);
-    j.head = last.head;
-  }
-  a.joins[cta] = j;
+// Whether all parts but the caller's of a group are parked: then the caller's need not be.  One warp; what the others have
+// written can be read behind it.
+__device__ __forceinline__ bool paged_others_parked(const uint32_t *arrived, int group) {
+  uint32_t n = 0;
+  if ((threadIdx.x & 31) == 0) asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(arrived) : "memory");
+  const bool all = __shfl_sync(0xffffffffu, n, 0) == (uint32_t)(group - 1);
+  if (all) __threadfence();
+  return all;
+}
+// The caller's warp has parked its part: whether it was the last of the group, as above.
+__device__ __forceinline__ bool paged_arrive_last(uint32_t *arrived, int group) {
+  __threadfence();
+  __syncwarp();
+  uint32_t before = 0;
+  if ((threadIdx.x & 31) == 0) before = atomicAdd(arrived, 1u);
+  const bool last = __shfl_sync(0xffffffffu, before, 0) == (uint32_t)(group - 1);
+  if (last) __threadfence();
+  return last;
 }
 
 // A launch may start while the one in front of it still runs (programmatic dependent launch): the front one says when the other
@@ -141,9 +140,9 @@ __device__ __forceinline__ void pdl_wait_for_front() { asm volatile("griddepcont
 #endif
 
 #ifdef __CUDACC__
-// A launch, with `beside` one that may start while the one in front of it in the stream still runs.
+// A launch that may start while the one in front of it in the stream still runs.
 template <class Kernel, class... Args>
-int ap_launch_beside(const char *what, Kernel kernel, int grid, int block, int bytes, cudaStream_t s, bool beside, const Args &...args) {
+int ap_launch_beside(const char *what, Kernel kernel, int grid, int block, int bytes, cudaStream_t s, const Args &...args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3((unsigned)block);
@@ -153,7 +152,7 @@ int ap_launch_beside(const char *what, Kernel kernel, int grid, int block, int b
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = beside ? 1 : 0;
+  cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "%s: %s", what, cudaGetErrorString(e));
   return OPS_OK;

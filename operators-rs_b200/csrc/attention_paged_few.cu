@@ -12,7 +12,7 @@
 //   warps 0-3  stage i goes to warp i % 4, which alone waits for it and frees it: S = Q K^T and O += P V for its 32 keys on
 //              m16n8k16 warp MMAs (the rows are the 16 of the MMA; a 128-row tcgen05 tile has nothing to chew on here), both
 //              operands by ldmatrix from the 128-byte-swizzled stage, the probabilities straight from the S registers.  At the
-//              end of a piece the four meet in shared memory.
+//              end of a piece the four meet in shared memory, and the CTA that comes last to a unit that several share joins its parts.
 //   warp 4     producer: a lane per box of a stage (32 / min(page, 32) boxes of K and of V), pages looked up a stage ahead
 //   warp 5     scheduler: finds the CTA's share, posts its pieces ahead
 //
@@ -58,7 +58,7 @@ struct FewPiece {
   int seq;  // -1: no more
   int row, n, len, head;
   int k0, k1;  // keys
-  int park;    // -1: the whole unit; else the slot of its part
+  int first, count;  // CTAs that have parts of the unit; 1: this is all of it
 };
 
 template <int DH, int NR> struct FewSmem {
@@ -102,13 +102,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
   auto piece_empty = [&](int i) { return bar0 + 8u * (2 * ST + 4 + FEW_RING + i); };
   const uint32_t meet_bar = bar0 + 8u * (2 * ST + 4 + 2 * FEW_RING);
   volatile FewPiece *pieces = reinterpret_cast<volatile FewPiece *>(base_ptr + Smem::OFF_PIECES);
-  __shared__ int gave_up;
+  __shared__ int gave_up, last_s;
   const PagedAttnArgs &a = f.a;
   int *status = a.batch.status + 1;  // of the waits
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = a.line.group;
 
-  pdl_let_next_come();
   PagedWalk walk;
   int total = 0;
   if (warp == FEW_CONSUMERS + FEW_PRODUCERS) {
@@ -134,6 +133,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     }
     mbar_init(meet_bar, FEW_CONSUMERS);
     fence_barrier_init();
+  } else if (warp == 1) {
+    pdl_wait_for_front();  // the counters have been cleared, this kernel's and the next one's: that may come
+    pdl_let_next_come();
   }
   __syncthreads();
 
@@ -141,9 +143,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
   if (warp == FEW_CONSUMERS + FEW_PRODUCERS) {
     // ------------------------------------------------------------------ scheduler
     if (lane == 0) {
-      PagedPiece last;
-      last.seq = -1;
-      bool front = false;
 #pragma unroll 1
       for (uint32_t i = 0; ok; ++i) {
         const PagedPiece q = paged_step(a.batch, a.line, walk);
@@ -158,14 +157,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           to.head = q.head;
           to.k0 = q.lo * FEW_KEYS;
           to.k1 = min(q.hi * FEW_KEYS, q.s.len);
-          to.park = q.whole() ? -1 : (int)blockIdx.x * 2 + q.slot();
+          const PagedParts parts = paged_parts(a.line, total, blockIdx.x, q);
+          to.first = parts.first;
+          to.count = parts.count;
         }
         mbar_arrive(piece_full(slot));
         if (q.seq < 0) break;
-        if (last.seq < 0) front = q.lo > 0;
-        last = q;
       }
-      paged_note_join(a, blockIdx.x, last, front, total);
     }
   } else if (warp >= FEW_CONSUMERS) {
     // ------------------------------------------------------------------ producers
@@ -263,7 +261,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       const int slot = i % FEW_RING;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(piece_full(slot), (i / FEW_RING) & 1u, status, 211)))) break;
       volatile FewPiece &p = pieces[slot];
-      const int seq = p.seq, row = p.row, n = p.n, len = p.len, head = p.head, k0 = p.k0, k1 = p.k1, park = p.park;
+      const int seq = p.seq, row = p.row, n = p.n, len = p.len, head = p.head, k0 = p.k0, k1 = p.k1, first = p.first, parts = p.count;
       __syncwarp();
       if (lane == 0) mbar_arrive(piece_empty(slot));
       if (seq < 0) break;
@@ -386,10 +384,29 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             *reinterpret_cast<float2 *>(o_s + (warp * ROWS + g + 8 * e) * Smem::O_LD + j * 8 + 2 * c) = make_float2(o[j][e * 2], o[j][e * 2 + 1]);
       }
       if (!(ok = meet())) break;
+      // outputs by thread: 4 columns of a row, all of which go through f(row, column)
+      auto each = [&](auto &&f) {
 #pragma unroll 1
-      for (int at = threadIdx.x; at < rows * (DH / 4); at += FEW_CONSUMERS * 32) {
-        const int r = at / (DH / 4), col = (at - r * (DH / 4)) * 4;
-        if (col >= a.dh) continue;
+        for (int at = threadIdx.x; at < rows * (DH / 4); at += FEW_CONSUMERS * 32) {
+          const int r = at / (DH / 4), col = (at - r * (DH / 4)) * 4;
+          if (col < a.dh) f(r, col);
+        }
+      };
+      // divided and written, or parked in a slot
+      auto leave = [&](int slot, int r, int col, float4 acc, float top, float den) {
+        if (slot < 0) {
+          const float inv = den > 0.f ? 1.f / den : 0.f;  // a row that sees nothing: zeros
+          const int tok = paged_div(r, a.line.by_group), gi = r - tok * group;
+          char *to = a.o + (long long)(row + tok) * a.o_t + (long long)(head * group + gi) * a.o_h + col * 2;
+          *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
+        } else {
+          const long long at = (long long)slot * ROWS + r;
+          *reinterpret_cast<float4 *>(a.parts + at * DH + col) = acc;
+          if (col == 0) a.parts_ml[at] = make_float2(top, den);
+        }
+      };
+      int node = (int)blockIdx.x - first;
+      each([&](int r, int col) {
         float2 ml[FEW_CONSUMERS];
         float top = -INFINITY;
 #pragma unroll
@@ -410,21 +427,66 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           acc.w = fmaf(v.w, weight, acc.w);
           den = fmaf(ml[w].y, weight, den);
         }
-        if (park < 0) {
-          const float inv = den > 0.f ? 1.f / den : 0.f;  // a row that sees nothing: zeros
-          const int tok = paged_div(r, a.line.by_group), gi = r - tok * group;
-          char *to = a.o + (long long)(row + tok) * a.o_t + (long long)(head * group + gi) * a.o_h + col * 2;
-          *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
-        } else {
-          float *to = a.parts + ((long long)park * ROWS + r) * (DH + AP_PAD);
-          *reinterpret_cast<float4 *>(to + col) = acc;
-          if (col == 0) *reinterpret_cast<float2 *>(to + DH) = make_float2(top, den);
+        leave(parts == 1 ? -1 : paged_slot(first, node), r, col, acc, top, den);
+      });
+      // Other CTAs have the other parts: the last of 16 neighbours joins theirs, the last of up to 16 such groups those.
+      int nodes = parts, span = 1;          // of the level of the tree: nodes, CTAs of one
+#pragma unroll 1
+      for (int level = 0; nodes > 1 && ok; ++level) {
+        const int g0 = node & ~(AP_FEW_JOIN - 1), together = min(AP_FEW_JOIN, nodes - g0);
+        if (!(ok = meet())) break;  // all have parked
+        if (warp == 0) {
+          // (a group of one has no counter: its CTA may hold the first group of the next unit)
+          const bool last = together == 1 || paged_arrive_last(a.arrived + (level * a.line.ctas + first + g0 * span) * 8, together);
+          if (lane == 0) last_s = last;
         }
+        if (!(ok = meet())) break;
+        if (!*reinterpret_cast<volatile int *>(&last_s)) break;
+        __threadfence();
+        node /= AP_FEW_JOIN;
+        nodes = (nodes + AP_FEW_JOIN - 1) / AP_FEW_JOIN;
+        each([&](int r, int col) {
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float top = -INFINITY, den = 0.f;
+          constexpr int DEEP = 8;
+#pragma unroll 1
+          for (int j0 = 0; j0 < together; j0 += DEEP) {
+            float4 v[DEEP];
+            float2 ml[DEEP];
+#pragma unroll
+            for (int e = 0; e < DEEP; ++e) {
+              v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+              ml[e] = make_float2(-INFINITY, 0.f);
+              if (j0 + e < together) {
+                const int k = (g0 + j0 + e) * span, slot = level == 0 ? paged_slot(first, k) : 2 * a.line.ctas + first + k;
+                const long long from = (long long)slot * ROWS + r;
+                ml[e] = __ldcg(a.parts_ml + from);
+                v[e] = __ldcg(reinterpret_cast<const float4 *>(a.parts + from * DH + col));
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < DEEP; ++e) {
+              const float next = fmaxf(top, ml[e].x), ref = next == -INFINITY ? 0.f : next;
+              const float wa = ap_ex2(top - ref), wb = ap_ex2(ml[e].x - ref);
+              den = den * wa + ml[e].y * wb;
+              acc.x = acc.x * wa + v[e].x * wb;
+              acc.y = acc.y * wa + v[e].y * wb;
+              acc.z = acc.z * wa + v[e].z * wb;
+              acc.w = acc.w * wa + v[e].w * wb;
+              top = next;
+            }
+          }
+          // joined groups have slots of their own behind the parts': other threads may still read these
+          leave(nodes == 1 ? -1 : 2 * a.line.ctas + first + g0 * span, r, col, acc, top, den);
+        });
+        span *= AP_FEW_JOIN;
       }
+      if (!ok) break;
       if (!(ok = meet())) break;  // ml_s and o_s are free again
     }
   }
   if (!ok) gave_up = 1;
+  if (warp == FEW_CONSUMERS) pdl_wait_for_front();  // no launch ends in front of the one it started beside
   __syncthreads();
   if (gave_up) __nanosleep(1000000);  // a wait ran out: let stray copies land before the CTA goes away
 }
@@ -437,8 +499,7 @@ static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap 
   const int bytes = FewSmem<DH, NR>::BYTES;
   cudaError_t e = cudaFuncSetAttribute(attention_paged_few_kernel<DH, BF, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
-  attention_paged_few_kernel<DH, BF, NR><<<f.a.line.ctas, FEW_THREADS, bytes, s>>>(k, v, f);
-  return check_launch("attention_paged(few rows)");
+  return ap_launch_beside("attention_paged(few rows)", attention_paged_few_kernel<DH, BF, NR>, f.a.line.ctas, FEW_THREADS, bytes, s, k, v, f);
 }
 template <int DH, int NR>
 static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, bool bf16, cudaStream_t s) {

@@ -17,6 +17,8 @@
 //     issued by its own lane, which has looked its page up a block ahead.  A box behind the sequence's end, or of a page that is
 //     not there, is asked for outside the map and arrives as zeros; the slots behind the end inside the last page are zeroed in
 //     shared memory (a zero probability does not hide a NaN there).
+//   - What several CTAs share of a unit is joined inside the launch (a kernel of its own for it cost 13 us of a 4096-token prompt's
+//     141): two parts by the last warp to come, more by all their CTAs' warps together.
 //   - One persistent CTA per SM takes an equal share of the line of all units' keys (paged_schedule.h): ragged chunks, one long
 //     chunk and few heads over a long past are all the same to it.  The pieces of its share follow each other without a
 //     pause: the scheduler warp posts them ahead, K, V and Q of the next piece load and its first scores run while the softmax
@@ -42,6 +44,7 @@ constexpr int TL_THREADS = 384;
 constexpr int TL_ROWS = 128;  // of a tile
 constexpr int TL_KEYS = AP_TILE_BLOCK;
 constexpr int TL_RING = 4;    // pieces posted ahead
+constexpr unsigned long long TL_HELP_NS = 100000;  // 100 us: parts of a unit end within a few
 constexpr int TL_READERS = 11;  // warps that read the ring: all but the scheduler
 
 // A piece as the scheduler posts it.
@@ -54,7 +57,7 @@ struct TilePiece {
   int lo, hi;     // key blocks of the unit that this CTA walks
   int blocks[2];  // ... of each tile, counted from lo
   int clean;      // local block whose V rows from len on are zeroed; -1: none
-  int park;       // -1: the piece is the whole unit; else the slot of the parts
+  int first, count;  // CTAs that have parts of the unit; 1: this is all of it
 };
 
 template <int DH> struct TileSmem {
@@ -72,11 +75,18 @@ template <int DH> struct TileSmem {
   static constexpr int BYTES = OFF_STAGE + 8 * 4096 + 1024;  // 1024: alignment
 };
 
+// A unit of more than two parts, one of them this CTA's, as the scheduler notes it for the end of the share.
+struct TileHelp {
+  int first, count;        // CTAs; count <= 2: none
+  int row, tokens, head;
+};
+
 struct TileArgs {
   PagedAttnArgs a;
   int per_tile;   // tokens of a tile: 128 / group
   int box_log2;   // rows of a K or V box: min(page, 64)
   int odd_scale;  // scale <= 0
+  int behind_clear;  // the launch in front is the one that clears the counters, not the few-rows kernel's
 };
 
 __device__ __forceinline__ float tl_max3(float a, float b, float c) {
@@ -117,10 +127,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   const int group = line.group;
   int *status = batch.status + 1;  // of the waits
   __shared__ int gave_up;
+  __shared__ TileHelp help[2];  // the unit that the share begins in, the one it ends in
 
   pdl_let_next_come();
   if (threadIdx.x == 0) {
     gave_up = 0;
+    help[0].count = help[1].count = 0;
     for (int t = 0; t < 2; ++t) {
       mbar_init(q_full(t), 1);
       mbar_init(q_empty(t), 1);
@@ -331,9 +343,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
     } else {
       // ------------------------------------------------------------------ scheduler
       if (lane == 0) {
-        PagedPiece last;
-        last.seq = -1;
-        bool front = false;
         bool ok = true;
 #pragma unroll 1
         for (uint32_t i = 0; ok; ++i) {
@@ -360,14 +369,21 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
             }
             const int end = q.s.len / TL_KEYS;  // the block the sequence ends in
             to.clean = (q.s.len & ((1 << g.box_log2) - 1)) && end >= q.lo && end < q.hi ? end - q.lo : -1;
-            to.park = q.whole() ? -1 : (int)blockIdx.x * 2 + q.slot();
+            const PagedParts parts = paged_parts(line, total, blockIdx.x, q);
+            to.first = parts.first;
+            to.count = parts.count;
+            if (parts.count > 2) {
+              TileHelp &u = help[q.lo > 0 ? 0 : 1];
+              u.first = parts.first;
+              u.count = parts.count;
+              u.row = q.s.row + t0;
+              u.tokens = q.s.n - t0;
+              u.head = q.head;
+            }
           }
           mbar_arrive(ring_full(slot));
           if (q.seq < 0) break;
-          if (last.seq < 0) front = q.lo > 0;
-          last = q;
         }
-        paged_note_join(g.a, blockIdx.x, last, front, total);
         if (!ok) gave_up = 1;
       }
     }
@@ -475,18 +491,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       }
       if (!ok) break;
       const bool there = tok < g.per_tile && mine < p.tokens;
-      const int park = p.park;
+      const int first = p.first, parts = p.count;
       const long long row = p.row + mine;
       const int q_head = p.head * group + gi;
       __syncwarp();
       if (lane == 0) mbar_arrive(ring_empty(slot));
-      float *parked = g.a.parts + ((long long)park * (2 * TL_ROWS) + t * TL_ROWS + r) * (DH + AP_PAD);
-      if (nblk == 0) {  // the tile has no block in this part of the unit, or no token at all
-        if (park >= 0) *reinterpret_cast<float2 *>(parked + DH) = make_float2(-INFINITY, 0.f);
-        continue;
+      if (nblk == 0 && parts == 1) continue;  // the unit has no tokens for this tile
+      bool own = nblk > 0;                    // whether there is an O: a tile may have no block in this part of its unit
+      if (own) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_final(t), o_count++ & 1u, status, 143)))) break;
+        tc_fence_after();
       }
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_final(t), o_count++ & 1u, status, 143)))) break;
-      tc_fence_after();
       // A row is one thread's, 512 or 256 bytes of it: written as it is, every store of a warp would touch 32 lines.  128 bytes of
       // the warp's 32 rows at a time turn in shared memory instead, 16-byte pieces swizzled by the row, and leave as whole lines
       // (a piece's end 5000 -> 1900 cycles).
@@ -502,21 +517,80 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         }
         __syncwarp();
       };
-      if (park >= 0) {
-        // one part of several: park the unnormalised O with its reference point and row sum (rows that are not there too: in bounds
-        // and never read)
-        *reinterpret_cast<float2 *>(parked + DH) = make_float2(m, l);
-        char *warp_rows = reinterpret_cast<char *>(parked) - (long long)lane * ((DH + AP_PAD) * 4);
+      // Other CTAs have the other parts of the unit.  Of two, the common case in a long line of units, each warp's rows are joined by
+      // whichever of the two warps comes last, from its tensor memory and the other's parked part.  More are parked, all of them, and
+      // joined at the end of the share (see below).
+      if (parts > 1) {
+        if (g.behind_clear) pdl_wait_for_front();  // else the counters were cleared before the few-rows kernel let this one come
+        const int k = (int)blockIdx.x - first;
+        auto rows_of = [&](int k) -> long long {  // this warp's rows of the unit's k-th part
+          return (long long)paged_slot(first, k) * (2 * TL_ROWS) + t * TL_ROWS + quarter * 32;
+        };
+        uint32_t *arrived = parts == 2 ? g.a.arrived + first * 8 + (warp - 4) : g.a.arrived + (line.ctas + first) * 8;
+        bool last = parts == 2 && paged_others_parked(arrived, 2);
+        if (!last) {
+          float *mine_at = g.a.parts + rows_of(k) * DH;
+          g.a.parts_ml[rows_of(k) + lane] = make_float2(m, l);
+          if (own) {
+#pragma unroll 1
+            for (int c = 0; c < DH; c += 32) {
+              uint32_t v[32];
+              tmem_ld_32x32(to + (uint32_t)c, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 8; ++e) turn(e, make_uint4(v[e * 4], v[e * 4 + 1], v[e * 4 + 2], v[e * 4 + 3]));
+              leave([&](int rr, int e) { return reinterpret_cast<char *>(mine_at + rr * DH + c + e * 4); });
+            }
+          }
+          last = paged_arrive_last(arrived, parts == 2 ? 2 : 8 * parts) && parts == 2;
+        }
+        if (!last) {
+          tc_fence_before();
+          continue;
+        }
+        const float *theirs = g.a.parts + rows_of(k ^ 1) * DH;
+        auto fetch = [&](int c, uint4 (&x)[8]) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const uint4 *>(theirs + (e * 4 + (lane >> 3)) * DH + (lane & 7) * 4 + c));
+        };
+        uint4 x[8];
+        fetch(0, x);
+        const float2 ml = __ldcg(g.a.parts_ml + rows_of(k ^ 1) + lane);
+        const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
+        const float w_own = ap_ex2(m - ref), w_their = ap_ex2(ml.x - ref);
+        l = __fadd_rn(__fmul_rn(l, w_own), __fmul_rn(ml.y, w_their));  // products and a sum: the same whichever of the two comes last
 #pragma unroll 1
         for (int c = 0; c < DH; c += 32) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int rr = e * 4 + (lane >> 3), piece = lane & 7;
+            *reinterpret_cast<uint4 *>(stage + rr * 128 + ((piece ^ (rr & 7)) << 4)) = x[e];
+          }
+          if (c + 32 < DH) fetch(c + 32, x);
+          __syncwarp();
           uint32_t v[32];
           tmem_ld_32x32(to + (uint32_t)c, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) turn(e, make_uint4(v[e * 4], v[e * 4 + 1], v[e * 4 + 2], v[e * 4 + 3]));
-          leave([&](int rr, int e) { return warp_rows + (long long)rr * ((DH + AP_PAD) * 4) + c * 4 + e * 16; });
+          for (int e = 0; e < 32; ++e)
+            if (!own) v[e] = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(stage + lane * 128 + ((e ^ (lane & 7)) << 4));
+            const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              // a part in which the row sees nothing may have left its o unwritten
+              const float their = w_their > 0.f ? __fmul_rn(__uint_as_float(z[q]), w_their) : 0.f;
+              v[e * 4 + q] = __float_as_uint(__fadd_rn(w_own > 0.f ? __fmul_rn(__uint_as_float(v[e * 4 + q]), w_own) : 0.f, their));
+            }
+          }
+          tmem_st_32x32(to + (uint32_t)c, v);
+          __syncwarp();
         }
-      } else {
+        tmem_wait_st();
+      }
+      {
         const float inv = l > 0.f ? __frcp_rn(l) : 0.f;  // a row that sees nothing: zeros
         char *orow = there ? g.a.o + row * g.a.o_t + (long long)q_head * g.a.o_h : nullptr;
 #pragma unroll 1
@@ -544,10 +618,84 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       }
       tc_fence_before();  // the next P of this tile says that O has been read
     }
+    // Units of more than two parts (few units, long pasts): their rows are dealt out, 16 rows by 32 columns at a time, to the warps
+    // of all their CTAs.  A warp waits a while for the last part, not for good: the warp that parks the last one finds
+    // nothing to wait for, so that whatever the others have left is done by it.
+    for (int h = 0; h < 2 && ok; ++h) {
+      const volatile TileHelp &u = help[h];
+      if (u.count <= 2) continue;
+      const int first = u.first, parts = u.count, tokens = u.tokens;
+      uint32_t *arrived = g.a.arrived + (line.ctas + first) * 8, *claimed = arrived + 1;
+      bool all = false;
+      const unsigned long long since = globaltimer_ns();
+      do {
+        uint32_t n = 0;
+        if (lane == 0) n = ld_acquire_gpu(arrived);
+        all = __shfl_sync(0xffffffffu, n, 0) == (uint32_t)(8 * parts);
+      } while (!all && __all_sync(0xffffffffu, globaltimer_ns() - since < TL_HELP_NS));
+      if (!all) continue;
+      __threadfence();
+      constexpr int COLUMNS = DH / 32, ROWS = 16, MINE = ROWS / 4, DEEP = 4;  // of a slice; a lane's rows of it; parts in flight
+#pragma unroll 1
+      while (true) {
+        uint32_t n = 0;
+        if (lane == 0) n = atomicAdd(claimed, 1u);
+        const int slice = (int)__shfl_sync(0xffffffffu, n, 0);
+        if (slice >= 2 * TL_ROWS / ROWS * COLUMNS) break;
+        const int rows0 = slice / COLUMNS * ROWS, col = slice % COLUMNS * 32 + (lane & 7) * 4;
+        const int tile_tokens = tokens - (rows0 >= TL_ROWS ? g.per_tile : 0);  // from the slice's tile on
+        if ((rows0 & (TL_ROWS - 1)) >= min(tile_tokens, g.per_tile) * group) continue;
+        // a lane: 4 columns of every fourth row
+        float4 acc[MINE];
+        float top[MINE], den[MINE];
+#pragma unroll
+        for (int e = 0; e < MINE; ++e) {
+          acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+          top[e] = -INFINITY;
+          den[e] = 0.f;
+        }
+#pragma unroll 1
+        for (int k0 = 0; k0 < parts; k0 += DEEP) {
+          float4 v[DEEP][MINE];
+          float2 ml[DEEP][MINE];
+#pragma unroll
+          for (int d = 0; d < DEEP; ++d) {
+            const long long from = (long long)paged_slot(first, min(k0 + d, parts - 1)) * (2 * TL_ROWS) + rows0 + (lane >> 3);
+#pragma unroll
+            for (int e = 0; e < MINE; ++e) {
+              ml[d][e] = __ldcg(g.a.parts_ml + from + e * 4);
+              v[d][e] = __ldcg(reinterpret_cast<const float4 *>(g.a.parts + (from + e * 4) * DH + col));
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+            for (int e = 0; e < MINE; ++e) {
+              if (k0 + d >= parts || ml[d][e].x == -INFINITY) continue;  // a row that saw nothing: its o may be unwritten
+              const float next = fmaxf(top[e], ml[d][e].x);
+              const float wa = ap_ex2(top[e] - next), wb = ap_ex2(ml[d][e].x - next);
+              den[e] = den[e] * wa + ml[d][e].y * wb;
+              acc[e].x = acc[e].x * wa + v[d][e].x * wb;
+              acc[e].y = acc[e].y * wa + v[d][e].y * wb;
+              acc[e].z = acc[e].z * wa + v[d][e].z * wb;
+              acc[e].w = acc[e].w * wa + v[d][e].w * wb;
+              top[e] = next;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < MINE; ++e) {
+          const int rr = (rows0 & (TL_ROWS - 1)) + e * 4 + (lane >> 3), tk = paged_div(rr, line.by_group), hd = rr - tk * group;
+          if (tk >= g.per_tile || tk >= tile_tokens || col >= g.a.dh) continue;
+          const float inv = den[e] > 0.f ? __frcp_rn(den[e]) : 0.f;
+          char *where = g.a.o + (long long)(u.row + (rows0 >= TL_ROWS ? g.per_tile : 0) + tk) * g.a.o_t + (long long)(u.head * group + hd) * g.a.o_h + col * 2;
+          *reinterpret_cast<uint2 *>(where) = make_uint2(ap_pack<BF>(acc[e].x * inv, acc[e].y * inv), ap_pack<BF>(acc[e].z * inv, acc[e].w * inv));
+        }
+      }
+    }
     if (!ok) gave_up = 1;
   }
 
-  if (warp == 3) pdl_wait_for_front();  // the few-rows kernel, beside which this one started, has ended when this one has
+  if (warp == 3) pdl_wait_for_front();  // no launch ends in front of the one it started beside
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -558,16 +706,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
 }
 
 template <int DH, bool BF>
-static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, bool beside, cudaStream_t s) {
+static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
   const int bytes = TileSmem<DH>::BYTES;
   cudaError_t e = cudaFuncSetAttribute(attention_paged_tile_kernel<DH, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
-  return ap_launch_beside("attention_paged(tiles)", attention_paged_tile_kernel<DH, BF>, g.a.line.ctas, TL_THREADS, bytes, s, beside, q, k, v, g);
+  return ap_launch_beside("attention_paged(tiles)", attention_paged_tile_kernel<DH, BF>, g.a.line.ctas, TL_THREADS, bytes, s, q, k, v, g);
 }
 
-int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool beside, cudaStream_t s) {
+int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, cudaStream_t s) {
   TileArgs g;
   g.a = a;
+  g.behind_clear = behind_clear;
   g.per_tile = TL_ROWS / a.line.group;
   g.odd_scale = !(a.scale_log2 > 0.f);
   g.box_log2 = a.batch.page_log2 < 6 ? a.batch.page_log2 : 6;
@@ -577,8 +726,8 @@ int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool beside, cudaStr
   if (!ap_encode(&q, bf16, a.q, q_dims, q_st, (uint32_t)a.line.group, (uint32_t)g.per_tile))
     return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
   OPS_TRY(attention_paged_maps(a, bf16, 1u << g.box_log2, &k, &v));
-  if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, beside, s) : tile_launch<64, false>(g, q, k, v, beside, s);
-  return bf16 ? tile_launch<128, true>(g, q, k, v, beside, s) : tile_launch<128, false>(g, q, k, v, beside, s);
+  if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, s) : tile_launch<64, false>(g, q, k, v, s);
+  return bf16 ? tile_launch<128, true>(g, q, k, v, s) : tile_launch<128, false>(g, q, k, v, s);
 }
 
 }  // namespace ops

@@ -6,8 +6,9 @@
 // CTA c of G takes the points [cut(c), cut(c + 1)): equal shares whatever the lengths are, one sequence of 30000 keys or a
 // thousand of 30.  A cut inside a unit falls between two of its key blocks (paged_block); the two CTAs beside it compute it by
 // the same integer arithmetic.  A CTA that has only part of a unit's blocks parks what it has, in one of its TWO slots — it can
-// hold the end of one unit and the beginning of another, never more — and a second kernel joins the parts of a unit in order.
-// So the scratch depends on G alone, and the result on the batch alone: no atomics, no order of arrival.
+// hold the end of one unit and the beginning of another, never more.  The parts of a unit are joined by
+// the last to come, or with its help (nobody's result waits for a CTA that is not there yet), always in the same order: the
+// scratch depends on G alone, the result on the batch alone, not on the order of arrival.
 //
 // A point is 2^shift keys, with the least shift that keeps every line the host can expect within 31 bits: the arithmetic is
 // 32-bit throughout, without a division by anything but what the host knows, and one warp of a CTA does it.  What the others
@@ -61,7 +62,7 @@ struct PagedLine {
   int block_log2;        // keys of a block
   int shift;             // log2 of the keys of a point
   int overhead;          // points in front of a unit's keys
-  int min_share, min_share_log2;  // no CTA gets fewer points than this, a power of two, as long as one has any
+  int min_share, min_share_log2;  // no CTA gets fewer points than this, a power of two and a block at least, as long as there are any
   int ctas;
   PagedDiv by_group, by_tokens, by_ctas;
 };
@@ -169,9 +170,32 @@ struct PagedPiece {
   int head, tile;
   int lo, hi, blocks;  // key blocks [lo, hi) of `blocks`
   int begin, cost;     // of the unit, on the line
-  OPS_HD bool whole() const { return lo == 0 && hi == blocks; }
-  OPS_HD int slot() const { return lo > 0 ? 0 : 1; }
 };
+
+// The CTAs [first, first + count) that have blocks of the unit, each some; 1: the piece is all of it.  (The unit's points may lie
+// in the shares of more, whose cuts leave them none: in front of its overhead's end, or behind its last block.)
+struct PagedParts {
+  int first, count;
+};
+OPS_HD PagedParts paged_parts(const PagedLine &l, int total, int cta, const PagedPiece &q) {
+  PagedParts p;
+  p.first = cta;
+  p.count = 1;
+  if (q.lo == 0 && q.hi == q.blocks) return p;
+  if (q.lo > 0) {
+    p.first = paged_first_behind(l, total, q.begin + 1) - 1;
+    OPS_ROLLED while (paged_block(l, q.cost, q.blocks, paged_cut(l, total, p.first + 1) - q.begin) == 0) ++p.first;
+  }
+  int end = cta + 1;
+  if (q.hi < q.blocks) {
+    end = paged_first_behind(l, total, q.begin + q.cost);
+    OPS_ROLLED while (paged_block(l, q.cost, q.blocks, paged_cut(l, total, end - 1) - q.begin) == q.blocks) --end;
+  }
+  p.count = end - p.first;
+  return p;
+}
+// The slot of the k-th part of a unit: its first is the end of its CTA's share, the others are the beginnings of theirs.
+OPS_HD int paged_slot(int first, int k) { return (first + k) * 2 + (k == 0 ? 1 : 0); }
 
 // Where a CTA is on its share: sequence `seq` begins at point `begin` of the line.
 struct PagedWalk {

@@ -1,5 +1,5 @@
 // Walks the schedule of random batches on the CPU: every key block of every unit belongs to exactly one CTA, a CTA parks at most
-// one part in each of its two slots, shares are even, and a unit's parts are found again from the cuts as the joining kernel does.
+// one part in each of its two slots, shares are even, and every part of a unit knows which CTAs have the others.
 #include <algorithm>
 #include <cstdio>
 #include <cstdlib>
@@ -40,7 +40,8 @@ int main() {
     l.tokens = tile ? 2 * (128 / l.group) : few;
     l.block_log2 = tile ? 7 : 6;
     const int block = 1 << l.block_log2;
-    const int overhead = pick(1, 600), min_share = pick(1, 900);
+    // (a share holds a block at least: no CTA in the middle of a unit goes without)
+    const int overhead = pick(1, 600), min_share = pick(1 << l.block_log2, 900);
     l.ctas = std::vector<int>{1, 3, 148, 296}[pick(0, 3)];
     std::vector<PagedSeq> seqs(pick(0, round_no % 10 ? 12 : 400));
     const int big = round_no % 7 ? 300 : 20000;
@@ -75,7 +76,11 @@ int main() {
     CHECK(active >= 1 && active <= l.ctas);
     CHECK(paged_cut(l, total, 0) == 0 && paged_cut(l, total, active) == total);
     auto at = [&](int i) { return seqs[i]; };
-    std::map<std::tuple<int, int, int>, std::vector<std::tuple<int, int, int>>> units;  // (seq, head, tile) -> (lo, hi, cta * 2 + slot) of the parts
+    struct Part {
+      int lo, hi, cta;
+      PagedParts parts;
+    };
+    std::map<std::tuple<int, int, int>, std::vector<Part>> units;  // (seq, head, tile) -> its parts
     std::map<std::tuple<int, int, int>, int> blocks;
     std::map<int, int> parked;
     for (int c = 0; c < active; ++c) {
@@ -85,14 +90,16 @@ int main() {
       for (PagedPiece q = paged_next(l, nseq, w, at); q.seq >= 0; q = paged_next(l, nseq, w, at)) {
         CHECK(++steps < 1000000);
         CHECK(q.lo < q.hi && q.hi <= q.blocks && q.lo >= 0);
-        if (!q.whole()) CHECK(++parked[c * 2 + q.slot()] == 1);
-        units[{q.seq, q.head, q.tile}].push_back({q.lo, q.hi, c * 2 + q.slot()});
+        const PagedParts parts = paged_parts(l, total, c, q);
+        CHECK((parts.count == 1) == (q.lo == 0 && q.hi == q.blocks));
+        if (parts.count > 1) CHECK(++parked[paged_slot(parts.first, c - parts.first)] == 1 && paged_slot(parts.first, c - parts.first) / 2 == c);
+        units[{q.seq, q.head, q.tile}].push_back({q.lo, q.hi, c, parts});
         blocks[{q.seq, q.head, q.tile}] = q.blocks;
         keys += (q.hi - q.lo);
       }
-      // a share is its points' blocks, to within the roundings at its two ends and the short last block and tile of a unit
-      // (a point of several keys rounds the ramp of a causal unit down)
-      if (l.shift == 0) CHECK(keys <= (((long long)(paged_cut(l, total, c + 1) - paged_cut(l, total, c)) << l.shift) / block + 2 + 2 * steps) * 9 / 8);
+      // a share is its points' blocks, to within the roundings at its two ends and the short last block and tile of a unit (a point
+      // of several keys rounds the ramp of a causal unit down)
+      if (l.shift == 0) CHECK(keys <= ((long long)(paged_cut(l, total, c + 1) - paged_cut(l, total, c)) / block + 2 + 2 * steps) * 9 / 8);
     }
     size_t want = 0;
     for (int i = 0; i < nseq; ++i) {
@@ -104,38 +111,16 @@ int main() {
     }
     CHECK(units.size() == want);
     for (auto &u : units) {
-      int next = 0;
+      int next = 0, k = 0;
       for (auto &part : u.second) {
-        CHECK(std::get<0>(part) == next);
-        next = std::get<1>(part);
+        CHECK(part.lo == next && part.parts.count == (int)u.second.size() && part.parts.first + k++ == part.cta);
+        next = part.hi;
       }
       CHECK(next == blocks[u.first]);
       const PagedSeq &s = seqs[std::get<0>(u.first)];
       const int keys = paged_keys(l, s, (std::get<2>(u.first) + 1) * l.tokens);
       CHECK((long long)blocks[u.first] * block >= keys && (keys == 0 || (long long)(blocks[u.first] - 1) * block < keys));
     }
-    // the joining kernel's view: the first cut inside a unit leads to all its parts
-    size_t joined = 0, split = 0;
-    for (auto &u : units) split += u.second.size() > 1;
-    for (int c = 1; c < active; ++c) {
-      const int cut = paged_cut(l, total, c);
-      int begin = 0;
-      int i = 0;
-      while (begin + paged_span(l, seqs[i]).head * l.nkvh <= cut) begin += paged_span(l, seqs[i++]).head * l.nkvh;
-      const PagedUnit u = paged_unit(paged_span(l, seqs[i]), cut - begin);
-      if (cut == begin + u.begin || paged_cut(l, total, c - 1) > begin + u.begin) continue;
-      const int nb = paged_blocks(l, seqs[i], u.tile);
-      std::vector<std::tuple<int, int, int>> parts;
-      for (int d = c - 1; d < active && paged_cut(l, total, d) < begin + u.begin + u.cost; ++d) {
-        const int from = begin + u.begin;
-        const int lo = paged_block(l, u.cost, nb, paged_cut(l, total, d) - from), hi = paged_block(l, u.cost, nb, paged_cut(l, total, d + 1) - from);
-        if (lo < hi) parts.push_back({lo, hi, d * 2 + (lo > 0 ? 0 : 1)});
-      }
-      auto found = units.find({i, u.head, u.tile});
-      CHECK(found != units.end() && found->second == parts);
-      joined += parts.size() > 1;
-    }
-    CHECK(joined == split);
     for (int k = 0; k < 20; ++k) {
       const int x = k ? 1 + (int)(rng() % (unsigned)total) : total;
       int c = 0;
