@@ -636,12 +636,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       if (!all) continue;
       __threadfence();
       constexpr int COLUMNS = DH / 32, ROWS = 16, MINE = ROWS / 4, DEEP = 4;  // of a slice; a lane's rows of it; parts in flight
+      uint32_t claim = 0;
+      if (lane == 0) claim = atomicAdd(claimed, 1u);
 #pragma unroll 1
       while (true) {
-        uint32_t n = 0;
-        if (lane == 0) n = atomicAdd(claimed, 1u);
-        const int slice = (int)__shfl_sync(0xffffffffu, n, 0);
+        const int slice = (int)__shfl_sync(0xffffffffu, claim, 0);
         if (slice >= 2 * TL_ROWS / ROWS * COLUMNS) break;
+        if (lane == 0) claim = atomicAdd(claimed, 1u);  // the next one's, while this one is joined
         const int rows0 = slice / COLUMNS * ROWS, col = slice % COLUMNS * 32 + (lane & 7) * 4;
         const int tile_tokens = tokens - (rows0 >= TL_ROWS ? g.per_tile : 0);  // from the slice's tile on
         if ((rows0 & (TL_ROWS - 1)) >= min(tile_tokens, g.per_tile) * group) continue;
