@@ -75,7 +75,7 @@ __device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLin
     if (!looking) {
       sum += cost;
       if (i0 < b.nseq) continue;
-      // (a lane's sum stays below 2^47: 2^16 sequences of 2^31 points; its halves add up in 32 bits)
+      sum = min(sum, 1ll << 40);  // far more than a line holds; the halves of 32 such sums add up in 32 bits
       sum = (long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum & 0xffffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum >> 24)) << 24);
       // sequences that share rows (seq_start falls) can put more on the line than the host allowed for: nothing is done then
       const int total = sum <= 0x7fffffff ? (int)sum : 0;
@@ -140,9 +140,10 @@ __device__ __forceinline__ void pdl_wait_for_front() { asm volatile("griddepcont
 #endif
 
 #ifdef __CUDACC__
-// A launch that may start while the one in front of it in the stream still runs.
+// A launch with `bytes` of shared memory that may start while the one in front of it in the stream still runs.
 template <class Kernel, class... Args>
 int ap_launch_beside(const char *what, Kernel kernel, int grid, int block, int bytes, cudaStream_t s, const Args &...args) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3((unsigned)block);
@@ -153,9 +154,10 @@ int ap_launch_beside(const char *what, Kernel kernel, int grid, int block, int b
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "%s: %s", what, cudaGetErrorString(e));
-  return OPS_OK;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e == cudaSuccess) return OPS_OK;
+  cudaGetLastError();  // not the next launch's to answer for
+  return fail(OPS_EXECUTION_FAILED, "%s: %s", what, cudaGetErrorString(e));
 }
 #endif
 

@@ -430,21 +430,23 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         leave(parts == 1 ? -1 : paged_slot(first, node), r, col, acc, top, den);
       });
       // Other CTAs have the other parts: the last of 16 neighbours joins theirs, the last of up to 16 such groups those.
-      int nodes = parts, span = 1;          // of the level of the tree: nodes, CTAs of one
+      int nodes = parts, span = 1;  // of the level of the tree: nodes, parts of one
 #pragma unroll 1
       for (int level = 0; nodes > 1 && ok; ++level) {
         const int g0 = node & ~(AP_FEW_JOIN - 1), together = min(AP_FEW_JOIN, nodes - g0);
-        if (!(ok = meet())) break;  // all have parked
+        const int one = span;  // parts of a node
+        node /= AP_FEW_JOIN;
+        nodes = (nodes + AP_FEW_JOIN - 1) / AP_FEW_JOIN;
+        span *= AP_FEW_JOIN;
+        if (together == 1) continue;  // as it was parked (it has neither a counter nor a slot: paged_group_slot)
+        if (!(ok = meet())) break;    // all have parked
         if (warp == 0) {
-          // (a group of one has no counter: its CTA may hold the first group of the next unit)
-          const bool last = together == 1 || paged_arrive_last(a.arrived + (level * a.line.ctas + first + g0 * span) * 8, together);
+          const bool last = paged_arrive_last(a.arrived + (level * a.line.ctas + first + g0 * one) * 8, together);
           if (lane == 0) last_s = last;
         }
         if (!(ok = meet())) break;
         if (!*reinterpret_cast<volatile int *>(&last_s)) break;
         __threadfence();
-        node /= AP_FEW_JOIN;
-        nodes = (nodes + AP_FEW_JOIN - 1) / AP_FEW_JOIN;
         each([&](int r, int col) {
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
           float top = -INFINITY, den = 0.f;
@@ -458,8 +460,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
               v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
               ml[e] = make_float2(-INFINITY, 0.f);
               if (j0 + e < together) {
-                const int k = (g0 + j0 + e) * span, slot = level == 0 ? paged_slot(first, k) : 2 * a.line.ctas + first + k;
-                const long long from = (long long)slot * ROWS + r;
+                const int k = (g0 + j0 + e) * one;
+                const long long from = (long long)paged_group_slot(a.line, first, k, min(one, parts - k)) * ROWS + r;
                 ml[e] = __ldcg(a.parts_ml + from);
                 v[e] = __ldcg(reinterpret_cast<const float4 *>(a.parts + from * DH + col));
               }
@@ -476,10 +478,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
               top = next;
             }
           }
-          // joined groups have slots of their own behind the parts': other threads may still read these
-          leave(nodes == 1 ? -1 : 2 * a.line.ctas + first + g0 * span, r, col, acc, top, den);
+          leave(nodes == 1 ? -1 : paged_group_slot(a.line, first, g0 * one, together * one), r, col, acc, top, den);
         });
-        span *= AP_FEW_JOIN;
       }
       if (!ok) break;
       if (!(ok = meet())) break;  // ml_s and o_s are free again
@@ -497,8 +497,6 @@ int attention_paged_few_ctas(const OpBase &base) { return base.sm_count; }
 template <int DH, bool BF, int NR>
 static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
   const int bytes = FewSmem<DH, NR>::BYTES;
-  cudaError_t e = cudaFuncSetAttribute(attention_paged_few_kernel<DH, BF, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
   return ap_launch_beside("attention_paged(few rows)", attention_paged_few_kernel<DH, BF, NR>, f.a.line.ctas, FEW_THREADS, bytes, s, k, v, f);
 }
 template <int DH, int NR>

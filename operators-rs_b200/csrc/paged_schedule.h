@@ -196,6 +196,10 @@ OPS_HD PagedParts paged_parts(const PagedLine &l, int total, int cta, const Page
 }
 // The slot of the k-th part of a unit: its first is the end of its CTA's share, the others are the beginnings of theirs.
 OPS_HD int paged_slot(int first, int k) { return (first + k) * 2 + (k == 0 ? 1 : 0); }
+// The slot of parts [k, k + size) joined, behind the slots of the parts: the CTA of the k-th part has one.  (A group of one stays where
+// it is: the CTA of a unit's last part may be the first of the next unit, whose first group has that slot.  In larger groups that
+// CTA is not the first.)
+OPS_HD int paged_group_slot(const PagedLine &l, int first, int k, int size) { return size == 1 ? paged_slot(first, k) : 2 * l.ctas + first + k; }
 
 // Where a CTA is on its share: sequence `seq` begins at point `begin` of the line.
 struct PagedWalk {

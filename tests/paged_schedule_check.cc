@@ -110,6 +110,16 @@ int main() {
       want += (size_t)p.tiles * l.nkvh;
     }
     CHECK(units.size() == want);
+    // the few-rows kernel joins a unit's parts 16 at a time: no two groups share a slot, or a slot with a part
+    std::map<int, int> joined;
+    for (auto &u : units) {
+      const int count = (int)u.second.size(), first = u.second[0].parts.first;
+      for (int k = 0; count > 16 && k < count; k += 16) {
+        const int size = std::min(16, count - k), slot = paged_group_slot(l, first, k, size);
+        if (size == 1) CHECK(slot == paged_slot(first, k));
+        else CHECK(slot >= 2 * l.ctas && slot < 3 * l.ctas && ++joined[slot] == 1);
+      }
+    }
     for (auto &u : units) {
       int next = 0, k = 0;
       for (auto &part : u.second) {
