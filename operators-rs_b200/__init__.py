@@ -438,8 +438,8 @@ class PagedBatch:
     batch serves every layer of a step."""
 
     def __init__(self, page_table, seq_start, kv_len, max_seq=0):
-        self._alive = (page_table, seq_start, kv_len)
-        self.operands = tuple([_operand(t, None if isinstance(t, TensorLayout) else t) for t in self._alive])
+        self.arrays = (page_table, seq_start, kv_len)
+        self.operands = tuple([_operand(t, None if isinstance(t, TensorLayout) else t) for t in self.arrays])
         self.max_seq = int(max_seq)
 
 

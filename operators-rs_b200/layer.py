@@ -14,8 +14,8 @@ how the partials and the residual meet.
 from dataclasses import dataclass
 
 from . import (ALL_REDUCE_AUTO, ATTENTION_MAX_RUNS, ATTENTION_RUN_RECORD_BYTES, MASK_CAUSAL, AllReduce, AllReduceArgs, Attention, AttentionArgs, AttentionPaged,
-               AttentionPagedArgs, FusedSoftmax, KvAppendPaged, KvAppendPagedArgs, MatMul, MatMulArgs, Rearrange, RmsNorm, RmsNormArgs, Rope, RopeArgs,
-               RopeNormArgs, Swiglu, SwigluArgs)
+               AttentionPagedArgs, FusedSoftmax, KvAppendPaged, KvAppendPagedArgs, MatMul, MatMulArgs, PagedBatch, Rearrange, RmsNorm, RmsNormArgs, Rope,
+               RopeArgs, RopeNormArgs, Swiglu, SwigluArgs)
 
 
 @dataclass
@@ -216,17 +216,19 @@ class DecoderLayer:
         q, k, v = heads[:, : self.nq], heads[:, self.nq: self.nq + self.nkv], heads[:, self.nq + self.nkv:]
         self.kv_append_paged.launch(KvAppendPagedArgs.of(q, q, k, v, k_pages, v_pages, pos, batch, cfg.theta, self.w.get("w_qk_norm"), cfg.eps))
         mark("kv_append_paged")
-        args = AttentionPagedArgs.of(q.permute(1, 0, 2), k_pages, v_pages, att_out.view(T, self.nq, cfg.dh).permute(1, 0, 2), batch, MASK_CAUSAL)
-        self.attention_paged.launch(args, self._paged_workspace(args))
+        q = q.permute(1, 0, 2)
+        args = AttentionPagedArgs.of(q, k_pages, v_pages, att_out.view(T, self.nq, cfg.dh).permute(1, 0, 2), batch, MASK_CAUSAL)
+        self.attention_paged.launch(args, self._paged_workspace(q, k_pages, v_pages, batch))
         mark("attention_paged")
         lane = self.lanes[0]
         return self._stage_mlp(lane, self._stage_o(lane, x, 0, T, mark), 0, T, mark)
 
-    def _paged_workspace(self, args):
-        """Scratch of attention_paged, kept between steps and grown when a step wants more."""
+    def _paged_workspace(self, q, k_pages, v_pages, batch):
+        """Scratch of attention_paged: enough for a step of any kind from the first one on, because a captured step goes on using it."""
         import torch
-        need = self.attention_paged.scheme(args)
-        if self.paged_ws is None or self.paged_ws.numel() < need:
+        if self.paged_ws is None:
+            any_step = PagedBatch(*batch.arrays)  # max_seq unknown: the most that a step takes
+            need = self.attention_paged.scheme(AttentionPagedArgs.of(q, k_pages, v_pages, q, any_step, MASK_CAUSAL))
             self.paged_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         return self.paged_ws
 
