@@ -297,7 +297,7 @@ void ops_attention_kv_cached_destroy(ops_attention_kv_cached *op);
  * two from 8 to 65536.  The rows of the step are the new tokens of all sequences, packed: sequence i owns the rows
  * [seq_start[i], seq_start[i + 1]) and, the new tokens included, the cache slots [0, kv_len[i]); slot s lies in page
  * page_table[i, s / page] at s % page.  Rows in front of seq_start[0] and from seq_start[nseq] on belong to nobody and are left as
- * they are, so a captured launch can be padded.  All three are device arrays of u32 (i32 is taken as its bits), read when the
+ * they are, so a captured launch can be padded.  Sequences may share pages; what two of them append to one slot is either's.  All three are device arrays of u32 (i32 is taken as its bits), read when the
  * kernels run: a captured graph may be replayed after they have changed.
  *
  * What the arrays hold is checked where it is used; nothing outside the tensors is ever read or written.  What is wrong sets
@@ -346,7 +346,9 @@ void ops_kv_append_paged_destroy(ops_kv_append_paged *op);
 /* attention_paged: o = softmax_mask(scale q k^T) v over the sequence's own slots, grouped-query heads.  q, o [nh, nt, dh] (the order
  * of ops_attention), nh a multiple of nkvh, up to 128 query heads per kv head.  With OPS_MASK_CAUSAL the j-th of n new tokens of a
  * sequence sees the slots [0, kv_len - n + j + 1), with OPS_MASK_NONE all kv_len; a row that sees nothing becomes zeros.  Slots
- * past kv_len are never used, whatever they hold.  Scores, softmax and sums are f32, the probabilities enter the second product
+ * past kv_len are never used, whatever they hold.  (Slots that only some of a sequence's new tokens see, the later new ones, are
+ * taken for all of them with a weight of zero: an infinite or NaN value there makes the others NaN, too.)  o lies apart from q and
+ * the cache.  The workspace is scratch of one launch at a time: launches that can run at the same time need one each.  Scores, softmax and sums are f32, the probabilities enter the second product
  * in the element type, o is rounded once.  f16 or bf16, dh a multiple of 8 up to 128, unit inner strides, every row 16-byte
  * aligned, positive strides. */
 typedef struct ops_attention_paged ops_attention_paged;

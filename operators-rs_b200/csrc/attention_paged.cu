@@ -180,6 +180,7 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   OPS_TRY(paged_launch_checks(name, &a->batch, &a->k_pages_layout, a->k_pages_base, &a->v_pages_layout, a->v_pages_base, m.paged, m.nt,
                               op ? op->h.status : nullptr, &g.batch));
   if (m.nt == 0 || m.nh == 0 || m.dh == 0 || m.paged.nseq == 0) return OPS_OK;
+  if (m.paged.npages == 0) return fail(OPS_SHAPE_NOT_SUPPORT, "attention_paged: a cache without pages");
   if (!op) return fail(OPS_ARGS_NOT_SUPPORT, "null handle");
   const OpBase &base = op->h.base;
   const PagedAttnPlan plan = attention_paged_plan(base, m.nh, m.paged.nkvh, m.dh, a->mask == OPS_MASK_CAUSAL, g.batch.max_seq, m.nt, m.paged.nseq,

@@ -556,6 +556,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         uint4 x[8];
         fetch(0, x);
         const float2 ml = __ldcg(g.a.parts_ml + rows_of(k ^ 1) + lane);
+        // a part in which the row sees nothing (its sum is zero: not a NaN) may have left its o unwritten
+        const bool own_counts = l != 0.f, their_counts = ml.y != 0.f;
         const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
         const float w_own = ap_ex2(m - ref), w_their = ap_ex2(ml.x - ref);
         l = __fadd_rn(__fmul_rn(l, w_own), __fmul_rn(ml.y, w_their));  // products and a sum: the same whichever of the two comes last
@@ -580,9 +582,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
             const uint32_t z[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              // a part in which the row sees nothing may have left its o unwritten
-              const float their = w_their > 0.f ? __fmul_rn(__uint_as_float(z[q]), w_their) : 0.f;
-              v[e * 4 + q] = __float_as_uint(__fadd_rn(w_own > 0.f ? __fmul_rn(__uint_as_float(v[e * 4 + q]), w_own) : 0.f, their));
+              const float their = their_counts ? __fmul_rn(__uint_as_float(z[q]), w_their) : 0.f;
+              v[e * 4 + q] = __float_as_uint(__fadd_rn(own_counts ? __fmul_rn(__uint_as_float(v[e * 4 + q]), w_own) : 0.f, their));
             }
           }
           tmem_st_32x32(to + (uint32_t)c, v);
@@ -672,7 +673,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           for (int d = 0; d < DEEP; ++d)
 #pragma unroll
             for (int e = 0; e < MINE; ++e) {
-              if (k0 + d >= parts || ml[d][e].x == -INFINITY) continue;  // a row that saw nothing: its o may be unwritten
+              if (k0 + d >= parts || ml[d][e].y == 0.f) continue;  // a row that saw nothing: its o may be unwritten
               const float next = fmaxf(top[e], ml[d][e].x);
               const float wa = ap_ex2(top[e] - next), wb = ap_ex2(ml[d][e].x - next);
               den[e] = den[e] * wa + ml[d][e].y * wb;
@@ -709,8 +710,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
 template <int DH, bool BF>
 static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
   const int bytes = TileSmem<DH>::BYTES;
-  cudaError_t e = cudaFuncSetAttribute(attention_paged_tile_kernel<DH, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention_paged: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
   return ap_launch_beside("attention_paged(tiles)", attention_paged_tile_kernel<DH, BF>, g.a.line.ctas, TL_THREADS, bytes, s, q, k, v, g);
 }
 

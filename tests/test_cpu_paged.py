@@ -127,6 +127,7 @@ def test_attention_paged_refusals(pkg):
     at_launch(pkg.STRIDES_NOT_SUPPORT, b=batch(pkg, table=L(pkg, pkg.I32, (3, 5), (40, 8))))
     at_launch(pkg.STRIDES_NOT_SUPPORT, b=batch(pkg, start=L(pkg, pkg.I32, (4,), (8,))))
     at_launch(pkg.SHAPE_NOT_SUPPORT, b=batch(pkg, table=L(pkg, pkg.I32, (3, 1 << 27))))  # 2^31 slots a sequence
+    at_launch(pkg.SHAPE_NOT_SUPPORT, k=L(pkg, F16, (0, 2, 16, 64)), v=L(pkg, F16, (0, 2, 16, 64)))  # nothing to point a tensor map at
     # nothing to do is not an error, null pointers or not
     for kw in ({"q": L(pkg, F16, (8, 0, 64)), "o": L(pkg, F16, (8, 0, 64))},
                {"b": batch(pkg, L(pkg, pkg.I32, (0, 5)), L(pkg, pkg.I32, (1,)), L(pkg, pkg.I32, (0,)))}):

@@ -390,6 +390,53 @@ def test_attention_paged_repeats_bit_for_bit(pkg, dev, ops):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("n,kv,nkvh,nh", [([1], [9000], 9, 18), ([1, 1, 1], [12000, 11000, 12500], 3, 3), ([40], [12000], 9, 36), ([20, 30, 300], [9000, 9500, 9800], 3, 12)])
+def test_attention_paged_units_of_many_parts(pkg, dev, ops, n, kv, nkvh, nh):
+    """Nine units over all SMs: 17 or 18 parts each, joined in two rounds; the second unit's first part is the CTA of the first
+    unit's last one.  Over and over: nothing depends on who comes when."""
+    b = ref.Batch(dev, F16, n, kv, nkvh, 128, 16, seed=5)
+    g = gen(dev, 5)
+    b.fill(g)
+    q = normal(g, (nh, b.nt, 128), F16)
+    want, tol = ref.attention(b, q, True, 128 ** -0.5)
+    o = torch.empty_like(q)
+    first = None
+    for _ in range(30):
+        o.fill_(7.0)
+        attend(pkg, ops.attention, b, q, o)
+        first = o.clone() if first is None else first
+        assert torch.equal(o, first)
+    near(o, want, tol, "o")
+    assert ops.attention.status() == 0
+
+
+@pytest.mark.parametrize("n,kv,nkvh", [([1], [3000], 1), ([1, 1], [40, 9000], 2), ([30], [2500], 2), ([150, 20], [400, 6000], 1), ([1500], [1500], 2)])
+def test_attention_paged_nan_queries(pkg, dev, ops, n, kv, nkvh):
+    """A NaN in a query is that row's alone, and shows, in however many parts the row is computed; so does one in a key, in all rows
+    that see it."""
+    b = ref.Batch(dev, F16, n, kv, nkvh, 64, 16, seed=7)
+    g = gen(dev, 7)
+    b.fill(g)
+    nh = 4 * nkvh
+    q = normal(g, (nh, b.nt, 64), F16)
+    want, tol = ref.attention(b, q, True, 0.125)
+    bent = q.clone()
+    for h in range(0, nh, 3):
+        bent[h, :: 7, 5] = math.nan
+    o = torch.zeros_like(q)
+    attend(pkg, ops.attention, b, bent, o)
+    hit = torch.isnan(bent).any(-1)
+    assert bool(torch.isnan(o[hit]).all())
+    near(o[~hit], want[~hit], tol[~hit], "the other rows")
+    page, slot = b.slots(0, 3, 4)
+    b.k_pages[page, 0, slot] = math.nan
+    attend(pkg, ops.attention, b, q, o)
+    sees = torch.zeros(nh, b.nt, dtype=torch.bool, device=dev)
+    sees[:4, max(0, 3 - (kv[0] - n[0])): n[0]] = True
+    assert bool(torch.isnan(o[sees]).all())
+    near(o[~sees], want[~sees], tol[~sees], "the other rows")
+
+
 def test_attention_paged_short_workspace(pkg, dev, ops):
     """Without one the operator says how much it wants (and Operator.launch gets it)."""
     b = ref.Batch(dev, F16, [1, 90], [5000, 100], 2, 128, 16, seed=8)
@@ -495,3 +542,37 @@ def test_layer_over_a_paged_cache(pkg, dev, norm):
             near(out[at: at + n[i]], want, 2e-2 * want.abs().div(4).clamp(min=1), f"request {i}, tokens {d}..{e}")
         done = kv
     assert layer.attention_paged.status() == 0 and layer.kv_append_paged.status() == 0
+
+
+def test_layer_captured_step_after_a_larger_one(pkg, dev):
+    """A captured step of single tokens goes on working after prompts have passed through the layer: its scratch is still there."""
+    layer_mod = importlib.import_module(graft.PKG_NAME + ".layer")
+    cfg = layer_mod.LayerConfig(d=512, nh=8, nkvh=2, dh=64, ffn=1024)
+    layer = layer_mod.DecoderLayer(cfg, _weights(dev, cfg, False), 256, dev)
+    ps = 16
+    k_pages, v_pages = (normal(gen(dev, k), (80, cfg.nkvh, ps, cfg.dh), F16) for k in (1, 2))
+    table = torch.arange(80, dtype=torch.int32, device=dev).view(2, 40)
+
+    def step(n, kv):
+        at = torch.cat([torch.arange(l - x, l) for x, l in zip(n, kv)])
+        batch = pkg.PagedBatch(table, torch.tensor([0, n[0], sum(n)], dtype=torch.int32, device=dev), torch.tensor(kv, dtype=torch.int32, device=dev), max(n))
+        return at.to(torch.int32).to(dev).view(torch.uint32), batch
+
+    rows = normal(gen(dev, 3), (2, cfg.d), F16)
+    x, (pos, batch) = rows.clone(), step([1, 1], [600, 513])
+    want = layer.forward_paged(x, pos, batch, k_pages, v_pages).clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.forward_paged(x, pos, batch, k_pages, v_pages)
+    keys, values = k_pages.clone(), v_pages.clone()
+    for n, kv in (([100, 30], [130, 40]), ([1, 60], [20, 70])):
+        p, b = step(n, kv)
+        layer.forward_paged(normal(gen(dev, 4), (sum(n), cfg.d), F16), p, b, k_pages, v_pages)
+    k_pages.copy_(keys)
+    v_pages.copy_(values)
+    junk = [torch.full((2 ** 20,), math.nan, device=dev) for _ in range(64)]  # takes what is free
+    for _ in range(3):
+        x.copy_(rows)
+        graph.replay()
+        assert torch.equal(out, want)
+    assert len(junk) == 64 and layer.attention_paged.status() == 0
