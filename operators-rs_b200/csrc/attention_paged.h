@@ -56,38 +56,57 @@ __device__ __forceinline__ uint32_t ap_pack(float lo, float hi) {  // first valu
   return *reinterpret_cast<uint32_t *>(&t);
 }
 
-// CTA `cta`'s share of the line, by one warp: the points of all sequences, then the one its share begins in.  `report` says
-// whether this CTA is the one that looks for what is wrong with the batch.  All lanes get the answer (at == end: nothing).
-__device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLine &l, int cta, bool report, PagedWalk *walk, int *total_out) {
+// CTA `cta`'s share of the line, for its warp `finder`: the points of all sequences, then the one its share begins in (at == end:
+// nothing).  Up to 32 sequences are that warp's alone; of more, every warp of the CTA adds up an even part first and the finder
+// looks for its sequence in one of the parts: all warps of the CTA call, and meet once.  (One warp alone took a round trip to
+// memory per 32 sequences, twice: 30 us of 2048 decoding requests' 116.)  `report` says whether this CTA is the one that looks
+// for what is wrong with the batch.
+template <int WARPS>
+__device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLine &l, int cta, bool report, int warp, int finder, PagedWalk *walk, int *total_out) {
+  static_assert(WARPS <= 32, "a lane per part");
+  __shared__ int parts[WARPS];  // points, or -1: too many
   const int lane = threadIdx.x & 31;
   walk->seq = walk->begin = walk->at = walk->end = 0;
   *total_out = 0;
+  const bool together = b.nseq > 32;
+  if (!together && warp != finder) return;
+  const int part = together ? (b.nseq + WARPS * 32 - 1) / (WARPS * 32) * 32 : 32;
+  int i0 = together ? warp * part : 0, end = min(b.nseq, i0 + part);
   long long sum = 0;
-  int lo = 0, hi = 0, before = 0;
-  // two passes through one copy of the code: all sequences for the sum, then up to the one that is looked for
-  bool looking = false;
+  int lo = 0, before = 0;
+  bool looking = false, picking = false;  // for a sequence, for a part; both passes run through one copy of the code
 #pragma unroll 1
-  for (int i0 = 0; i0 < b.nseq;) {
+  while (true) {
     const int i = i0 + lane;
     long long cost = 0;
-    if (i < b.nseq) cost = (long long)paged_span(l, paged_seq(b, i, report && !looking)).head * l.nkvh;
+    if (i < end) cost = (long long)paged_span(l, paged_seq(b, i, report && !looking)).head * l.nkvh;
     i0 += 32;
     if (!looking) {
       sum += cost;
-      if (i0 < b.nseq) continue;
+      if (i0 < end) continue;
       sum = min(sum, 1ll << 40);  // far more than a line holds; the halves of 32 such sums add up in 32 bits
       sum = (long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum & 0xffffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum >> 24)) << 24);
+      int mine = (int)sum;
+      if (together) {
+        if (lane == 0) parts[warp] = sum <= 0x7fffffff ? (int)sum : -1;
+        __syncthreads();
+        if (warp != finder) return;
+        mine = lane < WARPS ? parts[lane] : 0;
+        sum = __any_sync(0xffffffffu, mine < 0) ? 1ll << 40
+                                                : (long long)__reduce_add_sync(0xffffffffu, (unsigned)(mine & 0xffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(mine >> 16)) << 16);
+      }
       // sequences that share rows (seq_start falls) can put more on the line than the host allowed for: nothing is done then
       const int total = sum <= 0x7fffffff ? (int)sum : 0;
       if (report && total != sum && lane == 0) atomicCAS(b.status, 0, OPS_PAGED_BAD_ROWS);
       *total_out = total;
       lo = paged_cut(l, total, cta);
-      hi = paged_cut(l, total, cta + 1);
+      const int hi = paged_cut(l, total, cta + 1);
       if (lo >= hi) return;
+      walk->at = lo;
+      walk->end = hi;
       looking = true;
-      i0 = 0;
-      if (b.nseq > 32) continue;
-      i0 = 32;  // of up to 32 sequences the costs are at hand
+      picking = together;
+      if (picking) cost = mine;
     }
     int upto = (int)cost;
 #pragma unroll
@@ -98,14 +117,19 @@ __device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLin
     const unsigned here = __ballot_sync(0xffffffffu, before + upto - (int)cost <= lo && lo < before + upto);
     if (here) {
       const int at = __ffs(here) - 1;
-      walk->seq = i0 - 32 + at;
-      walk->begin = before + __shfl_sync(0xffffffffu, upto - (int)cost, at);
-      break;
+      before += __shfl_sync(0xffffffffu, upto - (int)cost, at);
+      if (!picking) {
+        walk->seq = i0 - 32 + at;
+        walk->begin = before;
+        break;
+      }
+      picking = false;
+      i0 = at * part;
+      end = min(b.nseq, i0 + part);
+      continue;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  walk->at = lo;
-  walk->end = hi;
 }
 
 // By one thread.

@@ -6,19 +6,27 @@
 // The work is reading K and V once, 4 dh bytes a key and kv head, HBM-bound.  The keys of all (sequence, kv head) pairs form one
 // line of which every CTA, one per SM, takes an equal share (paged_schedule.h), so ragged lengths cost nothing.  What keeps the
 // memory busy is bytes in flight: 6.4 TB/s at a loaded latency of about 3 us is 130 KB per SM, more than registers hold
-// (with every lane's loads in registers, 64 KB a CTA and two CTAs an SM: 3.7 TB/s).  So one warp streams pages into a ring
-// of 32-key stages by TMA, 192 KB deep and on through the ends of pieces, and four warps take the stages in turn:
+// (with every lane's loads in registers, 64 KB a CTA and two CTAs an SM: 3.7 TB/s).  So pages stream by TMA into a ring of
+// 32-key stages, 192 KB deep and on through the ends of pieces:
 //
-//   warps 0-3  stage i goes to warp i % 4, which alone waits for it and frees it: S = Q K^T and O += P V for its 32 keys on
-//              m16n8k16 warp MMAs (the rows are the 16 of the MMA; a 128-row tcgen05 tile has nothing to chew on here), both
-//              operands by ldmatrix from the 128-byte-swizzled stage, the probabilities straight from the S registers.  At the
-//              end of a piece the four meet in shared memory, and the CTA that comes last to a unit that several share joins its parts.
-//   warp 4     producer: a lane per box of a stage (32 / min(page, 32) boxes of K and of V), pages looked up a stage ahead
-//   warp 5     scheduler: finds the CTA's share, posts its pieces ahead
+//   warps 0-3  consumers: S = Q K^T and O += P V for a stage's 32 keys on m16n8k16 warp MMAs (the rows are the 8 or 16 of the MMA;
+//              a 128-row tcgen05 tile has nothing to chew on here), both operands by ldmatrix from the 128-byte-swizzled stage,
+//              the probabilities straight from the S registers: about 1400 clocks a stage, four stages at a time
+//   warps 4-7  producers, every fourth stage each (the boxes of one warp alone come to 3.4 TB/s): a lane per box of a stage
+//              (32 / min(page, 32) boxes of K and of V), pages looked up a stage ahead
+//   warp 8     scheduler: finds the CTA's share, posts its pieces ahead
+//
+// A long piece's stages go to the consumers in turn; at its end the four meet in shared memory, and the CTA that comes last to a
+// unit that several share joins its parts.  Meeting takes some 3000 clocks, more than the stages of a short sequence: a piece that
+// takes up half of the ring at most, is all of its unit and has more behind it goes to one consumer, who meets nobody, and the
+// four work on four pieces (2048 single tokens over 100 keys each: 116 us against 133; at the end of a share, where the
+// others would have nothing, together).
 //
 // A box behind the sequence's end, or of a page that is not there, is asked for outside the map and arrives as zeros; the slots
-// behind the end inside the last page are zeroed in the stage by the warp that owns it (a zero probability does not hide a
+// behind the end inside the last page are zeroed in the stage by the warp that takes it (a zero probability does not hide a
 // NaN there).  Every wait is bounded; when one runs out its code goes to the status word and all roles unwind.
+// Measured, 8 kv heads of 128: 61 requests over up to 4096 keys 98 us, 5.9 TB/s; eight over up to 32101 keys 106 us, 6.1 TB/s;
+// one over 1001 keys 9.9 us.
 #include <cuda.h>
 
 #include "attention_paged.h"
@@ -59,31 +67,49 @@ struct FewPiece {
   int row, n, len, head;
   int k0, k1;  // keys
   int first, count;  // CTAs that have parts of the unit; 1: this is all of it
+  int whose;         // consumer that does all of it; -1: the four together
 };
 
 template <int DH, int NR> struct FewSmem {
   static constexpr int ROWS = NR * 8;
   static constexpr int HALVES = DH / 64;
   static constexpr int OPERAND = FEW_KEYS * DH * 2;  // K or V of a stage: [half][32 keys][128 B], swizzled
-  // a multiple of the consumers, so that a slot of the ring is always the same warp's
+  // a multiple of the producers, so that a slot of the ring is always the same one's
   static constexpr int STAGES = DH == 64 ? 24 : NR == 1 ? 12 : 8;
   static constexpr int Q_LD = DH + 8;  // elements; rows fall on other banks
   static constexpr int O_LD = DH + 4;
   static constexpr int OFF_RING = 0;
-  static constexpr int OFF_Q = OFF_RING + STAGES * 2 * OPERAND;                 // [2][16][Q_LD] 16-bit
-  static constexpr int OFF_O = OFF_Q + 2 * 16 * Q_LD * 2;                       // [consumers][ROWS][O_LD] f32
+  static constexpr int OFF_Q = OFF_RING + STAGES * 2 * OPERAND;                 // [piece of the ring][ROWS][Q_LD] 16-bit
+  static constexpr int OFF_O = OFF_Q + FEW_RING * ROWS * Q_LD * 2;              // [consumers][ROWS][O_LD] f32
   static constexpr int OFF_ML = OFF_O + FEW_CONSUMERS * ROWS * O_LD * 4;        // [ROWS][consumers] (m, l)
   static constexpr int OFF_PIECES = OFF_ML + ROWS * FEW_CONSUMERS * 8;
   static constexpr int OFF_BAR = OFF_PIECES + FEW_RING * (int)sizeof(FewPiece);
-  static constexpr int NUM_BARS = 2 * STAGES + 4 + 2 * FEW_RING + 1;
-  static constexpr int BYTES = OFF_BAR + NUM_BARS * 8 + 1024;  // 1024: alignment
-  static_assert(STAGES % FEW_CONSUMERS == 0 && STAGES % FEW_PRODUCERS == 0 && OFF_BAR % 8 == 0 && OFF_O % 16 == 0, "layout");
+  static constexpr int NUM_BARS = 2 * STAGES + 3 * FEW_RING + 1;
+  static constexpr int OFF_ISSUED = OFF_BAR + NUM_BARS * 8;  // [STAGES] number of the stage that was last asked for in a slot of the ring, plus 1
+  static constexpr int BYTES = OFF_ISSUED + STAGES * 4 + 1024;  // 1024: alignment
+  static_assert(STAGES % FEW_PRODUCERS == 0 && OFF_BAR % 8 == 0 && OFF_O % 16 == 0, "layout");
 };
 
 struct FewArgs {
   PagedAttnArgs a;
   int box_log2;  // rows of a box: min(page, 32)
 };
+
+// A slot of the ring is not always the same consumer's: one that came early could take the phase before last of its barrier for the
+// one it wants.  So it waits for the barrier only once its stage has been asked for, which is when the one before has been used up.
+__device__ __forceinline__ bool few_wait_issued(const volatile uint32_t *issued, uint32_t stage, int *status, int code) {
+  if (*issued == stage) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (*issued == stage) return true;
+    if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) {
+      atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+}
 
 template <int DH, bool BF, int NR>
 __global__ void __launch_bounds__(FEW_THREADS, 1)
@@ -96,11 +122,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
   const uint32_t bar0 = base + Smem::OFF_BAR;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
-  auto q_full = [&](int b) { return bar0 + 8u * (2 * ST + b); };
-  auto q_empty = [&](int b) { return bar0 + 8u * (2 * ST + 2 + b); };
-  auto piece_full = [&](int i) { return bar0 + 8u * (2 * ST + 4 + i); };
-  auto piece_empty = [&](int i) { return bar0 + 8u * (2 * ST + 4 + FEW_RING + i); };
-  const uint32_t meet_bar = bar0 + 8u * (2 * ST + 4 + 2 * FEW_RING);
+  auto q_full = [&](int i) { return bar0 + 8u * (2 * ST + i); };
+  auto piece_full = [&](int i) { return bar0 + 8u * (2 * ST + FEW_RING + i); };
+  auto piece_empty = [&](int i) { return bar0 + 8u * (2 * ST + 2 * FEW_RING + i); };  // read, by the consumers with its q
+  const uint32_t meet_bar = bar0 + 8u * (2 * ST + 3 * FEW_RING);
+  volatile uint32_t *issued = reinterpret_cast<volatile uint32_t *>(base_ptr + Smem::OFF_ISSUED);
   volatile FewPiece *pieces = reinterpret_cast<volatile FewPiece *>(base_ptr + Smem::OFF_PIECES);
   __shared__ int gave_up, last_s;
   const PagedAttnArgs &a = f.a;
@@ -110,9 +136,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 
   PagedWalk walk;
   int total = 0;
-  if (warp == FEW_CONSUMERS + FEW_PRODUCERS) {
-    paged_locate(a.batch, a.line, blockIdx.x, blockIdx.x == 0, &walk, &total);
-  } else if (warp == FEW_CONSUMERS) {
+  paged_locate<FEW_THREADS / 32>(a.batch, a.line, blockIdx.x, blockIdx.x == 0, warp, FEW_CONSUMERS + FEW_PRODUCERS, &walk, &total);
+  if (warp == FEW_CONSUMERS) {
     if (lane == 0) {
       tma_prefetch_desc(&tmap_k);
       tma_prefetch_desc(&tmap_v);
@@ -122,12 +147,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     for (int s = 0; s < ST; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(q_full(b), 1);
-      mbar_init(q_empty(b), FEW_CONSUMERS);
+      issued[s] = 0;
     }
     for (int i = 0; i < FEW_RING; ++i) {
+      mbar_init(q_full(i), 1);
       mbar_init(piece_full(i), 1);
       mbar_init(piece_empty(i), FEW_CONSUMERS + FEW_PRODUCERS);
     }
@@ -143,6 +166,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
   if (warp == FEW_CONSUMERS + FEW_PRODUCERS) {
     // ------------------------------------------------------------------ scheduler
     if (lane == 0) {
+      uint32_t alone = 0;  // pieces given to one consumer
 #pragma unroll 1
       for (uint32_t i = 0; ok; ++i) {
         const PagedPiece q = paged_step(a.batch, a.line, walk);
@@ -160,6 +184,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           const PagedParts parts = paged_parts(a.line, total, blockIdx.x, q);
           to.first = parts.first;
           to.count = parts.count;
+          to.whose = parts.count == 1 && q.hi <= ST / 2 && walk.end - walk.at >= 2 * q.cost ? (int)(alone++ % FEW_CONSUMERS) : -1;
         }
         mbar_arrive(piece_full(slot));
         if (q.seq < 0) break;
@@ -197,7 +222,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       uint32_t st = ((uint32_t)producer - count) % FEW_PRODUCERS;
       int page = look_up(k0 + (int)st * FEW_KEYS);
       // the piece's q rows, zeros behind them: read now by the first producer, written once its first stage is asked for
-      constexpr int Q_VECS = 16 * DH / 8 / 32;  // 16-byte pieces a lane
+      constexpr int Q_VECS = ROWS * DH / 8 / 32;  // 16-byte pieces a lane
       uint4 qv[Q_VECS];
       bool q_due = producer == 0;
       if (q_due) {
@@ -217,6 +242,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           if (lane == 0) {
             ok = mbar_wait(empty(s), ((at / ST) & 1u) ^ 1u, status, 204);
             if (ok) mbar_arrive_expect_tx(full(s), 2 * Smem::OPERAND);
+            if (ok) issued[s] = at + 1;
           }
           ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0);
           if (!ok) break;
@@ -232,15 +258,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
         if (q_due) {
           q_due = false;
-          const int b = i & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(q_empty(b), ((i >> 1) & 1u) ^ 1u, status, 203));
+          // (the consumers have read what was there: this piece would not have been posted otherwise)
 #pragma unroll
           for (int e = 0; e < Q_VECS; ++e) {
             const int at = e * 32 + lane, qr = at / (DH / 8), col = (at - qr * (DH / 8)) * 8;
-            *reinterpret_cast<uint4 *>(base_ptr + Smem::OFF_Q + ((b * 16 + qr) * Smem::Q_LD + col) * 2) = qv[e];
+            *reinterpret_cast<uint4 *>(base_ptr + Smem::OFF_Q + ((slot * ROWS + qr) * Smem::Q_LD + col) * 2) = qv[e];
           }
           __syncwarp();
-          if (ok && lane == 0) mbar_arrive(q_full(b));
+          if (lane == 0) mbar_arrive(q_full(slot));
         }
       }
       count += stages;
@@ -261,35 +286,62 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       const int slot = i % FEW_RING;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(piece_full(slot), (i / FEW_RING) & 1u, status, 211)))) break;
       volatile FewPiece &p = pieces[slot];
-      const int seq = p.seq, row = p.row, n = p.n, len = p.len, head = p.head, k0 = p.k0, k1 = p.k1, first = p.first, parts = p.count;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(piece_empty(slot));
+      const int seq = p.seq, row = p.row, n = p.n, len = p.len, head = p.head, k0 = p.k0, k1 = p.k1, first = p.first, parts = p.count, whose = p.whose;
       if (seq < 0) break;
       const int rows = n * group;
+      const uint32_t stages = k1 > k0 ? (uint32_t)(k1 - k0 + FEW_KEYS - 1) / FEW_KEYS : 0u;
+      const bool mine = whose < 0 || whose == warp;
       uint32_t q[DH / 16][4];
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full(i & 1), (i >> 1) & 1u, status, 212)))) break;
+      if (mine) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full(slot), (i / FEW_RING) & 1u, status, 212)))) break;
+        const uint32_t q_at = base + Smem::OFF_Q + slot * ROWS * Smem::Q_LD * 2;
+        if (NR == 2) {
 #pragma unroll
-      for (int ks = 0; ks < DH / 16; ++ks)  // rows 0-7 | 8-15 of k 0-7, then of k 8-15
-        ldsm(base + Smem::OFF_Q + ((((i & 1) * 16 + (mi & 1) * 8 + mr) * Smem::Q_LD + ks * 16 + (mi >> 1) * 8) * 2), q[ks]);
+          for (int ks = 0; ks < DH / 16; ++ks)  // rows 0-7 | 8-15 of k 0-7, then of k 8-15
+            ldsm(q_at + (((mi & 1) * 8 + mr) * Smem::Q_LD + ks * 16 + (mi >> 1) * 8) * 2, q[ks]);
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < DH / 16; ks += 2) {  // k 0-7 | 8-15 of two steps; there are no rows 8-15
+            uint32_t two[4];
+            ldsm(q_at + (mr * Smem::Q_LD + ks * 16 + mi * 8) * 2, two);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              q[ks + e][0] = two[e * 2];
+              q[ks + e][2] = two[e * 2 + 1];
+              q[ks + e][1] = q[ks + e][3] = 0;
+            }
+          }
+        }
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_empty(i & 1));
+      if (lane == 0) mbar_arrive(piece_empty(slot));
+      if (!mine) {
+        count += stages;
+        continue;
+      }
       // last visible key of rows g and g + 8; every row sees the keys in front of `all`
-      int lim[2];
+      int lim[NR];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) lim[e] = a.line.causal ? len - n + paged_div(g + 8 * e, a.line.by_group) : len - 1;
+      for (int e = 0; e < NR; ++e) lim[e] = a.line.causal ? len - n + paged_div(g + 8 * e, a.line.by_group) : len - 1;
       const int all = min(k1, a.line.causal ? len - n + 1 : len);
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m is common to the four lanes of a row, l is this lane's share
+      float m[NR], l[NR];  // m is common to the four lanes of a row, l is this lane's share
+#pragma unroll
+      for (int e = 0; e < NR; ++e) {
+        m[e] = -INFINITY;
+        l[e] = 0.f;
+      }
       float o[DH / 8][4];
 #pragma unroll
       for (int j = 0; j < DH / 8; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
 
-      const uint32_t stages = k1 > k0 ? (uint32_t)(k1 - k0 + FEW_KEYS - 1) / FEW_KEYS : 0u;
+      const uint32_t step = whose < 0 ? FEW_CONSUMERS : 1;
 #pragma unroll 1
-      for (uint32_t st = ((uint32_t)warp - count) % FEW_CONSUMERS; st < stages; st += FEW_CONSUMERS) {
+      for (uint32_t st = whose < 0 ? ((uint32_t)warp - count) % FEW_CONSUMERS : 0u; st < stages; st += step) {
         const uint32_t at = count + st;
         const int s = at % ST, kb = k0 + (int)st * FEW_KEYS;
+        if (!(ok = __all_sync(0xffffffffu, few_wait_issued(issued + s, at + 1, status, 214)))) break;
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(full(s), (at / ST) & 1u, status, 213)))) break;
         const uint32_t ks_base = base + Smem::OFF_RING + s * (2 * Smem::OPERAND), vs_base = ks_base + Smem::OPERAND;
         if (kb + FEW_KEYS > len) {  // behind the end: may hold anything, a NaN too
@@ -317,9 +369,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             few_mma<BF>(x[np * 2 + 1], q[ks], b[2], b[3]);
           }
         uint32_t pa[2][4];  // the probabilities as the second product's A: 16 keys each
-        float al[2];
+        if (NR == 1) pa[0][1] = pa[0][3] = pa[1][1] = pa[1][3] = 0;
+        float al[NR];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < NR; ++e) {
           float mx = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -345,14 +398,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           l[e] = fmaf(l[e], al[e], sum);
           m[e] = m_new;
         }
-        if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+        if (__any_sync(0xffffffffu, al[0] != 1.f || al[NR - 1] != 1.f)) {
 #pragma unroll
-          for (int j = 0; j < DH / 8; ++j) {
-            o[j][0] *= al[0];
-            o[j][1] *= al[0];
-            o[j][2] *= al[1];
-            o[j][3] *= al[1];
-          }
+          for (int j = 0; j < DH / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 2 * NR; ++e) o[j][e] *= al[e >> 1];
         }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -370,13 +420,33 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       if (!ok) break;
       count += stages;
 
+#pragma unroll
+      for (int e = 0; e < NR; ++e) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      }
+      auto out_row = [&](int r) -> char * {
+        const int tok = paged_div(r, a.line.by_group), gi = r - tok * group;
+        return a.o + (long long)(row + tok) * a.o_t + (long long)(head * group + gi) * a.o_h;
+      };
+      if (whose >= 0) {  // nobody to wait for
+#pragma unroll
+        for (int e = 0; e < NR; ++e) {
+          if (g + 8 * e >= rows) continue;
+          const float inv = l[e] > 0.f ? 1.f / l[e] : 0.f;  // a row that sees nothing: zeros
+          char *to = out_row(g + 8 * e);
+#pragma unroll
+          for (int j = 0; j < DH / 8; ++j)
+            if (j * 8 < a.dh) *reinterpret_cast<uint32_t *>(to + (j * 8 + 2 * c) * 2) = ap_pack<BF>(o[j][e * 2] * inv, o[j][e * 2 + 1] * inv);
+        }
+        continue;
+      }
+
       // the four warps meet: each leaves its m, l and o, and the threads that finish an output weigh them
       float2 *ml_s = reinterpret_cast<float2 *>(base_ptr + Smem::OFF_ML);
       float *o_s = reinterpret_cast<float *>(base_ptr + Smem::OFF_O);
 #pragma unroll
       for (int e = 0; e < NR; ++e) {
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
         if (c == 0) ml_s[(g + 8 * e) * FEW_CONSUMERS + warp] = make_float2(m[e], l[e]);
         if (g + 8 * e < rows)
 #pragma unroll
@@ -396,9 +466,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       auto leave = [&](int slot, int r, int col, float4 acc, float top, float den) {
         if (slot < 0) {
           const float inv = den > 0.f ? 1.f / den : 0.f;  // a row that sees nothing: zeros
-          const int tok = paged_div(r, a.line.by_group), gi = r - tok * group;
-          char *to = a.o + (long long)(row + tok) * a.o_t + (long long)(head * group + gi) * a.o_h + col * 2;
-          *reinterpret_cast<uint2 *>(to) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
+          *reinterpret_cast<uint2 *>(out_row(r) + col * 2) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
         } else {
           const long long at = (long long)slot * ROWS + r;
           *reinterpret_cast<float4 *>(a.parts + at * DH + col) = acc;

@@ -130,6 +130,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   __shared__ TileHelp help[2];  // the unit that the share begins in, the one it ends in
 
   pdl_let_next_come();
+  PagedWalk walk;
+  int total = 0;
+  paged_locate<TL_THREADS / 32>(batch, line, blockIdx.x, blockIdx.x == 0, warp, 3, &walk, &total);
   if (threadIdx.x == 0) {
     gave_up = 0;
     help[0].count = help[1].count = 0;
@@ -154,9 +157,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
     }
     fence_barrier_init();
   }
-  PagedWalk walk;
-  int total = 0;
-  if (warp == 3) paged_locate(batch, line, blockIdx.x, blockIdx.x == 0, &walk, &total);
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
