@@ -209,11 +209,16 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   const bool bf16 = m.dt == OPS_DT_BF16;
   char *at = (char *)(((uintptr_t)ws + 255) / 256 * 256);
   PagedAttnArgs few = g, tile = g;
-  few.line = plan.few;
+  few.line = tile.beside = plan.few;
   few.arrived = (uint32_t *)at;
   few.parts = (float *)(at + plan.few_arrived + plan.tile_arrived);
   few.parts_ml = (float2 *)(few.parts + 3 * (usz)plan.few.ctas * plan.few_rows * plan.part_dh);
-  tile.line = plan.tile;
+  tile.line = few.beside = plan.tile;
+  if (plan.few.ctas && plan.tile.ctas)
+    for (int k = 0; k < AP_SHARES; ++k) {
+      few.by_ctas[k] = paged_div_by((uint32_t)paged_share(plan.few.ctas, k));
+      tile.by_ctas[k] = paged_div_by((uint32_t)std::max(1, plan.tile.ctas - paged_share(plan.tile.ctas, k)));
+    }
   tile.arrived = (uint32_t *)(at + plan.few_arrived);
   tile.parts = (float *)(at + plan.few_arrived + plan.tile_arrived + plan.few_parts);
   tile.parts_ml = (float2 *)(tile.parts + 2 * (usz)plan.tile.ctas * AP_TILE_ROWS * plan.part_dh);

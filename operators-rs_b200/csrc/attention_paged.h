@@ -11,6 +11,7 @@ namespace ops {
 constexpr int AP_MAX_DH = 128;
 constexpr int AP_MAX_GROUP = 128;
 constexpr int AP_MAX_CTAS = 256;  // of a kernel
+constexpr int AP_SHARES = 16;     // the few-rows kernel gets k / 16 of the CTAs where both kernels have work
 constexpr int AP_FEW_JOIN = 16, AP_LEVELS = 2;  // parts are joined in groups, the groups in turn: 16^2 is AP_MAX_CTAS
 
 struct PagedAttnArgs {
@@ -27,7 +28,12 @@ struct PagedAttnArgs {
   // lines, and (m, l), its reference point and sum
   float *parts;
   float2 *parts_ml;
+  PagedLine beside;             // the other kernel's line; ctas == 0: not launched
+  PagedDiv by_ctas[AP_SHARES];  // by the CTAs that this kernel takes of a launch of both, by paged_share
 };
+
+// The few-rows kernel's CTAs for k of 16 shares; the tile kernel gets the others.
+OPS_HD int paged_share(int ctas, int k) { return ctas * k / AP_SHARES > 0 ? ctas * k / AP_SHARES : 1; }
 
 // Tensor maps over the whole cache, boxes of 64 columns x `rows` slots of one head of one page, 128-byte swizzle.
 int attention_paged_maps(const PagedAttnArgs &a, bool bf16, uint32_t rows, CUtensorMap *k, CUtensorMap *v);
@@ -61,10 +67,21 @@ __device__ __forceinline__ uint32_t ap_pack(float lo, float hi) {  // first valu
 // looks for its sequence in one of the parts: all warps of the CTA call, and meet once.  (One warp alone took a round trip to
 // memory per 32 sequences, twice: 30 us of 2048 decoding requests' 116.)  `report` says whether this CTA is the one that looks
 // for what is wrong with the batch.
-template <int WARPS>
-__device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLine &l, int cta, bool report, int warp, int finder, PagedWalk *walk, int *total_out) {
+//
+// Where the line of the other kernel is not empty either, the two split the CTAs, and the SMs with them: the tile kernel's start on the
+// SMs that the few-rows kernel leaves.  One after the other, the first would leave the tensor cores idle and the second the memory;
+// and of the 148 SMs 96 are enough to read as fast as all (72: 89 %, 48: 63 %).  The split makes both take as long, by what a key costs
+// an SM: 4 dh bytes at 68 GB/s, or 4 dh flops for each of 256 rows at 7 TFLOP/s, 2.5 times as long (a chunk of 487 tokens beside 31
+// single ones over up to 2900 keys: 72 us, 86 one after the other).  Short sequences are bound by their number, not by the
+// memory, and gain nothing from fewer SMs (512 single tokens over 100 keys beside eight prompts of 700 tokens: 72 us, 66 one after
+// the other): then only a small share of the work runs beside the other's (64 of them: 47 us, 53 one after the other).  `l` comes
+// back with its CTAs.
+template <int WARPS, bool FEW>
+__device__ __forceinline__ void paged_locate(const PagedAttnArgs &a, PagedLine &l, int cta, bool report, int warp, int finder, PagedWalk *walk, int *total_out) {
   static_assert(WARPS <= 32, "a lane per part");
-  __shared__ int parts[WARPS];  // points, or -1: too many
+  __shared__ int parts[3][WARPS];  // points of the line (-1: too many), of the other in 64s, sequences with a few rows
+  const PagedBatch &b = a.batch;
+  const bool both = a.beside.ctas > 0;
   const int lane = threadIdx.x & 31;
   walk->seq = walk->begin = walk->at = walk->end = 0;
   *total_out = 0;
@@ -72,33 +89,66 @@ __device__ __forceinline__ void paged_locate(const PagedBatch &b, const PagedLin
   if (!together && warp != finder) return;
   const int part = together ? (b.nseq + WARPS * 32 - 1) / (WARPS * 32) * 32 : 32;
   int i0 = together ? warp * part : 0, end = min(b.nseq, i0 + part);
-  long long sum = 0;
+  long long sum = 0, sum_beside = 0;
+  int few_seqs = 0;
   int lo = 0, before = 0;
+  auto all_lanes = [](long long x) -> long long {  // the sum of non-negative numbers
+    x = min(x, 1ll << 40);  // far more than a line holds; the halves of 32 such sums add up in 32 bits
+    return (long long)__reduce_add_sync(0xffffffffu, (unsigned)(x & 0xffffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(x >> 24)) << 24);
+  };
   bool looking = false, picking = false;  // for a sequence, for a part; both passes run through one copy of the code
 #pragma unroll 1
   while (true) {
     const int i = i0 + lane;
     long long cost = 0;
-    if (i < end) cost = (long long)paged_span(l, paged_seq(b, i, report && !looking)).head * l.nkvh;
+    if (i < end) {
+      const PagedSeq s = paged_seq(b, i, report && !looking);
+      cost = (long long)paged_span(l, s).head * l.nkvh;
+      if (both && !looking) {
+        const long long other = (long long)paged_span(a.beside, s).head * l.nkvh;
+        sum_beside += other;
+        few_seqs += (FEW ? cost : other) > 0;
+      }
+    }
     i0 += 32;
     if (!looking) {
       sum += cost;
       if (i0 < end) continue;
-      sum = min(sum, 1ll << 40);  // far more than a line holds; the halves of 32 such sums add up in 32 bits
-      sum = (long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum & 0xffffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(sum >> 24)) << 24);
-      int mine = (int)sum;
+      sum = all_lanes(sum);
+      int mine = (int)sum, theirs = 0;
+      if (both) {  // to weigh the two lines against each other: near enough
+        theirs = __reduce_add_sync(0xffffffffu, (int)(sum_beside >> 6));
+        few_seqs = __reduce_add_sync(0xffffffffu, few_seqs);
+      }
       if (together) {
-        if (lane == 0) parts[warp] = sum <= 0x7fffffff ? (int)sum : -1;
+        if (lane == 0) {
+          parts[0][warp] = sum <= 0x7fffffff ? mine : -1;
+          parts[1][warp] = theirs;
+          parts[2][warp] = few_seqs;
+        }
         __syncthreads();
         if (warp != finder) return;
-        mine = lane < WARPS ? parts[lane] : 0;
-        sum = __any_sync(0xffffffffu, mine < 0) ? 1ll << 40
-                                                : (long long)__reduce_add_sync(0xffffffffu, (unsigned)(mine & 0xffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(mine >> 16)) << 16);
+        mine = lane < WARPS ? parts[0][lane] : 0;
+        sum = all_lanes(mine < 0 ? 1ll << 40 : mine);
+        if (both) {
+          theirs = __reduce_add_sync(0xffffffffu, lane < WARPS ? parts[1][lane] : 0);
+          few_seqs = __reduce_add_sync(0xffffffffu, lane < WARPS ? parts[2][lane] : 0);
+        }
       }
       // sequences that share rows (seq_start falls) can put more on the line than the host allowed for: nothing is done then
       const int total = sum <= 0x7fffffff ? (int)sum : 0;
       if (report && total != sum && lane == 0) atomicCAS(b.status, 0, OPS_PAGED_BAD_ROWS);
       *total_out = total;
+      if (both && total > 0 && theirs > 0) {
+        const float here = (float)total * (float)(1u << l.shift), there = (float)theirs * 64.f * (float)(1u << a.beside.shift);
+        const float few = FEW ? here : there, tile = 2.5f * (FEW ? there : here);  // in what a key costs the few-rows kernel
+        if (few >= 768.f * (float)(few_seqs * l.nkvh) || 13.f * few <= 3.f * tile) {  // 640 keys a unit and more, or 3 / 16 of the work
+          const int k = min(max(__float2int_rn(AP_SHARES * few / (few + tile)), 1), AP_SHARES * 3 / 4);
+          l.ctas = FEW ? paged_share(l.ctas, k) : l.ctas - paged_share(l.ctas, k);
+          l.by_ctas = a.by_ctas[k];
+        }
+      }
+      if (cta >= l.ctas) return;
       lo = paged_cut(l, total, cta);
       const int hi = paged_cut(l, total, cta + 1);
       if (lo >= hi) return;

@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 
   PagedWalk walk;
   int total = 0;
-  paged_locate<FEW_THREADS / 32>(a.batch, a.line, blockIdx.x, blockIdx.x == 0, warp, FEW_CONSUMERS + FEW_PRODUCERS, &walk, &total);
+  PagedLine line = a.line;  // the scheduler's, with the CTAs that have a part of it; `a.line.ctas` is what the workspace is laid out for
+  paged_locate<FEW_THREADS / 32, true>(a, line, blockIdx.x, blockIdx.x == 0, warp, FEW_CONSUMERS + FEW_PRODUCERS, &walk, &total);
   if (warp == FEW_CONSUMERS) {
     if (lane == 0) {
       tma_prefetch_desc(&tmap_k);
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       uint32_t alone = 0;  // pieces given to one consumer
 #pragma unroll 1
       for (uint32_t i = 0; ok; ++i) {
-        const PagedPiece q = paged_step(a.batch, a.line, walk);
+        const PagedPiece q = paged_step(a.batch, line, walk);
         const int slot = i % FEW_RING;
         if (!(ok = mbar_wait(piece_empty(slot), ((i / FEW_RING) & 1u) ^ 1u, status, 201))) break;
         volatile FewPiece &to = pieces[slot];
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           to.head = q.head;
           to.k0 = q.lo * FEW_KEYS;
           to.k1 = min(q.hi * FEW_KEYS, q.s.len);
-          const PagedParts parts = paged_parts(a.line, total, blockIdx.x, q);
+          const PagedParts parts = paged_parts(line, total, blockIdx.x, q);
           to.first = parts.first;
           to.count = parts.count;
           to.whose = parts.count == 1 && q.hi <= ST / 2 && walk.end - walk.at >= 2 * q.cost ? (int)(alone++ % FEW_CONSUMERS) : -1;

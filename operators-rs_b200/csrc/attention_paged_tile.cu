@@ -132,7 +132,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   pdl_let_next_come();
   PagedWalk walk;
   int total = 0;
-  paged_locate<TL_THREADS / 32>(batch, line, blockIdx.x, blockIdx.x == 0, warp, 3, &walk, &total);
+  PagedLine share = line;  // the scheduler's, with the CTAs that have a part of it; `line.ctas` is what the workspace is laid out for
+  paged_locate<TL_THREADS / 32, false>(g.a, share, blockIdx.x, blockIdx.x == 0, warp, 3, &walk, &total);
   if (threadIdx.x == 0) {
     gave_up = 0;
     help[0].count = help[1].count = 0;
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         bool ok = true;
 #pragma unroll 1
         for (uint32_t i = 0; ok; ++i) {
-          const PagedPiece q = paged_step(batch, line, walk);
+          const PagedPiece q = paged_step(batch, share, walk);
           const int slot = i % TL_RING;
           if (!(ok = mbar_wait(ring_empty(slot), ((i / TL_RING) & 1u) ^ 1u, status, 130))) break;
           volatile TilePiece &to = ring[slot];
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
             }
             const int end = q.s.len / TL_KEYS;  // the block the sequence ends in
             to.clean = (q.s.len & ((1 << g.box_log2) - 1)) && end >= q.lo && end < q.hi ? end - q.lo : -1;
-            const PagedParts parts = paged_parts(line, total, blockIdx.x, q);
+            const PagedParts parts = paged_parts(share, total, blockIdx.x, q);
             to.first = parts.first;
             to.count = parts.count;
             if (parts.count > 2) {
