@@ -196,13 +196,17 @@ __device__ __forceinline__ bool paged_others_parked(const uint32_t *arrived, int
   if (all) __threadfence();
   return all;
 }
-// The caller's warp has parked its part: whether it was the last of the group, as above.
-__device__ __forceinline__ bool paged_arrive_last(uint32_t *arrived, int group) {
+// The caller's warp has parked its part: the count as it was before.
+__device__ __forceinline__ uint32_t paged_arrive(uint32_t *arrived) {
   __threadfence();
   __syncwarp();
   uint32_t before = 0;
   if ((threadIdx.x & 31) == 0) before = atomicAdd(arrived, 1u);
-  const bool last = __shfl_sync(0xffffffffu, before, 0) == (uint32_t)(group - 1);
+  return __shfl_sync(0xffffffffu, before, 0);
+}
+// ... whether it was the last of the group, as above.
+__device__ __forceinline__ bool paged_arrive_last(uint32_t *arrived, int group) {
+  const bool last = paged_arrive(arrived) == (uint32_t)(group - 1);
   if (last) __threadfence();
   return last;
 }

@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   int *status = batch.status + 1;  // of the waits
   __shared__ int gave_up;
   __shared__ TileHelp help[2];  // the unit that the share begins in, the one it ends in
+  __shared__ uint32_t tickets[2][8];  // of the softmax warps for these: what paged_arrive said
 
   pdl_let_next_come();
   PagedWalk walk;
@@ -528,22 +529,27 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           return (long long)paged_slot(first, k) * (2 * TL_ROWS) + t * TL_ROWS + quarter * 32;
         };
         uint32_t *arrived = parts == 2 ? g.a.arrived + first * 8 + (warp - 4) : g.a.arrived + (line.ctas + first) * 8;
+        const bool counts = l != 0.f;  // a row that sees nothing in this part (a NaN is something) has zeros for its o, whatever V holds
         bool last = parts == 2 && paged_others_parked(arrived, 2);
         if (!last) {
           float *mine_at = g.a.parts + rows_of(k) * DH;
           g.a.parts_ml[rows_of(k) + lane] = make_float2(m, l);
-          if (own) {
 #pragma unroll 1
-            for (int c = 0; c < DH; c += 32) {
-              uint32_t v[32];
-              tmem_ld_32x32(to + (uint32_t)c, v);
-              tmem_wait_ld();
+          for (int c = 0; c < DH; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32(to + (uint32_t)c, v);
+            tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 8; ++e) turn(e, make_uint4(v[e * 4], v[e * 4 + 1], v[e * 4 + 2], v[e * 4 + 3]));
-              leave([&](int rr, int e) { return reinterpret_cast<char *>(mine_at + rr * DH + c + e * 4); });
-            }
+            for (int e = 0; e < 32; ++e)
+              if (!counts) v[e] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) turn(e, make_uint4(v[e * 4], v[e * 4 + 1], v[e * 4 + 2], v[e * 4 + 3]));
+            leave([&](int rr, int e) { return reinterpret_cast<char *>(mine_at + rr * DH + c + e * 4); });
           }
-          last = paged_arrive_last(arrived, parts == 2 ? 2 : 8 * parts) && parts == 2;
+          const uint32_t ticket = paged_arrive(arrived);
+          last = parts == 2 && ticket == 1;
+          if (last) __threadfence();
+          if (lane == 0) tickets[k == 0][warp - 4] = ticket;
         }
         if (!last) {
           tc_fence_before();
@@ -557,8 +563,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         uint4 x[8];
         fetch(0, x);
         const float2 ml = __ldcg(g.a.parts_ml + rows_of(k ^ 1) + lane);
-        // a part in which the row sees nothing (its sum is zero: not a NaN) may have left its o unwritten
-        const bool own_counts = l != 0.f, their_counts = ml.y != 0.f;
         const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
         const float w_own = ap_ex2(m - ref), w_their = ap_ex2(ml.x - ref);
         l = __fadd_rn(__fmul_rn(l, w_own), __fmul_rn(ml.y, w_their));  // products and a sum: the same whichever of the two comes last
@@ -575,16 +579,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           tmem_ld_32x32(to + (uint32_t)c, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!own) v[e] = 0;
-#pragma unroll
           for (int e = 0; e < 8; ++e) {
             const uint4 y = *reinterpret_cast<const uint4 *>(stage + lane * 128 + ((e ^ (lane & 7)) << 4));
             const uint32_t z[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const float their = their_counts ? __fmul_rn(__uint_as_float(z[q]), w_their) : 0.f;
-              v[e * 4 + q] = __float_as_uint(__fadd_rn(own_counts ? __fmul_rn(__uint_as_float(v[e * 4 + q]), w_own) : 0.f, their));
+              const float mine = counts ? __fmul_rn(__uint_as_float(v[e * 4 + q]), w_own) : 0.f;
+              v[e * 4 + q] = __float_as_uint(__fadd_rn(mine, __fmul_rn(__uint_as_float(z[q]), w_their)));
             }
           }
           tmem_st_32x32(to + (uint32_t)c, v);
@@ -621,78 +622,105 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       tc_fence_before();  // the next P of this tile says that O has been read
     }
     // Units of more than two parts (few units, long pasts): their rows are dealt out, 16 rows by 32 columns at a time, to the warps
-    // of all their CTAs.  A warp waits a while for the last part, not for good: the warp that parks the last one finds
-    // nothing to wait for, so that whatever the others have left is done by it.
+    // of all their CTAs in the order in which these parked their parts.  A warp waits a while for the last part, not for good: when
+    // its patience ends it marks its slices as left and goes, and the warp that parks the last part, which finds nothing to wait
+    // for, does what was left.  (A word counts the parts in its low half and those who left in its high half; who finds that all
+    // parts have come as it leaves stays.)
     for (int h = 0; h < 2 && ok; ++h) {
       const volatile TileHelp &u = help[h];
       if (u.count <= 2) continue;
       const int first = u.first, parts = u.count, tokens = u.tokens;
-      uint32_t *arrived = g.a.arrived + (line.ctas + first) * 8, *claimed = arrived + 1;
+      __syncwarp();
+      const uint32_t warps = 8 * (uint32_t)parts, arrival = tickets[h][warp - 4], ticket = arrival & 0xffffu;
+      uint32_t *arrived = g.a.arrived + (line.ctas + first) * 8;
+      auto left = [&](uint32_t t) -> uint32_t * {  // bits of the warps with tickets [8 k, 8 k + 8); the last CTA may be the first of the next unit
+        const int k = (int)(t >> 3);
+        return arrived + k * 8 + (k == parts - 1 ? 2 : 1);
+      };
       bool all = false;
       const unsigned long long since = globaltimer_ns();
       do {
         uint32_t n = 0;
         if (lane == 0) n = ld_acquire_gpu(arrived);
-        all = __shfl_sync(0xffffffffu, n, 0) == (uint32_t)(8 * parts);
+        all = (__shfl_sync(0xffffffffu, n, 0) & 0xffffu) == warps;
       } while (!all && __all_sync(0xffffffffu, globaltimer_ns() - since < TL_HELP_NS));
-      if (!all) continue;
-      __threadfence();
-      constexpr int COLUMNS = DH / 32, ROWS = 16, MINE = ROWS / 4, DEEP = 4;  // of a slice; a lane's rows of it; parts in flight
-      uint32_t claim = 0;
-      if (lane == 0) claim = atomicAdd(claimed, 1u);
-#pragma unroll 1
-      while (true) {
-        const int slice = (int)__shfl_sync(0xffffffffu, claim, 0);
-        if (slice >= 2 * TL_ROWS / ROWS * COLUMNS) break;
-        if (lane == 0) claim = atomicAdd(claimed, 1u);  // the next one's, while this one is joined
-        const int rows0 = slice / COLUMNS * ROWS, col = slice % COLUMNS * 32 + (lane & 7) * 4;
-        const int tile_tokens = tokens - (rows0 >= TL_ROWS ? g.per_tile : 0);  // from the slice's tile on
-        if ((rows0 & (TL_ROWS - 1)) >= min(tile_tokens, g.per_tile) * group) continue;
-        // a lane: 4 columns of every fourth row
-        float4 acc[MINE];
-        float top[MINE], den[MINE];
-#pragma unroll
-        for (int e = 0; e < MINE; ++e) {
-          acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-          top[e] = -INFINITY;
-          den[e] = 0.f;
+      if (!all) {
+        uint32_t n = 0;
+        if (lane == 0) {
+          atomicOr(left(ticket), 1u << (ticket & 7));
+          __threadfence();
+          n = atomicAdd(arrived, 0x10000u);
         }
+        if ((__shfl_sync(0xffffffffu, n, 0) & 0xffffu) != warps) continue;
+      }
+      __threadfence();
+      const bool heir = ticket == warps - 1 && arrival > 0xffffu;
+      uint32_t next = 0;
 #pragma unroll 1
-        for (int k0 = 0; k0 < parts; k0 += DEEP) {
-          float4 v[DEEP][MINE];
-          float2 ml[DEEP][MINE];
+      for (uint32_t whose = ticket; whose < warps; whose = next++) {
+        if (next > 0 && (whose == ticket || !(*reinterpret_cast<volatile uint32_t *>(left(whose)) >> (whose & 7) & 1u))) continue;
+        constexpr int COLUMNS = DH / 32, ROWS = 16, MINE = ROWS / 4, DEEP = 4;  // of a slice; a lane's rows of it; parts in flight
+#pragma unroll 1
+        for (int slice = (int)whose; slice < 2 * TL_ROWS / ROWS * COLUMNS; slice += (int)warps) {
+          const int rows0 = slice / COLUMNS * ROWS, col = slice % COLUMNS * 32 + (lane & 7) * 4;
+          const int tile_tokens = tokens - (rows0 >= TL_ROWS ? g.per_tile : 0);  // from the slice's tile on
+          if ((rows0 & (TL_ROWS - 1)) >= min(tile_tokens, g.per_tile) * group) continue;
+          // a lane: 4 columns of every fourth row
+          float4 acc[MINE];
+          float top[MINE], den[MINE];
 #pragma unroll
-          for (int d = 0; d < DEEP; ++d) {
-            const long long from = (long long)paged_slot(first, min(k0 + d, parts - 1)) * (2 * TL_ROWS) + rows0 + (lane >> 3);
+          for (int e = 0; e < MINE; ++e) {
+            acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            top[e] = -INFINITY;
+            den[e] = 0.f;
+          }
+#pragma unroll 1
+          for (int k0 = 0; k0 < parts; k0 += DEEP) {
+            float4 v[DEEP][MINE];
+            float2 ml[DEEP][MINE];
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) {
+              const long long from = (long long)paged_slot(first, k0 + d) * (2 * TL_ROWS) + rows0 + (lane >> 3);
+#pragma unroll
+              for (int e = 0; e < MINE; ++e) {
+                ml[d][e] = make_float2(-INFINITY, 0.f);
+                v[d][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k0 + d < parts) {
+                  ml[d][e] = __ldcg(g.a.parts_ml + from + e * 4);
+                  v[d][e] = __ldcg(reinterpret_cast<const float4 *>(g.a.parts + (from + e * 4) * DH + col));
+                }
+              }
+            }
 #pragma unroll
             for (int e = 0; e < MINE; ++e) {
-              ml[d][e] = __ldcg(g.a.parts_ml + from + e * 4);
-              v[d][e] = __ldcg(reinterpret_cast<const float4 *>(g.a.parts + (from + e * 4) * DH + col));
+              float next_top = top[e];
+#pragma unroll
+              for (int d = 0; d < DEEP; ++d) next_top = fmaxf(next_top, ml[d][e].x);
+              const float ref = next_top == -INFINITY ? 0.f : next_top, wa = ap_ex2(top[e] - ref);
+              top[e] = next_top;
+              den[e] *= wa;
+              acc[e] = make_float4(acc[e].x * wa, acc[e].y * wa, acc[e].z * wa, acc[e].w * wa);
+#pragma unroll
+              for (int d = 0; d < DEEP; ++d) {
+                const float w = ap_ex2(ml[d][e].x - ref);
+                den[e] = fmaf(ml[d][e].y, w, den[e]);
+                acc[e].x = fmaf(v[d][e].x, w, acc[e].x);
+                acc[e].y = fmaf(v[d][e].y, w, acc[e].y);
+                acc[e].z = fmaf(v[d][e].z, w, acc[e].z);
+                acc[e].w = fmaf(v[d][e].w, w, acc[e].w);
+              }
             }
           }
 #pragma unroll
-          for (int d = 0; d < DEEP; ++d)
-#pragma unroll
-            for (int e = 0; e < MINE; ++e) {
-              if (k0 + d >= parts || ml[d][e].y == 0.f) continue;  // a row that saw nothing: its o may be unwritten
-              const float next = fmaxf(top[e], ml[d][e].x);
-              const float wa = ap_ex2(top[e] - next), wb = ap_ex2(ml[d][e].x - next);
-              den[e] = den[e] * wa + ml[d][e].y * wb;
-              acc[e].x = acc[e].x * wa + v[d][e].x * wb;
-              acc[e].y = acc[e].y * wa + v[d][e].y * wb;
-              acc[e].z = acc[e].z * wa + v[d][e].z * wb;
-              acc[e].w = acc[e].w * wa + v[d][e].w * wb;
-              top[e] = next;
-            }
+          for (int e = 0; e < MINE; ++e) {
+            const int rr = (rows0 & (TL_ROWS - 1)) + e * 4 + (lane >> 3), tk = paged_div(rr, line.by_group), hd = rr - tk * group;
+            if (tk >= g.per_tile || tk >= tile_tokens || col >= g.a.dh) continue;
+            const float inv = den[e] > 0.f ? __frcp_rn(den[e]) : 0.f;
+            char *where = g.a.o + (long long)(u.row + (rows0 >= TL_ROWS ? g.per_tile : 0) + tk) * g.a.o_t + (long long)(u.head * group + hd) * g.a.o_h + col * 2;
+            *reinterpret_cast<uint2 *>(where) = make_uint2(ap_pack<BF>(acc[e].x * inv, acc[e].y * inv), ap_pack<BF>(acc[e].z * inv, acc[e].w * inv));
+          }
         }
-#pragma unroll
-        for (int e = 0; e < MINE; ++e) {
-          const int rr = (rows0 & (TL_ROWS - 1)) + e * 4 + (lane >> 3), tk = paged_div(rr, line.by_group), hd = rr - tk * group;
-          if (tk >= g.per_tile || tk >= tile_tokens || col >= g.a.dh) continue;
-          const float inv = den[e] > 0.f ? __frcp_rn(den[e]) : 0.f;
-          char *where = g.a.o + (long long)(u.row + (rows0 >= TL_ROWS ? g.per_tile : 0) + tk) * g.a.o_t + (long long)(u.head * group + hd) * g.a.o_h + col * 2;
-          *reinterpret_cast<uint2 *>(where) = make_uint2(ap_pack<BF>(acc[e].x * inv, acc[e].y * inv), ap_pack<BF>(acc[e].z * inv, acc[e].w * inv));
-        }
+        if (!heir) break;
       }
     }
     if (!ok) gave_up = 1;
