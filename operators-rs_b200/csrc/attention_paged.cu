@@ -224,7 +224,7 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   tile.parts_ml = (float2 *)(tile.parts + 2 * (usz)plan.tile.ctas * AP_TILE_ROWS * plan.part_dh);
   attention_paged_clear_kernel<<<1, 1024, 0, s>>>((uint4 *)at, (int)((plan.few_arrived + plan.tile_arrived) / 16));
   OPS_TRY(check_launch("attention_paged(clear)"));
-  if (plan.few.ctas) OPS_TRY(attention_paged_few(few, plan.few_rows, bf16, s));
-  if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, plan.few.ctas == 0, s));
+  if (plan.few.ctas) OPS_TRY(attention_paged_few(few, plan.few_rows, bf16, op->h.prepared, s));
+  if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, plan.few.ctas == 0, op->h.prepared, s));
   return OPS_OK;
 }

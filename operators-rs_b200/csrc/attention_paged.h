@@ -39,9 +39,9 @@ OPS_HD int paged_share(int ctas, int k) { return ctas * k / AP_SHARES > 0 ? ctas
 int attention_paged_maps(const PagedAttnArgs &a, bool bf16, uint32_t rows, CUtensorMap *k, CUtensorMap *v);
 // A 4-d map of 16-bit elements, 64 of the innermost dim and `box1` x `box2` of the next two a box, 128-byte swizzle.
 bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2);
-int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, cudaStream_t s);
+int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, std::atomic<unsigned> &prepared, cudaStream_t s);
 int attention_paged_few_ctas(const OpBase &base);
-int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, cudaStream_t s);
+int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, std::atomic<unsigned> &prepared, cudaStream_t s);
 constexpr int AP_FEW_BLOCK_LOG2 = 5, AP_FEW_BLOCK = 32, AP_TILE_BLOCK_LOG2 = 7, AP_TILE_BLOCK = 128;  // keys of a block
 constexpr int AP_TILE_ROWS = 256;                       // query rows of a unit of the tile kernel: two tiles
 
@@ -218,10 +218,15 @@ __device__ __forceinline__ void pdl_wait_for_front() { asm volatile("griddepcont
 #endif
 
 #ifdef __CUDACC__
-// A launch with `bytes` of shared memory that may start while the one in front of it in the stream still runs.
+// A launch with `bytes` of shared memory that may start while the one in front of it in the stream still runs.  `prepared`, the
+// handle's: bits of the kernels that have been told how much (`bit`: this one's).
 template <class Kernel, class... Args>
-int ap_launch_beside(const char *what, Kernel kernel, int grid, int block, int bytes, cudaStream_t s, const Args &...args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+int ap_launch_beside(const char *what, std::atomic<unsigned> &prepared, unsigned bit, Kernel kernel, int grid, int block, int bytes, cudaStream_t s, const Args &...args) {
+  cudaError_t e = cudaSuccess;
+  if (!(prepared.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) prepared.fetch_or(bit, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3((unsigned)block);

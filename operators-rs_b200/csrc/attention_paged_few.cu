@@ -564,23 +564,23 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 int attention_paged_few_ctas(const OpBase &base) { return base.sm_count; }
 
 template <int DH, bool BF, int NR>
-static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
+static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, std::atomic<unsigned> &prepared, cudaStream_t s) {
   const int bytes = FewSmem<DH, NR>::BYTES;
-  return ap_launch_beside("attention_paged(few rows)", attention_paged_few_kernel<DH, BF, NR>, f.a.line.ctas, FEW_THREADS, bytes, s, k, v, f);
+  return ap_launch_beside("attention_paged(few rows)", prepared, 1u << ((DH == 128) * 4 + BF * 2 + NR - 1), attention_paged_few_kernel<DH, BF, NR>, f.a.line.ctas, FEW_THREADS, bytes, s, k, v, f);
 }
 template <int DH, int NR>
-static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, bool bf16, cudaStream_t s) {
-  return bf16 ? few_launch<DH, true, NR>(f, k, v, s) : few_launch<DH, false, NR>(f, k, v, s);
+static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, bool bf16, std::atomic<unsigned> &prepared, cudaStream_t s) {
+  return bf16 ? few_launch<DH, true, NR>(f, k, v, prepared, s) : few_launch<DH, false, NR>(f, k, v, prepared, s);
 }
 
-int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, cudaStream_t s) {
+int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, std::atomic<unsigned> &prepared, cudaStream_t s) {
   FewArgs f;
   f.a = a;
   f.box_log2 = a.batch.page_log2 < 5 ? a.batch.page_log2 : 5;
   CUtensorMap k, v;
   OPS_TRY(attention_paged_maps(a, bf16, 1u << f.box_log2, &k, &v));
-  if (a.dh <= 64) return rows == 8 ? few_launch<64, 1>(f, k, v, bf16, s) : few_launch<64, 2>(f, k, v, bf16, s);
-  return rows == 8 ? few_launch<128, 1>(f, k, v, bf16, s) : few_launch<128, 2>(f, k, v, bf16, s);
+  if (a.dh <= 64) return rows == 8 ? few_launch<64, 1>(f, k, v, bf16, prepared, s) : few_launch<64, 2>(f, k, v, bf16, prepared, s);
+  return rows == 8 ? few_launch<128, 1>(f, k, v, bf16, prepared, s) : few_launch<128, 2>(f, k, v, bf16, prepared, s);
 }
 
 }  // namespace ops

@@ -737,12 +737,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
 }
 
 template <int DH, bool BF>
-static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
+static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, std::atomic<unsigned> &prepared, cudaStream_t s) {
   const int bytes = TileSmem<DH>::BYTES;
-  return ap_launch_beside("attention_paged(tiles)", attention_paged_tile_kernel<DH, BF>, g.a.line.ctas, TL_THREADS, bytes, s, q, k, v, g);
+  return ap_launch_beside("attention_paged(tiles)", prepared, 256u << ((DH == 128) * 2 + BF), attention_paged_tile_kernel<DH, BF>, g.a.line.ctas, TL_THREADS, bytes, s, q, k, v, g);
 }
 
-int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, cudaStream_t s) {
+int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, std::atomic<unsigned> &prepared, cudaStream_t s) {
   TileArgs g;
   g.a = a;
   g.behind_clear = behind_clear;
@@ -755,8 +755,8 @@ int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, c
   if (!ap_encode(&q, bf16, a.q, q_dims, q_st, (uint32_t)a.line.group, (uint32_t)g.per_tile))
     return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
   OPS_TRY(attention_paged_maps(a, bf16, 1u << g.box_log2, &k, &v));
-  if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, s) : tile_launch<64, false>(g, q, k, v, s);
-  return bf16 ? tile_launch<128, true>(g, q, k, v, s) : tile_launch<128, false>(g, q, k, v, s);
+  if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, prepared, s) : tile_launch<64, false>(g, q, k, v, prepared, s);
+  return bf16 ? tile_launch<128, true>(g, q, k, v, prepared, s) : tile_launch<128, false>(g, q, k, v, prepared, s);
 }
 
 }  // namespace ops

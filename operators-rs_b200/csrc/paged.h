@@ -1,5 +1,6 @@
 // paged.h — what the operators of a paged serving batch share: the batch as the kernels see it, its checks, the status words.
 #pragma once
+#include <atomic>
 #include <new>
 
 #include "common.h"
@@ -161,6 +162,7 @@ inline int rows16_checks(const char *op, const char *what, const ops_layout *l, 
 struct PagedHandle {
   OpBase base;
   int *status;
+  mutable std::atomic<unsigned> prepared{0};  // kernels whose shared memory has been reserved on the device
 };
 int paged_create(PagedHandle *h, int device);
 void paged_destroy(PagedHandle *h);
