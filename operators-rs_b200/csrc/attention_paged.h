@@ -142,7 +142,7 @@ __device__ __forceinline__ void paged_locate(const PagedAttnArgs &a, PagedLine &
       if (both && total > 0 && theirs > 0) {
         const float here = (float)total * (float)(1u << l.shift), there = (float)theirs * 64.f * (float)(1u << a.beside.shift);
         const float few = FEW ? here : there, tile = 2.5f * (FEW ? there : here);  // in what a key costs the few-rows kernel
-        if (few >= 768.f * (float)(few_seqs * l.nkvh) || 13.f * few <= 3.f * tile) {  // 640 keys a unit and more, or 3 / 16 of the work
+        if (few >= 768.f * (float)few_seqs * (float)l.nkvh || 13.f * few <= 3.f * tile) {  // 640 keys a unit and more, or 3 / 16 of the work
           const int k = min(max(__float2int_rn(AP_SHARES * few / (few + tile)), 1), AP_SHARES * 3 / 4);
           l.ctas = FEW ? paged_share(l.ctas, k) : l.ctas - paged_share(l.ctas, k);
           l.by_ctas = a.by_ctas[k];
