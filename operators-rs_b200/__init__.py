@@ -571,9 +571,9 @@ _raw_stream = None  # torch's own accessor, once CUDA is up: a hundredth of the 
 
 
 def current_stream(device=None):
-    """Torch's current stream of a device (an index; None: the current device)."""
+    """Torch's current stream of a device (an index or what torch takes for one; None: the current device)."""
     global _raw_stream
-    if _raw_stream is not None and device is not None:
+    if _raw_stream is not None and type(device) is int:
         return _raw_stream(device)
     import torch
     stream = torch.cuda.current_stream(device).cuda_stream

@@ -576,3 +576,14 @@ def test_layer_captured_step_after_a_larger_one(pkg, dev):
         graph.replay()
         assert torch.equal(out, want)
     assert len(junk) == 64 and layer.attention_paged.status() == 0
+
+
+def test_streams_of_every_kind_of_device(pkg, dev):
+    """A queue named by an index, a torch device, a string or nothing is torch's current stream."""
+    side = torch.cuda.Stream(dev)
+    for _ in range(2):
+        for device in (None, 0, dev, torch.device("cuda"), "cuda:0"):
+            assert pkg.TorchQueueAlloc(device).queue() == pkg.current_stream(device) == torch.cuda.current_stream().cuda_stream
+            with torch.cuda.stream(side):
+                assert pkg.TorchQueueAlloc(device).queue() == side.cuda_stream
+        pkg.Rope(0)
