@@ -7,7 +7,7 @@
 
 namespace ops {
 
-// Clears the counters of the launch.  The kernels that use them start beside it and wait for it where they first need them.
+// Clears the counters of the launch.  The kernel that uses them starts beside it and waits for it.
 __global__ void __launch_bounds__(1024) attention_paged_clear_kernel(uint4 *counters, int n) {
   pdl_let_next_come();
   for (int i = threadIdx.x; i < n; i += 1024) counters[i] = make_uint4(0, 0, 0, 0);
@@ -27,7 +27,8 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2) {
+// A 4-d map of 16-bit elements, 64 of the innermost dim and `box1` x `box2` of the next two a box, 128-byte swizzle.
+static bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t d[4], st[3];
@@ -39,12 +40,10 @@ bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int attention_paged_maps(const PagedAttnArgs &a, bool bf16, uint32_t rows, CUtensorMap *k, CUtensorMap *v) {
-  const usz dims[4] = {(usz)a.dh, (usz)1 << a.batch.page_log2, (usz)a.line.nkvh, a.batch.npages};
+static bool ap_encode_cache(const PagedAttnArgs &a, bool bf16, const PagedLineArgs &l, CUtensorMap *k, CUtensorMap *v) {
+  const usz dims[4] = {(usz)a.dh, (usz)1 << a.batch.page_log2, (usz)l.line.nkvh, a.batch.npages};
   const isz ks[3] = {a.kp_s, a.kp_h, a.kp_p}, vs[3] = {a.vp_s, a.vp_h, a.vp_p};
-  if (!ap_encode(k, bf16, a.k, dims, ks, rows, 1) || !ap_encode(v, bf16, a.v, dims, vs, rows, 1))
-    return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
-  return OPS_OK;
+  return ap_encode(k, bf16, a.k, dims, ks, 1u << l.box_log2, 1) && ap_encode(v, bf16, a.v, dims, vs, 1u << l.box_log2, 1);
 }
 
 struct PagedAttnMeta {
@@ -85,11 +84,11 @@ OPS_DEFINE_PAGED_HANDLE(attention_paged)
 
 namespace ops {
 
-// Which kernels a launch takes, and the scratch they want.  A sequence goes to the few-rows kernel when its new tokens times the
-// query heads of a kv head fit its rows; sequences with more go to the tile kernel.  What no sequence can need by max_seq is left
-// out of the launch.
+// The two lines of a launch and the scratch they want.  A sequence goes to the line of few rows when its new tokens times the query
+// heads of a kv head fit; sequences with more go to the tiles.  Where max_seq says that there are none, the launch is of the kernel
+// without tiles.
 struct PagedAttnPlan {
-  PagedLine few, tile;  // ctas == 0: not launched
+  PagedLine few, tile;  // ctas == 0: nothing can be on it
   int few_rows, part_dh;
   usz few_arrived, tile_arrived, few_parts, tile_parts;  // bytes
   usz bytes() const { return few_arrived + tile_arrived + few_parts + tile_parts + 256; }
@@ -131,7 +130,7 @@ static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, 
     p.few.rows_hi = p.few_rows;
     p.few.tokens = p.few_rows;
     p.few.block_log2 = AP_FEW_BLOCK_LOG2;
-    p.few.ctas = std::min(attention_paged_few_ctas(base), AP_MAX_CTAS);
+    p.few.ctas = std::min(base.sm_count, AP_MAX_CTAS);  // one a SM: the ring takes its shared memory
     line_scale(&p.few, nt, nseq, slots, 128, 128);
     p.few_arrived = up256((usz)AP_LEVELS * p.few.ctas * 8 * sizeof(uint32_t));
     p.few_parts = up256(3 * (usz)p.few.ctas * p.few_rows * (p.part_dh + 2) * sizeof(float));
@@ -208,23 +207,36 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   cudaStream_t s = (cudaStream_t)stream;
   const bool bf16 = m.dt == OPS_DT_BF16;
   char *at = (char *)(((uintptr_t)ws + 255) / 256 * 256);
-  PagedAttnArgs few = g, tile = g;
-  few.line = tile.beside = plan.few;
-  few.arrived = (uint32_t *)at;
-  few.parts = (float *)(at + plan.few_arrived + plan.tile_arrived);
-  few.parts_ml = (float2 *)(few.parts + 3 * (usz)plan.few.ctas * plan.few_rows * plan.part_dh);
-  tile.line = few.beside = plan.tile;
+  g.odd_scale = !(g.scale_log2 > 0.f);
+  g.per_tile = AP_TILE_ROWS / 2 / (int)(m.nh / m.paged.nkvh);
+  g.few.line = plan.few;
+  g.few.box_log2 = std::min(m.paged.page_log2, AP_FEW_BLOCK_LOG2);
+  g.few.arrived = (uint32_t *)at;
+  g.few.parts = (float *)(at + plan.few_arrived + plan.tile_arrived);
+  g.few.parts_ml = (float2 *)(g.few.parts + 3 * (usz)plan.few.ctas * plan.few_rows * plan.part_dh);
+  g.tile.line = plan.tile;
+  g.tile.box_log2 = std::min(m.paged.page_log2, 6);
+  g.tile.arrived = (uint32_t *)(at + plan.few_arrived);
+  g.tile.parts = (float *)(at + plan.few_arrived + plan.tile_arrived + plan.few_parts);
+  g.tile.parts_ml = (float2 *)(g.tile.parts + 2 * (usz)plan.tile.ctas * AP_TILE_ROWS * plan.part_dh);
   if (plan.few.ctas && plan.tile.ctas)
     for (int k = 0; k < AP_SHARES; ++k) {
-      few.by_ctas[k] = paged_div_by((uint32_t)paged_share(plan.few.ctas, k));
-      tile.by_ctas[k] = paged_div_by((uint32_t)std::max(1, plan.tile.ctas - paged_share(plan.tile.ctas, k)));
+      const int share = paged_share(plan.few.ctas, k);
+      g.few.by_ctas[k] = paged_div_by((uint32_t)share);
+      g.tile.by_ctas[k] = paged_div_by((uint32_t)std::max(1, plan.tile.ctas - share));
     }
-  tile.arrived = (uint32_t *)(at + plan.few_arrived);
-  tile.parts = (float *)(at + plan.few_arrived + plan.tile_arrived + plan.few_parts);
-  tile.parts_ml = (float2 *)(tile.parts + 2 * (usz)plan.tile.ctas * AP_TILE_ROWS * plan.part_dh);
+  PagedAttnMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  bool made = true;
+  if (plan.few.ctas) made = ap_encode_cache(g, bf16, g.few, &maps.few_k, &maps.few_v);
+  if (plan.tile.ctas) {
+    const usz q_dims[4] = {m.dh, (usz)plan.tile.group, m.nt, m.paged.nkvh};
+    const isz q_st[3] = {g.q_h, g.q_t, g.q_h * plan.tile.group};
+    made = made && ap_encode(&maps.tile_q, bf16, g.q, q_dims, q_st, (uint32_t)plan.tile.group, (uint32_t)g.per_tile) && ap_encode_cache(g, bf16, g.tile, &maps.tile_k, &maps.tile_v);
+  }
+  if (!made) return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
   attention_paged_clear_kernel<<<1, 1024, 0, s>>>((uint4 *)at, (int)((plan.few_arrived + plan.tile_arrived) / 16));
   OPS_TRY(check_launch("attention_paged(clear)"));
-  if (plan.few.ctas) OPS_TRY(attention_paged_few(few, plan.few_rows, bf16, op->h.prepared, s));
-  if (plan.tile.ctas) OPS_TRY(attention_paged_tile(tile, bf16, plan.few.ctas == 0, op->h.prepared, s));
+  OPS_TRY((bf16 ? attention_paged_run_bf16 : attention_paged_run_f16)(maps, g, plan.few_rows, plan.tile.ctas > 0, op->h.prepared, s));
   return OPS_OK;
 }

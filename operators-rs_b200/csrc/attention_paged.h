@@ -11,8 +11,20 @@ namespace ops {
 constexpr int AP_MAX_DH = 128;
 constexpr int AP_MAX_GROUP = 128;
 constexpr int AP_MAX_CTAS = 256;  // of a kernel
-constexpr int AP_SHARES = 16;     // the few-rows kernel gets k / 16 of the CTAs where both kernels have work
+constexpr int AP_SHARES = 16;     // the few-rows line gets k / 16 of the CTAs where both have work
 constexpr int AP_FEW_JOIN = 16, AP_LEVELS = 2;  // parts are joined in groups, the groups in turn: 16^2 is AP_MAX_CTAS
+
+// A line of work (paged_schedule.h) with the scratch of its units' parts.
+struct PagedLineArgs {
+  PagedLine line;     // ctas == 0: nothing can be on it
+  int box_log2;       // rows of a K or V box
+  uint32_t *arrived;  // [AP_LEVELS][line.ctas][8]: parts of a group that are parked; zero when they are first used
+  // parked parts, [2 * line.ctas, and line.ctas more of few rows][rows of a unit]: unnormalised o, DH floats in whole lines, and
+  // (m, l), its reference point and sum
+  float *parts;
+  float2 *parts_ml;
+  PagedDiv by_ctas[AP_SHARES];  // by the CTAs that are this line's where both have work, by paged_share
+};
 
 struct PagedAttnArgs {
   const char *q, *k, *v;
@@ -21,27 +33,23 @@ struct PagedAttnArgs {
   long long kp_p, kp_h, kp_s, vp_p, vp_h, vp_s;  // byte strides: page, head, slot
   int nh, dh;
   float scale_log2;  // scale * log2(e): the softmax runs in powers of two
+  int odd_scale;     // scale <= 0
+  int per_tile;      // tokens of a tile: 128 / query heads of a kv head
   PagedBatch batch;
-  PagedLine line;
-  uint32_t *arrived;  // [AP_LEVELS][line.ctas][8]: parts of a group that are parked; zero when the launch begins
-  // parked parts, [2 * line.ctas, and line.ctas more for the few-rows kernel][rows of a unit]: unnormalised o, DH floats in whole
-  // lines, and (m, l), its reference point and sum
-  float *parts;
-  float2 *parts_ml;
-  PagedLine beside;             // the other kernel's line; ctas == 0: not launched
-  PagedDiv by_ctas[AP_SHARES];  // by the CTAs that this kernel takes of a launch of both, by paged_share
+  PagedLineArgs few, tile;
 };
 
-// The few-rows kernel's CTAs for k of 16 shares; the tile kernel gets the others.
+// The few-rows line's CTAs for k of 16 shares; the tiles get the others.
 OPS_HD int paged_share(int ctas, int k) { return ctas * k / AP_SHARES > 0 ? ctas * k / AP_SHARES : 1; }
 
-// Tensor maps over the whole cache, boxes of 64 columns x `rows` slots of one head of one page, 128-byte swizzle.
-int attention_paged_maps(const PagedAttnArgs &a, bool bf16, uint32_t rows, CUtensorMap *k, CUtensorMap *v);
-// A 4-d map of 16-bit elements, 64 of the innermost dim and `box1` x `box2` of the next two a box, 128-byte swizzle.
-bool ap_encode(CUtensorMap *map, bool bf16, const void *ptr, const usz (&dims)[4], const isz (&strides)[3], uint32_t box1, uint32_t box2);
-int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, std::atomic<unsigned> &prepared, cudaStream_t s);
-int attention_paged_few_ctas(const OpBase &base);
-int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, std::atomic<unsigned> &prepared, cudaStream_t s);
+// Tensor maps: K and V of the whole cache, boxes of 64 columns x 2^box_log2 slots of one head of one page; the queries, boxes of 64
+// columns x the heads of a group x the tokens of a tile.
+struct PagedAttnMaps {
+  CUtensorMap few_k, few_v, tile_q, tile_k, tile_v;
+};
+// Launches the kernel for few rows alone (tiles == false) or for both, of 8 or 16 few rows.  `prepared`: the handle's.
+int attention_paged_run_f16(const PagedAttnMaps &maps, const PagedAttnArgs &a, int few_rows, bool tiles, std::atomic<unsigned> &prepared, cudaStream_t s);
+int attention_paged_run_bf16(const PagedAttnMaps &maps, const PagedAttnArgs &a, int few_rows, bool tiles, std::atomic<unsigned> &prepared, cudaStream_t s);
 constexpr int AP_FEW_BLOCK_LOG2 = 5, AP_FEW_BLOCK = 32, AP_TILE_BLOCK_LOG2 = 7, AP_TILE_BLOCK = 128;  // keys of a block
 constexpr int AP_TILE_ROWS = 256;                       // query rows of a unit of the tile kernel: two tiles
 
@@ -62,116 +70,135 @@ __device__ __forceinline__ uint32_t ap_pack(float lo, float hi) {  // first valu
   return *reinterpret_cast<uint32_t *>(&t);
 }
 
-// CTA `cta`'s share of the line, for its warp `finder`: the points of all sequences, then the one its share begins in (at == end:
-// nothing).  Up to 32 sequences are that warp's alone; of more, every warp of the CTA adds up an even part first and the finder
-// looks for its sequence in one of the parts: all warps of the CTA call, and meet once.  (One warp alone took a round trip to
-// memory per 32 sequences, twice: 30 us of 2048 decoding requests' 116.)  `report` says whether this CTA is the one that looks
-// for what is wrong with the batch.
+// What of the two lines is this CTA's, by its warps `few_finder` and `tile_finder` (TILES), for all behind the next barrier.  All sequences' points are added up, then the sequence that the share
+// begins in is looked for.  Up to 32 sequences are the finders' alone; of more, every warp of the CTA adds up an even part
+// first and a finder looks for its sequence in one of the parts: all warps call, and meet once.  (One warp alone took a round trip
+// to memory per 32 sequences, twice: 30 us of 2048 decoding requests' 116.)  CTA 0 looks for what is wrong with the batch.
 //
-// Where the line of the other kernel is not empty either, the two split the CTAs, and the SMs with them: the tile kernel's start on the
-// SMs that the few-rows kernel leaves.  One after the other, the first would leave the tensor cores idle and the second the memory;
-// and of the 148 SMs 96 are enough to read as fast as all (72: 89 %, 48: 63 %).  The split makes both take as long, by what a key costs
-// an SM: 4 dh bytes at 68 GB/s, or 4 dh flops for each of 256 rows at 7 TFLOP/s, 2.5 times as long (a chunk of 487 tokens beside 31
-// single ones over up to 2900 keys: 72 us, 86 one after the other).  Short sequences are bound by their number, not by the
-// memory, and gain nothing from fewer SMs (512 single tokens over 100 keys beside eight prompts of 700 tokens: 72 us, 66 one after
-// the other): then only a small share of the work runs beside the other's (64 of them: 47 us, 53 one after the other).  `l` comes
-// back with its CTAs.
-template <int WARPS, bool FEW>
-__device__ __forceinline__ void paged_locate(const PagedAttnArgs &a, PagedLine &l, int cta, bool report, int warp, int finder, PagedWalk *walk, int *total_out) {
+// Where neither line is empty the two split the CTAs, and the SMs with them.  One after the other, the first would leave the
+// tensor cores idle and the second the memory; and of the 148 SMs 96 are enough to read as fast as all (72: 89 %, 48: 63 %).  The
+// split makes both take as long, by what a key costs an SM: 4 dh bytes at 68 GB/s, or 4 dh flops for each of 256 rows at
+// 7 TFLOP/s, 2.5 times as long (a chunk of 487 tokens beside 31 single ones over up to 2900 keys: 64 us, 86 one after the other).
+// Short sequences are bound by their number, not by the memory, and gain nothing from fewer SMs (512 single tokens over 100
+// keys beside eight prompts of 700 tokens: 72 us, 66 one after the other): then only a small share of the work runs beside the
+// other's (64 of them: 47 us, 53 one after the other).
+struct PagedShare {
+  int cta;  // place on the line, -1: nothing there
+  int total;
+  int ctas;  // that have a part of it
+  PagedDiv by_ctas;
+  PagedWalk walk;
+};
+__device__ __forceinline__ PagedLine paged_shared_line(const PagedLine &l, const PagedShare &s) {
+  PagedLine mine = l;
+  mine.ctas = s.ctas;
+  mine.by_ctas = s.by_ctas;
+  return mine;
+}
+
+template <int WARPS, bool TILES>
+__device__ __forceinline__ void paged_locate(const PagedAttnArgs &a, int warp, int few_finder, int tile_finder, PagedShare (&shares)[2]) {
   static_assert(WARPS <= 32, "a lane per part");
-  __shared__ int parts[3][WARPS];  // points of the line (-1: too many), of the other in 64s, sequences with a few rows
+  __shared__ int parts[3][WARPS];  // points of the lines (-1: too many), sequences of few rows
   const PagedBatch &b = a.batch;
-  const bool both = a.beside.ctas > 0;
-  const int lane = threadIdx.x & 31;
-  walk->seq = walk->begin = walk->at = walk->end = 0;
-  *total_out = 0;
+  const int lane = threadIdx.x & 31, nkvh = a.few.line.nkvh;
+  const bool few = !TILES || warp == few_finder, finder = warp == few_finder || (TILES && warp == tile_finder), report = blockIdx.x == 0;
+  PagedShare &mine = shares[few ? 0 : 1];
+  if (finder && lane == 0) mine.cta = -1;
   const bool together = b.nseq > 32;
-  if (!together && warp != finder) return;
+  if (!together && !finder) return;
   const int part = together ? (b.nseq + WARPS * 32 - 1) / (WARPS * 32) * 32 : 32;
   int i0 = together ? warp * part : 0, end = min(b.nseq, i0 + part);
-  long long sum = 0, sum_beside = 0;
-  int few_seqs = 0;
-  int lo = 0, before = 0;
+  long long few_sum = 0, tile_sum = 0;
+  int few_seqs = 0, lo = 0, hi = 0, cta = 0, total = 0, before = 0;
+  PagedLine line = few ? a.few.line : a.tile.line;
   auto all_lanes = [](long long x) -> long long {  // the sum of non-negative numbers
     x = min(x, 1ll << 40);  // far more than a line holds; the halves of 32 such sums add up in 32 bits
     return (long long)__reduce_add_sync(0xffffffffu, (unsigned)(x & 0xffffff)) + ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(x >> 24)) << 24);
   };
+  auto fits = [](long long x) -> int { return x <= 0x7fffffff ? (int)x : -1; };
   bool looking = false, picking = false;  // for a sequence, for a part; both passes run through one copy of the code
 #pragma unroll 1
   while (true) {
     const int i = i0 + lane;
-    long long cost = 0;
+    long long few_cost = 0, tile_cost = 0;
     if (i < end) {
       const PagedSeq s = paged_seq(b, i, report && !looking);
-      cost = (long long)paged_span(l, s).head * l.nkvh;
-      if (both && !looking) {
-        const long long other = (long long)paged_span(a.beside, s).head * l.nkvh;
-        sum_beside += other;
-        few_seqs += (FEW ? cost : other) > 0;
-      }
+      few_cost = (long long)paged_span(a.few.line, s).head * nkvh;
+      if (TILES) tile_cost = (long long)paged_span(a.tile.line, s).head * nkvh;
     }
+    int cost = (int)(few ? few_cost : tile_cost);
     i0 += 32;
     if (!looking) {
-      sum += cost;
+      few_sum += few_cost;
+      if (TILES) {
+        tile_sum += tile_cost;
+        few_seqs += few_cost > 0;
+      }
       if (i0 < end) continue;
-      sum = all_lanes(sum);
-      int mine = (int)sum, theirs = 0;
-      if (both) {  // to weigh the two lines against each other: near enough
-        theirs = __reduce_add_sync(0xffffffffu, (int)(sum_beside >> 6));
+      few_sum = all_lanes(few_sum);
+      if (TILES) {
+        tile_sum = all_lanes(tile_sum);
         few_seqs = __reduce_add_sync(0xffffffffu, few_seqs);
       }
       if (together) {
         if (lane == 0) {
-          parts[0][warp] = sum <= 0x7fffffff ? mine : -1;
-          parts[1][warp] = theirs;
+          parts[0][warp] = fits(few_sum);
+          parts[1][warp] = fits(tile_sum);
           parts[2][warp] = few_seqs;
         }
         __syncthreads();
-        if (warp != finder) return;
-        mine = lane < WARPS ? parts[0][lane] : 0;
-        sum = all_lanes(mine < 0 ? 1ll << 40 : mine);
-        if (both) {
-          theirs = __reduce_add_sync(0xffffffffu, lane < WARPS ? parts[1][lane] : 0);
+        if (!finder) return;
+        const int f = lane < WARPS ? parts[0][lane] : 0, t = lane < WARPS ? parts[1][lane] : 0;
+        few_sum = all_lanes(f < 0 ? 1ll << 40 : f);
+        if (TILES) {
+          tile_sum = all_lanes(t < 0 ? 1ll << 40 : t);
           few_seqs = __reduce_add_sync(0xffffffffu, lane < WARPS ? parts[2][lane] : 0);
         }
+        cost = few ? f : t;
       }
-      // sequences that share rows (seq_start falls) can put more on the line than the host allowed for: nothing is done then
-      const int total = sum <= 0x7fffffff ? (int)sum : 0;
-      if (report && total != sum && lane == 0) atomicCAS(b.status, 0, OPS_PAGED_BAD_ROWS);
-      *total_out = total;
-      if (both && total > 0 && theirs > 0) {
-        const float here = (float)total * (float)(1u << l.shift), there = (float)theirs * 64.f * (float)(1u << a.beside.shift);
-        const float few = FEW ? here : there, tile = 2.5f * (FEW ? there : here);  // in what a key costs the few-rows kernel
-        if (few >= 768.f * (float)few_seqs * (float)l.nkvh || 13.f * few <= 3.f * tile) {  // 640 keys a unit and more, or 3 / 16 of the work
-          const int k = min(max(__float2int_rn(AP_SHARES * few / (few + tile)), 1), AP_SHARES * 3 / 4);
-          l.ctas = FEW ? paged_share(l.ctas, k) : l.ctas - paged_share(l.ctas, k);
-          l.by_ctas = a.by_ctas[k];
+      // sequences that share rows (seq_start falls) can put more on a line than the host allowed for: nothing is done then
+      const int few_total = max(0, fits(few_sum)), tile_total = max(0, fits(tile_sum));
+      if (report && few && (few_total != few_sum || tile_total != tile_sum) && lane == 0) atomicCAS(b.status, 0, OPS_PAGED_BAD_ROWS);
+      total = few ? few_total : tile_total;
+      cta = blockIdx.x;
+      if (TILES && few_total > 0 && tile_total > 0) {
+        const float few_keys = (float)few_total * (float)(1u << a.few.line.shift);
+        const float tile_keys = 2.5f * (float)tile_total * (float)(1u << a.tile.line.shift);  // in what a key of few rows costs
+        if (few_keys >= 768.f * (float)few_seqs * (float)nkvh || 13.f * few_keys <= 3.f * tile_keys) {  // 640 keys a unit and more, or 3 / 16 of the work
+          const int k = min(max(__float2int_rn(AP_SHARES * few_keys / (few_keys + tile_keys)), 1), AP_SHARES * 3 / 4);
+          const int few_ctas = paged_share(a.few.line.ctas, k);
+          line.ctas = few ? few_ctas : a.tile.line.ctas - few_ctas;
+          line.by_ctas = few ? a.few.by_ctas[k] : a.tile.by_ctas[k];
+          if (!few) cta -= few_ctas;
         }
       }
-      if (cta >= l.ctas) return;
-      lo = paged_cut(l, total, cta);
-      const int hi = paged_cut(l, total, cta + 1);
+      if (cta < 0 || cta >= line.ctas) return;
+      lo = paged_cut(line, total, cta);
+      hi = paged_cut(line, total, cta + 1);
       if (lo >= hi) return;
-      walk->at = lo;
-      walk->end = hi;
       looking = true;
       picking = together;
-      if (picking) cost = mine;
     }
-    int upto = (int)cost;
+    int upto = cost;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
-    const unsigned here = __ballot_sync(0xffffffffu, before + upto - (int)cost <= lo && lo < before + upto);
+    const unsigned here = __ballot_sync(0xffffffffu, before + upto - cost <= lo && lo < before + upto);
     if (here) {
       const int at = __ffs(here) - 1;
-      before += __shfl_sync(0xffffffffu, upto - (int)cost, at);
+      before += __shfl_sync(0xffffffffu, upto - cost, at);
       if (!picking) {
-        walk->seq = i0 - 32 + at;
-        walk->begin = before;
-        break;
+        if (lane == 0) {
+          mine.cta = cta;
+          mine.total = total;
+          mine.ctas = line.ctas;
+          mine.by_ctas = line.by_ctas;
+          mine.walk = {i0 - 32 + at, before, lo, hi};
+        }
+        return;
       }
       picking = false;
       i0 = at * part;
@@ -212,7 +239,7 @@ __device__ __forceinline__ bool paged_arrive_last(uint32_t *arrived, int group) 
 }
 
 // A launch may start while the one in front of it still runs (programmatic dependent launch): the front one says when the other
-// may come, the other waits for all of its results.
+// may come, the other waits for all of its results.  (Here: the kernel that clears the counters, the one that uses them.)
 __device__ __forceinline__ void pdl_let_next_come() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_for_front() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 #endif

@@ -1,4 +1,4 @@
-// attention_paged_few.cu — attention over a paged cache for sequences with a handful of query rows (a decode step, a few drafted
+// attention_paged_few.cuh — attention over a paged cache for sequences with a handful of query rows (a decode step, a few drafted
 // tokens): at most 8 or 16 rows = new tokens x query heads per kv head.
 //
 //   o_r = sum_j 2^(x_rj - m_r) v_j / sum_j 2^(x_rj - m_r),  x_rj = scale log2(e) q_r . k_j,  one pass with a running m_r
@@ -27,8 +27,7 @@
 // NaN there).  Every wait is bounded; when one runs out its code goes to the status word and all roles unwind.
 // Measured, 8 kv heads of 128: 61 requests over up to 4096 keys 98 us, 5.9 TB/s; eight over up to 32101 keys 106 us, 6.1 TB/s;
 // one over 1001 keys 9.9 us.
-#include <cuda.h>
-
+#pragma once
 #include "attention_paged.h"
 #include "device_utils.cuh"
 #include "sm100_ptx.cuh"
@@ -83,16 +82,16 @@ template <int DH, int NR> struct FewSmem {
   static constexpr int OFF_O = OFF_Q + FEW_RING * ROWS * Q_LD * 2;              // [consumers][ROWS][O_LD] f32
   static constexpr int OFF_ML = OFF_O + FEW_CONSUMERS * ROWS * O_LD * 4;        // [ROWS][consumers] (m, l)
   static constexpr int OFF_PIECES = OFF_ML + ROWS * FEW_CONSUMERS * 8;
-  static constexpr int OFF_BAR = OFF_PIECES + FEW_RING * (int)sizeof(FewPiece);
+  static constexpr int BYTES = OFF_PIECES + FEW_RING * (int)sizeof(FewPiece) + 1024;  // 1024: alignment
   static constexpr int NUM_BARS = 2 * STAGES + 3 * FEW_RING + 1;
-  static constexpr int OFF_ISSUED = OFF_BAR + NUM_BARS * 8;  // [STAGES] number of the stage that was last asked for in a slot of the ring, plus 1
-  static constexpr int BYTES = OFF_ISSUED + STAGES * 4 + 1024;  // 1024: alignment
-  static_assert(STAGES % FEW_PRODUCERS == 0 && OFF_BAR % 8 == 0 && OFF_O % 16 == 0, "layout");
+  static_assert(STAGES % FEW_PRODUCERS == 0 && OFF_O % 16 == 0, "layout");
 };
 
-struct FewArgs {
-  PagedAttnArgs a;
-  int box_log2;  // rows of a box: min(page, 32)
+// What lies outside the dynamic shared memory, which the tiles of the same launch use after it.
+template <int DH, int NR> struct FewShared {
+  unsigned long long bars[FewSmem<DH, NR>::NUM_BARS];
+  uint32_t issued[FewSmem<DH, NR>::STAGES];  // number of the stage that was last asked for in a slot of the ring, plus 1
+  int last;
 };
 
 // A slot of the ring is not always the same consumer's: one that came early could take the phase before last of its barrier for the
@@ -111,66 +110,46 @@ __device__ __forceinline__ bool few_wait_issued(const volatile uint32_t *issued,
   }
 }
 
+template <int DH, int NR> __device__ __forceinline__ void few_init(FewShared<DH, NR> &sh) {  // one thread
+  constexpr int ST = FewSmem<DH, NR>::STAGES;
+  const uint32_t bar0 = smem_u32(sh.bars);
+  for (int i = 0; i < 2 * ST + 2 * FEW_RING; ++i) mbar_init(bar0 + 8u * i, 1);  // full, empty, q_full, piece_full
+  for (int i = 0; i < FEW_RING; ++i) mbar_init(bar0 + 8u * (2 * ST + 2 * FEW_RING + i), FEW_CONSUMERS + FEW_PRODUCERS);  // piece_empty
+  mbar_init(bar0 + 8u * (2 * ST + 3 * FEW_RING), FEW_CONSUMERS);  // meet_bar
+  for (int s = 0; s < ST; ++s) sh.issued[s] = 0;
+}
+
+// The CTA's share of the line of few rows.  Whether no wait ran out.
 template <int DH, bool BF, int NR>
-__global__ void __launch_bounds__(FEW_THREADS, 1)
-    attention_paged_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ FewArgs f) {
+__device__ __forceinline__ bool few_rows(const CUtensorMap &tmap_k, const CUtensorMap &tmap_v, const PagedAttnArgs &a, uint8_t *base_ptr, FewShared<DH, NR> &sh,
+                                         const PagedShare &share) {
   typedef FewSmem<DH, NR> Smem;
   constexpr int ST = Smem::STAGES, ROWS = Smem::ROWS;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t bar0 = base + Smem::OFF_BAR;
+  const uint32_t base = smem_u32(base_ptr), bar0 = smem_u32(sh.bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
   auto q_full = [&](int i) { return bar0 + 8u * (2 * ST + i); };
   auto piece_full = [&](int i) { return bar0 + 8u * (2 * ST + FEW_RING + i); };
   auto piece_empty = [&](int i) { return bar0 + 8u * (2 * ST + 2 * FEW_RING + i); };  // read, by the consumers with its q
   const uint32_t meet_bar = bar0 + 8u * (2 * ST + 3 * FEW_RING);
-  volatile uint32_t *issued = reinterpret_cast<volatile uint32_t *>(base_ptr + Smem::OFF_ISSUED);
+  volatile uint32_t *issued = sh.issued;
   volatile FewPiece *pieces = reinterpret_cast<volatile FewPiece *>(base_ptr + Smem::OFF_PIECES);
-  __shared__ int gave_up, last_s;
-  const PagedAttnArgs &a = f.a;
-  int *status = a.batch.status + 1;  // of the waits
+  const PagedLine &line = a.few.line;  // `line.ctas`: what the scratch is laid out for
+  int *status = a.batch.status + 1;    // of the waits
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int group = a.line.group;
-
-  PagedWalk walk;
-  int total = 0;
-  PagedLine line = a.line;  // the scheduler's, with the CTAs that have a part of it; `a.line.ctas` is what the workspace is laid out for
-  paged_locate<FEW_THREADS / 32, true>(a, line, blockIdx.x, blockIdx.x == 0, warp, FEW_CONSUMERS + FEW_PRODUCERS, &walk, &total);
-  if (warp == FEW_CONSUMERS) {
-    if (lane == 0) {
-      tma_prefetch_desc(&tmap_k);
-      tma_prefetch_desc(&tmap_v);
-    }
-  } else if (threadIdx.x == 0) {
-    gave_up = 0;
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
-      issued[s] = 0;
-    }
-    for (int i = 0; i < FEW_RING; ++i) {
-      mbar_init(q_full(i), 1);
-      mbar_init(piece_full(i), 1);
-      mbar_init(piece_empty(i), FEW_CONSUMERS + FEW_PRODUCERS);
-    }
-    mbar_init(meet_bar, FEW_CONSUMERS);
-    fence_barrier_init();
-  } else if (warp == 1) {
-    pdl_wait_for_front();  // the counters have been cleared, this kernel's and the next one's: that may come
-    pdl_let_next_come();
-  }
-  __syncthreads();
+  const int group = line.group, cta = share.cta;
 
   bool ok = true;
   if (warp == FEW_CONSUMERS + FEW_PRODUCERS) {
     // ------------------------------------------------------------------ scheduler
     if (lane == 0) {
+      const PagedLine shared = paged_shared_line(line, share);
+      const int total = share.total;
+      PagedWalk walk = share.walk;
       uint32_t alone = 0;  // pieces given to one consumer
 #pragma unroll 1
       for (uint32_t i = 0; ok; ++i) {
-        const PagedPiece q = paged_step(a.batch, line, walk);
+        const PagedPiece q = paged_step(a.batch, shared, walk);
         const int slot = i % FEW_RING;
         if (!(ok = mbar_wait(piece_empty(slot), ((i / FEW_RING) & 1u) ^ 1u, status, 201))) break;
         volatile FewPiece &to = pieces[slot];
@@ -182,7 +161,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           to.head = q.head;
           to.k0 = q.lo * FEW_KEYS;
           to.k1 = min(q.hi * FEW_KEYS, q.s.len);
-          const PagedParts parts = paged_parts(line, total, blockIdx.x, q);
+          const PagedParts parts = paged_parts(shared, total, cta, q);
           to.first = parts.first;
           to.count = parts.count;
           to.whose = parts.count == 1 && q.hi <= ST / 2 && walk.end - walk.at >= 2 * q.cost ? (int)(alone++ % FEW_CONSUMERS) : -1;
@@ -191,10 +170,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         if (q.seq < 0) break;
       }
     }
-  } else if (warp >= FEW_CONSUMERS) {
+  } else if (warp >= FEW_CONSUMERS && warp < FEW_CONSUMERS + FEW_PRODUCERS) {
     // ------------------------------------------------------------------ producers
     const int producer = warp - FEW_CONSUMERS;
-    const int box = 1 << f.box_log2, boxes = FEW_KEYS >> f.box_log2;  // of K; as many of V
+    const int box = 1 << a.few.box_log2, boxes = FEW_KEYS >> a.few.box_log2;  // of K; as many of V
     const int lg = a.batch.page_log2, in_page = (1 << lg) - 1;
     const bool values = lane >= boxes;
     const int r = (values ? lane - boxes : lane) * box;  // the lane's first row of a stage
@@ -230,7 +209,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < Q_VECS; ++e) {
           const int at = e * 32 + lane, qr = at / (DH / 8), col = (at - qr * (DH / 8)) * 8;
-          const int tok = paged_div(qr, a.line.by_group), gi = qr - tok * group;
+          const int tok = paged_div(qr, line.by_group), gi = qr - tok * group;
           qv[e] = make_uint4(0, 0, 0, 0);
           if (tok < n && col < a.dh) qv[e] = ld_global_16(a.q + (long long)(row + tok) * a.q_t + (long long)(head * group + gi) * a.q_h + col * 2);
         }
@@ -271,7 +250,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       }
       count += stages;
     }
-  } else {
+  } else if (warp < FEW_CONSUMERS) {
     // ------------------------------------------------------------------ consumers
     const int g = lane >> 2, c = lane & 3;
     // ldmatrix: lane l names row l % 8 of matrix l / 8
@@ -323,8 +302,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       // last visible key of rows g and g + 8; every row sees the keys in front of `all`
       int lim[NR];
 #pragma unroll
-      for (int e = 0; e < NR; ++e) lim[e] = a.line.causal ? len - n + paged_div(g + 8 * e, a.line.by_group) : len - 1;
-      const int all = min(k1, a.line.causal ? len - n + 1 : len);
+      for (int e = 0; e < NR; ++e) lim[e] = line.causal ? len - n + paged_div(g + 8 * e, line.by_group) : len - 1;
+      const int all = min(k1, line.causal ? len - n + 1 : len);
       float m[NR], l[NR];  // m is common to the four lanes of a row, l is this lane's share
 #pragma unroll
       for (int e = 0; e < NR; ++e) {
@@ -427,7 +406,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
       }
       auto out_row = [&](int r) -> char * {
-        const int tok = paged_div(r, a.line.by_group), gi = r - tok * group;
+        const int tok = paged_div(r, line.by_group), gi = r - tok * group;
         return a.o + (long long)(row + tok) * a.o_t + (long long)(head * group + gi) * a.o_h;
       };
       if (whose >= 0) {  // nobody to wait for
@@ -470,11 +449,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           *reinterpret_cast<uint2 *>(out_row(r) + col * 2) = make_uint2(ap_pack<BF>(acc.x * inv, acc.y * inv), ap_pack<BF>(acc.z * inv, acc.w * inv));
         } else {
           const long long at = (long long)slot * ROWS + r;
-          *reinterpret_cast<float4 *>(a.parts + at * DH + col) = acc;
-          if (col == 0) a.parts_ml[at] = make_float2(top, den);
+          *reinterpret_cast<float4 *>(a.few.parts + at * DH + col) = acc;
+          if (col == 0) a.few.parts_ml[at] = make_float2(top, den);
         }
       };
-      int node = (int)blockIdx.x - first;
+      int node = cta - first;
       each([&](int r, int col) {
         float2 ml[FEW_CONSUMERS];
         float top = -INFINITY;
@@ -510,11 +489,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         if (together == 1) continue;  // as it was parked (it has neither a counter nor a slot: paged_group_slot)
         if (!(ok = meet())) break;    // all have parked
         if (warp == 0) {
-          const bool last = paged_arrive_last(a.arrived + (level * a.line.ctas + first + g0 * one) * 8, together);
-          if (lane == 0) last_s = last;
+          const bool last = paged_arrive_last(a.few.arrived + (level * line.ctas + first + g0 * one) * 8, together);
+          if (lane == 0) *const_cast<volatile int *>(&sh.last) = last;
         }
         if (!(ok = meet())) break;
-        if (!*reinterpret_cast<volatile int *>(&last_s)) break;
+        if (!*const_cast<volatile int *>(&sh.last)) break;
         __threadfence();
         each([&](int r, int col) {
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -530,9 +509,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
               ml[e] = make_float2(-INFINITY, 0.f);
               if (j0 + e < together) {
                 const int k = (g0 + j0 + e) * one;
-                const long long from = (long long)paged_group_slot(a.line, first, k, min(one, parts - k)) * ROWS + r;
-                ml[e] = __ldcg(a.parts_ml + from);
-                v[e] = __ldcg(reinterpret_cast<const float4 *>(a.parts + from * DH + col));
+                const long long from = (long long)paged_group_slot(line, first, k, min(one, parts - k)) * ROWS + r;
+                ml[e] = __ldcg(a.few.parts_ml + from);
+                v[e] = __ldcg(reinterpret_cast<const float4 *>(a.few.parts + from * DH + col));
               }
             }
 #pragma unroll
@@ -547,40 +526,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
               top = next;
             }
           }
-          leave(nodes == 1 ? -1 : paged_group_slot(a.line, first, g0 * one, together * one), r, col, acc, top, den);
+          leave(nodes == 1 ? -1 : paged_group_slot(line, first, g0 * one, together * one), r, col, acc, top, den);
         });
       }
       if (!ok) break;
       if (!(ok = meet())) break;  // ml_s and o_s are free again
     }
   }
-  if (!ok) gave_up = 1;
-  if (warp == FEW_CONSUMERS) pdl_wait_for_front();  // no launch ends in front of the one it started beside
-  __syncthreads();
-  if (gave_up) __nanosleep(1000000);  // a wait ran out: let stray copies land before the CTA goes away
-}
-
-// One CTA per SM: the ring takes its shared memory.
-int attention_paged_few_ctas(const OpBase &base) { return base.sm_count; }
-
-template <int DH, bool BF, int NR>
-static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, std::atomic<unsigned> &prepared, cudaStream_t s) {
-  const int bytes = FewSmem<DH, NR>::BYTES;
-  return ap_launch_beside("attention_paged(few rows)", prepared, 1u << ((DH == 128) * 4 + BF * 2 + NR - 1), attention_paged_few_kernel<DH, BF, NR>, f.a.line.ctas, FEW_THREADS, bytes, s, k, v, f);
-}
-template <int DH, int NR>
-static int few_launch(const FewArgs &f, const CUtensorMap &k, const CUtensorMap &v, bool bf16, std::atomic<unsigned> &prepared, cudaStream_t s) {
-  return bf16 ? few_launch<DH, true, NR>(f, k, v, prepared, s) : few_launch<DH, false, NR>(f, k, v, prepared, s);
-}
-
-int attention_paged_few(const PagedAttnArgs &a, int rows, bool bf16, std::atomic<unsigned> &prepared, cudaStream_t s) {
-  FewArgs f;
-  f.a = a;
-  f.box_log2 = a.batch.page_log2 < 5 ? a.batch.page_log2 : 5;
-  CUtensorMap k, v;
-  OPS_TRY(attention_paged_maps(a, bf16, 1u << f.box_log2, &k, &v));
-  if (a.dh <= 64) return rows == 8 ? few_launch<64, 1>(f, k, v, bf16, prepared, s) : few_launch<64, 2>(f, k, v, bf16, prepared, s);
-  return rows == 8 ? few_launch<128, 1>(f, k, v, bf16, prepared, s) : few_launch<128, 2>(f, k, v, bf16, prepared, s);
+  return ok;
 }
 
 }  // namespace ops

@@ -1,4 +1,4 @@
-// attention_paged_tile.cu — attention over a paged cache for sequences with more query rows than the few-rows kernel holds: chunks
+// attention_paged_tile.cuh — attention over a paged cache for sequences with more query rows than the few-rows kernel holds: chunks
 // of a prompt, whole prompts, many query heads per kv head.
 //
 //   o_r = sum_j 2^(x_rj - m_r) v_j / sum_j 2^(x_rj - m_r),  x_rj = scale log2(e) q_r . k_j,  one pass with a running m_r
@@ -34,8 +34,7 @@
 // of their cycles each (a block's two products and its powers take turns less than perfectly; a polynomial for 1 in 8, 4, 3 or 2
 // powers: 141, 148, 147, 176 us); 1024 tokens of 4 heads over 8025 keys 35 us, of which some 5 are spent until the first scores and
 // 8 on parking and joining.
-#include <cuda.h>
-
+#pragma once
 #include "attention_paged.h"
 #include "device_utils.cuh"
 #include "sm100_ptx.cuh"
@@ -71,10 +70,8 @@ template <int DH> struct TileSmem {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + 2 * TILE;
   static constexpr int OFF_V = OFF_K + STAGES * TILE;
-  static constexpr int OFF_BAR = OFF_V + STAGES * TILE;
   static constexpr int NUM_BARS = 12 + 2 * TL_RING + 5 * STAGES;
-  static constexpr int OFF_TMEM_SLOT = OFF_BAR + NUM_BARS * 8;
-  static constexpr int OFF_RING = (OFF_TMEM_SLOT + 16 + 15) / 16 * 16;
+  static constexpr int OFF_RING = OFF_V + STAGES * TILE;
   static constexpr int OFF_STAGE = (OFF_RING + TL_RING * (int)sizeof(TilePiece) + 15) / 16 * 16;  // 4 KB a softmax warp: 32 rows x 128 B
   static constexpr int BYTES = OFF_STAGE + 8 * 4096 + 1024;  // 1024: alignment
 };
@@ -85,12 +82,12 @@ struct TileHelp {
   int row, tokens, head;
 };
 
-struct TileArgs {
-  PagedAttnArgs a;
-  int per_tile;   // tokens of a tile: 128 / group
-  int box_log2;   // rows of a K or V box: min(page, 64)
-  int odd_scale;  // scale <= 0
-  int behind_clear;  // the launch in front is the one that clears the counters, not the few-rows kernel's
+// What lies outside the dynamic shared memory.
+template <int DH> struct TileShared {
+  unsigned long long bars[TileSmem<DH>::NUM_BARS];
+  TileHelp help[2];        // the unit that the share begins in, the one it ends in
+  uint32_t tickets[2][8];  // of the softmax warps for these: what paged_arrive said
+  uint32_t tmem;           // address
 };
 
 __device__ __forceinline__ float tl_max3(float a, float b, float c) {
@@ -99,16 +96,24 @@ __device__ __forceinline__ float tl_max3(float a, float b, float c) {
   return r;
 }
 
+template <int DH> __device__ __forceinline__ void tile_init(TileShared<DH> &sh) {  // one thread
+  constexpr int ST = TileSmem<DH>::STAGES;
+  const uint32_t bar0 = smem_u32(sh.bars);
+  for (int i = 0; i < TileSmem<DH>::NUM_BARS; ++i) {
+    const bool p_full = i >= 6 && i < 10, ring_empty = i >= 12 + TL_RING && i < 12 + 2 * TL_RING;
+    mbar_init(bar0 + 8u * i, p_full ? 4 : ring_empty ? TL_READERS : 1);
+  }
+  static_assert(TileSmem<DH>::NUM_BARS == 12 + 2 * TL_RING + 5 * ST, "the barriers that tiles() names");
+  sh.help[0].count = sh.help[1].count = 0;
+}
+
+// The CTA's share of the line of tiles.  Whether no wait ran out.
 template <int DH, bool BF>
-__global__ void __launch_bounds__(TL_THREADS, 1)
-    attention_paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                                const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ TileArgs g) {
+__device__ __forceinline__ bool tiles(const CUtensorMap &tmap_q, const CUtensorMap &tmap_k, const CUtensorMap &tmap_v, const PagedAttnArgs &a, uint8_t *base_ptr,
+                                      TileShared<DH> &sh, const PagedShare &share) {
   typedef TileSmem<DH> Smem;
   constexpr int HALVES = Smem::HALVES, ST = Smem::STAGES, TILE = Smem::TILE;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t *base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t bar0 = base + Smem::OFF_BAR;
+  const uint32_t base = smem_u32(base_ptr), bar0 = smem_u32(sh.bars);
   auto q_full = [&](int t) { return bar0 + 8u * (0 + t); };
   auto q_empty = [&](int t) { return bar0 + 8u * (2 + t); };    // last QK of the piece's tile done
   auto s_full = [&](int t) { return bar0 + 8u * (4 + t); };     // S complete (tensor pipe -> softmax)
@@ -121,61 +126,16 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
   auto v_full = [&](int s) { return bar0 + 8u * (12 + 2 * TL_RING + 2 * ST + s); };
   auto v_empty = [&](int s) { return bar0 + 8u * (12 + 2 * TL_RING + 3 * ST + s); };
   auto v_clean = [&](int s) { return bar0 + 8u * (12 + 2 * TL_RING + 4 * ST + s); };  // a stage's, so that no phase is overrun
-  const uint32_t tmem_slot = base + Smem::OFF_TMEM_SLOT;
-  uint32_t *tmem_slot_ptr = reinterpret_cast<uint32_t *>(base_ptr + Smem::OFF_TMEM_SLOT);
   volatile TilePiece *ring = reinterpret_cast<volatile TilePiece *>(base_ptr + Smem::OFF_RING);
+  volatile TileHelp *help = sh.help;
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // known to be uniform
-  const PagedBatch &batch = g.a.batch;
-  const PagedLine &line = g.a.line;
+  const PagedBatch &batch = a.batch;
+  const PagedLine &line = a.tile.line;  // `line.ctas`: what the scratch is laid out for
   const int group = line.group;
   int *status = batch.status + 1;  // of the waits
-  __shared__ int gave_up;
-  __shared__ TileHelp help[2];  // the unit that the share begins in, the one it ends in
-  __shared__ uint32_t tickets[2][8];  // of the softmax warps for these: what paged_arrive said
-
-  pdl_let_next_come();
-  PagedWalk walk;
-  int total = 0;
-  PagedLine share = line;  // the scheduler's, with the CTAs that have a part of it; `line.ctas` is what the workspace is laid out for
-  paged_locate<TL_THREADS / 32, false>(g.a, share, blockIdx.x, blockIdx.x == 0, warp, 3, &walk, &total);
-  if (threadIdx.x == 0) {
-    gave_up = 0;
-    help[0].count = help[1].count = 0;
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(q_full(t), 1);
-      mbar_init(q_empty(t), 1);
-      mbar_init(s_full(t), 1);
-      mbar_init(p_full(t, 0), 4);
-      mbar_init(p_full(t, 1), 4);
-      mbar_init(o_final(t), 1);
-    }
-    for (int i = 0; i < TL_RING; ++i) {
-      mbar_init(ring_full(i), 1);
-      mbar_init(ring_empty(i), TL_READERS);
-    }
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(k_full(s), 1);
-      mbar_init(k_empty(s), 1);
-      mbar_init(v_full(s), 1);
-      mbar_init(v_empty(s), 1);
-      mbar_init(v_clean(s), 1);
-    }
-    fence_barrier_init();
-  }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmap_q);
-    tma_prefetch_desc(&tmap_k);
-    tma_prefetch_desc(&tmap_v);
-  }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot_ptr;
+  const uint32_t tmem_base = sh.tmem;
+  bool ok = true;
   // tensor memory columns: S0 | S1 | O0 | O1, 128 each; the P of a tile overwrites the first 64 columns of its S
   auto s_col = [&](int t) { return (uint32_t)(t * 128); };
   auto o_col = [&](int t) { return (uint32_t)(256 + t * 128); };
@@ -185,10 +145,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
     if (warp == 0 || warp == 2) {
       // ------------------------------------------------------------------ producers: one warp, a lane per box
       const bool keys = warp == 0;
-      const int box = 1 << g.box_log2, boxes = TL_KEYS >> g.box_log2;
+      const int box = 1 << a.tile.box_log2, boxes = TL_KEYS >> a.tile.box_log2;
       const int lg = batch.page_log2, in_page = (1 << lg) - 1;
       uint32_t count = 0, q_count[2] = {0, 0};
-      bool ok = true;
       for (uint32_t i = 0; ok; ++i) {
         const int slot = i % TL_RING;
         ok = mbar_wait(ring_full(slot), (i / TL_RING) & 1u, status, keys ? 101 : 102);
@@ -217,10 +176,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
             if (lane == 0) {
               ok = mbar_wait(q_empty(t), (q_count[t] & 1u) ^ 1u, status, 103 + t);
               if (ok) {
-                mbar_arrive_expect_tx(q_full(t), (uint32_t)(group * g.per_tile * HALVES * 128));
+                mbar_arrive_expect_tx(q_full(t), (uint32_t)(group * a.per_tile * HALVES * 128));
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h)
-                  tma_load_4d(base + Smem::OFF_Q + t * TILE + h * (TL_ROWS * 128), &tmap_q, q_full(t), h * 64, 0, row + t * g.per_tile, head);
+                  tma_load_4d(base + Smem::OFF_Q + t * TILE + h * (TL_ROWS * 128), &tmap_q, q_full(t), h * 64, 0, row + t * a.per_tile, head);
               }
             }
             ++q_count[t];
@@ -252,7 +211,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
             // the slots behind the end share a page with the last ones and may hold anything, a NaN too
             ok = __all_sync(0xffffffffu, mbar_wait(full, (count / ST) & 1u, status, 107));
             if (!ok) break;
-            const int r0 = len % TL_KEYS, r1 = (r0 + box - 1) >> g.box_log2 << g.box_log2;
+            const int r0 = len % TL_KEYS, r1 = (r0 + box - 1) >> a.tile.box_log2 << a.tile.box_log2;
             for (int e = lane; e < (r1 - r0) * HALVES * 8; e += 32) {
               const int r = r0 + e / (HALVES * 8), piece = e % (HALVES * 8);
               *reinterpret_cast<uint4 *>(base_ptr + Smem::OFF_V + s * TILE + ((r >> 6) * HALVES + (piece >> 3)) * 8192 + (r & 63) * 128 + (piece & 7) * 16) =
@@ -264,7 +223,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           }
         }
       }
-      if (!ok) gave_up = 1;
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMA issuer
       // the whole warp walks along, one lane issues
@@ -277,7 +235,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         const uint64_t v_desc = make_smem_desc_sw128(base + Smem::OFF_V, 8192, 1024);
         auto all_wait = [&](uint32_t bar, uint32_t parity, int code) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code)); };
         uint32_t count = 0, cleaned = 0 /* a bit per stage */, q_count[2] = {0, 0}, p_count[2] = {0, 0};
-        bool ok = true;
         for (uint32_t i = 0; ok; ++i) {
           const int slot = i % TL_RING;
           if (!(ok = all_wait(ring_full(slot), (i / TL_RING) & 1u, 120))) break;
@@ -344,15 +301,16 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           if (clean >= 0) cleaned ^= 1u << ((count + (uint32_t)clean) % ST);
           count += (uint32_t)blocks;
         }
-        if (!ok) gave_up = 1;
       }
     } else {
       // ------------------------------------------------------------------ scheduler
       if (lane == 0) {
-        bool ok = true;
+        const PagedLine shared = paged_shared_line(line, share);
+        const int total = share.total;
+        PagedWalk walk = share.walk;
 #pragma unroll 1
         for (uint32_t i = 0; ok; ++i) {
-          const PagedPiece q = paged_step(batch, share, walk);
+          const PagedPiece q = paged_step(batch, shared, walk);
           const int slot = i % TL_RING;
           if (!(ok = mbar_wait(ring_empty(slot), ((i / TL_RING) & 1u) ^ 1u, status, 130))) break;
           volatile TilePiece &to = ring[slot];
@@ -369,17 +327,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
             to.hi = q.hi;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const int seen = paged_keys(line, q.s, t0 + (t + 1) * g.per_tile);
-              const int all = t0 + t * g.per_tile < q.s.n ? max(1, (seen + TL_KEYS - 1) / TL_KEYS) : 0;
+              const int seen = paged_keys(line, q.s, t0 + (t + 1) * a.per_tile);
+              const int all = t0 + t * a.per_tile < q.s.n ? max(1, (seen + TL_KEYS - 1) / TL_KEYS) : 0;
               to.blocks[t] = max(0, min(all, q.hi) - q.lo);
             }
             const int end = q.s.len / TL_KEYS;  // the block the sequence ends in
-            to.clean = (q.s.len & ((1 << g.box_log2) - 1)) && end >= q.lo && end < q.hi ? end - q.lo : -1;
-            const PagedParts parts = paged_parts(share, total, blockIdx.x, q);
+            to.clean = (q.s.len & ((1 << a.tile.box_log2) - 1)) && end >= q.lo && end < q.hi ? end - q.lo : -1;
+            const PagedParts parts = paged_parts(shared, total, share.cta, q);
             to.first = parts.first;
             to.count = parts.count;
             if (parts.count > 2) {
-              TileHelp &u = help[q.lo > 0 ? 0 : 1];
+              volatile TileHelp &u = help[q.lo > 0 ? 0 : 1];
               u.first = parts.first;
               u.count = parts.count;
               u.row = q.s.row + t0;
@@ -390,7 +348,6 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           mbar_arrive(ring_full(slot));
           if (q.seq < 0) break;
         }
-        if (!ok) gave_up = 1;
       }
     }
   } else {
@@ -402,9 +359,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const int tok = paged_div(r, line.by_group), gi = r - tok * group;
     const uint32_t ta = tmem_base + lane_addr + s_col(t), to = tmem_base + lane_addr + o_col(t);
-    const float mult = g.odd_scale ? 1.f : g.a.scale_log2;
-    uint32_t s_count = 0, o_count = 0;
-    bool ok = true;
+    const float mult = a.odd_scale ? 1.f : a.scale_log2;
+    uint32_t phases = 0;  // bit 0: of s_full, bit 1: of o_final
 #pragma unroll 1
     for (uint32_t i = 0; ok; ++i) {
       const int slot = i % TL_RING;
@@ -412,13 +368,14 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       volatile TilePiece &p = ring[slot];
       if (!p.valid) break;
       const int nblk = p.blocks[t];
-      const int mine = t * g.per_tile + tok;  // token of the unit
+      const int mine = t * a.per_tile + tok;  // token of the unit
       const int limit = line.causal ? min(p.len - 1, p.off + mine) : p.len - 1;  // last slot this row may see
       int kv0 = p.lo * TL_KEYS;
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int j = 0; j < nblk; ++j, kv0 += TL_KEYS) {
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), s_count++ & 1u, status, 142)))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), phases & 1u, status, 142)))) break;
+        phases ^= 1u;
         tc_fence_after();
         uint32_t x[4][32];
 #pragma unroll
@@ -426,11 +383,11 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         tmem_wait_ld();
         // Rare cases first, each in a branch of its own that whole warps take or leave, so that the common path is an addition, a
         // power, a multiply-add and half a maximum and half a conversion per score.
-        if (g.odd_scale) {  // not positive: the maximum of the products is not the product of the maximum
+        if (a.odd_scale) {  // not positive: the maximum of the products is not the product of the maximum
 #pragma unroll
           for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[q][e] = __float_as_uint(__uint_as_float(x[q][e]) * g.a.scale_log2);
+            for (int e = 0; e < 32; ++e) x[q][e] = __float_as_uint(__uint_as_float(x[q][e]) * a.scale_log2);
         }
         if (__any_sync(0xffffffffu, kv0 + TL_KEYS - 1 > limit)) {  // the diagonal, or the end: what a row does not see weighs nothing
 #pragma unroll
@@ -496,7 +453,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
         l += sum.x + sum.y;
       }
       if (!ok) break;
-      const bool there = tok < g.per_tile && mine < p.tokens;
+      const bool there = tok < a.per_tile && mine < p.tokens;
       const int first = p.first, parts = p.count;
       const long long row = p.row + mine;
       const int q_head = p.head * group + gi;
@@ -505,7 +462,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       if (nblk == 0 && parts == 1) continue;  // the unit has no tokens for this tile
       bool own = nblk > 0;                    // whether there is an O: a tile may have no block in this part of its unit
       if (own) {
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_final(t), o_count++ & 1u, status, 143)))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_final(t), phases >> 1, status, 143)))) break;
+        phases ^= 2u;
         tc_fence_after();
       }
       // A row is one thread's, 512 or 256 bytes of it: written as it is, every store of a warp would touch 32 lines.  128 bytes of
@@ -527,17 +485,16 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       // whichever of the two warps comes last, from its tensor memory and the other's parked part.  More are parked, all of them, and
       // joined at the end of the share (see below).
       if (parts > 1) {
-        if (g.behind_clear) pdl_wait_for_front();  // else the counters were cleared before the few-rows kernel let this one come
-        const int k = (int)blockIdx.x - first;
+        const int k = *(const volatile int *)&share.cta - first;
         auto rows_of = [&](int k) -> long long {  // this warp's rows of the unit's k-th part
           return (long long)paged_slot(first, k) * (2 * TL_ROWS) + t * TL_ROWS + quarter * 32;
         };
-        uint32_t *arrived = parts == 2 ? g.a.arrived + first * 8 + (warp - 4) : g.a.arrived + (line.ctas + first) * 8;
+        uint32_t *arrived = parts == 2 ? a.tile.arrived + first * 8 + (warp - 4) : a.tile.arrived + (line.ctas + first) * 8;
         const bool counts = l != 0.f;  // a row that sees nothing in this part (a NaN is something) has zeros for its o, whatever V holds
         bool last = parts == 2 && paged_others_parked(arrived, 2);
         if (!last) {
-          float *mine_at = g.a.parts + rows_of(k) * DH;
-          g.a.parts_ml[rows_of(k) + lane] = make_float2(m, l);
+          float *mine_at = a.tile.parts + rows_of(k) * DH;
+          a.tile.parts_ml[rows_of(k) + lane] = make_float2(m, l);
 #pragma unroll 1
           for (int c = 0; c < DH; c += 32) {
             uint32_t v[32];
@@ -553,20 +510,20 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           const uint32_t ticket = paged_arrive(arrived);
           last = parts == 2 && ticket == 1;
           if (last) __threadfence();
-          if (lane == 0) tickets[k == 0][warp - 4] = ticket;
+          if (lane == 0) sh.tickets[k == 0][warp - 4] = ticket;
         }
         if (!last) {
           tc_fence_before();
           continue;
         }
-        const float *theirs = g.a.parts + rows_of(k ^ 1) * DH;
+        const float *theirs = a.tile.parts + rows_of(k ^ 1) * DH;
         auto fetch = [&](int c, uint4 (&x)[8]) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const uint4 *>(theirs + (e * 4 + (lane >> 3)) * DH + (lane & 7) * 4 + c));
         };
         uint4 x[8];
         fetch(0, x);
-        const float2 ml = __ldcg(g.a.parts_ml + rows_of(k ^ 1) + lane);
+        const float2 ml = __ldcg(a.tile.parts_ml + rows_of(k ^ 1) + lane);
         const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
         const float w_own = ap_ex2(m - ref), w_their = ap_ex2(ml.x - ref);
         l = __fadd_rn(__fmul_rn(l, w_own), __fmul_rn(ml.y, w_their));  // products and a sum: the same whichever of the two comes last
@@ -599,7 +556,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       }
       {
         const float inv = l > 0.f ? __frcp_rn(l) : 0.f;  // a row that sees nothing: zeros
-        char *orow = there ? g.a.o + row * g.a.o_t + (long long)q_head * g.a.o_h : nullptr;
+        char *orow = there ? a.o + row * a.o_t + (long long)q_head * a.o_h : nullptr;
 #pragma unroll 1
         for (int c = 0; c < DH; c += 64) {
 #pragma unroll
@@ -619,7 +576,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
           }
           leave([&](int rr, int e) -> char * {
             char *whose = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), rr));
-            return whose && c + e * 8 < g.a.dh ? whose + (c + e * 8) * 2 : nullptr;
+            return whose && c + e * 8 < a.dh ? whose + (c + e * 8) * 2 : nullptr;
           });
         }
       }
@@ -635,8 +592,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
       if (u.count <= 2) continue;
       const int first = u.first, parts = u.count, tokens = u.tokens;
       __syncwarp();
-      const uint32_t warps = 8 * (uint32_t)parts, arrival = tickets[h][warp - 4], ticket = arrival & 0xffffu;
-      uint32_t *arrived = g.a.arrived + (line.ctas + first) * 8;
+      const uint32_t warps = 8 * (uint32_t)parts, arrival = sh.tickets[h][warp - 4], ticket = arrival & 0xffffu;
+      uint32_t *arrived = a.tile.arrived + (line.ctas + first) * 8;
       auto left = [&](uint32_t t) -> uint32_t * {  // bits of the warps with tickets [8 k, 8 k + 8); the last CTA may be the first of the next unit
         const int k = (int)(t >> 3);
         return arrived + k * 8 + (k == parts - 1 ? 2 : 1);
@@ -667,8 +624,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
 #pragma unroll 1
         for (int slice = (int)whose; slice < 2 * TL_ROWS / ROWS * COLUMNS; slice += (int)warps) {
           const int rows0 = slice / COLUMNS * ROWS, col = slice % COLUMNS * 32 + (lane & 7) * 4;
-          const int tile_tokens = tokens - (rows0 >= TL_ROWS ? g.per_tile : 0);  // from the slice's tile on
-          if ((rows0 & (TL_ROWS - 1)) >= min(tile_tokens, g.per_tile) * group) continue;
+          const int tile_tokens = tokens - (rows0 >= TL_ROWS ? a.per_tile : 0);  // from the slice's tile on
+          if ((rows0 & (TL_ROWS - 1)) >= min(tile_tokens, a.per_tile) * group) continue;
           // a lane: 4 columns of every fourth row
           float4 acc[MINE];
           float top[MINE], den[MINE];
@@ -690,8 +647,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
                 ml[d][e] = make_float2(-INFINITY, 0.f);
                 v[d][e] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (k0 + d < parts) {
-                  ml[d][e] = __ldcg(g.a.parts_ml + from + e * 4);
-                  v[d][e] = __ldcg(reinterpret_cast<const float4 *>(g.a.parts + (from + e * 4) * DH + col));
+                  ml[d][e] = __ldcg(a.tile.parts_ml + from + e * 4);
+                  v[d][e] = __ldcg(reinterpret_cast<const float4 *>(a.tile.parts + (from + e * 4) * DH + col));
                 }
               }
             }
@@ -718,49 +675,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < MINE; ++e) {
             const int rr = (rows0 & (TL_ROWS - 1)) + e * 4 + (lane >> 3), tk = paged_div(rr, line.by_group), hd = rr - tk * group;
-            if (tk >= g.per_tile || tk >= tile_tokens || col >= g.a.dh) continue;
+            if (tk >= a.per_tile || tk >= tile_tokens || col >= a.dh) continue;
             const float inv = den[e] > 0.f ? __frcp_rn(den[e]) : 0.f;
-            char *where = g.a.o + (long long)(u.row + (rows0 >= TL_ROWS ? g.per_tile : 0) + tk) * g.a.o_t + (long long)(u.head * group + hd) * g.a.o_h + col * 2;
+            char *where = a.o + (long long)(u.row + (rows0 >= TL_ROWS ? a.per_tile : 0) + tk) * a.o_t + (long long)(u.head * group + hd) * a.o_h + col * 2;
             *reinterpret_cast<uint2 *>(where) = make_uint2(ap_pack<BF>(acc[e].x * inv, acc[e].y * inv), ap_pack<BF>(acc[e].z * inv, acc[e].w * inv));
           }
         }
         if (!heir) break;
       }
     }
-    if (!ok) gave_up = 1;
   }
-
-  if (warp == 3) pdl_wait_for_front();  // no launch ends in front of the one it started beside
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    if (gave_up) __nanosleep(1000000);  // a wait ran out: let stray copies land before the CTA goes away
-    tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
-  }
-}
-
-template <int DH, bool BF>
-static int tile_launch(const TileArgs &g, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, std::atomic<unsigned> &prepared, cudaStream_t s) {
-  const int bytes = TileSmem<DH>::BYTES;
-  return ap_launch_beside("attention_paged(tiles)", prepared, 256u << ((DH == 128) * 2 + BF), attention_paged_tile_kernel<DH, BF>, g.a.line.ctas, TL_THREADS, bytes, s, q, k, v, g);
-}
-
-int attention_paged_tile(const PagedAttnArgs &a, bool bf16, bool behind_clear, std::atomic<unsigned> &prepared, cudaStream_t s) {
-  TileArgs g;
-  g.a = a;
-  g.behind_clear = behind_clear;
-  g.per_tile = TL_ROWS / a.line.group;
-  g.odd_scale = !(a.scale_log2 > 0.f);
-  g.box_log2 = a.batch.page_log2 < 6 ? a.batch.page_log2 : 6;
-  CUtensorMap q, k, v;
-  const usz q_dims[4] = {(usz)a.dh, (usz)a.line.group, (usz)a.batch.nt, (usz)a.line.nkvh};
-  const isz q_st[3] = {a.q_h, a.q_t, a.q_h * a.line.group};
-  if (!ap_encode(&q, bf16, a.q, q_dims, q_st, (uint32_t)a.line.group, (uint32_t)g.per_tile))
-    return fail(OPS_EXECUTION_FAILED, "attention_paged: cuTensorMapEncodeTiled failed");
-  OPS_TRY(attention_paged_maps(a, bf16, 1u << g.box_log2, &k, &v));
-  if (a.dh <= 64) return bf16 ? tile_launch<64, true>(g, q, k, v, prepared, s) : tile_launch<64, false>(g, q, k, v, prepared, s);
-  return bf16 ? tile_launch<128, true>(g, q, k, v, prepared, s) : tile_launch<128, false>(g, q, k, v, prepared, s);
+  return ok;
 }
 
 }  // namespace ops
