@@ -489,6 +489,7 @@ __device__ __forceinline__ bool few_rows(const CUtensorMap &tmap_k, const CUtens
         if (together == 1) continue;  // as it was parked (it has neither a counter nor a slot: paged_group_slot)
         if (!(ok = meet())) break;    // all have parked
         if (warp == 0) {
+          pdl_wait_for_front();  // the counters have been cleared
           const bool last = paged_arrive_last(a.few.arrived + (level * line.ctas + first + g0 * one) * 8, together);
           if (lane == 0) *const_cast<volatile int *>(&sh.last) = last;
         }

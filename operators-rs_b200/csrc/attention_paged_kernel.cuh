@@ -40,7 +40,6 @@ __global__ void __launch_bounds__(TILES ? TL_THREADS : FEW_THREADS, 1)
       tma_prefetch_desc(&maps.tile_v);
     }
   }
-  if (warp == 5) pdl_wait_for_front();  // the counters have been cleared
   if (TILES && warp == 1) {
     tmem_alloc(smem_u32(&tile_sh.tmem), 512);
     tmem_relinquish();
@@ -65,6 +64,7 @@ __global__ void __launch_bounds__(TILES ? TL_THREADS : FEW_THREADS, 1)
     __syncthreads();
     tc_fence_after();
   }
+  pdl_wait_for_front();  // (no launch ends in front of the one it started beside; who uses the counters has waited for them to be cleared)
   if (*(volatile int *)&gave_up) __nanosleep(1000000);  // a wait ran out: let stray copies land before the CTA goes away
   if (TILES && threadIdx.x >> 5 == 1) tmem_dealloc(tile_sh.tmem, 512);
 }

@@ -485,6 +485,7 @@ __device__ __forceinline__ bool tiles(const CUtensorMap &tmap_q, const CUtensorM
       // whichever of the two warps comes last, from its tensor memory and the other's parked part.  More are parked, all of them, and
       // joined at the end of the share (see below).
       if (parts > 1) {
+        pdl_wait_for_front();  // the counters have been cleared
         const int k = *(const volatile int *)&share.cta - first;
         auto rows_of = [&](int k) -> long long {  // this warp's rows of the unit's k-th part
           return (long long)paged_slot(first, k) * (2 * TL_ROWS) + t * TL_ROWS + quarter * 32;
