@@ -314,7 +314,7 @@ typedef struct {
   ops_layout page_table_layout; const void *page_table_base; /* [nseq, width], rows contiguous */
   ops_layout seq_start_layout; const void *seq_start_base;   /* [nseq + 1] */
   ops_layout kv_len_layout; const void *kv_len_base;         /* [nseq] */
-  size_t max_seq; /* no sequence has more new tokens than this; 0: unknown (a step of single tokens then costs an idle launch) */
+  size_t max_seq; /* no sequence has more new tokens than this; 0: unknown (the launch is then made for chunks, too) */
 } ops_paged_batch;
 
 /* kv_append_paged: q_out <- rotated q (q_out may be q); k rotated and v as it is into the pages of their slots.  The rotation is

@@ -1,4 +1,4 @@
-// attention_paged_tile.cuh — attention over a paged cache for sequences with more query rows than the few-rows kernel holds: chunks
+// attention_paged_tile.cuh — attention over a paged cache for sequences with more query rows than attention_paged_few.cuh takes: chunks
 // of a prompt, whole prompts, many query heads per kv head.
 //
 //   o_r = sum_j 2^(x_rj - m_r) v_j / sum_j 2^(x_rj - m_r),  x_rj = scale log2(e) q_r . k_j,  one pass with a running m_r
@@ -30,7 +30,7 @@
 //            front takes the tensor pipe: the next stage is not free earlier)
 //   warp 3   scheduler
 // Every wait is bounded; when one runs out its code goes to the status word and all roles unwind to the common teardown.
-// Measured, heads of 128: a 4096-token prompt of 32 heads 131 us, 1.05 PFLOP/s, the tensor pipe and the special-function unit at 57 %
+// Measured, heads of 128: a 4096-token prompt of 32 heads 132 us, 1.04 PFLOP/s, the tensor pipe and the special-function unit at 55 %
 // of their cycles each (a block's two products and its powers take turns less than perfectly; a polynomial for 1 in 8, 4, 3 or 2
 // powers: 141, 148, 147, 176 us); 1024 tokens of 4 heads over 8025 keys 35 us, of which some 5 are spent until the first scores and
 // 8 on parking and joining.
