@@ -235,6 +235,22 @@ def test_attention_paged_many_sequences(pkg, dev, ops):
     check_attention(pkg, dev, ops.attention, ref.Batch(dev, F16, n, kv, 1, 64, 16, seed=1), 2)
 
 
+@pytest.mark.parametrize("nseq,nh,nkvh,dh,new,most", [(700, 16, 1, 128, 1, 120), (400, 6, 2, 80, 2, 200), (500, 8, 8, 64, 1, 90), (450, 14, 2, 64, 2, 330)])
+def test_attention_paged_many_short_sequences(pkg, dev, ops, nseq, nh, nkvh, dh, new, most):
+    """Sequences that one warp takes alone, some of nothing, some too long for that, the last ones of a share taken together."""
+    kv = [(i * 53) % most + new if i % 17 else (0 if i % 2 else 5 * most) for i in range(nseq)]
+    check_attention(pkg, dev, ops.attention, ref.Batch(dev, BF16 if nseq % 2 else F16, [new] * nseq, kv, nkvh, dh, 16, seed=2, max_seq=new), nh)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,kv,nh,nkvh,dh", [([1] * 20 + [200], [3000 + 7 * i for i in range(20)] + [900], 8, 2, 128),       # long single tokens: side by side
+                                             ([1, 600, 1, 500], [300, 700, 40, 500], 4, 2, 64),                              # a small share of the work
+                                             ([1] * 60 + [90, 1], [60 + i for i in range(60)] + [4000, 9], 16, 2, 64),       # short ones beside a long past
+                                             ([2] * 40 + [300], [1500] * 40 + [1300], 4, 4, 96)])
+def test_attention_paged_chunks_beside_single_tokens(pkg, dev, ops, causal, n, kv, nh, nkvh, dh):
+    check_attention(pkg, dev, ops.attention, ref.Batch(dev, BF16, n, kv, nkvh, dh, 32, seed=4, pad=2), nh, causal)
+
+
 @pytest.mark.parametrize("n,kv", [([1], [40000]), ([1, 1], [30, 20001]), ([200], [20000]), ([2, 64], [16000, 9001])])
 def test_attention_paged_long(pkg, dev, ops, n, kv):
     check_attention(pkg, dev, ops.attention, ref.Batch(dev, BF16, n, kv, 2, 128, 64, seed=9), 8)
