@@ -14,7 +14,10 @@
 // pos * (theta^(-2k/dh) / 2 pi), in f64 and reduced there: in f32 it would be off by pos * 2^-24 rad.
 // What bounded it first was instruction issue (full-range sincospi, 64-bit address arithmetic per vector: 70 us for 8192 rows of
 // 40 heads of 128); with angles reduced in f64 in front of the special-function unit, pointers that step and packed f32 pairs
-// it streams: 33 us, 5.1 TB/s.  Reads and writes both bypass what other kernels keep in L2 (either alone changes nothing: 43 us).
+// it streams: 33 us.  The norm was 5 us of that, each vector's chain of shuffles behind the last one's: with the sums of a round
+// side by side 30 us, 5.6 TB/s (6 blocks an SM; with 7, or the weights loaded ahead of the sums, registers spill: 31, 37 us.  The
+// append takes 7: 30.2 us for seven prompts against 31.2 with 6).  Reads and writes both bypass what other kernels keep in L2
+// (either alone changed nothing).
 #include <type_traits>
 
 #include "device_utils.cuh"
@@ -61,13 +64,19 @@ __device__ __forceinline__ void pairs_of(uint4 v, float2 (&f)[4], __nv_bfloat16)
 #pragma unroll
   for (int e = 0; e < 4; ++e) f[e] = __bfloat1622float2(h[e]);
 }
-template <class T> __device__ __forceinline__ void load_pairs(const T *p, float2 (&f)[4]) { pairs_of(ld_global_16(p), f, T()); }
-__device__ __forceinline__ void load_pairs(const float *p, float2 (&f)[4]) {
-  const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-  f[0] = make_float2(a.x, a.y);
-  f[1] = make_float2(a.z, a.w);
-  f[2] = make_float2(b.x, b.y);
-  f[3] = make_float2(b.z, b.w);
+// ... of a row of weights, as they are loaded
+template <class T> struct RowPiece {
+  typedef uint4 type;
+};
+struct __align__(16) EightFloats {
+  float v[8];
+};
+template <> struct RowPiece<float> {
+  typedef EightFloats type;
+};
+__device__ __forceinline__ void pairs_of(const EightFloats &v, float2 (&f)[4], float) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = make_float2(v.v[2 * e], v.v[2 * e + 1]);
 }
 __device__ __forceinline__ uint32_t pair_to(float2 v, __half) {
   const __half2 h = __float22half2_rn(v);
@@ -79,7 +88,7 @@ __device__ __forceinline__ uint32_t pair_to(float2 v, __nv_bfloat16) {
 }
 
 template <class E, class W, bool NORM, bool APPEND, int RN_UNROLL>
-__global__ void __launch_bounds__(RN_WARPS * 32) rotate_heads_kernel(const __grid_constant__ RotateArgs a, const __grid_constant__ RotateTurns turns) {
+__global__ void __launch_bounds__(RN_WARPS * 32, APPEND ? 7 : 6) rotate_heads_kernel(const __grid_constant__ RotateArgs a, const __grid_constant__ RotateTurns turns) {
   const int lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * RN_WARPS + (threadIdx.x >> 5);
   const int tok = (int)(item / a.slices), slice = (int)(item - (long long)tok * a.slices);
@@ -127,6 +136,27 @@ __global__ void __launch_bounds__(RN_WARPS * 32) rotate_heads_kernel(const __gri
         if (active && h + u * at_once < hi) x[u] = ld_stream_16(src + u * src_step);
       }
       if (rotated) turn();
+      // the sums of a round side by side: the shuffles of a step wait together, not in turn
+      float r[RN_UNROLL];
+      if (rotated && NORM) {
+#pragma unroll
+        for (int u = 0; u < RN_UNROLL; ++u) {
+          float2 f[4];
+          pairs_of(x[u], f, E());
+          float2 ss = __fmul2_rn(f[0], f[0]);
+#pragma unroll
+          for (int e = 1; e < 4; ++e) ss = __ffma2_rn(f[e], f[e], ss);
+          r[u] = ss.x + ss.y;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          if (o < a.lanes) {
+#pragma unroll
+            for (int u = 0; u < RN_UNROLL; ++u) r[u] += __shfl_xor_sync(0xffffffffu, r[u], o);
+          }
+#pragma unroll
+        for (int u = 0; u < RN_UNROLL; ++u) r[u] = rsqrtf(fmaf(r[u], a.inv_dh, a.eps));
+      }
 #pragma unroll
       for (int u = 0; u < RN_UNROLL; ++u) {
         const bool there = active && h + u * at_once < hi;
@@ -134,18 +164,12 @@ __global__ void __launch_bounds__(RN_WARPS * 32) rotate_heads_kernel(const __gri
           float2 f[4];
           pairs_of(x[u], f, E());
           if (NORM) {
-            float2 ss = __fmul2_rn(f[0], f[0]);
-#pragma unroll
-            for (int e = 1; e < 4; ++e) ss = __ffma2_rn(f[e], f[e], ss);
-            float sum = ss.x + ss.y;
-            for (int o = a.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const float r = rsqrtf(fmaf(sum, a.inv_dh, a.eps));
             float2 wt[4];
+            typename RowPiece<W>::type weight = typename RowPiece<W>::type();
+            if (there) weight = *reinterpret_cast<const typename RowPiece<W>::type *>(w + u * w_step);
+            pairs_of(weight, wt, W());
 #pragma unroll
-            for (int e = 0; e < 4; ++e) wt[e] = make_float2(0.f, 0.f);
-            if (there) load_pairs(reinterpret_cast<const W *>(w + u * w_step), wt);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = __fmul2_rn(f[e], __fmul2_rn(wt[e], make_float2(r, r)));
+            for (int e = 0; e < 4; ++e) f[e] = __fmul2_rn(f[e], __fmul2_rn(wt[e], make_float2(r[u], r[u])));
           }
           uint32_t y[4];
 #pragma unroll
@@ -205,9 +229,9 @@ static const RotateTurns &rotate_turns(float theta, usz dh) {
 
 // Warps per token.  About 16 warps an SM hide a round trip to memory; with no more than that, and few heads a warp, a round of two
 // vectors a lane is enough (a round of four spends instructions on vectors that are not there: 64 rows of 40 heads 3.8 against
-// 3.3 us, 1777 rows of 5 heads 5.5 against 4.5).  Otherwise a warp walks a whole token in rounds of four, or half of one as long
-// as that makes no more than 48 warps an SM (8192 rows of 40 heads: 33.0 us against 36.4 in rounds of two, 36.4 with twice the
-// warps; ragged prompts of 48 heads: 30.8 us against 33.4 with 16 warps an SM).
+// 3.2 us, 1777 rows of 5 heads 5.5 against 4.4).  Otherwise a warp walks a whole token in rounds of four, or half of one as long
+// as that makes no more than 48 warps an SM (8192 rows of 40 heads: 29.9 us against 33.3 with twice the warps; ragged prompts of
+// 48 heads: 30.2 us against 32.6 with 32 warps an SM; rounds of two were a tenth slower in both).
 static int rotate_split(const OpBase &base, RotateArgs *a, int heads) {
   a->lanes = 1;
   while (a->lanes * 8 < a->dh) a->lanes *= 2;
