@@ -32,7 +32,8 @@
 // Every wait is bounded; when one runs out its code goes to the status word and all roles unwind to the common teardown.
 // Measured, heads of 128: a 4096-token prompt of 32 heads 132 us, 1.04 PFLOP/s, the tensor pipe and the special-function unit at 55 %
 // of their cycles each (a block's two products and its powers take turns less than perfectly; a polynomial for 1 in 8, 4, 3 or 2
-// powers: 141, 148, 147, 176 us); 1024 tokens of 4 heads over 8025 keys 35 us, of which some 5 are spent until the first scores and
+// powers: 141, 148, 147, 176 us; scores made and used 64 keys at a time, so that nothing waits for a whole block's: 136 us, the two
+// tiles' powers then coincide); 1024 tokens of 4 heads over 8025 keys 35 us, of which some 5 are spent until the first scores and
 // 8 on parking and joining.
 #pragma once
 #include "attention_paged.h"
