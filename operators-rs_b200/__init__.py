@@ -439,6 +439,9 @@ class PagedBatch:
 
     def __init__(self, page_table, seq_start, kv_len, max_seq=0):
         self.arrays = (page_table, seq_start, kv_len)
+        for t in self.arrays:
+            if getattr(t, "is_cuda", None) is False:  # schedulers make them on the host: the easiest mistake of all
+                raise ValueError("page_table, seq_start and kv_len are read by the kernels: device tensors expected")
         self.operands = tuple([_operand(t, None if isinstance(t, TensorLayout) else t) for t in self.arrays])
         self.max_seq = int(max_seq)
 

@@ -174,6 +174,15 @@ def test_kv_append_paged_refusals(pkg):
     at_launch(pkg.STRIDES_NOT_SUPPORT, w_base=P16 + 2)
 
 
+def test_batch_of_host_tensors_is_refused(pkg):
+    import torch
+    table, start, length = torch.zeros(3, 5, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    for arrays in ((table, L(pkg, pkg.I32, (4,)), L(pkg, pkg.I32, (3,))), (L(pkg, pkg.I32, (3, 5)), start, L(pkg, pkg.I32, (3,))),
+                   (L(pkg, pkg.I32, (3, 5)), L(pkg, pkg.I32, (4,)), length)):
+        with pytest.raises(ValueError, match="device tensors"):
+            pkg.PagedBatch(*arrays)
+
+
 def test_rope_norm_refusals(pkg):
     F16, op = pkg.F16, "rope_norm"
 
