@@ -91,6 +91,11 @@ template <class E, class W, bool NORM, bool APPEND, int RN_UNROLL>
 __global__ void __launch_bounds__(RN_WARPS * 32, APPEND ? 7 : 6) rotate_heads_kernel(const __grid_constant__ RotateArgs a, const __grid_constant__ RotateTurns turns) {
   const int lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * RN_WARPS + (threadIdx.x >> 5);
+  if (APPEND) {
+    // What is wrong with the batch, a lane per sequence: rows alone do not show it (none may find its way to a sequence whose
+    // start falls).  Warps that have no sequence, nearly all, go on at once.
+    for (long long i = item * 32 + lane; i < a.batch.nseq; i += (long long)gridDim.x * (RN_WARPS * 32)) paged_seq(a.batch, (int)i, true);
+  }
   const int tok = (int)(item / a.slices), slice = (int)(item - (long long)tok * a.slices);
   if (tok >= a.nt) return;
   const int sub = lane & (a.lanes - 1);   // which 8 elements of the head
@@ -190,7 +195,7 @@ __global__ void __launch_bounds__(RN_WARPS * 32, APPEND ? 7 : 6) rotate_heads_ke
   // the token's slot in the cache
   const int i = paged_find(a.batch, (uint32_t)tok);
   if (i < 0) return;
-  const PagedSeq s = paged_seq(a.batch, i, slice == a.slices - 1 && lane == 0);
+  const PagedSeq s = paged_seq(a.batch, i, false);
   const long long slot = (long long)a.batch.len[i] - s.n + (tok - s.row);  // by the length as given: a cut one would move the token
   int wrong = 0;
   uint32_t page = 0;

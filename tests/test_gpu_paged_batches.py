@@ -1,0 +1,47 @@
+"""Batches that the paged operators have to report or to survive, beside those of test_gpu_paged.py."""
+import math
+
+import pytest
+import torch
+
+import paged_reference as ref
+from test_gpu_paged import BF16, EPS, F16, THETA, attend, gen, near, normal
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ kv_append_paged: the whole batch is looked at
+@pytest.mark.parametrize("start,bad", [([3, 0], True),               # every row is in front of the first sequence, or behind the last
+                                       ([0, 4, 2, 6], True),         # rows 2 and 3 are claimed twice
+                                       ([0, 6, 6, 2, 6], True),      # a fall between sequences that own no row
+                                       ([0, 6, 900, 6], True),       # past the step's rows, and back
+                                       ([0, 2, 2, 6], False), ([2, 2, 6], False)])
+@pytest.mark.parametrize("nt", [6, 40])
+def test_kv_append_paged_reports_starts_that_fall(pkg, dev, start, bad, nt):
+    op = pkg.KvAppendPaged(0)
+    nseq, ps = len(start) - 1, 16
+    k_pages, v_pages = (torch.full((nseq, 2, ps, 64), math.nan, dtype=F16, device=dev) for _ in range(2))
+    ints = [torch.tensor(x, dtype=torch.int32, device=dev) for x in ([[i] for i in range(nseq)], start, [ps] * nseq)]
+    qkv = normal(gen(dev, 1), (nt, 8, 64), F16)
+    pos = torch.arange(nt, dtype=torch.int32, device=dev).view(torch.uint32)
+    op.launch(pkg.KvAppendPagedArgs.of(qkv[:, :4].clone(), qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], k_pages, v_pages, pos, pkg.PagedBatch(*ints), THETA))
+    assert op.status() == (pkg.PAGED_BAD_ROWS if bad else 0)
+
+
+def test_kv_append_paged_reports_a_length_of_an_idle_sequence(pkg, dev):
+    """As attention_paged does: kv_len beyond what the table maps, though none of the step's rows is the sequence's."""
+    op = pkg.KvAppendPaged(0)
+    n = 300
+    k_pages, v_pages = (torch.zeros(2, 2, 16, 64, dtype=F16, device=dev) for _ in range(2))
+    for at in (0, 150, n - 1):
+        length = torch.zeros(n, dtype=torch.int32, device=dev)
+        length[at] = 17
+        start = torch.zeros(n + 1, dtype=torch.int32, device=dev)
+        if at < n - 1:
+            start[n], length[n - 1] = 2, 2  # two rows, the last sequence's
+        qkv = normal(gen(dev, 1), (2, 8, 64), F16)
+        pos = torch.arange(2, dtype=torch.int32, device=dev).view(torch.uint32)
+        batch = pkg.PagedBatch(torch.zeros(n, 1, dtype=torch.int32, device=dev), start, length)
+        op.launch(pkg.KvAppendPagedArgs.of(qkv[:, :4].clone(), qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], k_pages, v_pages, pos, batch, THETA))
+        assert op.status() == pkg.PAGED_BAD_LENGTH
+        op.status_reset()
