@@ -286,6 +286,15 @@ class _PackedArgs(_ArgsBase):
             dims += [s * unit for s in strides]
         packer.pack_into(buf, 0, *values, *tail, *dims)
 
+    def check_home(self, device):
+        """Refuses operands that a kernel on `device` cannot follow: those of the host (not pinned) or of another device."""
+        for t in self._alive:
+            where = getattr(t, "get_device", None)  # (an address or a layout has none: the caller's word)
+            if where is not None:
+                where = where()
+                if where != device and (where >= 0 or not t.is_pinned()):
+                    raise ValueError(f"operand of shape {tuple(t.shape)} on {t.device}: device tensors of cuda:{device} expected")
+
 
 _NO_WEIGHT = (F32, (), (), 1, None)  # beside a null weight the layout is never looked at
 
@@ -452,7 +461,7 @@ class KvAppendPagedArgs(_PackedArgs):
 
     def __init__(self, q_out_layout, q_out_base, q_layout, q_base, k_layout, k_base, v_layout, v_base, k_pages_layout, k_pages_base,
                  v_pages_layout, v_pages_base, p_layout, p_base, w_layout, w_base, batch, epsilon, theta):
-        self._alive = (q_out_base, q_base, k_base, v_base, k_pages_base, v_pages_base, p_base, w_base, batch)
+        self._alive = (q_out_base, q_base, k_base, v_base, k_pages_base, v_pages_base, p_base, w_base, *batch.arrays)
         self._fill((_operand(q_out_layout, q_out_base), _operand(q_layout, q_base), _operand(k_layout, k_base), _operand(v_layout, v_base),
                     _operand(k_pages_layout, k_pages_base), _operand(v_pages_layout, v_pages_base), _operand(p_layout, p_base),
                     _NO_WEIGHT if w_layout is None else _operand(w_layout, w_base), *batch.operands), (batch.max_seq, epsilon, theta))
@@ -467,7 +476,7 @@ class AttentionPagedArgs(_PackedArgs):
     TAIL = "QB3xf"  # batch.max_seq, mask, scale
 
     def __init__(self, q_layout, q_base, k_pages_layout, k_pages_base, v_pages_layout, v_pages_base, o_layout, o_base, batch, mask, scale):
-        self._alive = (q_base, k_pages_base, v_pages_base, o_base, batch)
+        self._alive = (q_base, k_pages_base, v_pages_base, o_base, *batch.arrays)
         self._fill((_operand(q_layout, q_base), _operand(k_pages_layout, k_pages_base), _operand(v_pages_layout, v_pages_base),
                     _operand(o_layout, o_base), *batch.operands), (batch.max_seq, mask, scale))
 
@@ -665,6 +674,7 @@ class Rope(Operator):
 
     def launch_norm(self, args, queue_alloc=None):
         """ops_rope_norm_launch: every head normalised, weighted and rotated in one pass."""
+        args.check_home(self.device)
         self._last_args = args
         rc = lib().ops_rope_norm_launch(self._h, args.byref(), current_stream(self.device) if queue_alloc is None else queue_alloc.queue())
         if rc != OK:
@@ -740,6 +750,12 @@ class AttentionKvCached(Operator):
 
 
 class _PagedOperator(Operator):
+    def launch(self, args, workspace=None, queue_alloc=None):
+        args.check_home(self.device)
+        if hasattr(workspace, "get_device") and (workspace.get_device() != self.device or not workspace.is_contiguous()):
+            raise ValueError(f"workspace: a contiguous tensor of cuda:{self.device} expected")
+        super().launch(args, workspace, queue_alloc)
+
     def status(self):
         """0, or what the device found wrong first (PAGED_BAD_*; from 100 on a bounded wait ran out).  Synchronises."""
         return getattr(lib(), f"ops_{self.NAME}_status")(self._h)

@@ -227,3 +227,57 @@ def test_no_device_no_operator(pkg, cls):
     with pytest.raises(pkg.SchemeError) as e:
         getattr(pkg, cls)(0)
     assert e.value.kind == pkg.EXECUTION_FAILED and "no CPU path" in e.value.info
+
+
+class _Queue:
+    """A queue that needs no device."""
+
+    def queue(self):
+        return 0
+
+
+def _without_device(pkg, cls, calls):
+    """An operator whose launches end in `calls`."""
+    op = getattr(pkg, cls).__new__(getattr(pkg, cls))
+    op.device, op._h = 0, None
+    op._launch = lambda *a: calls.append(a) or 0
+    return op
+
+
+def test_operands_of_the_host_never_reach_a_kernel(pkg, monkeypatch):
+    """A host tensor among the operands is refused where it would be launched; layouts and addresses are the caller's word."""
+    import torch
+    calls = []
+    host = {name: torch.zeros(shape, dtype=dt) for name, shape, dt in (
+        ("x", (7, 10, 64), torch.float16), ("q", (7, 8, 64), torch.float16), ("k", (7, 2, 64), torch.float16),
+        ("pages", (10, 2, 16, 64), torch.float16), ("p", (7,), torch.uint32), ("w", (10, 64), torch.float16))}
+
+    def bent(args, launch, cls):
+        with pytest.raises(ValueError, match="cuda:0 expected"):
+            launch(_without_device(pkg, cls, calls), args)
+
+    F16 = pkg.F16
+    lay = {"q": L(pkg, F16, (7, 8, 64)), "k": L(pkg, F16, (7, 2, 64)), "pages": L(pkg, F16, (10, 2, 16, 64)), "p": L(pkg, pkg.U32, (7,)), "w": L(pkg, F16, (10, 64))}
+    operands = ["q", "q", "k", "k", "pages", "pages", "p", "w"]
+    run = lambda op, args: op.launch(args, None, _Queue())  # noqa: E731
+    for which in range(len(operands)):
+        bases = [host[name] if i == which else P16 for i, name in enumerate(operands)]
+        bent(pkg.KvAppendPagedArgs(*(x for name, base in zip(operands, bases) for x in (lay[name], base)), batch(pkg), 1e-5, 1e4), run, "KvAppendPaged")
+    q, pages = L(pkg, F16, (8, 7, 64)), lay["pages"]
+    operands = [(q, host["q"].transpose(0, 1)), (pages, host["pages"]), (pages, host["pages"]), (q, host["q"].transpose(0, 1))]
+    for which in range(4):
+        bent(pkg.AttentionPagedArgs(*(x for i, (layout, t) in enumerate(operands) for x in (layout, t if i == which else P16)), batch(pkg), 1, 0.125), run, "AttentionPaged")
+    monkeypatch.setattr(pkg.lib(), "ops_rope_norm_launch", lambda *a: calls.append(a) or 0)
+    x = L(pkg, F16, (7, 10, 64))
+    operands = [(x, host["x"]), (x, host["x"]), (lay["p"], host["p"]), (lay["w"], host["w"])]
+    for which in range(4):
+        bent(pkg.RopeNormArgs(*(y for i, (layout, t) in enumerate(operands) for y in (layout, t if i == which else P16)), 1e-5, 1e4),
+             lambda op, args: op.launch_norm(args, _Queue()), "Rope")
+    with pytest.raises(ValueError, match="workspace"):
+        _without_device(pkg, "AttentionPaged", calls).launch(attention_args(pkg), torch.zeros(1 << 20, dtype=torch.uint8), _Queue())
+    assert not calls
+    # addresses pass
+    run(_without_device(pkg, "AttentionPaged", calls), attention_args(pkg))
+    run(_without_device(pkg, "KvAppendPaged", calls), append_args(pkg))
+    _without_device(pkg, "Rope", calls).launch_norm(norm_args(pkg), _Queue())
+    assert len(calls) == 3
