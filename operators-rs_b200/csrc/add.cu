@@ -223,7 +223,7 @@ OPS_API int ops_add_rows_create(int device, ops_add_rows **out) {
   int rc = init_base(&h->base, device);
   if (rc == OPS_OK) {
     cudaSetDevice(device);
-    if (cudaMalloc(&h->status_dev, sizeof(int)) != cudaSuccess || cudaMemset(h->status_dev, 0, sizeof(int)) != cudaSuccess)
+    if (cudaMalloc(&h->status_dev, sizeof(int)) != cudaSuccess || zero_words(h->status_dev, sizeof(int)) != cudaSuccess)
       rc = fail(OPS_EXECUTION_FAILED, "add_rows: cannot allocate the status word");
   }
   if (rc != OPS_OK) {

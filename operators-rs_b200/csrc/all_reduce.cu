@@ -545,7 +545,7 @@ OPS_API int ops_comm_init_rank(int device, int rank, int group_size, const uint8
     }
     c->has_nccl = true;
   }
-  if (cudaMalloc(&c->status_dev, sizeof(int)) != cudaSuccess || cudaMemset(c->status_dev, 0, sizeof(int)) != cudaSuccess) {
+  if (cudaMalloc(&c->status_dev, sizeof(int)) != cudaSuccess || zero_words(c->status_dev, sizeof(int)) != cudaSuccess) {
     delete c;
     return fail(OPS_EXECUTION_FAILED, "all_reduce: cannot allocate the status word");
   }

@@ -159,11 +159,11 @@ OPS_API int ops_attention_create(int device, ops_attention **out) {
   if (rc == OPS_OK) rc = ops_mat_mul_create(device, &h->mat_mul);
   if (rc == OPS_OK) {
     cudaSetDevice(device);
-    if (cudaMalloc(&h->status_dev, sizeof(int)) != cudaSuccess || cudaMemset(h->status_dev, 0, sizeof(int)) != cudaSuccess)
+    if (cudaMalloc(&h->status_dev, sizeof(int)) != cudaSuccess || zero_words(h->status_dev, sizeof(int)) != cudaSuccess)
       rc = fail(OPS_EXECUTION_FAILED, "attention: cannot allocate the status word");
     else if (cudaMalloc(&h->decode_scratch, attention_decode_scratch_bytes()) != cudaSuccess ||
              cudaMalloc(&h->decode_tickets, attention_decode_ticket_bytes()) != cudaSuccess ||
-             cudaMemset(h->decode_tickets, 0, attention_decode_ticket_bytes()) != cudaSuccess)
+             zero_words(h->decode_tickets, attention_decode_ticket_bytes()) != cudaSuccess)
       rc = fail(OPS_EXECUTION_FAILED, "attention: cannot allocate the decode scratch");
   }
   if (rc != OPS_OK) {
@@ -209,8 +209,8 @@ OPS_API int ops_attention_status_reset(ops_attention *op) {
   if (!op) return fail(OPS_ARGS_NOT_SUPPORT, "null handle");
   cudaSetDevice(op->base.device);
   cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMemset(op->status_dev, 0, sizeof(int));
-  if (e == cudaSuccess && op->decode_tickets) e = cudaMemset(op->decode_tickets, 0, attention_decode_ticket_bytes());
+  if (e == cudaSuccess) e = zero_words(op->status_dev, sizeof(int));
+  if (e == cudaSuccess && op->decode_tickets) e = zero_words(op->decode_tickets, attention_decode_ticket_bytes());
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "attention status reset: %s", cudaGetErrorString(e));
   return ops_mat_mul_status_reset(op->mat_mul);
 }

@@ -53,6 +53,13 @@ struct OpBase {
 };
 int init_base(OpBase *b, int device);
 
+// Zeroes a handle's own device words, on the current device, and waits until they are zero: cudaMemset returns before it has run, and
+// a stream that does not wait for the default one could see the words change under its launches.
+inline cudaError_t zero_words(void *words, usz bytes) {
+  const cudaError_t e = cudaMemset(words, 0, bytes);
+  return e == cudaSuccess ? cudaStreamSynchronize(0) : e;
+}
+
 // Makes `device` current for a launch and gives the caller's current device back.
 class DeviceGuard {
  public:

@@ -999,13 +999,13 @@ OPS_API int ops_mat_mul_create(int device, ops_mat_mul **out) {
     return rc;
   }
   cudaSetDevice(device);
-  if (cudaMalloc(&h->st.status_dev, sizeof(int)) != cudaSuccess || cudaMemset(h->st.status_dev, 0, sizeof(int)) != cudaSuccess) {
+  if (cudaMalloc(&h->st.status_dev, sizeof(int)) != cudaSuccess || zero_words(h->st.status_dev, sizeof(int)) != cudaSuccess) {
     delete h;
     return fail(OPS_EXECUTION_FAILED, "mat_mul: cannot allocate the status word");
   }
   const size_t ws_bytes = (size_t)GEMM_SPLIT_MAX_UNITS * GEMM_BM * 256 * sizeof(float), tk_bytes = (size_t)GEMM_SPLIT_MAX_UNITS * 16 * sizeof(unsigned int);
   if (cudaMalloc(&h->st.split_ws, ws_bytes) != cudaSuccess || cudaMalloc(&h->st.split_tickets, tk_bytes) != cudaSuccess ||
-      cudaMemset(h->st.split_tickets, 0, tk_bytes) != cudaSuccess) {
+      zero_words(h->st.split_tickets, tk_bytes) != cudaSuccess) {
     cudaGetLastError();  // without the scratch the kernel simply runs its last wave unsplit
     if (h->st.split_ws) cudaFree(h->st.split_ws);
     if (h->st.split_tickets) cudaFree(h->st.split_tickets);
@@ -1039,8 +1039,8 @@ OPS_API int ops_mat_mul_status_reset(ops_mat_mul *op) {
   if (!op) return fail(OPS_ARGS_NOT_SUPPORT, "null handle");
   cudaSetDevice(op->base.device);
   cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMemset(op->st.status_dev, 0, sizeof(int));
-  if (e == cudaSuccess && op->st.split_tickets) e = cudaMemset(op->st.split_tickets, 0, (size_t)GEMM_SPLIT_MAX_UNITS * 16 * sizeof(unsigned int));
+  if (e == cudaSuccess) e = zero_words(op->st.status_dev, sizeof(int));
+  if (e == cudaSuccess && op->st.split_tickets) e = zero_words(op->st.split_tickets, (size_t)GEMM_SPLIT_MAX_UNITS * 16 * sizeof(unsigned int));
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "mat_mul status reset: %s", cudaGetErrorString(e));
   return OPS_OK;
 }

@@ -7,7 +7,7 @@ int paged_create(PagedHandle *h, int device) {
   h->status = nullptr;
   OPS_TRY(init_base(&h->base, device));
   DeviceGuard guard(device);
-  if (cudaMalloc(&h->status, 2 * sizeof(int)) != cudaSuccess || cudaMemset(h->status, 0, 2 * sizeof(int)) != cudaSuccess) {
+  if (cudaMalloc(&h->status, 2 * sizeof(int)) != cudaSuccess || zero_words(h->status, 2 * sizeof(int)) != cudaSuccess) {
     cudaGetLastError();
     if (h->status) cudaFree(h->status);
     return fail(OPS_EXECUTION_FAILED, "cannot allocate the status words");
@@ -29,7 +29,7 @@ int paged_status(const PagedHandle *h) {
 int paged_status_reset(PagedHandle *h) {
   DeviceGuard guard(h->base.device);
   cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMemset(h->status, 0, 2 * sizeof(int));
+  if (e == cudaSuccess) e = zero_words(h->status, 2 * sizeof(int));
   if (e != cudaSuccess) return fail(OPS_EXECUTION_FAILED, "status reset: %s", cudaGetErrorString(e));
   return OPS_OK;
 }

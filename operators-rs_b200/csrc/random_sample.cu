@@ -1148,7 +1148,7 @@ OPS_API int ops_random_sample_create(int device, ops_random_sample **out) {
   }
   cudaSetDevice(device);
   if (cudaMalloc(&h->arg_scratch, ARGMAX_OWN_ROWS * sizeof(ArgmaxScratch)) != cudaSuccess ||
-      cudaMemset(h->arg_scratch, 0, ARGMAX_OWN_ROWS * sizeof(ArgmaxScratch)) != cudaSuccess) {
+      zero_words(h->arg_scratch, ARGMAX_OWN_ROWS * sizeof(ArgmaxScratch)) != cudaSuccess) {
     cudaGetLastError();  // without it the argmax path takes its records from the caller's workspace
     if (h->arg_scratch) cudaFree(h->arg_scratch);
     h->arg_scratch = nullptr;

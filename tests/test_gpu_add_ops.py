@@ -87,3 +87,23 @@ def test_add_rows_out_of_range_index_is_reported(pkg, synth, dev):
     op.launch(pkg.AddRowsArgs.of(dst, src, idx))
     assert op.status() == 1  # the crate's CPU operator asserts idx < k; here the row is skipped and the status word set
     assert dst[0, 1].eq(1).all() and dst[0, 0].eq(2).all() and dst[0, 2].eq(2).all()
+
+
+def test_add_rows_status_of_a_handle_made_on_a_busy_device(pkg, dev):
+    """What a launch on a stream of its own reports stays, although the default stream was busy when the handle was made."""
+    dst = torch.ones(1, 3, 16, dtype=torch.float16, device=dev)
+    src = torch.ones(4, 16, dtype=torch.float16, device=dev)
+    idx = torch.tensor([[0, 9, 3]], dtype=torch.int32, device=dev).view(torch.uint32)
+    side = torch.cuda.Stream(dev)
+
+    def launch(op):
+        with torch.cuda.stream(side):
+            op.launch(pkg.AddRowsArgs.of(dst, src, idx))
+
+    launch(pkg.AddRows(0))  # a kernel's first launch may wait for the device
+    torch.cuda.synchronize()
+    torch.cuda._sleep(300_000_000)  # some 0.2 s of the default stream
+    op = pkg.AddRows(0)
+    launch(op)
+    torch.cuda.synchronize()
+    assert op.status() == 1

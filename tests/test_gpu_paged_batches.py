@@ -45,3 +45,32 @@ def test_kv_append_paged_reports_a_length_of_an_idle_sequence(pkg, dev):
         op.launch(pkg.KvAppendPagedArgs.of(qkv[:, :4].clone(), qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], k_pages, v_pages, pos, batch, THETA))
         assert op.status() == pkg.PAGED_BAD_LENGTH
         op.status_reset()
+
+
+# ------------------------------------------------------------------------------------------------ status words
+@pytest.mark.parametrize("cls", ["KvAppendPaged", "AttentionPaged"])
+def test_status_of_a_handle_made_on_a_busy_device(pkg, dev, cls):
+    """What a launch on a stream of its own reports stays, although the default stream was busy when the handle was made: the
+    words are clear before the handle is there, not some time after."""
+    b = ref.Batch(dev, F16, [1], [20], 2, 64, 16, seed=1)
+    b.fill(gen(dev, 1))
+    b.page_table[0, 1] = b.npages
+    qkv = normal(gen(dev, 2), (1, 8, 64), F16)
+    pos = torch.zeros(1, dtype=torch.int32, device=dev).view(torch.uint32)
+    o, ws, side = torch.zeros(4, 1, 64, dtype=F16, device=dev), torch.empty(64 << 20, dtype=torch.uint8, device=dev), torch.cuda.Stream(dev)
+
+    def launch(op):
+        with torch.cuda.stream(side):
+            if cls == "KvAppendPaged":
+                op.launch(pkg.KvAppendPagedArgs.of(qkv[:, :4], qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], b.k_pages, b.v_pages, pos, b.descriptor(pkg), THETA))
+            else:
+                attend(pkg, op, b, qkv[:, :4].permute(1, 0, 2), o, ws=ws)
+
+    launch(getattr(pkg, cls)(0))  # a kernel's first launch may wait for the device
+    torch.cuda.synchronize()
+    torch.cuda._sleep(300_000_000)  # some 0.2 s of the default stream
+    op = getattr(pkg, cls)(0)
+    launch(op)
+    assert op.status() == pkg.PAGED_BAD_PAGE
+    op.status_reset()
+    assert op.status() == 0
