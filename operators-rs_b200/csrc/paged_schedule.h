@@ -207,8 +207,16 @@ struct PagedWalk {
   int begin, at, end;
 };
 
-// The next piece of the share (an empty one is passed over).  Seqs: seq index -> PagedSeq.
-template <class Seqs> OPS_HD PagedPiece paged_next(const PagedLine &l, int nseq, PagedWalk &w, const Seqs &seqs) {
+// Whether a sequence with rows [r0, r1) can have points on the line (max_seq may still rule it out).
+OPS_HD bool paged_rows_fit(const PagedLine &l, uint32_t r0, uint32_t r1) {
+  if (r1 <= r0) return false;
+  const unsigned long long rows = (unsigned long long)(r1 - r0) * (unsigned)l.group;
+  return rows >= (unsigned)l.rows_lo && rows <= (unsigned)l.rows_hi;
+}
+
+// The next piece of the share (an empty one is passed over).  Seqs: seq index -> PagedSeq.  Skip: the first sequence from the given
+// one on that has points on the line, or any in front of it; it is asked when one without any has been met.
+template <class Seqs, class Skip> OPS_HD PagedPiece paged_next(const PagedLine &l, int nseq, PagedWalk &w, const Seqs &seqs, const Skip &skip) {
   PagedPiece q;
   q.seq = -1;
   OPS_ROLLED while (w.at < w.end && w.seq < nseq) {
@@ -218,6 +226,7 @@ template <class Seqs> OPS_HD PagedPiece paged_next(const PagedLine &l, int nseq,
     if (w.at >= w.begin + all) {
       w.begin += all;
       ++w.seq;
+      if (all == 0) w.seq = skip(w.seq);
       continue;
     }
     const PagedUnit u = paged_unit(p, w.at - w.begin);
@@ -234,6 +243,9 @@ template <class Seqs> OPS_HD PagedPiece paged_next(const PagedLine &l, int nseq,
     break;
   }
   return q;
+}
+template <class Seqs> OPS_HD PagedPiece paged_next(const PagedLine &l, int nseq, PagedWalk &w, const Seqs &seqs) {
+  return paged_next(l, nseq, w, seqs, [](int seq) { return seq; });
 }
 
 }  // namespace ops

@@ -281,3 +281,13 @@ def test_operands_of_the_host_never_reach_a_kernel(pkg, monkeypatch):
     run(_without_device(pkg, "KvAppendPaged", calls), append_args(pkg))
     _without_device(pkg, "Rope", calls).launch_norm(norm_args(pkg), _Queue())
     assert len(calls) == 3
+
+
+def test_schedule_of_sparse_batches_on_the_cpu(tmp_path):
+    """Sequences without work on a line are passed over in runs."""
+    exe = str(tmp_path / "paged_schedule_sparse_check")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "paged_schedule_sparse_check.cc")
+    built = subprocess.run([shutil.which("g++") or "g++", "-O2", "-std=c++17", src, "-o", exe], capture_output=True, text=True)
+    assert built.returncode == 0, built.stderr
+    ran = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert ran.returncode == 0 and "schedule ok" in ran.stdout, ran.stdout

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_paged import BF16, EPS, F16, THETA, attend, gen, near, normal
+from test_gpu_paged import EPS, F16, THETA, attend, check_attention, gen, near, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +74,13 @@ def test_status_of_a_handle_made_on_a_busy_device(pkg, dev, cls):
     assert op.status() == pkg.PAGED_BAD_PAGE
     op.status_reset()
     assert op.status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ work far apart
+@pytest.mark.parametrize("n,past", [([300] + [0] * 3000 + [200], 300),                   # idle sequences between two chunks
+                                    ([70] + [1] * 300 + [0] * 33 + [60, 0, 0, 80], 90),  # single tokens, which the tiles have nothing of
+                                    ([0] * 200 + [1] + [0] * 5000 + [1], 2500),          # ... and single tokens far apart
+                                    ([1] + [40] * 5 + [0] * 129 + [40] * 3 + [1] * 2, 700)])
+def test_attention_paged_sequences_far_apart(pkg, dev, n, past):
+    kv = [m + (past + 13 * i % 50 if m else 0) for i, m in enumerate(n)]
+    check_attention(pkg, dev, pkg.AttentionPaged(0), ref.Batch(dev, F16, n, kv, 2, 64, 16, seed=4, pad=3), 4)
