@@ -366,6 +366,10 @@ int ops_attention_paged_scheme(ops_attention_paged *op, const ops_attention_page
 int ops_attention_paged_launch(const ops_attention_paged *op, const ops_attention_paged_args *args, void *ws, size_t ws_len, void *stream);
 int ops_attention_paged_status(const ops_attention_paged *op);
 int ops_attention_paged_status_reset(ops_attention_paged *op);
+/* How long the SMs that share more than two parts of a few query rows wait for one another before the last one is left to join them
+ * alone (100 us when a handle is made, 1 s at most; taken by the launches that follow).  Outputs do not depend on it, bit for bit:
+ * it is there so that the rare case, SMs that come to a launch late, can be brought about. */
+int ops_attention_paged_set_patience(ops_attention_paged *op, uint64_t nanoseconds);
 void ops_attention_paged_destroy(ops_attention_paged *op);
 
 /* ---------------------------------------------------------------------------------------------

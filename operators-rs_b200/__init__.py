@@ -771,6 +771,10 @@ class KvAppendPaged(_PagedOperator):
 class AttentionPaged(_PagedOperator):
     NAME = "attention_paged"
 
+    def set_patience(self, nanoseconds):
+        """ops_attention_paged_set_patience: how long parts of query rows wait for one another; outputs do not depend on it."""
+        _check(lib().ops_attention_paged_set_patience(self._h, ctypes.c_uint64(nanoseconds)), False)
+
 
 class RandomSample(Operator):
     NAME = "random_sample"
@@ -946,6 +950,6 @@ EXPORTS = [
     "ops_comm_init_rank", "ops_comm_rank", "ops_comm_group_size", "ops_comm_destroy", "ops_comm_p2p_export",
     "ops_comm_p2p_attach", "ops_comm_p2p_status", "ops_comm_p2p_reset", "ops_comm_p2p_direct", "ops_comm_nvls_attach", "ops_all_reduce_add_launch",
     "ops_rope_norm_launch", "ops_kv_append_paged_status", "ops_kv_append_paged_status_reset", "ops_attention_paged_status",
-    "ops_attention_paged_status_reset",
+    "ops_attention_paged_status_reset", "ops_attention_paged_set_patience",
     "ops_rms_norm_add_launch", "ops_comm_create_loopback", "ops_all_reduce_set_algo", "ops_add_rows_status", "ops_mat_mul_all_reduce_launch",
 ]

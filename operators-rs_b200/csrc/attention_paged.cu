@@ -82,6 +82,13 @@ using namespace ops;
 
 OPS_DEFINE_PAGED_HANDLE(attention_paged)
 
+OPS_API int ops_attention_paged_set_patience(ops_attention_paged *op, uint64_t nanoseconds) {
+  if (!op) return fail(OPS_ARGS_NOT_SUPPORT, "null handle");
+  if (nanoseconds > 1000000000u) return fail(OPS_ARGS_NOT_SUPPORT, "attention_paged: a patience of %llu ns, 1 s at most expected", (unsigned long long)nanoseconds);
+  op->h.patience.store(nanoseconds, std::memory_order_relaxed);
+  return OPS_OK;
+}
+
 namespace ops {
 
 // The two lines of a launch and the scratch they want.  A sequence goes to the line of few rows when its new tokens times the query
@@ -207,6 +214,7 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
   cudaStream_t s = (cudaStream_t)stream;
   const bool bf16 = m.dt == OPS_DT_BF16;
   char *at = (char *)(((uintptr_t)ws + 255) / 256 * 256);
+  g.patience = op->h.patience.load(std::memory_order_relaxed);
   g.odd_scale = !(g.scale_log2 > 0.f);
   g.per_tile = AP_TILE_ROWS / 2 / (int)(m.nh / m.paged.nkvh);
   g.few.line = plan.few;

@@ -35,6 +35,7 @@ struct PagedAttnArgs {
   float scale_log2;  // scale * log2(e): the softmax runs in powers of two
   int odd_scale;     // scale <= 0
   int per_tile;      // tokens of a tile: 128 / query heads of a kv head
+  unsigned long long patience;  // ns that a warp waits for the other parts of a unit of more than two
   PagedBatch batch;
   PagedLineArgs few, tile;
 };

@@ -48,7 +48,6 @@ constexpr int TL_THREADS = 384;
 constexpr int TL_ROWS = 128;  // of a tile
 constexpr int TL_KEYS = AP_TILE_BLOCK;
 constexpr int TL_RING = 4;    // pieces posted ahead
-constexpr unsigned long long TL_HELP_NS = 100000;  // 100 us: parts of a unit end within a few
 constexpr int TL_READERS = 11;  // warps that read the ring: all but the scheduler
 
 // A piece as the scheduler posts it.
@@ -606,7 +605,7 @@ __device__ __forceinline__ bool tiles(const CUtensorMap &tmap_q, const CUtensorM
         uint32_t n = 0;
         if (lane == 0) n = ld_acquire_gpu(arrived);
         all = (__shfl_sync(0xffffffffu, n, 0) & 0xffffu) == warps;
-      } while (!all && __all_sync(0xffffffffu, globaltimer_ns() - since < TL_HELP_NS));
+      } while (!all && __all_sync(0xffffffffu, globaltimer_ns() - since < a.patience));
       if (!all) {
         uint32_t n = 0;
         if (lane == 0) {

@@ -163,6 +163,7 @@ struct PagedHandle {
   OpBase base;
   int *status;
   mutable std::atomic<unsigned> prepared{0};  // kernels whose shared memory has been reserved on the device
+  std::atomic<unsigned long long> patience{100000};  // attention_paged's, ns: parts of a unit end within a few us of each other
 };
 int paged_create(PagedHandle *h, int device);
 void paged_destroy(PagedHandle *h);

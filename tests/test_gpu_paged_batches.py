@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_paged import EPS, F16, THETA, attend, check_attention, gen, near, normal
+from test_gpu_paged import BF16, F16, THETA, attend, check_attention, gen, near, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +84,34 @@ def test_status_of_a_handle_made_on_a_busy_device(pkg, dev, cls):
 def test_attention_paged_sequences_far_apart(pkg, dev, n, past):
     kv = [m + (past + 13 * i % 50 if m else 0) for i, m in enumerate(n)]
     check_attention(pkg, dev, pkg.AttentionPaged(0), ref.Batch(dev, F16, n, kv, 2, 64, 16, seed=4, pad=3), 4)
+
+
+# ------------------------------------------------------------------------------------------------ parts that do not wait for one another
+@pytest.mark.parametrize("n,kv,nkvh,nh,dh", [([40], [12000], 9, 36, 128), ([20, 30, 300], [9000, 9500, 9800], 3, 12, 128), ([33], [20000], 1, 8, 64),
+                                             ([1, 700], [3000, 6000], 1, 4, 128)])
+def test_attention_paged_units_whose_parts_do_not_wait(pkg, dev, n, kv, nkvh, nh, dh):
+    """Units of many parts, joined by all their warps together when they meet, by the last to come when the others have left: bit
+    for bit the same, from a patience that none outlasts through one that some do to the ordinary one."""
+    op = pkg.AttentionPaged(0)
+    b = ref.Batch(dev, BF16, n, kv, nkvh, dh, 16, seed=6)
+    g = gen(dev, 6)
+    b.fill(g)
+    q = normal(g, (nh, b.nt, dh), BF16)
+    want = torch.empty_like(q)
+    ws = attend(pkg, op, b, q, want)
+    near(want, *ref.attention(b, q, True, dh ** -0.5), "o")
+    o = torch.empty_like(q)
+    for patience in [0] * 30 + [500, 1000, 2000, 4000] * 15 + [100000]:
+        op.set_patience(patience)
+        o.fill_(7.0)
+        ws.fill_(0xff)
+        attend(pkg, op, b, q, o, ws=ws)
+        assert torch.equal(o, want), patience
+    assert op.status() == 0
+
+
+def test_attention_paged_patience_is_bounded(pkg, dev):
+    op = pkg.AttentionPaged(0)
+    with pytest.raises(pkg.SchemeError):
+        op.set_patience(10 ** 9 + 1)
+    op.set_patience(10 ** 9)
