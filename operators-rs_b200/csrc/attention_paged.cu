@@ -91,69 +91,24 @@ OPS_API int ops_attention_paged_set_patience(ops_attention_paged *op, uint64_t n
 
 namespace ops {
 
-// The two lines of a launch and the scratch they want.  A sequence goes to the line of few rows when its new tokens times the query
-// heads of a kv head fit; sequences with more go to the tiles.  Where max_seq says that there are none, the launch is of the kernel
-// without tiles.
-struct PagedAttnPlan {
-  PagedLine few, tile;  // ctas == 0: nothing can be on it
-  int few_rows, part_dh;
+// The two lines of a launch and the scratch they want.  Where max_seq says that there are no tiles, the launch is of the kernel
+// without them.
+struct PagedAttnPlan : PagedLines {
+  int part_dh;
   usz few_arrived, tile_arrived, few_parts, tile_parts;  // bytes
   usz bytes() const { return few_arrived + tile_arrived + few_parts + tile_parts + 256; }
 };
 
 static usz up256(usz n) { return (n + 255) / 256 * 256; }
 
-// The least shift with which a line cannot pass 31 bits: units, at most all rows in tiles and one more per sequence, of at most
-// all slots and rows.  `overhead`, `min_share`: keys.
-static void line_scale(PagedLine *l, usz nt, usz nseq, usz slots, int overhead, int min_share) {
-  const double units = ((double)(nt / (usz)l->tokens) + (double)nseq) * l->nkvh, keys = (double)slots + (double)nt + l->tokens + overhead;
-  l->shift = 0;
-  while (l->shift < 30 && units * (std::ldexp(keys, -l->shift) + 4.0) > 2147483647.0) ++l->shift;
-  l->overhead = std::max(1, overhead >> l->shift);
-  l->min_share = std::max(1, min_share >> l->shift);  // a power of two
-  l->min_share_log2 = 0;
-  while ((1 << l->min_share_log2) < l->min_share) ++l->min_share_log2;
-  l->by_tokens = paged_div_by((uint32_t)l->tokens);
-  l->by_ctas = paged_div_by((uint32_t)l->ctas);
-}
-
 static PagedAttnPlan attention_paged_plan(const OpBase &base, usz nh, usz nkvh, usz dh, bool causal, uint32_t max_seq, usz nt, usz nseq, usz slots) {
   PagedAttnPlan p;
-  memset(&p, 0, sizeof(p));
-  const usz group = nh / nkvh, most = max_seq == 0xffffffffu ? 0xffffffffull : (usz)max_seq * group;
-  // 16 rows cost the kernel a third of its ring; 8 are enough for one token of up to 8 heads
-  p.few_rows = group <= 8 && !(most > 8 && most <= 16) ? 8 : 16;
+  static_cast<PagedLines &>(p) = paged_lines(base.sm_count, nh, nkvh, causal, max_seq, nt, nseq, slots);
   p.part_dh = dh <= 64 ? 64 : 128;
-  PagedLine l;
-  memset(&l, 0, sizeof(l));
-  l.nkvh = (int)nkvh;
-  l.group = (int)group;
-  l.by_group = paged_div_by((uint32_t)group);
-  l.causal = causal;
-  l.max_seq = max_seq > 0x7fffffffu ? 0x7fffffff : (int)max_seq;
-  p.few = p.tile = l;
-  if (group <= (usz)p.few_rows) {
-    p.few.rows_lo = 1;
-    p.few.rows_hi = p.few_rows;
-    p.few.tokens = p.few_rows;
-    p.few.block_log2 = AP_FEW_BLOCK_LOG2;
-    p.few.ctas = std::min(base.sm_count, AP_MAX_CTAS);  // one a SM: the ring takes its shared memory
-    line_scale(&p.few, nt, nseq, slots, 128, 128);
-    p.few_arrived = up256((usz)AP_LEVELS * p.few.ctas * 8 * sizeof(uint32_t));
-    p.few_parts = up256(3 * (usz)p.few.ctas * p.few_rows * (p.part_dh + 2) * sizeof(float));
-    p.tile.rows_lo = p.few_rows + 1;
-  } else {
-    p.tile.rows_lo = 1;
-  }
-  if (most >= (usz)p.tile.rows_lo) {
-    p.tile.rows_hi = 0x7fffffff;
-    p.tile.tokens = AP_TILE_ROWS / 2 / (int)group * 2;
-    p.tile.block_log2 = AP_TILE_BLOCK_LOG2;
-    p.tile.ctas = std::min(base.sm_count, AP_MAX_CTAS);
-    line_scale(&p.tile, nt, nseq, slots, 512, 512);
-    p.tile_arrived = up256((usz)AP_LEVELS * p.tile.ctas * 8 * sizeof(uint32_t));
-    p.tile_parts = up256(2 * (usz)p.tile.ctas * AP_TILE_ROWS * (p.part_dh + 2) * sizeof(float));
-  }
+  p.few_arrived = up256((usz)AP_LEVELS * p.few.ctas * 8 * sizeof(uint32_t));
+  p.few_parts = up256(3 * (usz)p.few.ctas * p.few_rows * (p.part_dh + 2) * sizeof(float));
+  p.tile_arrived = up256((usz)AP_LEVELS * p.tile.ctas * 8 * sizeof(uint32_t));
+  p.tile_parts = up256(2 * (usz)p.tile.ctas * AP_TILE_ROWS * (p.part_dh + 2) * sizeof(float));
   return p;
 }
 

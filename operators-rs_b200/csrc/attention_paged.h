@@ -10,9 +10,6 @@ namespace ops {
 
 constexpr int AP_MAX_DH = 128;
 constexpr int AP_MAX_GROUP = 128;
-constexpr int AP_MAX_CTAS = 256;  // of a kernel
-constexpr int AP_SHARES = 16;     // the few-rows line gets k / 16 of the CTAs where both have work
-constexpr int AP_FEW_JOIN = 16, AP_LEVELS = 2;  // parts are joined in groups, the groups in turn: 16^2 is AP_MAX_CTAS
 
 // A line of work (paged_schedule.h) with the scratch of its units' parts.
 struct PagedLineArgs {
@@ -40,9 +37,6 @@ struct PagedAttnArgs {
   PagedLineArgs few, tile;
 };
 
-// The few-rows line's CTAs for k of 16 shares; the tiles get the others.
-OPS_HD int paged_share(int ctas, int k) { return ctas * k / AP_SHARES > 0 ? ctas * k / AP_SHARES : 1; }
-
 // Tensor maps: K and V of the whole cache, boxes of 64 columns x 2^box_log2 slots of one head of one page; the queries, boxes of 64
 // columns x the heads of a group x the tokens of a tile.
 struct PagedAttnMaps {
@@ -51,8 +45,6 @@ struct PagedAttnMaps {
 // Launches the kernel for few rows alone (tiles == false) or for both, of 8 or 16 few rows.  `prepared`: the handle's.
 int attention_paged_run_f16(const PagedAttnMaps &maps, const PagedAttnArgs &a, int few_rows, bool tiles, std::atomic<unsigned> &prepared, cudaStream_t s);
 int attention_paged_run_bf16(const PagedAttnMaps &maps, const PagedAttnArgs &a, int few_rows, bool tiles, std::atomic<unsigned> &prepared, cudaStream_t s);
-constexpr int AP_FEW_BLOCK_LOG2 = 5, AP_FEW_BLOCK = 32, AP_TILE_BLOCK_LOG2 = 7, AP_TILE_BLOCK = 128;  // keys of a block
-constexpr int AP_TILE_ROWS = 256;                       // query rows of a unit of the tile kernel: two tiles
 
 #ifdef __CUDACC__
 __device__ __forceinline__ float ap_ex2(float x) {

@@ -14,6 +14,9 @@
 // 32-bit throughout, without a division by anything but what the host knows, and one warp of a CTA does it.  What the others
 // wait for at the start of a launch is this.
 #pragma once
+#include <algorithm>
+#include <cmath>
+#include <cstddef>
 #include <cstdint>
 
 #ifdef __CUDACC__
@@ -66,6 +69,70 @@ struct PagedLine {
   int ctas;
   PagedDiv by_group, by_tokens, by_ctas;
 };
+
+constexpr int AP_MAX_CTAS = 256;  // of a kernel
+constexpr int AP_SHARES = 16;     // the few-rows line gets k / 16 of the CTAs where both have work
+constexpr int AP_FEW_JOIN = 16, AP_LEVELS = 2;  // parts are joined in groups, the groups in turn: 16^2 is AP_MAX_CTAS
+constexpr int AP_FEW_BLOCK_LOG2 = 5, AP_FEW_BLOCK = 32, AP_TILE_BLOCK_LOG2 = 7, AP_TILE_BLOCK = 128;  // keys of a block
+constexpr int AP_TILE_ROWS = 256;                       // query rows of a unit of the tile kernel: two tiles
+
+// The few-rows line's CTAs for k of 16 shares; the tiles get the others.
+OPS_HD int paged_share(int ctas, int k) { return ctas * k / AP_SHARES > 0 ? ctas * k / AP_SHARES : 1; }
+
+// The lines of a launch.  A sequence goes to the line of few rows when its new tokens times the query heads of a kv head fit;
+// sequences with more go to the tiles.
+struct PagedLines {
+  PagedLine few, tile;  // ctas == 0: nothing can be on it
+  int few_rows;
+};
+
+// The least shift with which a line cannot pass 31 bits: units, at most all rows in tiles and one more per sequence, of at most
+// all slots and rows.  `overhead`, `min_share`: keys.
+inline void paged_line_scale(PagedLine *l, size_t nt, size_t nseq, size_t slots, int overhead, int min_share) {
+  const double units = ((double)(nt / (size_t)l->tokens) + (double)nseq) * l->nkvh, keys = (double)slots + (double)nt + l->tokens + overhead;
+  l->shift = 0;
+  while (l->shift < 30 && units * (std::ldexp(keys, -l->shift) + 4.0) > 2147483647.0) ++l->shift;
+  l->overhead = std::max(1, overhead >> l->shift);
+  l->min_share = std::max(1, min_share >> l->shift);  // a power of two
+  l->min_share_log2 = 0;
+  while ((1 << l->min_share_log2) < l->min_share) ++l->min_share_log2;
+  l->by_tokens = paged_div_by((uint32_t)l->tokens);
+  l->by_ctas = paged_div_by((uint32_t)l->ctas);
+}
+
+// For nt rows and nseq sequences of up to `slots` slots; max_seq: 0xffffffff when unknown.
+inline PagedLines paged_lines(int sm_count, size_t nh, size_t nkvh, bool causal, uint32_t max_seq, size_t nt, size_t nseq, size_t slots) {
+  PagedLines p = PagedLines();
+  const size_t group = nh / nkvh, most = max_seq == 0xffffffffu ? 0xffffffffull : (size_t)max_seq * group;
+  // 16 rows cost the kernel a third of its ring; 8 are enough for one token of up to 8 heads
+  p.few_rows = group <= 8 && !(most > 8 && most <= 16) ? 8 : 16;
+  PagedLine l = PagedLine();
+  l.nkvh = (int)nkvh;
+  l.group = (int)group;
+  l.by_group = paged_div_by((uint32_t)group);
+  l.causal = causal;
+  l.max_seq = max_seq > 0x7fffffffu ? 0x7fffffff : (int)max_seq;
+  p.few = p.tile = l;
+  if (group <= (size_t)p.few_rows) {
+    p.few.rows_lo = 1;
+    p.few.rows_hi = p.few_rows;
+    p.few.tokens = p.few_rows;
+    p.few.block_log2 = AP_FEW_BLOCK_LOG2;
+    p.few.ctas = std::min(sm_count, AP_MAX_CTAS);  // one a SM: the ring takes its shared memory
+    paged_line_scale(&p.few, nt, nseq, slots, 128, 128);
+    p.tile.rows_lo = p.few_rows + 1;
+  } else {
+    p.tile.rows_lo = 1;
+  }
+  if (most >= (size_t)p.tile.rows_lo) {
+    p.tile.rows_hi = 0x7fffffff;
+    p.tile.tokens = AP_TILE_ROWS / 2 / (int)group * 2;
+    p.tile.block_log2 = AP_TILE_BLOCK_LOG2;
+    p.tile.ctas = std::min(sm_count, AP_MAX_CTAS);
+    paged_line_scale(&p.tile, nt, nseq, slots, 512, 512);
+  }
+  return p;
+}
 
 // What one sequence puts on the line: per kv head `tiles` units, the p-th of base + ramp * (p + 1) points, the overhead among
 // them.  (Causal tiles see `tokens` keys more each; the last one may see fewer, which the line does not bother to know.)

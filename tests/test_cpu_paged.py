@@ -291,3 +291,13 @@ def test_schedule_of_sparse_batches_on_the_cpu(tmp_path):
     assert built.returncode == 0, built.stderr
     ran = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert ran.returncode == 0 and "schedule ok" in ran.stdout, ran.stdout
+
+
+def test_schedule_of_launches_on_the_cpu(tmp_path):
+    """The lines as a launch makes them: slots, counters and marks are nobody's twice."""
+    exe = str(tmp_path / "paged_schedule_launch_check")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "paged_schedule_launch_check.cc")
+    built = subprocess.run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-Wall", src, "-o", exe], capture_output=True, text=True)
+    assert built.returncode == 0, built.stderr
+    ran = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert ran.returncode == 0 and "schedule ok" in ran.stdout, ran.stdout
