@@ -115,3 +115,127 @@ def test_attention_paged_patience_is_bounded(pkg, dev):
     with pytest.raises(pkg.SchemeError):
         op.set_patience(10 ** 9 + 1)
     op.set_patience(10 ** 9)
+
+
+# ------------------------------------------------------------------------------------------------ values that no score may meet
+# Past and chunk by kernel: few rows, a few drafted tokens, tiles in one part, tiles of many parts.
+SPECIAL = [([1, 1], [700, 40], 2), ([3, 2], [900, 40], 2), ([300, 20], [400, 50], 4), ([40, 30], [9000, 300], 4)]
+
+
+def plain(b, i, q, scale, hidden=()):
+    """Sequence i's rows over its slots but `hidden`, in doubles: ([nh, n, dh], tolerance as ref.attention derives it, slots a row sees)."""
+    n, l, r0 = b.n[i], b.kv[i], int(b.start[i])
+    page, slot = b.slots(i, 0, l)
+    see = torch.arange(l, device=q.device)[None] <= torch.arange(l - n, l, device=q.device)[:, None]
+    see[:, list(hidden)] = False
+    out, tol = [], []
+    for h in range(q.shape[0]):
+        kv = h // (q.shape[0] // b.nkvh)
+        k, v = b.k_pages[page, kv, slot].double().clone(), b.v_pages[page, kv, slot].double().clone()
+        k[list(hidden)], v[list(hidden)] = 0, 0
+        x = q[h, r0: r0 + n].double()
+        size = (x.abs() @ k.abs().T * scale).amax(-1, keepdim=True)
+        p = torch.softmax((x @ k.T * scale).masked_fill(~see, -math.inf), -1)
+        o = p @ v
+        move = ref.HALF_STEP[b.dt] + 2 * b.dh * 2.0 ** -23 * size + 2.0 ** -20
+        out.append(o)
+        tol.append(ref.HALF_STEP[b.dt] * o.abs() + (1 + ref.HALF_STEP[b.dt]) * (move * (p @ v.abs()) + l * ref.LEAST[b.dt] * v.abs().amax()) + ref.LEAST[b.dt])
+    return torch.stack(out), torch.stack(tol), see
+
+
+def special(pkg, dev, dt, case, positive=False):
+    n, kv, nh = SPECIAL[case]
+    b = ref.Batch(dev, dt, n, kv, 1, 64, 16, seed=case)
+    g = gen(dev, case)
+    b.fill(g)
+    q = normal(g, (nh, b.nt, 64), dt)
+    return b, (q.abs() + 0.1 if positive else q)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("case", [1, 2, 3])
+def test_attention_paged_keys_of_later_tokens(pkg, dev, dt, value, case):
+    """A key that only the sequence's last token sees shows in no other row, whatever it holds."""
+    b, q = special(pkg, dev, dt, case)
+    wants = [plain(b, i, q, 0.125) for i in range(2)]
+    page, slot = b.slots(0, b.kv[0] - 1, b.kv[0])
+    b.k_pages[page, :, slot] = value
+    o = torch.zeros_like(q)
+    attend(pkg, pkg.AttentionPaged(0), b, q, o)
+    near(o[:, : b.n[0] - 1], wants[0][0][:, :-1], wants[0][1][:, :-1], "the rows in front")
+    near(o[:, b.n[0]:], *wants[1][:2], "the other sequence")
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("case", [1, 2, 3])
+def test_attention_paged_values_of_later_tokens(pkg, dev, dt, value, case):
+    """A value of the last token's that is no number shows in the rows that see it, in no other sequence, and in no unit of rows in
+    front of which ends before its block of keys (rows that share a block with it are documented to take it with a weight of zero)."""
+    b, q = special(pkg, dev, dt, case)
+    wants = [plain(b, i, q, 0.125) for i in range(2)]
+    page, slot = b.slots(0, b.kv[0] - 1, b.kv[0])
+    b.v_pages[page, :, slot] = value
+    o = torch.zeros_like(q)
+    attend(pkg, pkg.AttentionPaged(0), b, q, o)
+    assert not torch.isfinite(o[:, b.n[0] - 1]).any()
+    near(o[:, b.n[0]:], *wants[1][:2], "the other sequence")
+    unit = 2 * (128 // q.shape[0])  # tokens of two tiles, the heads sharing one kv head
+    for t0 in range(0, b.n[0] if case > 1 else 0, unit):
+        if b.kv[0] - b.n[0] + t0 + unit <= (b.kv[0] - 1) // 128 * 128:
+            near(o[:, t0: t0 + unit], wants[0][0][:, t0: t0 + unit], wants[0][1][:, t0: t0 + unit], f"tokens from {t0} on")
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("case", [0, 1, 2, 3])
+@pytest.mark.parametrize("hidden", ["first", "some", "most"])
+def test_attention_paged_scores_of_minus_infinity(pkg, dev, dt, case, hidden):
+    """Keys of -inf against positive queries weigh nothing: the first blocks of a row entirely, single ones, all but a few."""
+    b, q = special(pkg, dev, dt, case, positive=True)
+    l = b.kv[0]
+    past = l - b.n[0]
+    which = {"first": range(0, min(257, past)), "some": range(0, l, 3), "most": [s for s in range(l) if s % 97 or s > past]}[hidden]
+    want, tol, see = plain(b, 0, q, 0.125, which)
+    page, slot = b.slots(0, 0, l)
+    b.k_pages[page[list(which)], :, slot[list(which)]] = -math.inf
+    o = torch.zeros_like(q)
+    attend(pkg, pkg.AttentionPaged(0), b, q, o)
+    rows = see.any(-1)
+    near(o[:, : b.n[0]][:, rows], want[:, rows], tol[:, rows], "o")
+    near(o[:, b.n[0]:], *plain(b, 1, q, 0.125)[:2], "the other sequence")
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("case", [0, 1, 2, 3])
+def test_attention_paged_scores_of_infinity(pkg, dev, dt, case):
+    """A score of +inf makes its row NaN, as the formula does (infinity less infinity), in however many parts; no other row."""
+    b, q = special(pkg, dev, dt, case, positive=True)
+    wants = [plain(b, i, q, 0.125) for i in range(2)]
+    at = b.kv[0] - b.n[0] // 2 - 1  # the later half of the new tokens see it
+    page, slot = b.slots(0, at, at + 1)
+    b.k_pages[page, :, slot] = math.inf
+    o = torch.zeros_like(q)
+    attend(pkg, pkg.AttentionPaged(0), b, q, o)
+    sees = wants[0][2][:, at]
+    assert bool(torch.isnan(o[:, : b.n[0]][:, sees]).all())
+    near(o[:, : b.n[0]][:, ~sees], wants[0][0][:, ~sees], wants[0][1][:, ~sees], "rows in front of it")
+    near(o[:, b.n[0]:], *wants[1][:2], "the other sequence")
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("case", [0, 1, 2, 3])
+def test_attention_paged_infinite_values(pkg, dev, dt, case):
+    """An infinite value that all rows see with some weight makes its column infinite in all of them, and no other column."""
+    b, q = special(pkg, dev, dt, case)
+    q = q * 0.25  # scores of a fraction: no weight rounds to zero
+    want, tol, see = plain(b, 0, q, 0.125)
+    page, slot = b.slots(0, 5, 6)
+    b.v_pages[page, :, slot, 7] = math.inf
+    b.v_pages[page, :, slot, 9] = -math.inf
+    o = torch.zeros_like(q)
+    attend(pkg, pkg.AttentionPaged(0), b, q, o)
+    got = o[:, : b.n[0]]
+    assert bool((got[..., 7] == math.inf).all()) and bool((got[..., 9] == -math.inf).all())
+    rest = [c for c in range(64) if c not in (7, 9)]
+    near(got[..., rest], want[..., rest], tol[..., rest], "the other columns")
