@@ -142,10 +142,11 @@ OPS_API int ops_attention_paged_launch(const ops_attention_paged *op, const ops_
                               op ? op->h.status : nullptr, &g.batch));
   if (m.nt == 0 || m.nh == 0 || m.dh == 0 || m.paged.nseq == 0) return OPS_OK;
   if (m.paged.npages == 0) return fail(OPS_SHAPE_NOT_SUPPORT, "attention_paged: a cache without pages");
-  if (!op) return fail(OPS_ARGS_NOT_SUPPORT, "null handle");
-  const OpBase &base = op->h.base;
+  const OpBase base = op ? op->h.base : OpBase{0, 148};
   const PagedAttnPlan plan = attention_paged_plan(base, m.nh, m.paged.nkvh, m.dh, a->mask == OPS_MASK_CAUSAL, g.batch.max_seq, m.nt, m.paged.nseq,
                                                 m.paged.width * m.paged.page);
+  if (!plan.fit) return fail(OPS_SHAPE_NOT_SUPPORT, "attention_paged: more than some 2^29 units of a sequence, a kv head and its query rows");
+  if (!op) return fail(OPS_ARGS_NOT_SUPPORT, "null handle");
   if (!ws || ws_len < plan.bytes()) return need_workspace(plan.bytes());
   g.q = (const char *)a->q_base;
   g.q_h = a->q_layout.strides[0];

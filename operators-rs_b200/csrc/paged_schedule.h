@@ -84,25 +84,29 @@ OPS_HD int paged_share(int ctas, int k) { return ctas * k / AP_SHARES > 0 ? ctas
 struct PagedLines {
   PagedLine few, tile;  // ctas == 0: nothing can be on it
   int few_rows;
+  bool fit;  // whatever the device finds in the batch, both fit in 31 bits
 };
 
-// The least shift with which a line cannot pass 31 bits: units, at most all rows in tiles and one more per sequence, of at most
-// all slots and rows.  `overhead`, `min_share`: keys.
-inline void paged_line_scale(PagedLine *l, size_t nt, size_t nseq, size_t slots, int overhead, int min_share) {
-  const double units = ((double)(nt / (size_t)l->tokens) + (double)nseq) * l->nkvh, keys = (double)slots + (double)nt + l->tokens + overhead;
+// The least shift with which a line cannot pass 31 bits: units, at most all rows in tiles and one more per sequence with rows, of at
+// most all slots and rows; false: there is none.  `overhead`, `min_share`: keys.
+inline bool paged_line_scale(PagedLine *l, size_t nt, size_t nseq, size_t slots, int overhead, int min_share) {
+  const double units = ((double)(nt / (size_t)l->tokens) + (double)std::min(nseq, nt)) * l->nkvh, keys = (double)slots + (double)nt + l->tokens + overhead;
+  auto fits = [&] { return units * (std::ldexp(keys, -l->shift) + 4.0) <= 2147483647.0; };
   l->shift = 0;
-  while (l->shift < 30 && units * (std::ldexp(keys, -l->shift) + 4.0) > 2147483647.0) ++l->shift;
+  while (l->shift < 30 && !fits()) ++l->shift;
   l->overhead = std::max(1, overhead >> l->shift);
   l->min_share = std::max(1, min_share >> l->shift);  // a power of two
   l->min_share_log2 = 0;
   while ((1 << l->min_share_log2) < l->min_share) ++l->min_share_log2;
   l->by_tokens = paged_div_by((uint32_t)l->tokens);
   l->by_ctas = paged_div_by((uint32_t)l->ctas);
+  return fits();
 }
 
 // For nt rows and nseq sequences of up to `slots` slots; max_seq: 0xffffffff when unknown.
 inline PagedLines paged_lines(int sm_count, size_t nh, size_t nkvh, bool causal, uint32_t max_seq, size_t nt, size_t nseq, size_t slots) {
   PagedLines p = PagedLines();
+  p.fit = true;
   const size_t group = nh / nkvh, most = max_seq == 0xffffffffu ? 0xffffffffull : (size_t)max_seq * group;
   // 16 rows cost the kernel a third of its ring; 8 are enough for one token of up to 8 heads
   p.few_rows = group <= 8 && !(most > 8 && most <= 16) ? 8 : 16;
@@ -119,7 +123,7 @@ inline PagedLines paged_lines(int sm_count, size_t nh, size_t nkvh, bool causal,
     p.few.tokens = p.few_rows;
     p.few.block_log2 = AP_FEW_BLOCK_LOG2;
     p.few.ctas = std::min(sm_count, AP_MAX_CTAS);  // one a SM: the ring takes its shared memory
-    paged_line_scale(&p.few, nt, nseq, slots, 128, 128);
+    p.fit = paged_line_scale(&p.few, nt, nseq, slots, 128, 128);
     p.tile.rows_lo = p.few_rows + 1;
   } else {
     p.tile.rows_lo = 1;
@@ -129,7 +133,7 @@ inline PagedLines paged_lines(int sm_count, size_t nh, size_t nkvh, bool causal,
     p.tile.tokens = AP_TILE_ROWS / 2 / (int)group * 2;
     p.tile.block_log2 = AP_TILE_BLOCK_LOG2;
     p.tile.ctas = std::min(sm_count, AP_MAX_CTAS);
-    paged_line_scale(&p.tile, nt, nseq, slots, 512, 512);
+    p.fit = paged_line_scale(&p.tile, nt, nseq, slots, 512, 512) && p.fit;
   }
   return p;
 }

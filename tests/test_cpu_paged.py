@@ -301,3 +301,16 @@ def test_schedule_of_launches_on_the_cpu(tmp_path):
     assert built.returncode == 0, built.stderr
     ran = subprocess.run([exe], capture_output=True, text=True, timeout=300)
     assert ran.returncode == 0 and "schedule ok" in ran.stdout, ran.stdout
+
+
+@pytest.mark.parametrize("rows,nseq,nkvh,fits", [(7, 3, 2, True), (1 << 20, 1 << 20, 8, True), (1 << 28, 1 << 28, 2, False), (1 << 29, 1, 128, False), (1, 1 << 27, 8, True)])
+def test_attention_paged_refuses_more_units_than_a_line_holds(pkg, rows, nseq, nkvh, fits):
+    """The device would find that they do not fit, write nothing and blame the batch."""
+    F16, I32 = pkg.F16, pkg.I32
+    q, kv = L(pkg, F16, (128, rows, 8)), L(pkg, F16, (10, nkvh, 16, 8))
+    b = batch(pkg, L(pkg, I32, (nseq, 5)), L(pkg, I32, (nseq + 1,)), L(pkg, I32, (nseq,)))
+    args = attention_args(pkg, q=q, o=q, k=kv, v=kv, b=b)
+    if fits:
+        assert passes(pkg, "attention_paged", args)
+    else:
+        assert launch(pkg, "attention_paged", args) == pkg.SHAPE_NOT_SUPPORT and "units" in pkg.last_error(), pkg.last_error()
