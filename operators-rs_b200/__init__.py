@@ -453,6 +453,8 @@ class PagedBatch:
                 raise ValueError("page_table, seq_start and kv_len are read by the kernels: device tensors expected")
         self.operands = tuple([_operand(t, None if isinstance(t, TensorLayout) else t) for t in self.arrays])
         self.max_seq = int(max_seq)
+        if not 0 <= self.max_seq < 1 << 64:
+            raise ValueError(f"max_seq = {max_seq}: a number of tokens expected, 0 where it is unknown")
 
 
 class KvAppendPagedArgs(_PackedArgs):

@@ -314,3 +314,9 @@ def test_attention_paged_refuses_more_units_than_a_line_holds(pkg, rows, nseq, n
         assert passes(pkg, "attention_paged", args)
     else:
         assert launch(pkg, "attention_paged", args) == pkg.SHAPE_NOT_SUPPORT and "units" in pkg.last_error(), pkg.last_error()
+
+
+def test_batch_of_a_negative_max_seq_is_refused(pkg):
+    for wrong in (-1, 1 << 64):
+        with pytest.raises(ValueError, match="max_seq"):
+            batch(pkg, max_seq=wrong)
