@@ -320,3 +320,71 @@ def test_batch_of_a_negative_max_seq_is_refused(pkg):
     for wrong in (-1, 1 << 64):
         with pytest.raises(ValueError, match="max_seq"):
             batch(pkg, max_seq=wrong)
+
+
+def test_argument_structs_are_those_of_the_header(pkg, tmp_path):
+    """What the Python mirror packs by hand, read back by code that was compiled against the header."""
+    lib = str(tmp_path / "libpaged_structs_check.so")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "paged_structs_check.cc")
+    built = subprocess.run([shutil.which("g++") or "g++", "-O1", "-std=c++17", "-Wall", "-shared", "-fPIC", src, "-o", lib], capture_output=True, text=True)
+    assert built.returncode == 0, built.stderr
+    read = ctypes.CDLL(lib)
+    bases = iter(range(0x1000, 0x100000, 0x1000))
+
+    def field(name, dt, rank):
+        base = next(bases)
+        shape, strides = tuple(base + i for i in range(rank)), tuple(-base - i for i in range(rank))
+        line = f"{name} dt {dt} shape {' '.join(map(str, shape))} strides {' '.join(map(str, strides))} base {base:x}"
+        return pkg.TensorLayout(dt, shape, strides), base, line
+
+    def check(function, make, names, tail, with_batch):
+        fields = [field(name, dt, rank) for name, dt, rank in names]
+        flat = [x for layout, base, _ in fields for x in (layout, base)]
+        lines = [line for _, _, line in fields]
+        more = []
+        if with_batch:
+            arrays = [field(name, pkg.U32, rank) for name, rank in (("page_table", 2), ("seq_start", 1), ("kv_len", 1))]
+            b = pkg.PagedBatch(*(layout for layout, _, _ in arrays), 123456789012345)
+            b.operands = tuple((*o[:-1], base) for o, (_, base, _) in zip(b.operands, arrays))
+            more, lines = [b], lines + [line for _, _, line in arrays] + ["max_seq 123456789012345"]
+        args = make(*flat, *more)
+        front = 32  # an operand: u32 dt, u32 ndim, two pointers; its base
+        size = len(names) * front + (3 * front + 8 if with_batch else 0) + 8
+        fn = getattr(read, function)
+        fn.restype = ctypes.c_char_p
+        fn.argtypes = [ctypes.c_void_p]
+        assert fn(args.byref()).decode().splitlines() == lines + [f"{tail} size {size}"]
+
+    F16, BF16 = pkg.F16, pkg.BF16
+    check("read_rope_norm", lambda *a: pkg.RopeNormArgs(*a, 0.25, 512.0), [("y", F16, 3), ("x", F16, 3), ("p", pkg.U64, 1), ("w", pkg.F32, 2)],
+          "epsilon 0.25 theta 512", False)
+    check("read_kv_append_paged", lambda *a: pkg.KvAppendPagedArgs(*a, 0.25, 512.0),
+          [("q_out", F16, 3), ("q", F16, 3), ("k", BF16, 3), ("v", F16, 3), ("k_pages", BF16, 4), ("v_pages", F16, 4), ("p", pkg.U32, 1), ("w", F16, 2)],
+          "epsilon 0.25 theta 512", True)
+    check("read_attention_paged", lambda *a: pkg.AttentionPagedArgs(*a, 1, 0.125),
+          [("q", F16, 3), ("k_pages", BF16, 4), ("v_pages", F16, 4), ("o", BF16, 3)], "mask 1 scale 0.125", True)
+
+
+@pytest.mark.parametrize("tp", [1, 2, 4])
+def test_norm_weights_of_the_heads_are_cut_with_them(pkg, tp):
+    """Every head of a rank's shard has the weights that it has in the whole layer."""
+    import importlib
+
+    import numpy as np
+
+    import __graft_entry__ as graft
+    layer = importlib.import_module(graft.PKG_NAME + ".layer")
+    nh, nkvh, dh, d, ffn = 12, 4, 8, 6, 16
+    cfg = layer.LayerConfig(d=d, nh=nh, nkvh=nkvh, dh=dh, ffn=ffn)
+    heads = np.arange(nh + 2 * nkvh, dtype=np.float32)
+    w = {"w_norm1": np.ones(d), "w_norm2": np.ones(d), "w_qkv": np.repeat(heads, dh)[None].repeat(d, 0), "w_o": np.ones((nh * dh, d)),
+         "w_gu": np.ones((d, 2 * ffn)), "w_down": np.ones((ffn, d)), "w_qk_norm": np.repeat(heads[: nh + nkvh, None], dh, 1)}
+    seen = []
+    for rank in range(tp):
+        cut = layer.shard_weights(w, rank, tp, cfg)
+        n = (nh + nkvh) // tp
+        assert cut["w_qk_norm"].shape == (n, dh)
+        of_columns = cut["w_qkv"][0].reshape(-1, dh)[:n]
+        assert np.array_equal(of_columns, cut["w_qk_norm"])
+        seen += cut["w_qk_norm"][:, 0].tolist()
+    assert sorted(seen) == heads[: nh + nkvh].tolist()
