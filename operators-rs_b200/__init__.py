@@ -257,12 +257,24 @@ def _operand(layout, base):
     return info[0], layout.shape, layout.stride(), info[1], layout.data_ptr() if base is layout else ptr(base)
 
 
+_devices = 0
+
+
+def _one_device():
+    global _devices
+    if _devices == 0:
+        import torch
+        _devices = torch.cuda.device_count()
+    return _devices == 1
+
+
 class _PackedArgs(_ArgsBase):
     """An args struct written in one go: `operands` layouts, each followed by its base pointer, then TAIL; the shapes and
     strides that the layouts point to lie behind it in the same buffer.  (A decode step makes several of these per layer: one
     ctypes object per layout costs 5 us each, a step's kernels run for less.)"""
     TAIL = ""   # struct format of what follows the operands
     _plans = {}
+    _batch = None
 
     def _fill(self, operands, tail):
         """operands: as `_operand` makes them."""
@@ -288,7 +300,16 @@ class _PackedArgs(_ArgsBase):
 
     def check_home(self, device):
         """Refuses operands that a kernel on `device` cannot follow: those of the host (not pinned) or of another device."""
-        for t in self._alive:
+        try:
+            for t in self._alive:
+                if not t.is_cuda:
+                    break
+            else:
+                if _one_device():  # (the batch's arrays are the device's, or there would be no batch)
+                    return
+        except AttributeError:
+            pass
+        for t in self._alive + (self._batch.arrays if self._batch is not None else ()):
             where = getattr(t, "get_device", None)  # (an address or a layout has none: the caller's word)
             if where is not None:
                 where = where()
@@ -463,7 +484,8 @@ class KvAppendPagedArgs(_PackedArgs):
 
     def __init__(self, q_out_layout, q_out_base, q_layout, q_base, k_layout, k_base, v_layout, v_base, k_pages_layout, k_pages_base,
                  v_pages_layout, v_pages_base, p_layout, p_base, w_layout, w_base, batch, epsilon, theta):
-        self._alive = (q_out_base, q_base, k_base, v_base, k_pages_base, v_pages_base, p_base, w_base, *batch.arrays)
+        self._alive = (q_out_base, q_base, k_base, v_base, k_pages_base, v_pages_base, p_base, *(() if w_base is None else (w_base,)))
+        self._batch = batch
         self._fill((_operand(q_out_layout, q_out_base), _operand(q_layout, q_base), _operand(k_layout, k_base), _operand(v_layout, v_base),
                     _operand(k_pages_layout, k_pages_base), _operand(v_pages_layout, v_pages_base), _operand(p_layout, p_base),
                     _NO_WEIGHT if w_layout is None else _operand(w_layout, w_base), *batch.operands), (batch.max_seq, epsilon, theta))
@@ -478,7 +500,8 @@ class AttentionPagedArgs(_PackedArgs):
     TAIL = "QB3xf"  # batch.max_seq, mask, scale
 
     def __init__(self, q_layout, q_base, k_pages_layout, k_pages_base, v_pages_layout, v_pages_base, o_layout, o_base, batch, mask, scale):
-        self._alive = (q_base, k_pages_base, v_pages_base, o_base, *batch.arrays)
+        self._alive = (q_base, k_pages_base, v_pages_base, o_base)
+        self._batch = batch
         self._fill((_operand(q_layout, q_base), _operand(k_pages_layout, k_pages_base), _operand(v_pages_layout, v_pages_base),
                     _operand(o_layout, o_base), *batch.operands), (batch.max_seq, mask, scale))
 
@@ -754,9 +777,9 @@ class AttentionKvCached(Operator):
 class _PagedOperator(Operator):
     def launch(self, args, workspace=None, queue_alloc=None):
         args.check_home(self.device)
-        if hasattr(workspace, "get_device") and (workspace.get_device() != self.device or not workspace.is_contiguous()):
+        if workspace is not None and hasattr(workspace, "get_device") and (workspace.get_device() != self.device or not workspace.is_contiguous()):
             raise ValueError(f"workspace: a contiguous tensor of cuda:{self.device} expected")
-        super().launch(args, workspace, queue_alloc)
+        Operator.launch(self, args, workspace, queue_alloc)
 
     def status(self):
         """0, or what the device found wrong first (PAGED_BAD_*; from 100 on a bounded wait ran out).  Synchronises."""

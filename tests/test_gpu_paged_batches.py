@@ -239,3 +239,20 @@ def test_attention_paged_infinite_values(pkg, dev, dt, case):
     assert bool((got[..., 7] == math.inf).all()) and bool((got[..., 9] == -math.inf).all())
     rest = [c for c in range(64) if c not in (7, 9)]
     near(got[..., rest], want[..., rest], tol[..., rest], "the other columns")
+
+
+def test_operands_of_the_host_are_refused_beside_those_of_the_device(pkg, dev):
+    b = ref.Batch(dev, F16, [1], [20], 2, 64, 16, seed=1)
+    b.fill(gen(dev, 1))
+    q, ws = normal(gen(dev, 2), (4, 1, 64), F16), torch.empty(64 << 20, dtype=torch.uint8, device=dev)
+    op, o = pkg.AttentionPaged(0), torch.zeros(4, 1, 64, dtype=F16, device=dev)
+    attend(pkg, op, b, q, o, ws=ws)
+    want = o.clone()
+    for bent in ((q.cpu(), b.k_pages, b.v_pages, o), (q, b.k_pages.cpu(), b.v_pages, o), (q, b.k_pages, b.v_pages.cpu(), o), (q, b.k_pages, b.v_pages, o.cpu())):
+        with pytest.raises(ValueError, match="cuda:0 expected"):
+            op.launch(pkg.AttentionPagedArgs.of(*bent, b.descriptor(pkg)), ws)
+    for short in (ws.cpu(), ws[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            op.launch(pkg.AttentionPagedArgs.of(q, b.k_pages, b.v_pages, o, b.descriptor(pkg)), short)
+    attend(pkg, op, b, q, o, ws=ws)
+    assert torch.equal(o, want)
