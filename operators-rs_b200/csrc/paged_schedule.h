@@ -59,7 +59,7 @@ struct PagedSeq {
 
 struct PagedLine {
   int nkvh, group, causal;
-  int rows_lo, rows_hi;  // the sequences on this line: rows_lo <= n * group <= rows_hi (n > 0)
+  int rows_lo, rows_hi;  // the sequences on this line: rows_lo <= n * group <= rows_hi (n > 0); 0x7fffffff: no upper bound
   int max_seq;           // ... and n <= max_seq
   int tokens;            // query tokens of a unit
   int block_log2;        // keys of a block
@@ -153,7 +153,7 @@ OPS_HD PagedSpan paged_span(const PagedLine &l, const PagedSeq &s) {
   PagedSpan p;
   p.tiles = p.base = p.ramp = p.head = 0;
   const long long rows = (long long)s.n * l.group;
-  if (s.n <= 0 || s.n > l.max_seq || rows < l.rows_lo || rows > l.rows_hi) return p;
+  if (s.n <= 0 || s.n > l.max_seq || rows < l.rows_lo || (rows > l.rows_hi && l.rows_hi != 0x7fffffff)) return p;
   p.tiles = s.n <= l.tokens ? 1 : paged_div(s.n + l.tokens - 1, l.by_tokens);
   const bool ramped = l.causal && p.tiles > 1;
   p.base = l.overhead + paged_points(l, ramped ? (s.len > s.n ? s.len - s.n : 0) : (s.len > 0 ? s.len : 1));
@@ -282,7 +282,7 @@ struct PagedWalk {
 OPS_HD bool paged_rows_fit(const PagedLine &l, uint32_t r0, uint32_t r1) {
   if (r1 <= r0) return false;
   const unsigned long long rows = (unsigned long long)(r1 - r0) * (unsigned)l.group;
-  return rows >= (unsigned)l.rows_lo && rows <= (unsigned)l.rows_hi;
+  return rows >= (unsigned)l.rows_lo && (rows <= (unsigned)l.rows_hi || l.rows_hi == 0x7fffffff);
 }
 
 // The next piece of the share (an empty one is passed over).  Seqs: seq index -> PagedSeq.  Skip: the first sequence from the given

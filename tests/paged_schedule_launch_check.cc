@@ -103,6 +103,14 @@ static int check(const PagedLine &line, int ctas, const std::vector<PagedSeq> &s
 }
 
 int main() {
+  // a sequence of more query rows than 31 bits count, one of them alone and behind a single token
+  for (int n : {1 << 24, (1 << 24) + 1, 1 << 26})
+    for (int past : {0, 1000}) {
+      const PagedLines lines = paged_lines(148, 128, 1, true, 0xffffffffu, (size_t)n + 1, 2, (size_t)n + past);
+      const std::vector<PagedSeq> seqs{{0, 1, 1}, {1, n, n + past}};
+      CHECK(lines.fit && paged_span(lines.tile, seqs[1]).tiles == (n + lines.tile.tokens - 1) / lines.tile.tokens);
+      CHECK(paged_rows_fit(lines.tile, 1, 1 + (uint32_t)n) && !paged_rows_fit(lines.tile, 1, 1));
+    }
   std::mt19937 rng(11);
   auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
   for (round_no = 0; round_no < 1500; ++round_no) {
