@@ -307,6 +307,7 @@ void ops_attention_kv_cached_destroy(ops_attention_kv_cached *op);
  *                         slots than new tokens; tokens without a slot of the table are not written
  *   OPS_PAGED_BAD_ROWS    seq_start decreases or passes nt (cut to that), or a sequence has more new tokens than max_seq (attention
  *                         leaves its rows as they are)
+ * Both operators look at every sequence for the latter two, whether rows find their way to it or not.
  * Codes from 100 on: a bounded wait inside a kernel ran out (the launch's output is undefined then).
  * ------------------------------------------------------------------------------------------- */
 enum { OPS_PAGED_BAD_PAGE = 1, OPS_PAGED_BAD_LENGTH = 2, OPS_PAGED_BAD_ROWS = 3 };

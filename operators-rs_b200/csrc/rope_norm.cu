@@ -15,9 +15,10 @@
 // What bounded it first was instruction issue (full-range sincospi, 64-bit address arithmetic per vector: 70 us for 8192 rows of
 // 40 heads of 128); with angles reduced in f64 in front of the special-function unit, pointers that step and packed f32 pairs
 // it streams: 33 us.  The norm was 5 us of that, each vector's chain of shuffles behind the last one's: with the sums of a round
-// side by side 30 us, 5.6 TB/s (6 blocks an SM; with 7, or the weights loaded ahead of the sums, registers spill: 31, 37 us.  The
-// append takes 7: 30.2 us for seven prompts against 31.2 with 6).  Reads and writes both bypass what other kernels keep in L2
-// (either alone changed nothing).
+// side by side 30 us, 5.6 TB/s (6 blocks an SM; with 7, or the weights loaded ahead of the sums, registers spill: 31, 37 us).  The
+// append takes 7 blocks all the same: in rounds of four with norms it spills (32 to 46 bytes of stores, 76 to 88 of loads a thread, at
+// 72 registers), and seven prompts take 30.4 us against 31.2 with 6.  Reads and writes both bypass what other kernels keep in
+// L2 (either alone changed nothing for these kernels; the attention behind an append was not timed with them).
 #include <type_traits>
 
 #include "device_utils.cuh"
