@@ -629,7 +629,15 @@ class TorchQueueAlloc:
 
     def alloc(self, size):
         import torch
-        return torch.empty(max(int(size), 1), dtype=torch.uint8, device=self.device if self.device is not None else "cuda")
+        def make():
+            return torch.empty(max(int(size), 1), dtype=torch.uint8, device=self.device if self.device is not None else "cuda")
+
+        if self.stream is None or self.stream == current_stream(self.device):
+            return make()
+        # of the queue's stream: what the allocator has for another one may still be in use there, and would be handed on there, once
+        # dropped, before the queue has got past its launch
+        with torch.cuda.stream(torch.cuda.ExternalStream(self.stream, device=self.device) if self.stream else torch.cuda.default_stream(self.device)):
+            return make()
 
 
 class Operator:
@@ -671,7 +679,7 @@ class Operator:
             need = lib().ops_last_workspace_need()
             own = (queue_alloc or TorchQueueAlloc(self.device)).alloc(need)
             rc = self._launch(self._h, args.byref(), own.data_ptr(), need, stream)
-            self._last_ws = own  # stream-ordered reuse by torch's allocator keeps this safe once dropped
+            self._last_ws = own  # torch's allocator hands it on in the order of the queue's stream: safe once dropped
         if rc != OK:
             _check(rc, True)
 

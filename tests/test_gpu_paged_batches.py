@@ -256,3 +256,40 @@ def test_operands_of_the_host_are_refused_beside_those_of_the_device(pkg, dev):
             op.launch(pkg.AttentionPagedArgs.of(q, b.k_pages, b.v_pages, o, b.descriptor(pkg)), short)
     attend(pkg, op, b, q, o, ws=ws)
     assert torch.equal(o, want)
+
+
+# ------------------------------------------------------------------------------------------------ workspaces of a stream of the caller's
+def test_workspace_of_another_stream_is_not_handed_on_while_it_is_used(pkg, dev):
+    """A launch on a queue of the caller's own, without a workspace: what the mirror allocates for it is that queue's, neither what
+    the current stream may still be using nor, once the next launch has dropped it, what the current stream is given next."""
+    b = ref.Batch(dev, F16, [1, 90], [5000, 100], 2, 128, 16, seed=8)
+    g = gen(dev, 8)
+    b.fill(g)
+    q = normal(g, (8, b.nt, 128), F16)
+    outs = [torch.zeros_like(q) for _ in range(3)]
+    op = pkg.AttentionPaged(0)
+    args = [pkg.AttentionPagedArgs.of(q, b.k_pages, b.v_pages, o, b.descriptor(pkg)) for o in outs]
+    need = op.scheme(args[0])
+    op.launch(args[0], torch.empty(need, dtype=torch.uint8, device=dev))
+    for side in [torch.cuda.Stream(dev) for _ in range(6)]:  # some share a queue of the device's with the current stream: those wait anyway
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+        queue = pkg.TorchQueueAlloc(dev, side.cuda_stream)
+        free = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr()  # the current stream's, until here
+        op.launch(args[1], None, queue)
+        assert op._last_ws.data_ptr() != free
+        op.launch(args[2], None, queue)  # drops the first one's workspace
+        mine = [torch.full((need,), 77, dtype=torch.uint8, device=dev) for _ in range(4)]  # of the current stream
+        torch.cuda.synchronize()
+        assert all(bool((x == 77).all()) for x in mine)
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+        del mine
+
+
+def test_queues_of_every_kind_allocate(pkg, dev):
+    side = torch.cuda.Stream(dev)
+    for device in (None, 0, dev, "cuda:0"):
+        for stream in (None, 0, side.cuda_stream, torch.cuda.current_stream().cuda_stream):
+            mem = pkg.TorchQueueAlloc(device, stream).alloc(1000)
+            assert mem.is_cuda and mem.numel() == 1000 and mem.get_device() == 0
