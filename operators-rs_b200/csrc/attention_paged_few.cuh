@@ -11,7 +11,9 @@
 //
 //   warps 0-3  consumers: S = Q K^T and O += P V for a stage's 32 keys on m16n8k16 warp MMAs (the rows are the 8 or 16 of the MMA;
 //              a 128-row tcgen05 tile has nothing to chew on here), both operands by ldmatrix from the 128-byte-swizzled stage,
-//              the probabilities straight from the S registers: about 1400 clocks a stage, four stages at a time
+//              the probabilities straight from the S registers: about 1400 clocks a stage, four stages at a time.  They round to
+//              the element type there, as the warp MMA wants (half a step each, at random over the keys: against 64 bits the output
+//              is off by at most 1.3 times what its own rounding is off by); the sums that they are divided by do not
 //   warps 4-7  producers, every fourth stage each (the boxes of one warp alone come to 3.4 TB/s): a lane per box of a stage
 //              (32 / min(page, 32) boxes of K and of V), pages looked up a stage ahead
 //   warp 8     scheduler: finds the CTA's share, posts its pieces ahead
